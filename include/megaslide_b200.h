@@ -56,6 +56,9 @@ extern "C" {
                                     had issued, skipped every phase that reads the copied keys, and its
                                     results are not valid */
 
+#define MSL_STATUS_ROTARY_INDEX 8u /* rotary positions: an index outside its axis; that axis of the token is
+                                      left unrotated, the results are not valid */
+
 /* kernel family */
 #define MSL_ALGO_AUTO 0 /* tensor-core envelope kernels when supported (bf16, head_dim % 8 == 0, <= 128) */
 #define MSL_ALGO_SIMT 1 /* CUDA-core gather kernels (float32 and bf16, any head_dim <= 128) */
@@ -249,6 +252,119 @@ int msl_offsets_absmax(const float* offsets, int64_t rows, int64_t ld, const flo
 /* Element-type conversion float32 -> dtype of a [rows, cols] matrix (row strides in elements). */
 int msl_convert_f32(const float* src, int64_t src_ld, void* dst, int64_t dst_ld, int32_t dtype,
                     int64_t rows, int64_t cols, void* stream);
+
+/* ----------------------------------------------------------------------------------------------
+ * Rotary positions with several axes, alone and in one pass with the per-head RMS norm of queries and
+ * keys.  No counterpart in the reference (it adds a learned table of positions, model.py:128-131).
+ *
+ * A head's first axis_t + axis_h + axis_w channels turn in pairs: pair p is channels (2p, 2p+1)
+ * (interleaved) or (p, p + R/2), R the number of turning channels; the first axis_t/2 pairs turn by the
+ * token's time position, the next axis_h/2 by its row, the last axis_w/2 by its column.  The remaining
+ * channels pass.  table: float32 (cos, sin) of every position and pair of an axis, the axes one after the
+ * other: [frames, axis_t/2, 2], [height, axis_h/2, 2], [width, axis_w/2, 2].
+ * Token n of a sample has t = frame0 + n / (height*width), h, w as in x[B, N, C]; or, with index (int32
+ * [index_rows, 3], row r of the call using index row r % index_rows), the three table rows it names.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct msl_rotary_geometry {
+  int64_t rows;                  /* tokens of the call, all samples */
+  int64_t tokens;                /* tokens of a sample (grid positions restart there) */
+  int32_t frames, height, width; /* extents of the table */
+  int32_t frame0;                /* time position of a sample's first token (grid positions) */
+  int32_t axis_t, axis_h, axis_w;
+  int32_t head_dim;              /* even, <= 256 */
+  int32_t interleaved;
+  int32_t dtype;                 /* MSL_DTYPE_* of the token rows */
+} msl_rotary_geometry;
+
+/* y = rotated x, both [rows, >= heads*head_dim]; y may be x.  inverse != 0 turns the other way, which is
+ * the backward pass.  status (may be NULL) receives MSL_STATUS_ROTARY_INDEX. */
+int msl_rope3d(const msl_rotary_geometry* geom, int32_t heads, const void* x, int64_t x_ld, const float* table,
+               const int32_t* index, int64_t index_rows, int32_t inverse, void* y, int64_t y_ld, uint32_t* status,
+               void* stream);
+
+/* Operands of the norm + rotation of queries [rows, heads*head_dim] and keys [rows, kv_heads*head_dim]
+ * (kv_heads may be 0: queries alone).  weights: [head_dim] of weight_dtype, shared by the heads; NULL = ones.
+ * table NULL: no rotation.  q_out / k_out may be q / k.  The fields from dq_out on are the backward's:
+ * dq_out, dk_out gradients of the results; dq, dk gradients of q, k (may be dq_out, dk_out); dq_weight,
+ * dk_weight [head_dim] of weight_dtype, or both NULL. */
+typedef struct msl_qk_norm_io {
+  const void* q; int64_t q_ld;
+  const void* k; int64_t k_ld;
+  const void* q_weight; const void* k_weight;
+  void* q_out; int64_t q_out_ld;
+  void* k_out; int64_t k_out_ld;
+  const float* table;
+  const int32_t* index; int64_t index_rows;
+  uint32_t* status;
+  int32_t heads, kv_heads, weight_dtype;
+  float eps;
+  const void* dq_out; int64_t dq_out_ld;
+  const void* dk_out; int64_t dk_out_ld;
+  void* dq; int64_t dq_ld;
+  void* dk; int64_t dk_ld;
+  void* dq_weight; void* dk_weight;
+} msl_qk_norm_io;
+
+/* out = rotate(x / sqrt(mean(x^2) + eps) * weight), per token and head, statistics in float32. */
+int msl_qk_norm_rope_fwd(const msl_rotary_geometry* geom, const msl_qk_norm_io* io, void* stream);
+/* Bytes of workspace that msl_qk_norm_rope_bwd needs for the weights' gradients (0 without them). */
+size_t msl_qk_norm_rope_bwd_workspace_bytes(const msl_rotary_geometry* geom, const msl_qk_norm_io* io);
+/* Gradients of q, k and the weights; sums in a fixed order (the same result on every run). */
+int msl_qk_norm_rope_bwd(const msl_rotary_geometry* geom, const msl_qk_norm_io* io, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* ----------------------------------------------------------------------------------------------
+ * Gated feed-forward block  y = (act(g) * u) w_out^T + b_out,  [g u] = x w_in^T + b_in,
+ * x [rows, dim], w_in [2*hidden, dim] (gate rows, then up rows), w_out [dim, hidden].  No counterpart in
+ * the reference (its MLP is fc1, GELU, fc2, model.py:21-37).
+ * ---------------------------------------------------------------------------------------------- */
+#define MSL_ACT_SILU 0
+#define MSL_ACT_GELU 1 /* erf form */
+
+typedef struct msl_ffn_geometry {
+  int64_t rows;
+  int32_t dim, hidden;
+  int32_t dtype;      /* MSL_DTYPE_* of every operand */
+  int32_t activation; /* MSL_ACT_* */
+} msl_ffn_geometry;
+
+/* Matrices are contiguous rows of their width except x, y, dy and dx (row strides given).  h [rows, hidden]
+ * is the gated product that the second projection reads; gu [rows, 2*hidden] receives g and u, which the
+ * backward reads (NULL = not kept).  Backward: dgu [rows, 2*hidden] is scratch (the gradients of g and u);
+ * dx, dw_in, dw_out, db_in, db_out are written where they are not NULL. */
+typedef struct msl_ffn_io {
+  const void* x; int64_t x_ld;
+  const void* w_in; const void* b_in;
+  const void* w_out; const void* b_out;
+  void* h; void* gu;
+  void* y; int64_t y_ld;
+  const void* dy; int64_t dy_ld;
+  void* dgu;
+  void* dx; int64_t dx_ld;
+  void* dw_in; void* dw_out; void* db_in; void* db_out;
+  uint32_t* status; /* MSL_STATUS_TIMEOUT, as in the attention (may be NULL) */
+} msl_ffn_io;
+
+size_t msl_gated_ffn_workspace_bytes(const msl_ffn_geometry* geom, int32_t backward);
+int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,
+                      void* stream);
+int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* ----------------------------------------------------------------------------------------------
+ * Global gradient norm over many tensors, and clipping (the device counterpart of the norm and scale
+ * of the reference's optimizer step, infinity/video/trainer.py:575-599).  src, dst, numel and dtype are host
+ * arrays of `count` entries, read before the call returns.
+ * ---------------------------------------------------------------------------------------------- */
+size_t msl_grad_norm_workspace_bytes(const int64_t* numel, int32_t count);
+/* *norm (device float32) = sqrt(extra_sumsq + sum of squares of every element), accumulated in float32
+ * and joined in double, in a fixed order. */
+int msl_grad_norm(const void* const* src, const int64_t* numel, const int32_t* dtype, int32_t count,
+                  double extra_sumsq, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+/* msl_grad_norm, then dst = src * min(1, max_norm / (norm + 1e-6)) (dst of src's type; may be src). */
+int msl_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int32_t count,
+                  double extra_sumsq, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 int32_t msl_abi_version(void);
 /* Kernel launches issued by this library since it was loaded (all threads). */

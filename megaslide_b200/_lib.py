@@ -24,6 +24,7 @@ MSL_DTYPE_BF16 = 1
 MSL_STATUS_HALO_MISS = 1
 MSL_STATUS_TC_RANGE = 2
 MSL_STATUS_TIMEOUT = 4
+MSL_STATUS_ROTARY_INDEX = 8
 MSL_ALGO_AUTO = 0
 MSL_ALGO_SIMT = 1
 MSL_ALGO_TC = 2
@@ -31,6 +32,8 @@ MSL_EPI_NONE = 0
 MSL_EPI_GELU = 1
 MSL_EPI_GELU_GRAD = 2
 MSL_EPI_ACCUM = 3
+MSL_ACT_SILU = 0
+MSL_ACT_GELU = 1
 MSL_NOALLOC_SCRATCH_BYTES = 64 * 1024 * 1024
 
 _i32 = ctypes.c_int32
@@ -87,6 +90,44 @@ class DwconvGeometry(ctypes.Structure):
     ]
 
 
+class RotaryGeometry(ctypes.Structure):
+    """Mirror of ``msl_rotary_geometry``."""
+
+    _fields_ = [
+        ("rows", _i64), ("tokens", _i64), ("frames", _i32), ("height", _i32), ("width", _i32), ("frame0", _i32),
+        ("axis_t", _i32), ("axis_h", _i32), ("axis_w", _i32), ("head_dim", _i32), ("interleaved", _i32), ("dtype", _i32),
+    ]
+
+
+class QkNormIO(ctypes.Structure):
+    """Mirror of ``msl_qk_norm_io``."""
+
+    _fields_ = [
+        ("q", _vp), ("q_ld", _i64), ("k", _vp), ("k_ld", _i64), ("q_weight", _vp), ("k_weight", _vp),
+        ("q_out", _vp), ("q_out_ld", _i64), ("k_out", _vp), ("k_out_ld", _i64),
+        ("table", _vp), ("index", _vp), ("index_rows", _i64), ("status", _vp),
+        ("heads", _i32), ("kv_heads", _i32), ("weight_dtype", _i32), ("eps", _f32),
+        ("dq_out", _vp), ("dq_out_ld", _i64), ("dk_out", _vp), ("dk_out_ld", _i64),
+        ("dq", _vp), ("dq_ld", _i64), ("dk", _vp), ("dk_ld", _i64), ("dq_weight", _vp), ("dk_weight", _vp),
+    ]
+
+
+class FfnGeometry(ctypes.Structure):
+    """Mirror of ``msl_ffn_geometry``."""
+
+    _fields_ = [("rows", _i64), ("dim", _i32), ("hidden", _i32), ("dtype", _i32), ("activation", _i32)]
+
+
+class FfnIO(ctypes.Structure):
+    """Mirror of ``msl_ffn_io``."""
+
+    _fields_ = [
+        ("x", _vp), ("x_ld", _i64), ("w_in", _vp), ("b_in", _vp), ("w_out", _vp), ("b_out", _vp), ("h", _vp), ("gu", _vp),
+        ("y", _vp), ("y_ld", _i64), ("dy", _vp), ("dy_ld", _i64), ("dgu", _vp), ("dx", _vp), ("dx_ld", _i64),
+        ("dw_in", _vp), ("dw_out", _vp), ("db_in", _vp), ("db_out", _vp), ("status", _vp),
+    ]
+
+
 # name -> (restype, argtypes); the full exported surface of include/megaslide_b200.h
 SIGNATURES = {
     "msl_dsa_attn_fwd": (ctypes.c_int, [ctypes.POINTER(DsaGeometry), ctypes.POINTER(DsaFwdIO), _vp]),
@@ -103,6 +144,17 @@ SIGNATURES = {
                                                _vp, _vp]),
     "msl_offsets_absmax": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i32, _i32, _f32, _vp, _vp]),
     "msl_convert_f32": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp]),
+    "msl_rope3d": (ctypes.c_int, [ctypes.POINTER(RotaryGeometry), _i32, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _vp]),
+    "msl_qk_norm_rope_fwd": (ctypes.c_int, [ctypes.POINTER(RotaryGeometry), ctypes.POINTER(QkNormIO), _vp]),
+    "msl_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RotaryGeometry), ctypes.POINTER(QkNormIO)]),
+    "msl_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(RotaryGeometry), ctypes.POINTER(QkNormIO), _vp, ctypes.c_size_t,
+                                            _vp]),
+    "msl_gated_ffn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FfnGeometry), _i32]),
+    "msl_gated_ffn_fwd": (ctypes.c_int, [ctypes.POINTER(FfnGeometry), ctypes.POINTER(FfnIO), _vp, ctypes.c_size_t, _vp]),
+    "msl_gated_ffn_bwd": (ctypes.c_int, [ctypes.POINTER(FfnGeometry), ctypes.POINTER(FfnIO), _vp, ctypes.c_size_t, _vp]),
+    "msl_grad_norm_workspace_bytes": (ctypes.c_size_t, [_vp, _i32]),
+    "msl_grad_norm": (ctypes.c_int, [_vp, _vp, _vp, _i32, ctypes.c_double, _vp, _vp, ctypes.c_size_t, _vp]),
+    "msl_grad_clip": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, ctypes.c_double, _f32, _vp, _vp, ctypes.c_size_t, _vp]),
     "msl_host_accumulate": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, ctypes.POINTER(ctypes.c_double)]),
     "msl_host_adamw": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _f32, _i64, _f32, _vp, _i32]),
     "msl_abi_version": (_i32, []),

@@ -1,0 +1,54 @@
+"""Global gradient norm over many tensors and clipping on the kernels of csrc/grad_norm.cu: two launches for the
+norm or for norm and scaling, whatever the number of tensors, and no wait for the GPU."""
+
+from __future__ import annotations
+
+import math
+from typing import Iterable, List, Optional, Sequence, Union
+
+import torch
+from torch import Tensor
+
+from . import ops
+
+Tensors = Union[Tensor, Iterable[Optional[Tensor]]]
+
+
+def _list(tensors: Tensors) -> List[Tensor]:
+    """The tensors of a call; of parameters (which require gradients) their gradients, where they have one."""
+    ts = [tensors] if isinstance(tensors, Tensor) else [t for t in tensors if t is not None]
+    return [t.detach() if not isinstance(t, torch.nn.Parameter) else t.grad for t in ts
+            if not isinstance(t, torch.nn.Parameter) or t.grad is not None]
+
+
+def _check(extra_sumsq: float) -> float:
+    if not extra_sumsq >= 0:
+        raise ValueError(f"extra_sumsq must be >= 0, got {extra_sumsq}")
+    return float(extra_sumsq)
+
+
+def grad_norm(tensors: Tensors, extra_sumsq: float = 0.0) -> Tensor:
+    """2-norm of all elements of the tensors together (float32 or bfloat16, contiguous, on one CUDA device; parameters
+    stand for their gradients), as a 0-dim float32 tensor on their device.  extra_sumsq: a sum of squares held
+    elsewhere (on the host, on other ranks) that belongs to the norm.  Without tensors the norm of extra_sumsq
+    alone, on the CPU."""
+    ts = _list(tensors)
+    extra = _check(extra_sumsq)
+    if not ts:
+        return torch.tensor(math.sqrt(extra))
+    return ops.grad_norm(ts, extra_sumsq=extra)
+
+
+def clip_grad_norm_(tensors: Tensors, max_norm: float, *, out: Optional[Sequence[Tensor]] = None,
+                    extra_sumsq: float = 0.0) -> Tensor:
+    """Scales the tensors (parameters: their gradients) by min(1, max_norm / (norm + 1e-6)) and returns the norm
+    before that, as grad_norm does; nothing waits for the GPU.  out: tensors of the same dtypes and sizes that
+    receive the result in place of the tensors themselves (slices of one flat buffer, say).  A norm that is not finite
+    reaches the results as the formula says (an infinite norm: zeros, and NaN for its infinite elements)."""
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    ts = _list(tensors)
+    extra = _check(extra_sumsq)
+    if not ts:
+        return torch.tensor(math.sqrt(extra))
+    return ops.grad_norm(ts, ts if out is None else list(out), float(max_norm), extra)

@@ -9,6 +9,7 @@
 
 #include "dsa_attn.cuh"
 #include "megaslide_b200.h"
+#include "msl_abi.cuh"
 
 namespace {
 
@@ -162,6 +163,29 @@ int fill_conv(const msl_dwconv_geometry* g, msl::ConvParams& P) {
 namespace msl {
 // Records an error for msl_last_error() from another translation unit of the library.
 int record_error(int code, const char* msg) { return fail(code, "%s", msg); }
+
+int failf(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+
+void count_launches(unsigned n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
+
+int sm_count() {
+  static std::atomic<int> cached[64];
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  v = cached[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
+    cached[dev].store(v, std::memory_order_relaxed);
+  }
+  return v;
+}
 }  // namespace msl
 
 extern "C" {

@@ -1,0 +1,307 @@
+// Gated feed-forward block, forward and backward: the products on the CUDA cores (float32, and bf16
+// widths that no 16-byte row allows), the bias gradients, and the entry points.
+//
+//   [g u] = x w_in^T + b_in;  h = act(g) u;  y = h w_out^T + b_out
+//   dh = dy w_out;  dg = dh u act'(g);  du = dh act(g);  dx = [dg du] w_in;  dw_in = [dg du]^T x;
+//   dw_out = dy^T h;  db_in, db_out = column sums of [dg du], dy
+
+#include "gated_ffn.cuh"
+
+namespace msl {
+namespace ffn {
+
+constexpr int kTM = 64, kTN = 64, kTK = 16;
+
+// One 64 x 64 tile per block, 4 x 4 results per thread (twice as many for the gate).
+template <typename T, int EPI, bool AM, bool BM>
+__global__ void __launch_bounds__(256) product_simt_kernel(const Product P) {
+  constexpr int NB = EPI == kGate ? 2 : 1;
+  __shared__ float As[kTK][kTM + 4], Bs[NB][kTK][kTN + 4];
+  const T* const A = static_cast<const T*>(P.a);
+  const T* const B = static_cast<const T*>(P.b);
+  const long long m0 = static_cast<long long>(blockIdx.x) * kTM, n0 = static_cast<long long>(blockIdx.y) * kTN;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[NB][4][4] = {};
+  for (long long k0 = 0; k0 < P.K; k0 += kTK) {
+#pragma unroll
+    for (int i = 0; i < kTM * kTK / 256; ++i) {
+      const int e = i * 256 + threadIdx.x;
+      const int m = AM ? e % kTM : e / kTK, k = AM ? e / kTM : e % kTK;
+      const bool in = m0 + m < P.M && k0 + k < P.K;
+      As[k][m] = in ? to_f32<T>(A[AM ? (k0 + k) * P.lda + m0 + m : (m0 + m) * P.lda + k0 + k]) : 0.f;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < kTN * kTK / 256; ++i) {
+        const int e = i * 256 + threadIdx.x;
+        const int n = BM ? e % kTN : e / kTK, k = BM ? e / kTN : e % kTK;
+        const bool in = n0 + n < P.N && k0 + k < P.K;
+        const long long row = n0 + n + (b ? P.N : 0);
+        Bs[b][k][n] = in ? to_f32<T>(B[BM ? (k0 + k) * P.ldb + row : row * P.ldb + k0 + k]) : 0.f;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTK; ++k) {
+      const float4 a = *reinterpret_cast<const float4*>(&As[k][ty * 4]);
+      const float av[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const float4 v = *reinterpret_cast<const float4*>(&Bs[b][k][tx * 4]);
+        const float bv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[b][i][j] = fmaf(av[i], bv[j], acc[b][i][j]);
+      }
+    }
+    __syncthreads();
+  }
+  const T* const bias = static_cast<const T*>(P.bias);
+  T* const out = static_cast<T*>(P.out);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long m = m0 + ty * 4 + i;
+    if (m >= P.M) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long n = n0 + tx * 4 + j;
+      if (n >= P.N) continue;
+      if (EPI == kPlain) {
+        out[m * P.ldo + n] = from_f32<T>(acc[0][i][j] + (bias ? to_f32<T>(bias[n]) : 0.f));
+      } else if (EPI == kGate) {
+        const float g = acc[0][i][j] + (bias ? to_f32<T>(bias[n]) : 0.f);
+        const float u = acc[NB - 1][i][j] + (bias ? to_f32<T>(bias[P.N + n]) : 0.f);
+        out[m * P.ldo + n] = from_f32<T>(act_value<sizeof(T) == 2>(g, P.act) * u);
+        if (P.gu_out) {
+          T* const gu = static_cast<T*>(P.gu_out) + m * 2 * P.N;
+          gu[n] = from_f32<T>(g);
+          gu[P.N + n] = from_f32<T>(u);
+        }
+      } else {
+        const T* const gu = static_cast<const T*>(P.gu) + m * 2 * P.N;
+        float da;
+        const float a = act_value_grad<sizeof(T) == 2>(to_f32<T>(gu[n]), P.act, da);
+        out[m * 2 * P.N + n] = from_f32<T>(acc[0][i][j] * to_f32<T>(gu[P.N + n]) * da);
+        out[m * 2 * P.N + P.N + n] = from_f32<T>(acc[0][i][j] * a);
+      }
+    }
+  }
+}
+
+template <typename T, int EPI>
+static cudaError_t launch_simt(const Product& p, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((p.M + kTM - 1) / kTM), static_cast<unsigned>((p.N + kTN - 1) / kTN));
+  if (p.a_major && p.b_major) product_simt_kernel<T, EPI, true, true><<<grid, 256, 0, s>>>(p);
+  else if (p.a_major) return cudaErrorInvalidValue;
+  else if (p.b_major) product_simt_kernel<T, EPI, false, true><<<grid, 256, 0, s>>>(p);
+  else product_simt_kernel<T, EPI, false, false><<<grid, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_product_simt(const Product& p, cudaStream_t s) {
+  const bool bf = p.dtype == MSL_DTYPE_BF16;
+  switch (p.epilogue) {
+    case kPlain: return bf ? launch_simt<__nv_bfloat16, kPlain>(p, s) : launch_simt<float, kPlain>(p, s);
+    case kGate: return bf ? launch_simt<__nv_bfloat16, kGate>(p, s) : launch_simt<float, kGate>(p, s);
+    default: return bf ? launch_simt<__nv_bfloat16, kDgate>(p, s) : launch_simt<float, kDgate>(p, s);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ column sums
+
+// partial[slice][c] = sum of the slice's rows; 32 columns x 8 rows of threads.
+template <typename T>
+__global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x, long long ld, long long rows, int cols, long long per,
+                                                         float* __restrict__ partial) {
+  __shared__ float part[8][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+  const long long r1 = min(rows, (blockIdx.y + 1LL) * per);
+  float t = 0.f;
+  if (c < cols)
+    for (long long r = blockIdx.y * per + y; r < r1; r += 8) t += to_f32<T>(x[r * ld + c]);
+  part[y][threadIdx.x & 31] = t;
+  __syncthreads();
+  if (y == 0 && c < cols) {
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += part[i][threadIdx.x];
+    partial[static_cast<size_t>(blockIdx.y) * cols + c] = t;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) column_join_kernel(const float* __restrict__ partial, int slices, int cols, T* __restrict__ out) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float t = 0.f;
+  for (int s = 0; s < slices; ++s) t += partial[static_cast<size_t>(s) * cols + c];
+  out[c] = from_f32<T>(t);
+}
+
+constexpr int kSlices = 64;
+
+static cudaError_t column_sums(int dtype, const void* x, long long ld, long long rows, int cols, void* out, float* partial, cudaStream_t s) {
+  const long long per = (rows + kSlices - 1) / kSlices;
+  const int slices = static_cast<int>((rows + per - 1) / per);
+  const dim3 grid((cols + 31) / 32, slices);
+  if (dtype == MSL_DTYPE_BF16) {
+    column_sum_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), ld, rows, cols, per, partial);
+    column_join_kernel<<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, static_cast<__nv_bfloat16*>(out));
+  } else {
+    column_sum_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(x), ld, rows, cols, per, partial);
+    column_join_kernel<<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, static_cast<float*>(out));
+  }
+  count_launches(2);
+  return cudaGetLastError();
+}
+
+static int run(const Product& p, cudaStream_t s) {
+  const cudaError_t e = launch_product_simt(p, s);
+  if (e != cudaSuccess) return cuda_failf(e, "product_simt_kernel launch");
+  count_launches(1);
+  return MSL_OK;
+}
+
+static int check(const msl_ffn_geometry* g, const msl_ffn_io* io) {
+  if (!g) return failf(MSL_ERR_INVALID, "geometry is NULL");
+  if (g->rows < 0 || g->dim < 1 || g->hidden < 1) return failf(MSL_ERR_INVALID, "rows must be >= 0, dim and hidden >= 1");
+  if (g->dtype != MSL_DTYPE_F32 && g->dtype != MSL_DTYPE_BF16) return failf(MSL_ERR_INVALID, "unknown dtype %d", g->dtype);
+  if (g->activation != MSL_ACT_SILU && g->activation != MSL_ACT_GELU) return failf(MSL_ERR_INVALID, "unknown activation %d", g->activation);
+  if (g->dim > (1 << 21) || g->hidden > (1 << 20)) return failf(MSL_ERR_UNSUPPORTED, "dim or hidden is over 2^20");
+  if (g->rows > (1LL << 31)) return failf(MSL_ERR_UNSUPPORTED, "rows is over 2^31");
+  if (!io) return failf(MSL_ERR_INVALID, "io is NULL");
+  return MSL_OK;
+}
+
+static Product product(const msl_ffn_geometry* g, const msl_ffn_io* io) {
+  Product p{};
+  p.dtype = g->dtype;
+  p.act = g->activation;
+  p.status = io->status;
+  return p;
+}
+
+}  // namespace ffn
+}  // namespace msl
+
+using namespace msl;
+
+extern "C" {
+
+size_t msl_gated_ffn_workspace_bytes(const msl_ffn_geometry* geom, int32_t backward) {
+  msl_ffn_io none{};
+  if (ffn::check(geom, &none) || !backward) return 0;
+  return sizeof(float) * ffn::kSlices * (2 * static_cast<size_t>(geom->hidden) > static_cast<size_t>(geom->dim) ? 2 * static_cast<size_t>(geom->hidden)
+                                                                                                              : static_cast<size_t>(geom->dim));
+}
+
+int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  int rc = ffn::check(geom, io);
+  if (rc) return rc;
+  const long long M = geom->rows, C = geom->dim, F = geom->hidden;
+  if (!io->w_in || !io->w_out) return failf(MSL_ERR_INVALID, "w_in and w_out are required");
+  if (M == 0) return MSL_OK;
+  if (!io->x || !io->h || !io->y) return failf(MSL_ERR_INVALID, "x, h and y are required");
+  if (io->x_ld < C || io->y_ld < C) return failf(MSL_ERR_INVALID, "row strides must be >= dim = %lld", C);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  ffn::Product p = ffn::product(geom, io);
+  p.epilogue = ffn::kGate;
+  p.a = io->x; p.lda = io->x_ld;
+  p.b = io->w_in; p.ldb = C;
+  p.out = io->h; p.ldo = F;
+  p.bias = io->b_in;
+  p.gu_out = io->gu;
+  p.M = M; p.N = F; p.K = C;
+  rc = ffn::run(p, s);
+  if (rc) return rc;
+  p = ffn::product(geom, io);
+  p.epilogue = ffn::kPlain;
+  p.a = io->h; p.lda = F;
+  p.b = io->w_out; p.ldb = F;
+  p.out = io->y; p.ldo = io->y_ld;
+  p.bias = io->b_out;
+  p.M = M; p.N = C; p.K = F;
+  return ffn::run(p, s);
+}
+
+int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  int rc = ffn::check(geom, io);
+  if (rc) return rc;
+  const long long M = geom->rows, C = geom->dim, F = geom->hidden;
+  const size_t es = geom->dtype == MSL_DTYPE_BF16 ? 2 : 4;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    struct { void* p; size_t n; } zero[] = {{io->dw_in, 2 * F * C * es}, {io->dw_out, C * F * es}, {io->db_in, 2 * F * es}, {io->db_out, C * es}};
+    for (const auto& z : zero) {
+      const cudaError_t e = z.p ? cudaMemsetAsync(z.p, 0, z.n, s) : cudaSuccess;
+      if (e != cudaSuccess) return cuda_failf(e, "clearing the weights' gradients");
+    }
+    return MSL_OK;
+  }
+  const bool inner = io->dx || io->dw_in || io->db_in;  // wants the gradients of g and u
+  if (!io->dy || io->dy_ld < C) return failf(MSL_ERR_INVALID, "dy (row stride >= dim) is required");
+  if (inner && (!io->w_out || !io->gu || !io->dgu)) return failf(MSL_ERR_INVALID, "w_out, gu and dgu are required");
+  if (io->dx && (!io->w_in || io->dx_ld < C)) return failf(MSL_ERR_INVALID, "dx needs w_in and a row stride >= dim");
+  if (io->dw_in && (!io->x || io->x_ld < C)) return failf(MSL_ERR_INVALID, "dw_in needs x");
+  if (io->dw_out && !io->h) return failf(MSL_ERR_INVALID, "dw_out needs h");
+  if (io->db_in || io->db_out) {
+    const size_t need = msl_gated_ffn_workspace_bytes(geom, 1);
+    if (!workspace || workspace_bytes < need)
+      return failf(MSL_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
+    if (!multiple_of(workspace, 16)) return failf(MSL_ERR_INVALID, "workspace must be 16-byte aligned");
+  }
+  ffn::Product p;
+  if (inner) {
+    p = ffn::product(geom, io);
+    p.epilogue = ffn::kDgate;
+    p.a = io->dy; p.lda = io->dy_ld;
+    p.b = io->w_out; p.ldb = F; p.b_major = true;  // [K = dim, N = hidden]
+    p.out = io->dgu; p.ldo = 2 * F;
+    p.gu = io->gu;
+    p.M = M; p.N = F; p.K = C;
+    rc = ffn::run(p, s);
+    if (rc) return rc;
+  }
+  if (io->dx) {
+    p = ffn::product(geom, io);
+    p.a = io->dgu; p.lda = 2 * F;
+    p.b = io->w_in; p.ldb = C; p.b_major = true;  // [K = 2 hidden, N = dim]
+    p.out = io->dx; p.ldo = io->dx_ld;
+    p.M = M; p.N = C; p.K = 2 * F;
+    rc = ffn::run(p, s);
+    if (rc) return rc;
+  }
+  if (io->dw_in) {
+    p = ffn::product(geom, io);
+    p.a = io->dgu; p.lda = 2 * F; p.a_major = true;  // [K = rows, M = 2 hidden]
+    p.b = io->x; p.ldb = io->x_ld; p.b_major = true;  // [K = rows, N = dim]
+    p.out = io->dw_in; p.ldo = C;
+    p.M = 2 * F; p.N = C; p.K = M;
+    rc = ffn::run(p, s);
+    if (rc) return rc;
+  }
+  if (io->dw_out) {
+    p = ffn::product(geom, io);
+    p.a = io->dy; p.lda = io->dy_ld; p.a_major = true;  // [K = rows, M = dim]
+    p.b = io->h; p.ldb = F; p.b_major = true;           // [K = rows, N = hidden]
+    p.out = io->dw_out; p.ldo = F;
+    p.M = C; p.N = F; p.K = M;
+    rc = ffn::run(p, s);
+    if (rc) return rc;
+  }
+  float* const partial = static_cast<float*>(workspace);
+  if (io->db_in) {
+    const cudaError_t e = ffn::column_sums(geom->dtype, io->dgu, 2 * F, M, static_cast<int>(2 * F), io->db_in, partial, s);
+    if (e != cudaSuccess) return cuda_failf(e, "column_sum_kernel launch");
+  }
+  if (io->db_out) {
+    const cudaError_t e = ffn::column_sums(geom->dtype, io->dy, io->dy_ld, M, static_cast<int>(C), io->db_out, partial, s);
+    if (e != cudaSuccess) return cuda_failf(e, "column_sum_kernel launch");
+  }
+  return MSL_OK;
+}
+
+}  // extern "C"

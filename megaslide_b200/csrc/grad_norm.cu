@@ -1,0 +1,294 @@
+// Global gradient norm over many tensors, and clipping.
+//
+//   norm = sqrt(extra + sum over tensors of sum_i g_i^2),   out = g * min(1, max_norm / (norm + 1e-6))
+//
+// Bound by bytes: the norm reads everything once, the scaling reads it again (the factor is known only
+// when the last element has been read) and writes it.  The tensors are cut into chunks of kChunk
+// elements; a block takes an equal share of consecutive chunks, whatever the tensors' sizes, so two
+// launches serve any number of tensors up to kMaxTensors (more take further launches).  The table of
+// tensors travels in the kernel's parameters: no copy to the device, nothing to keep alive.
+// Sums: float32 in a thread's part of a chunk, double from there on, joined in a fixed order (the same result on
+// every run on the same kind of GPU).
+
+#include <math.h>
+
+#include "msl_abi.cuh"
+#include "msl_common.cuh"
+
+namespace msl {
+namespace clip {
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 8192;       // elements: 256 threads x 4 loads of 8 bf16
+constexpr int kMaxTensors = 896;   // of a launch: 30 KB of the 32 KB that parameters may take
+constexpr int kBlocksPerSm = 4;
+
+struct Table {
+  const void* src[kMaxTensors];
+  void* dst[kMaxTensors];
+  long long numel[kMaxTensors];
+  unsigned first[kMaxTensors + 1];  // chunks before the tensor; [count] = all
+  unsigned char bf16[kMaxTensors];
+  int count;
+};
+
+// last tensor whose first chunk is <= c (tensors without elements have no chunk and are never it)
+__device__ __forceinline__ int tensor_of(const Table& t, unsigned c) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void sum_span(const T* p, int n, float& acc) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
+  for (int i = threadIdx.x; i < head; i += kThreads) { const float v = to_f32<T>(p[i]); acc = fmaf(v, v, acc); }
+  const uint4* const q = reinterpret_cast<const uint4*>(p + head);
+  const int nv = (n - head) / kPer;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nv; i += kThreads) {
+    const uint4 w = __ldg(q + i);
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) { const float v = to_f32<T>(e[j]); acc = fmaf(v, v, acc); }
+  }
+  for (int i = head + nv * kPer + threadIdx.x; i < n; i += kThreads) { const float v = to_f32<T>(p[i]); acc = fmaf(v, v, acc); }
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_span(const T* p, T* o, int n, float c) {
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
+  int nv = (n - head) / kPer;
+  if ((reinterpret_cast<uintptr_t>(o + head) & 15) != 0) nv = 0;  // source and result are not aligned alike
+  for (int i = threadIdx.x; i < head; i += kThreads) o[i] = from_f32<T>(to_f32<T>(p[i]) * c);
+  const uint4* const q = reinterpret_cast<const uint4*>(p + head);
+  uint4* const r = reinterpret_cast<uint4*>(o + head);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nv; i += kThreads) {
+    uint4 w = q[i];
+    T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) e[j] = from_f32<T>(to_f32<T>(e[j]) * c);
+    r[i] = w;
+  }
+#pragma unroll 4
+  for (int i = head + nv * kPer + threadIdx.x; i < n; i += kThreads) o[i] = from_f32<T>(to_f32<T>(p[i]) * c);
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[kThreads / 32];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) v += part[i];
+  __syncthreads();
+  return v;
+}
+
+// the chunks of this block: an equal share of `total`
+__device__ __forceinline__ void share(unsigned total, unsigned& c0, unsigned& c1) {
+  c0 = static_cast<unsigned>(static_cast<unsigned long long>(total) * blockIdx.x / gridDim.x);
+  c1 = static_cast<unsigned>(static_cast<unsigned long long>(total) * (blockIdx.x + 1) / gridDim.x);
+}
+
+__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ Table t, double* __restrict__ partial) {
+  unsigned c0, c1;
+  share(t.first[t.count], c0, c1);
+  // a chunk's 32 squares of a thread add up in float32, the chunks in double: thousands of squares of bf16
+  // numbers, whose few bits leave many ties, drift by 5e-6 in one float32 sum
+  double sum = 0.0;
+  if (c0 < c1) {
+    int k = tensor_of(t, c0);
+    for (unsigned c = c0; c < c1; ++c) {
+      while (c >= t.first[k + 1]) ++k;
+      const long long at = static_cast<long long>(c - t.first[k]) * kChunk;
+      const int n = static_cast<int>(min(static_cast<long long>(kChunk), t.numel[k] - at));
+      float acc = 0.f;
+      if (t.bf16[k]) sum_span(static_cast<const __nv_bfloat16*>(t.src[k]) + at, n, acc);
+      else sum_span(static_cast<const float*>(t.src[k]) + at, n, acc);
+      sum += static_cast<double>(acc);
+    }
+  }
+  const double s = block_sum(sum);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// every block joins the same sums in the same order
+__device__ __forceinline__ float join(const double* __restrict__ partial, int n, double extra) {
+  double v = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) v += partial[i];
+  return static_cast<float>(sqrt(block_sum(v) + extra));
+}
+
+__global__ void __launch_bounds__(kThreads) norm_kernel(const double* __restrict__ partial, int n, double extra, float* norm) {
+  const float v = join(partial, n, extra);
+  if (threadIdx.x == 0) *norm = v;
+}
+
+__global__ void __launch_bounds__(kThreads)
+    scale_kernel(const __grid_constant__ Table t, const double* __restrict__ partial, int n, double extra, float max_norm, float* norm) {
+  const float v = join(partial, n, extra);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
+  float f = max_norm / (v + 1e-6f);
+  f = f > 1.f ? 1.f : f;  // a NaN stays a NaN
+  unsigned c0, c1;
+  share(t.first[t.count], c0, c1);
+  if (c0 >= c1) return;
+  int k = tensor_of(t, c0);
+  for (unsigned c = c0; c < c1; ++c) {
+    while (c >= t.first[k + 1]) ++k;
+    const long long at = static_cast<long long>(c - t.first[k]) * kChunk;
+    const int m = static_cast<int>(min(static_cast<long long>(kChunk), t.numel[k] - at));
+    if (t.bf16[k]) scale_span(static_cast<const __nv_bfloat16*>(t.src[k]) + at, static_cast<__nv_bfloat16*>(t.dst[k]) + at, m, f);
+    else scale_span(static_cast<const float*>(t.src[k]) + at, static_cast<float*>(t.dst[k]) + at, m, f);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+
+long long chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+
+int grid_of(long long chunks) {
+  const long long most = static_cast<long long>(sm_count()) * kBlocksPerSm;
+  return static_cast<int>(chunks < most ? (chunks > 0 ? chunks : 1) : most);
+}
+
+// Fills a table with up to kMaxTensors tensors from `at` on; returns the next tensor.
+int fill(Table& t, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int count, int at) {
+  long long chunks = 0;
+  int k = 0;
+  for (; at < count && k < kMaxTensors; ++at) {
+    const long long c = chunks_of(numel[at]);
+    if (c == 0) continue;
+    if (chunks + c > 0x7fffffffLL && k > 0) break;
+    t.src[k] = src[at];
+    t.dst[k] = dst ? dst[at] : nullptr;
+    t.numel[k] = numel[at];
+    t.bf16[k] = dtype[at] == MSL_DTYPE_BF16;
+    t.first[k] = static_cast<unsigned>(chunks);
+    chunks += c;
+    ++k;
+  }
+  t.count = k;
+  t.first[k] = static_cast<unsigned>(chunks);
+  return at;
+}
+
+// Blocks of every launch over these tensors together (the sums of a launch follow those before it).
+long long all_blocks(const int64_t* numel, int count) {
+  long long n = 0;
+  int at = 0;
+  do {
+    long long chunks = 0;
+    int k = 0;
+    for (; at < count && k < kMaxTensors; ++at) {
+      const long long c = chunks_of(numel[at]);
+      if (c == 0) continue;
+      if (chunks + c > 0x7fffffffLL && k > 0) break;
+      chunks += c;
+      ++k;
+    }
+    n += grid_of(chunks);
+  } while (at < count);
+  return n;
+}
+
+int check(const void* const* src, void* const* dst, bool scale, const int64_t* numel, const int32_t* dtype, int32_t count,
+          double extra, const float* norm, void* workspace, size_t bytes) {
+  if (count < 0) return failf(MSL_ERR_INVALID, "count must be >= 0");
+  if (count > 0 && (!src || !numel || !dtype || (scale && !dst))) return failf(MSL_ERR_INVALID, "src, dst, numel and dtype are required");
+  if (!norm) return failf(MSL_ERR_INVALID, "norm is required");
+  if (!(extra >= 0.0)) return failf(MSL_ERR_INVALID, "extra_sumsq must be >= 0");
+  for (int i = 0; i < count; ++i) {
+    if (numel[i] < 0) return failf(MSL_ERR_INVALID, "tensor %d: numel must be >= 0", i);
+    if (dtype[i] != MSL_DTYPE_F32 && dtype[i] != MSL_DTYPE_BF16) return failf(MSL_ERR_INVALID, "tensor %d: unknown dtype %d", i, dtype[i]);
+    if (numel[i] == 0) continue;
+    if (!src[i] || (scale && !dst[i])) return failf(MSL_ERR_INVALID, "tensor %d: NULL", i);
+    const unsigned es = dtype[i] == MSL_DTYPE_BF16 ? 2 : 4;
+    if (!multiple_of(src[i], es) || (scale && !multiple_of(dst[i], es)))
+      return failf(MSL_ERR_INVALID, "tensor %d: not aligned to its elements", i);
+    if (chunks_of(numel[i]) > 0x7fffffffLL) return failf(MSL_ERR_UNSUPPORTED, "tensor %d: too many elements", i);
+  }
+  const size_t need = sizeof(double) * static_cast<size_t>(all_blocks(numel, count));
+  if (!workspace || bytes < need) return failf(MSL_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? bytes : 0);
+  if (!multiple_of(workspace, 8)) return failf(MSL_ERR_INVALID, "workspace must be 8-byte aligned");
+  return MSL_OK;
+}
+
+}  // namespace clip
+}  // namespace msl
+
+using namespace msl;
+
+static int sum_squares(clip::Table& t, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype,
+                       int32_t count, double* partial, cudaStream_t s, int* blocks) {
+  int at = 0, n = 0;
+  do {
+    at = clip::fill(t, src, dst, numel, dtype, count, at);
+    const int g = clip::grid_of(t.first[t.count]);
+    clip::sumsq_kernel<<<g, clip::kThreads, 0, s>>>(t, partial + n);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_failf(e, "sumsq_kernel launch");
+    count_launches(1);
+    n += g;
+  } while (at < count);
+  *blocks = n;
+  return MSL_OK;
+}
+
+extern "C" {
+
+size_t msl_grad_norm_workspace_bytes(const int64_t* numel, int32_t count) {
+  if (count < 0 || (count > 0 && !numel)) return 0;
+  return sizeof(double) * static_cast<size_t>(clip::all_blocks(numel, count));
+}
+
+int msl_grad_norm(const void* const* src, const int64_t* numel, const int32_t* dtype, int32_t count,
+                  double extra_sumsq, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = clip::check(src, nullptr, false, numel, dtype, count, extra_sumsq, norm, workspace, workspace_bytes);
+  if (rc) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  double* const partial = static_cast<double*>(workspace);
+  static thread_local clip::Table t;
+  int n = 0;
+  rc = sum_squares(t, src, nullptr, numel, dtype, count, partial, s, &n);
+  if (rc) return rc;
+  clip::norm_kernel<<<1, clip::kThreads, 0, s>>>(partial, n, extra_sumsq, norm);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_failf(e, "norm_kernel launch");
+  count_launches(1);
+  return MSL_OK;
+}
+
+int msl_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int32_t count,
+                  double extra_sumsq, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  if (!(max_norm >= 0.f)) return failf(MSL_ERR_INVALID, "max_norm must be >= 0");
+  int rc = clip::check(src, dst, true, numel, dtype, count, extra_sumsq, norm, workspace, workspace_bytes);
+  if (rc) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  double* const partial = static_cast<double*>(workspace);
+  static thread_local clip::Table t;
+  int n = 0;
+  rc = sum_squares(t, src, dst, numel, dtype, count, partial, s, &n);
+  if (rc) return rc;
+  int at = 0;
+  do {
+    at = clip::fill(t, src, dst, numel, dtype, count, at);
+    clip::scale_kernel<<<clip::grid_of(t.first[t.count]), clip::kThreads, 0, s>>>(t, partial, n, extra_sumsq, max_norm, norm);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_failf(e, "scale_kernel launch");
+    count_launches(1);
+  } while (at < count);
+  return MSL_OK;
+}
+
+}  // extern "C"

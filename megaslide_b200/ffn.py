@@ -1,0 +1,87 @@
+"""Gated feed-forward block on the kernels of csrc/gated_ffn.cu.
+
+    y = (act(x Wg^T + bg) * (x Wu^T + bu)) w_out^T + b_out,   w_in = [Wg; Wu]
+
+Both projections, their biases, the activation and the product are one kernel; the second projection is another.
+The backward keeps the two projections and the gated product, and is one kernel for the gradients of the
+projections (product with w_out, the activation's derivative and the products) and one for each of dx, dw_in and
+dw_out.  float32 or bfloat16 operands, float32 sums; the intermediate results are rounded to the operands' type,
+in which the next product reads them.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch import Tensor
+
+from . import ops
+
+
+def _rows_of(x: Tensor) -> Tensor:
+    """[..., C] as a [rows, C] row view (a copy where the strides allow none)."""
+    x2 = x.reshape(-1, x.shape[-1])
+    if (x2.stride(1) != 1 and x2.shape[1] > 1) or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
+        x2 = x2.contiguous()
+    return x2
+
+
+def _status(dev: torch.device):
+    sw = ops.status_word(dev)
+    sw.poll()
+    return sw
+
+
+class GatedFFNFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_in, w_out, b_in, b_out, activation):
+        x2 = _rows_of(x)
+        y, h, gu = ops.gated_ffn_fwd(x2, w_in, w_out, b_in, b_out, activation, keep=True, status=ops.status_word(x.device).word)
+        ctx.save_for_backward(x2, w_in, w_out, b_in, b_out, h, gu)
+        ctx.activation = activation
+        ctx.x_shape = x.shape
+        return y.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, w_in, w_out, b_in, b_out, h, gu = ctx.saved_tensors
+        sw = _status(x2.device)
+        dx, dw_in, dw_out, db_in, db_out = ops.gated_ffn_bwd(x2, w_in, w_out, h, gu, _rows_of(dy), b_in, b_out, ctx.activation,
+                                                             needs=ctx.needs_input_grad[:5], status=sw.word)
+        sw.post()
+        return dx.view(ctx.x_shape) if dx is not None else None, dw_in, dw_out, db_in, db_out, None
+
+
+def gated_ffn(x: Tensor, w_in: Tensor, w_out: Tensor, b_in: Optional[Tensor] = None, b_out: Optional[Tensor] = None,
+              activation: str = "silu") -> Tensor:
+    """y [..., dim] of x [..., dim]; w_in [2 * hidden, dim] holds the gate's rows, then the other's; w_out [dim, hidden];
+    activation "silu" or "gelu" (erf form).  One dtype (float32 or bfloat16) for all.  Differentiable in everything."""
+    if not x.is_cuda:
+        raise RuntimeError("x must be a CUDA tensor (no CPU fallback)")
+    if x.dim() < 1:
+        raise ValueError("x must be [..., dim]")
+    ops.dtype_code(x.dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out)):
+        return GatedFFNFunction.apply(x, w_in, w_out, b_in, b_out, activation)
+    return ops.gated_ffn_fwd(_rows_of(x), w_in, w_out, b_in, b_out, activation, status=ops.status_word(x.device).word)[0].view(x.shape)
+
+
+class GatedMLP(nn.Module):
+    """The gated block as a module: fc1 (2 * intermediate_size rows: gate, then the other) and fc2, as nn.Linear
+    parameters.  Under CUDA autocast to bfloat16 it computes in bfloat16, like nn.Linear."""
+
+    def __init__(self, hidden_size: int, intermediate_size: int, dropout: float = 0.0, activation: str = "silu"):
+        super().__init__()
+        ops.activation_code(activation)
+        self.fc1 = nn.Linear(hidden_size, 2 * intermediate_size)
+        self.fc2 = nn.Linear(intermediate_size, hidden_size)
+        self.dropout = nn.Dropout(dropout)
+        self.activation = activation
+
+    def forward(self, x: Tensor) -> Tensor:
+        p = (x, self.fc1.weight, self.fc2.weight, self.fc1.bias, self.fc2.bias)
+        if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+            p = tuple(t.to(torch.bfloat16) for t in p)
+        return self.dropout(gated_ffn(*p, activation=self.activation))

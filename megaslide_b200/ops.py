@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from contextlib import contextmanager
+from contextlib import contextmanager, nullcontext
 from dataclasses import dataclass
 from typing import List, Optional, Tuple
 
@@ -76,11 +76,11 @@ class StatusWord:
     """The per-device status word the attention kernels OR their MSL_STATUS_* bits into (device int32),
     read back without stalling the host: after every call an asynchronous copy into pinned memory is
     enqueued with an event, and the next call (poll) reads that copy once its event has completed.  A
-    halo miss or a timed-out TMA wait (results not valid) raises MslError there, at most one call late;
+    halo miss, a timed-out TMA wait or a position outside its axis (results not valid) raises MslError there, at most one call late;
     check() reads the word synchronously.  MSL_STATUS_TC_RANGE is informational (the kernels computed
     such tiles with the CUDA-core gather)."""
 
-    BAD = _lib.MSL_STATUS_HALO_MISS | _lib.MSL_STATUS_TIMEOUT
+    BAD = _lib.MSL_STATUS_HALO_MISS | _lib.MSL_STATUS_TIMEOUT | _lib.MSL_STATUS_ROTARY_INDEX
 
     def __init__(self, device: torch.device):
         self.word = torch.zeros(1, dtype=torch.int32, device=device)
@@ -103,6 +103,11 @@ class StatusWord:
                 what.append("a sample corner fell outside the K/V frames the call was given (halo miss)")
             if v & _lib.MSL_STATUS_TIMEOUT:
                 what.append("a tensor-core CTA's TMA copies did not complete within a second")
+            if v & _lib.MSL_STATUS_ROTARY_INDEX:
+                what.append("a rotary position index was outside its axis")
+            if v & self.BAD == _lib.MSL_STATUS_ROTARY_INDEX:
+                raise _lib.MslError("msl_rope3d / msl_qk_norm_rope", _lib.MSL_ERR_CUDA,
+                                    "a previous call produced invalid results: " + "; ".join(what))
             raise _lib.MslError("msl_dsa_attn", _lib.MSL_ERR_CUDA,
                                 "a previous attention call produced invalid results: " + "; ".join(what))
 
@@ -465,3 +470,272 @@ def convert_f32(src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
                                          dtype_code(dst.dtype), src.shape[0], src.shape[1], _stream(src.device))
     _lib.check("msl_convert_f32", rc)
     return dst
+
+
+_HERE = nullcontext()
+
+
+def _on(dev: torch.device):
+    """Context that makes `dev` current; nothing to do where it is."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+@dataclass(frozen=True)
+class RotaryShape:
+    """Geometry of a rotary call (mirrors ``msl_rotary_geometry``): `tokens` of each of `batch` samples, the
+    table's extents (frames, height, width), the channels each axis turns, the heads' width."""
+
+    batch: int
+    tokens: int
+    video_shape: Tuple[int, int, int]
+    axes: Tuple[int, int, int]
+    head_dim: int
+    frame0: int = 0
+    interleaved: bool = True
+
+    def geometry(self, dtype: torch.dtype) -> "_lib.RotaryGeometry":
+        t, h, w = self.video_shape
+        at, ah, aw = self.axes
+        return _lib.RotaryGeometry(self.batch * self.tokens, max(self.tokens, 1), t, h, w, self.frame0, at, ah, aw, self.head_dim,
+                                   1 if self.interleaved else 0, dtype_code(dtype))
+
+
+def _check_positions(shape: RotaryShape, table: Optional[torch.Tensor], index: Optional[torch.Tensor], dev: torch.device) -> int:
+    """Checks a rotary call's table and index; returns the rows of the index (0 without one)."""
+    if table is None:
+        return 0
+    (t, h, w), (at, ah, aw) = shape.video_shape, shape.axes
+    want = (t * at + h * ah + w * aw) // 2
+    if table.dtype != torch.float32 or table.numel() != 2 * want or not table.is_contiguous():
+        raise ValueError(f"table must be a contiguous float32 tensor of {want} (cos, sin) pairs (rotary_table), got {tuple(table.shape)} {table.dtype}")
+    if table.device != dev:
+        raise RuntimeError("table must be on the tokens' CUDA device")
+    if index is None:
+        return 0
+    if index.dtype != torch.int32 or not index.is_contiguous() or index.shape[-1:] != (3,):
+        raise ValueError(f"index must be a contiguous int32 tensor [..., tokens, 3], got {tuple(index.shape)} {index.dtype}")
+    rows = index.numel() // 3
+    if rows not in (shape.tokens, shape.batch * shape.tokens):
+        raise ValueError(f"index names {rows} tokens, the call has {shape.tokens} in each of {shape.batch} samples")
+    if index.device != dev:
+        raise RuntimeError("index must be on the tokens' CUDA device")
+    return rows
+
+
+def rope3d(shape: RotaryShape, heads: int, x: torch.Tensor, table: torch.Tensor, index: Optional[torch.Tensor] = None,
+           inverse: bool = False, out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates the heads of x [rows, >= heads*head_dim] (row view) by their tokens' positions; ``inverse`` turns
+    back, which is the backward pass.  ``out`` may be x."""
+    _need_cuda(x, table, index)
+    index_rows = _check_positions(shape, table, index, x.device)
+    if out is None:
+        out = torch.empty(x.shape[0], heads * shape.head_dim, device=x.device, dtype=x.dtype)
+    g = shape.geometry(x.dtype)
+    with _on(x.device):
+        rc = _call("msl_rope3d", x.device, lambda: _lib.load().msl_rope3d(
+            ctypes.byref(g), heads, _ptr(x), _rows(x, "x"), _ptr(table), _ptr(index), index_rows, 1 if inverse else 0,
+            _ptr(out), _rows(out, "out"), _ptr(status), _stream(x.device)))
+    _lib.check("msl_rope3d", rc)
+    return out
+
+
+def _qk_io(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weight, k_weight, eps, table, index, status) -> "_lib.QkNormIO":
+    _need_cuda(q, k, q_weight, k_weight, table, index)
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"q and k must have the same dtype, got {q.dtype} and {k.dtype}")
+    wdt = torch.float32
+    for w, nm in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is None:
+            continue
+        if w.numel() != shape.head_dim or not w.is_contiguous():
+            raise ValueError(f"{nm} must be a contiguous tensor of head_dim = {shape.head_dim} elements, got {tuple(w.shape)}")
+        wdt = w.dtype
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise TypeError("q_weight and k_weight must have the same dtype")
+    io = _lib.QkNormIO()
+    io.index_rows = _check_positions(shape, table, index, q.device)
+    io.q, io.q_ld = _ptr(q), _rows(q, "q")
+    if kv_heads:
+        io.k, io.k_ld = _ptr(k), _rows(k, "k")
+    io.q_weight, io.k_weight = _ptr(q_weight), _ptr(k_weight)
+    io.table, io.index, io.status = _ptr(table), _ptr(index), _ptr(status)
+    io.heads, io.kv_heads, io.weight_dtype, io.eps = heads, kv_heads, dtype_code(wdt), eps
+    return io
+
+
+def qk_norm_rope_fwd(shape: RotaryShape, heads: int, kv_heads: int, q: torch.Tensor, k: Optional[torch.Tensor],
+                     q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float = 1e-6,
+                     table: Optional[torch.Tensor] = None, index: Optional[torch.Tensor] = None,
+                     q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """RMS norm of every head of q [rows, >= heads*head_dim] and k [rows, >= kv_heads*head_dim] (row views) times
+    the weights (None = ones), then the rotation (none without a table).  q_out / k_out may be q / k; kv_heads = 0
+    takes q alone."""
+    io = _qk_io(shape, heads, kv_heads, q, k, q_weight, k_weight, eps, table, index, status)
+    if q_out is None:
+        q_out = torch.empty(q.shape[0], heads * shape.head_dim, device=q.device, dtype=q.dtype)
+    io.q_out, io.q_out_ld = _ptr(q_out), _rows(q_out, "q_out")
+    if kv_heads:
+        if k_out is None:
+            k_out = torch.empty(k.shape[0], kv_heads * shape.head_dim, device=k.device, dtype=k.dtype)
+        io.k_out, io.k_out_ld = _ptr(k_out), _rows(k_out, "k_out")
+    g = shape.geometry(q.dtype)
+    with _on(q.device):
+        rc = _call("msl_qk_norm_rope_fwd", q.device, lambda: _lib.load().msl_qk_norm_rope_fwd(
+            ctypes.byref(g), ctypes.byref(io), _stream(q.device)))
+    _lib.check("msl_qk_norm_rope_fwd", rc)
+    return q_out, k_out
+
+
+def qk_norm_rope_bwd(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weight, k_weight, dq_out, dk_out, eps: float = 1e-6,
+                     table=None, index=None, dq=None, dk=None, weight_grads: bool = True, status=None):
+    """Backward of qk_norm_rope_fwd: (dq, dk, dq_weight, dk_weight); the weights' gradients are None for weights
+    that are None and where ``weight_grads`` is false.  dq / dk may be dq_out / dk_out."""
+    io = _qk_io(shape, heads, kv_heads, q, k, q_weight, k_weight, eps, table, index, status)
+    _need_cuda(dq_out, dk_out)
+    if dq is None:
+        dq = torch.empty(q.shape[0], heads * shape.head_dim, device=q.device, dtype=q.dtype)
+    io.dq_out, io.dq_out_ld, io.dq, io.dq_ld = _ptr(dq_out), _rows(dq_out, "dq_out"), _ptr(dq), _rows(dq, "dq")
+    if kv_heads:
+        if dk is None:
+            dk = torch.empty(k.shape[0], kv_heads * shape.head_dim, device=k.device, dtype=k.dtype)
+        io.dk_out, io.dk_out_ld, io.dk, io.dk_ld = _ptr(dk_out), _rows(dk_out, "dk_out"), _ptr(dk), _rows(dk, "dk")
+    dgq = torch.empty_like(q_weight) if weight_grads and q_weight is not None else None
+    dgk = torch.empty_like(k_weight) if weight_grads and k_weight is not None and kv_heads else None
+    io.dq_weight, io.dk_weight = _ptr(dgq), _ptr(dgk)
+    g = shape.geometry(q.dtype)
+    lib = _lib.load()
+    with _on(q.device):
+        need = int(lib.msl_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(g), ctypes.byref(io)))
+        ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        rc = _call("msl_qk_norm_rope_bwd", q.device, lambda: lib.msl_qk_norm_rope_bwd(
+            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _stream(q.device)))
+    _lib.check("msl_qk_norm_rope_bwd", rc)
+    return dq, dk, dgq, dgk
+
+
+_ACTIVATIONS = {"silu": _lib.MSL_ACT_SILU, "gelu": _lib.MSL_ACT_GELU}
+
+
+def activation_code(name: str) -> int:
+    try:
+        return _ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {name!r}") from None
+
+
+def _ffn_check(x, w_in, w_out, b_in, b_out) -> Tuple[int, int, int]:
+    """(rows, dim, hidden) of a gated feed-forward call, its operands checked."""
+    _need_cuda(x, w_in, w_out, b_in, b_out)
+    M, C = x.shape
+    if w_in.dim() != 2 or w_in.shape[0] % 2 or w_in.shape[1] != C:
+        raise ValueError(f"w_in must be [2 * hidden, {C}], got {tuple(w_in.shape)}")
+    F = w_in.shape[0] // 2
+    if tuple(w_out.shape) != (C, F):
+        raise ValueError(f"w_out must be {(C, F)}, got {tuple(w_out.shape)}")
+    for t, n, nm in ((b_in, 2 * F, "b_in"), (b_out, C, "b_out")):
+        if t is not None and (t.dim() != 1 or t.numel() != n):
+            raise ValueError(f"{nm} must be [{n}], got {tuple(t.shape)}")
+    for t, nm in ((w_in, "w_in"), (w_out, "w_out"), (b_in, "b_in"), (b_out, "b_out")):
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise TypeError(f"{nm} must have x's dtype {x.dtype}, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{nm} must be contiguous")
+        if t.device != x.device:
+            raise RuntimeError(f"{nm} must be on x's CUDA device")
+    return M, C, F
+
+
+def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
+                  b_out: Optional[torch.Tensor] = None, activation: str = "silu", keep: bool = False,
+                  status: Optional[torch.Tensor] = None):
+    """Gated feed-forward block on x [rows, >= dim] (row view).  Returns (y, h, gu): h [rows, hidden] the gated
+    product, gu [rows, 2 * hidden] the two projections where ``keep`` (for the backward), else None."""
+    M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
+    h = torch.empty(M, F, device=x.device, dtype=x.dtype)
+    gu = torch.empty(M, 2 * F, device=x.device, dtype=x.dtype) if keep else None
+    y = torch.empty(M, C, device=x.device, dtype=x.dtype)
+    g = _lib.FfnGeometry(M, C, F, dtype_code(x.dtype), activation_code(activation))
+    io = _lib.FfnIO()
+    io.x, io.x_ld, io.w_in, io.b_in, io.w_out, io.b_out = _ptr(x), _rows(x, "x"), _ptr(w_in), _ptr(b_in), _ptr(w_out), _ptr(b_out)
+    io.h, io.gu, io.y, io.y_ld, io.status = _ptr(h), _ptr(gu), _ptr(y), C, _ptr(status)
+    lib = _lib.load()
+    with _on(x.device):
+        need = int(lib.msl_gated_ffn_workspace_bytes(ctypes.byref(g), 0))
+        ws = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
+        rc = _call("msl_gated_ffn_fwd", x.device, lambda: lib.msl_gated_ffn_fwd(
+            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _stream(x.device)))
+    _lib.check("msl_gated_ffn_fwd", rc)
+    return y, h, gu
+
+
+def gated_ffn_bwd(x, w_in, w_out, h, gu, dy, b_in=None, b_out=None, activation: str = "silu",
+                  needs=(True, True, True, True, True), status: Optional[torch.Tensor] = None):
+    """Backward of gated_ffn_fwd(keep=True): (dx, dw_in, dw_out, db_in, db_out); ``needs`` says which are computed
+    (the others, and those of biases that are None, are None)."""
+    M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
+    _need_cuda(h, gu, dy)
+    dev, dt = x.device, x.dtype
+    needs = (needs[0], needs[1], needs[2], needs[3] and b_in is not None, needs[4] and b_out is not None)
+    dx = torch.empty(M, C, device=dev, dtype=dt) if needs[0] else None
+    dw_in = torch.empty_like(w_in) if needs[1] else None
+    dw_out = torch.empty_like(w_out) if needs[2] else None
+    db_in = torch.empty_like(b_in) if needs[3] else None
+    db_out = torch.empty_like(b_out) if needs[4] else None
+    dgu = torch.empty(M, 2 * F, device=dev, dtype=dt) if needs[0] or needs[1] or needs[3] else None
+    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation))
+    io = _lib.FfnIO()
+    io.x, io.x_ld, io.w_in, io.w_out = _ptr(x), _rows(x, "x"), _ptr(w_in), _ptr(w_out)
+    io.h, io.gu, io.dy, io.dy_ld, io.dgu = _ptr(h), _ptr(gu), _ptr(dy), _rows(dy, "dy"), _ptr(dgu)
+    io.dx, io.dx_ld, io.dw_in, io.dw_out, io.db_in, io.db_out = _ptr(dx), C, _ptr(dw_in), _ptr(dw_out), _ptr(db_in), _ptr(db_out)
+    io.status = _ptr(status)
+    lib = _lib.load()
+    with _on(dev):
+        need = int(lib.msl_gated_ffn_workspace_bytes(ctypes.byref(g), 1))
+        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+        rc = _call("msl_gated_ffn_bwd", dev, lambda: lib.msl_gated_ffn_bwd(
+            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _stream(dev)))
+    _lib.check("msl_gated_ffn_bwd", rc)
+    return dx, dw_in, dw_out, db_in, db_out
+
+
+def grad_norm(src: List[torch.Tensor], dst: Optional[List[torch.Tensor]] = None, max_norm: float = 0.0,
+              extra_sumsq: float = 0.0) -> torch.Tensor:
+    """sqrt(extra_sumsq + the sum of squares of every element of the contiguous CUDA tensors `src`), a 0-dim
+    float32 tensor; with ``dst`` also dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)) (dst[i] may be src[i])."""
+    if not src:
+        raise ValueError("no tensors")
+    dev = src[0].device
+    n = len(src)
+    if dst is not None and len(dst) != n:
+        raise ValueError(f"{n} tensors, but {len(dst)} to write")
+    for ts, nm in ((src, "tensor"), (dst or (), "out")):
+        for i, t in enumerate(ts):
+            if not t.is_cuda or t.device != dev:
+                raise RuntimeError(f"{nm} {i} must be on the same CUDA device as the first tensor (no CPU fallback)")
+            if not t.is_contiguous():
+                raise ValueError(f"{nm} {i} must be contiguous")
+    if dst is not None:
+        for i, (a, b) in enumerate(zip(src, dst)):
+            if a.dtype != b.dtype or a.numel() != b.numel():
+                raise ValueError(f"out {i} must have the tensor's dtype and size, got {b.numel()} {b.dtype} for {a.numel()} {a.dtype}")
+    numel = (ctypes.c_int64 * n)(*[t.numel() for t in src])
+    dtypes = (ctypes.c_int32 * n)(*[dtype_code(t.dtype) for t in src])
+    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in src])
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    lib = _lib.load()
+    with _on(dev):
+        need = int(lib.msl_grad_norm_workspace_bytes(numel, n))
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        if dst is None:
+            name = "msl_grad_norm"
+            rc = _call(name, dev, lambda: lib.msl_grad_norm(ptrs, numel, dtypes, n, extra_sumsq, _ptr(norm), _ptr(ws), need, _stream(dev)))
+        else:
+            name = "msl_grad_clip"
+            outs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst])
+            rc = _call(name, dev, lambda: lib.msl_grad_clip(ptrs, outs, numel, dtypes, n, extra_sumsq, max_norm, _ptr(norm),
+                                                            _ptr(ws), need, _stream(dev)))
+    _lib.check(name, rc)
+    return norm
