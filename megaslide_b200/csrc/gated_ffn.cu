@@ -157,8 +157,9 @@ static cudaError_t column_sums(int dtype, const void* x, long long ld, long long
 }
 
 static int run(const Product& p, cudaStream_t s) {
-  const cudaError_t e = launch_product_simt(p, s);
-  if (e != cudaSuccess) return cuda_failf(e, "product_simt_kernel launch");
+  const bool tc = tc_applies(p);
+  const cudaError_t e = tc ? launch_product_tc(p, s) : launch_product_simt(p, s);
+  if (e != cudaSuccess) return cuda_failf(e, tc ? "product_kernel launch" : "product_simt_kernel launch");
   count_launches(1);
   return MSL_OK;
 }

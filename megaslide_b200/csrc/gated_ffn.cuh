@@ -55,6 +55,9 @@ __device__ __forceinline__ float act_value_grad(float g, int act, float& da) {
 }
 
 cudaError_t launch_product_simt(const Product& p, cudaStream_t s);
+// Tensor-core form (gated_ffn_tc.cu), and whether the operands allow it.
+bool tc_applies(const Product& p);
+cudaError_t launch_product_tc(const Product& p, cudaStream_t s);
 
 }  // namespace ffn
 }  // namespace msl
