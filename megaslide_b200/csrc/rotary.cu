@@ -8,11 +8,14 @@
 // Bound by bytes: every element is read once and written once (the backward reads x again instead of
 // keeping r, which costs nothing, as the norm's gradient needs x anyway).
 //
-// Layout: a warp takes one token and goes through its heads, first the queries', then the keys'.  A head
-// is cut into slots of 2V channels, V pairs; a lane keeps one slot (SL of them where V is small) for the
-// whole call, so the cosines and sines of a token are loaded once and serve all its heads, and the
-// gradients of the weights add up in registers.  32 / (lanes of a head) heads go through together, whole
-// rows of adjacent 16-byte loads; the sums of a head are shuffles among its lanes.
+// Layout: a block works on the queries or on the keys; a warp takes a few consecutive tokens, one after the
+// other, and goes through a token's heads.  A head is cut into slots of 2V channels, V pairs; a lane keeps one
+// slot (SL of them where V is small) for the whole call, so the cosines and sines of a token are loaded once and
+// serve all its heads, and the gradients of the weights add up in registers.  32 / (lanes of a head) heads go
+// through together, whole rows of adjacent loads; the sums of a head are shuffles among its lanes.
+// With that the limit is the instructions of an element, not the bytes, so the arithmetic goes two pairs at
+// a time (fma.rn.f32x2), the weights are multiplied into the cosines and sines once per token, and lanes
+// without a head load a neighbour's instead of branching (they only never store).
 
 #include "msl_abi.cuh"
 #include "msl_common.cuh"
@@ -26,7 +29,8 @@ struct Params {
   void* y[2];
   long long x_ld[2], dy_ld[2], y_ld[2];
   const void* weight[2];
-  float* partial;  // [blocks][2][d] sums of the weights' gradients
+  float* partial;  // [blocks][d] sums of the weights' gradients
+  int blocks0;     // blocks of the queries; the others are the keys'
   int heads[2];
   int w_bf16;
   const float2* table;
@@ -34,13 +38,32 @@ struct Params {
   long long index_rows;
   uint32_t* status;
   long long rows, tokens;
-  int splits;  // warps that share a token's heads
+  int splits;     // warps that share a token's heads
+  int group;      // consecutive tokens of a warp
+  int table_vec;  // the table's entries of a slot are one axis' and 16-byte aligned
   int size[3], npair[3];
   int frame0, HW, W;
   int d, R;
   int lanes;  // of a head
   float eps, inv_d, sign;
 };
+
+// ------------------------------------------------------------------------------------------ two at a time
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
 
 template <int BYTES>
 struct Word;
@@ -49,245 +72,322 @@ template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<8> { using type = uint2; };
 template <> struct Word<16> { using type = uint4; };
 
-// N elements at p, aligned to their size or 16 bytes, whichever is less
+// N elements between p and registers, in words of their size or 16 bytes, whichever is less
 template <typename T, int N>
-__device__ __forceinline__ void load(const T* p, float* o) {
+__device__ __forceinline__ void load(const T* p, T* o) {
   constexpr int kBytes = N * static_cast<int>(sizeof(T)), kWord = kBytes < 16 ? kBytes : 16;
-  constexpr int kPer = kWord / static_cast<int>(sizeof(T));
   using W = typename Word<kWord>::type;
 #pragma unroll
-  for (int i = 0; i < N / kPer; ++i) {
-    const W w = reinterpret_cast<const W*>(p)[i];
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) o[i * kPer + j] = to_f32<T>(e[j]);
-  }
+  for (int i = 0; i < kBytes / kWord; ++i) reinterpret_cast<W*>(o)[i] = reinterpret_cast<const W*>(p)[i];
 }
-
 template <typename T, int N>
-__device__ __forceinline__ void store(T* p, const float* o) {
+__device__ __forceinline__ void store(T* p, const T* o) {
   constexpr int kBytes = N * static_cast<int>(sizeof(T)), kWord = kBytes < 16 ? kBytes : 16;
-  constexpr int kPer = kWord / static_cast<int>(sizeof(T));
   using W = typename Word<kWord>::type;
 #pragma unroll
-  for (int i = 0; i < N / kPer; ++i) {
-    W w;
-    T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) e[j] = from_f32<T>(o[i * kPer + j]);
-    reinterpret_cast<W*>(p)[i] = w;
-  }
+  for (int i = 0; i < kBytes / kWord; ++i) reinterpret_cast<W*>(p)[i] = reinterpret_cast<const W*>(o)[i];
 }
 
-// Sum over the `lanes` adjacent lanes of a head, on each of them, always in the same order.
+// A lane's V * SL pairs of one head, as they lie in memory.
+template <typename T, int V, int SL, bool INTER>
+struct alignas(16) Raw {
+  T e[SL][2 * V];
+
+  // `hi` elements after the slot's first half lies its second
+  __device__ __forceinline__ void get(const T* const (&slot)[SL], const int (&hi)[SL]) {
+#pragma unroll
+    for (int s = 0; s < SL; ++s) {
+      if constexpr (INTER && V > 1) {
+        load<T, 2 * V>(slot[s], e[s]);
+      } else {
+        load<T, V>(slot[s], e[s]);
+        load<T, V>(slot[s] + hi[s], e[s] + V);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(T* const (&slot)[SL], const int (&hi)[SL], const bool (&valid)[SL]) const {
+#pragma unroll
+    for (int s = 0; s < SL; ++s) {
+      if (!valid[s]) continue;
+      if constexpr (INTER && V > 1) {
+        store<T, 2 * V>(slot[s], e[s]);
+      } else {
+        store<T, V>(slot[s], e[s]);
+        store<T, V>(slot[s] + hi[s], e[s] + V);
+      }
+    }
+  }
+  // pair j = (first, second); two pairs a float2
+  __device__ __forceinline__ void split(float2 (&a)[V * SL / 2], float2 (&b)[V * SL / 2]) const {
+#pragma unroll
+    for (int j = 0; j < V * SL; ++j) {
+      const int s = j / V, i = j % V;
+      const float x = to_f32<T>(e[s][INTER ? 2 * i : i]), y = to_f32<T>(e[s][INTER ? 2 * i + 1 : V + i]);
+      (j & 1 ? a[j / 2].y : a[j / 2].x) = x;
+      (j & 1 ? b[j / 2].y : b[j / 2].x) = y;
+    }
+  }
+  __device__ __forceinline__ void join(const float2 (&a)[V * SL / 2], const float2 (&b)[V * SL / 2]) {
+#pragma unroll
+    for (int j = 0; j < V * SL; ++j) {
+      const int s = j / V, i = j % V;
+      e[s][INTER ? 2 * i : i] = from_f32<T>(j & 1 ? a[j / 2].y : a[j / 2].x);
+      e[s][INTER ? 2 * i + 1 : V + i] = from_f32<T>(j & 1 ? b[j / 2].y : b[j / 2].x);
+    }
+  }
+};
+
+// Sum over the adjacent lanes of a head, on each of them, always in the same order.  LC: their number where
+// it is a power of two known to the compiler, else 0.
+template <int LC>
 __device__ __forceinline__ float head_sum(float v, int lanes, int in_head, int first) {
-  if ((lanes & (lanes - 1)) == 0) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  if constexpr (LC > 0) {
+#pragma unroll
+    for (int o = LC >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
   }
-  for (int o = 1; o < lanes; o <<= 1) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    if (o >= lanes) break;
     const float t = __shfl_down_sync(kFull, v, o);
     if (in_head + o < lanes) v += t;
   }
   return __shfl_sync(kFull, v, first);
 }
 
-template <typename T, int V, int SL, bool INTER, bool NORM, bool BWD>
-__global__ void __launch_bounds__(256) rotary_kernel(const Params P) {
-  constexpr int U = BWD ? (SL == 1 && V <= 4 ? 2 : 1) : (SL == 1 ? (V <= 4 ? 4 : 2) : 1);  // heads in flight
+enum Mode : int { kRotate = 0, kForward = 1, kBackward = 2 };
+
+template <typename T, int V, int SL, bool INTER, int MODE, int LC>
+__global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1) rotary_kernel(const __grid_constant__ Params P) {
+  constexpr int NP = V * SL, N2 = NP / 2;         // pairs of a lane
+  // heads in flight, and blocks a SM (the launch bounds): measured together on 262144 x 24 x 64 and 131072 x 16 x 72 in
+  // bf16; forward 3 and 3 blocks 850 us, 2 and 3 740, 1 and 4 830; backward 2 and 2 1035, 1 and 3 1700, 1 and 4 1270;
+  // rotation alone 3 and 3 145 us, 2 and 3 211, 1 and 4 174
+  constexpr int U = MODE == kRotate ? 3 : 2;
+  constexpr bool NORM = MODE != kRotate, BWD = MODE == kBackward;
+  using R = Raw<T, V, SL, INTER>;
   const int lane = threadIdx.x & 31;
-  const int L = P.lanes;
+  const int L = LC > 0 ? LC : P.lanes;
   const int seg = lane / L, in_head = lane - seg * L;
   const int per_warp = 32 / L;  // heads of one step
   const int nslots = P.d / (2 * V), turning = P.R / (2 * V);
   const bool mine = seg < per_warp;
   const int first = min(seg, per_warp - 1) * L;
+  // queries or keys
+  const int o = static_cast<int>(blockIdx.x) >= P.blocks0 ? 1 : 0;
+  const unsigned block = blockIdx.x - (o ? P.blocks0 : 0), nblocks = o ? gridDim.x - P.blocks0 : P.blocks0;
+  const int nh = P.heads[o];
+  const int units = (nh + per_warp - 1) / per_warp;
 
-  int lo[SL], hi[SL];
+  int lo[SL], hi[SL];  // the slot's first channel, and from there to its second half
   bool valid[SL];
-  float w[2][SL][2 * V];
-  float acc[2][SL][2 * V];
 #pragma unroll
   for (int s = 0; s < SL; ++s) {
     const int slot = in_head + s * L;
     valid[s] = mine && slot < nslots;
-    const bool turns = slot < turning;
-    lo[s] = !INTER && turns ? slot * V : slot * 2 * V;
-    hi[s] = !INTER && turns ? P.R / 2 + slot * V : slot * 2 * V + V;
-    if (NORM) {
+    const bool turns = valid[s] && slot < turning;
+    lo[s] = !valid[s] ? 0 : !INTER && turns ? slot * V : slot * 2 * V;
+    hi[s] = !INTER && turns ? P.R / 2 : V;
+  }
+  // channel of a pair's first (k = 0) or second (k = 1) element
+  auto channel = [&](int j, int k) {
+    const int s = j / V, i = j % V;
+    return INTER ? lo[s] + 2 * i + k : lo[s] + (k ? hi[s] : 0) + i;
+  };
+  float2 wa[NORM ? N2 : 1], wb[NORM ? N2 : 1];  // weights of the pairs' first and second channels
+  float2 ga[BWD ? N2 : 1], gb[BWD ? N2 : 1];    // sums of their gradients
+  if (NORM) {
+    const void* const weight = P.weight[o];
 #pragma unroll
-      for (int o = 0; o < 2; ++o) {
+    for (int j = 0; j < NP; ++j) {
+      float w[2] = {1.f, 1.f};
+      if (weight) {
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) {
-          const int ch = (i < V ? lo[s] : hi[s] - V) + i;
-          w[o][s][i] = 1.f;
-          if (P.weight[o] && valid[s])
-            w[o][s][i] = P.w_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(P.weight[o])[ch])
-                                  : static_cast<const float*>(P.weight[o])[ch];
-          acc[o][s][i] = 0.f;
-        }
+        for (int k = 0; k < 2; ++k)
+          w[k] = P.w_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(weight)[channel(j, k)]) : static_cast<const float*>(weight)[channel(j, k)];
       }
+      (j & 1 ? wa[j / 2].y : wa[j / 2].x) = w[0];
+      (j & 1 ? wb[j / 2].y : wb[j / 2].x) = w[1];
+    }
+    if (BWD) {
+#pragma unroll
+      for (int j = 0; j < N2; ++j) ga[j] = gb[j] = both(0.f);
     }
   }
+  // where the lane's pairs lie in the table: axis and entry of position 0
   const int start1 = P.npair[0], start2 = P.npair[0] + P.npair[1];
-  const long long off1 = static_cast<long long>(P.size[0]) * P.npair[0];
-  const long long off2 = off1 + static_cast<long long>(P.size[1]) * P.npair[1];
-  const int units0 = (P.heads[0] + per_warp - 1) / per_warp, units1 = (P.heads[1] + per_warp - 1) / per_warp;
-  const int units = units0 + units1;
+  const int off1 = P.size[0] * P.npair[0], off2 = off1 + P.size[1] * P.npair[1];
+  int entry[NP];
+  unsigned axes = 0;  // 2 bits a pair: the axis, 3 where the pair does not turn
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int slot = in_head + j / V * L, p = slot * V + j % V;
+    const bool turns = valid[j / V] && slot < turning;
+    const int a = p < start1 ? 0 : p < start2 ? 1 : 2;
+    entry[j] = a == 0 ? p : a == 1 ? off1 + p - start1 : off2 + p - start2;
+    axes |= (turns ? a : 3u) << (2 * j);
+  }
   const int chunk = (units + P.splits - 1) / P.splits;
-
-  const long long nitems = P.rows * P.splits;
-  const long long step = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-  for (long long item = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); item < nitems;
-       item += step) {
-    const long long row = P.splits == 1 ? item : item / P.splits;
-    const int u0 = P.splits == 1 ? 0 : static_cast<int>(item - row * P.splits) * chunk;
-    const int u1 = min(units, u0 + chunk);
-    float cs[SL][V], sn[SL][V];
-#pragma unroll
-    for (int s = 0; s < SL; ++s)
-#pragma unroll
-      for (int i = 0; i < V; ++i) { cs[s][i] = 1.f; sn[s][i] = 0.f; }
-    if (turning > 0) {
-      int pos[3];
-      bool out = false;
-      if (P.index) {
-        const int* ix = P.index + (row % P.index_rows) * 3;
-#pragma unroll
-        for (int a = 0; a < 3; ++a) {
-          pos[a] = ix[a];
-          if (P.npair[a] > 0 && static_cast<unsigned>(pos[a]) >= static_cast<unsigned>(P.size[a])) { pos[a] = -1; out = true; }
-        }
-        if (out && lane == 0 && P.status) atomicOr(P.status, MSL_STATUS_ROTARY_INDEX);
+  const long long nitems = (P.rows + P.group - 1) / P.group * P.splits;
+  const long long step = static_cast<long long>(nblocks) * (blockDim.x >> 5);
+  for (long long item = static_cast<long long>(block) * (blockDim.x >> 5) + (threadIdx.x >> 5); item < nitems; item += step) {
+    const long long grp = P.splits == 1 ? item : item / P.splits;
+    const int b0 = P.splits == 1 ? 0 : static_cast<int>(item - grp * P.splits) * chunk;
+    const int b1 = min(units, b0 + chunk);
+    if (b0 >= b1) continue;
+    const long long row0 = grp * P.group;
+    const long long row1 = min(P.rows, row0 + P.group);
+    long long n = 0;  // token of its sample
+    int pos[3] = {0, 0, 0};
+    if (turning > 0 && !P.index) {
+      int f, rest;
+      if (P.tokens <= 0x7fffffffLL && P.rows <= 0x7fffffffLL) {
+        const unsigned t = static_cast<unsigned>(row0) % static_cast<unsigned>(P.tokens);
+        n = t;
+        f = t / static_cast<unsigned>(P.HW);
+        rest = t - f * P.HW;
       } else {
-        const long long n = row % P.tokens;
-        const int f = static_cast<int>(n / P.HW), rest = static_cast<int>(n - static_cast<long long>(f) * P.HW);
-        pos[0] = P.frame0 + f;
-        pos[1] = rest / P.W;
-        pos[2] = rest - pos[1] * P.W;
+        n = row0 % P.tokens;
+        f = static_cast<int>(n / P.HW);
+        rest = static_cast<int>(n - static_cast<long long>(f) * P.HW);
       }
+      pos[0] = P.frame0 + f;
+      pos[1] = rest / P.W;
+      pos[2] = rest - pos[1] * P.W;
+    }
+    for (long long row = row0; row < row1; ++row) {
+      float2 cs[N2], sn[N2];
 #pragma unroll
-      for (int s = 0; s < SL; ++s) {
-        const int slot = in_head + s * L;
-        if (valid[s] && slot < turning) {
+      for (int j = 0; j < N2; ++j) { cs[j] = both(1.f); sn[j] = both(0.f); }
+      if (turning > 0) {
+        if (P.index) {
+          const int* ix = P.index + (row % P.index_rows) * 3;
+          bool out = false;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int p = slot * V + i;
-            const int a = p < start1 ? 0 : p < start2 ? 1 : 2;
+          for (int a = 0; a < 3; ++a) {
+            pos[a] = ix[a];
+            if (P.npair[a] > 0 && static_cast<unsigned>(pos[a]) >= static_cast<unsigned>(P.size[a])) { pos[a] = -1; out = true; }
+          }
+          if (out && lane == 0 && P.status) atomicOr(P.status, MSL_STATUS_ROTARY_INDEX);
+        }
+        if (P.table_vec) {  // every axis has whole slots, on 16-byte boundaries
+          const int a = axes & 3u;
+          const int at = a == 0 ? pos[0] : a == 1 ? pos[1] : pos[2];
+          if (a < 3 && at >= 0) {
+            const float4* const c = reinterpret_cast<const float4*>(P.table + entry[0] + at * (a == 0 ? P.npair[0] : a == 1 ? P.npair[1] : P.npair[2]));
+#pragma unroll
+            for (int j = 0; j < N2; ++j) {
+              const float4 v = __ldg(c + j);
+              cs[j] = make_float2(v.x, v.z);
+              sn[j] = make_float2(v.y, v.w);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            const int a = (axes >> (2 * j)) & 3u;
             const int at = a == 0 ? pos[0] : a == 1 ? pos[1] : pos[2];
-            const long long base = a == 0 ? p : a == 1 ? off1 + p - start1 : off2 + p - start2;
-            if (at >= 0) {
-              const float2 c = __ldg(P.table + base + static_cast<long long>(at) * P.npair[a]);
-              cs[s][i] = c.x;
-              sn[s][i] = c.y * P.sign;
+            if (a < 3 && at >= 0) {
+              const float2 c = __ldg(P.table + entry[j] + at * (a == 0 ? P.npair[0] : a == 1 ? P.npair[1] : P.npair[2]));
+              (j & 1 ? cs[j / 2].y : cs[j / 2].x) = c.x;
+              (j & 1 ? sn[j / 2].y : sn[j / 2].x) = c.y;
             }
           }
         }
+        if (!P.index) {  // the next token's place
+          if (++pos[2] == P.W) {
+            pos[2] = 0;
+            if (++pos[1] == P.size[1]) { pos[1] = 0; ++pos[0]; }
+          }
+          if (++n == P.tokens) { n = 0; pos[0] = P.frame0; pos[1] = pos[2] = 0; }
+        }
       }
-    }
+      // forward: y_a = r (x_a A + x_b B), y_b = r (x_b C + x_a D), the weights inside; a rotation alone: r = 1.
+      // backward: n_a = dy_a A + dy_b B, n_b = dy_b A + dy_a D, the inverse rotation
+      float2 A[N2], B[N2], C[N2], D[N2];
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int nh = P.heads[o];
-      const int b0 = o == 0 ? u0 : max(u0 - units0, 0), b1 = o == 0 ? min(u1, units0) : u1 - units0;
+      for (int j = 0; j < N2; ++j) {
+        const float2 s = P.sign < 0.f ? neg(sn[j]) : sn[j];
+        A[j] = MODE == kForward ? mul2(cs[j], wa[j]) : cs[j];
+        B[j] = neg(MODE == kForward ? mul2(s, wb[j]) : s);
+        C[j] = MODE == kForward ? mul2(cs[j], wb[j]) : cs[j];
+        D[j] = MODE == kForward ? mul2(s, wa[j]) : s;
+      }
       const T* const xr = static_cast<const T*>(P.x[o]) + row * P.x_ld[o];
       const T* const gr = BWD ? static_cast<const T*>(P.dy[o]) + row * P.dy_ld[o] : nullptr;
       T* const yr = static_cast<T*>(P.y[o]) + row * P.y_ld[o];
       for (int b = b0; b < b1; b += U) {
-        float e[U][SL][2 * V], g[BWD ? U : 1][SL][2 * V];
-        bool on[U][SL];
+        R raw[U], rdy[BWD ? U : 1];
+        int at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int h = (b + u) * per_warp + seg;
+          if (u > 0 && b + u >= b1) break;
+          at[u] = min((b + u) * per_warp + seg, nh - 1) * P.d;
+          const T* from[SL];
 #pragma unroll
-          for (int s = 0; s < SL; ++s) {
-            on[u][s] = valid[s] && b + u < b1 && h < nh;
-            const T* const p = xr + static_cast<long long>(h) * P.d;
-            const T* const q = BWD ? gr + static_cast<long long>(h) * P.d : nullptr;
-            if (on[u][s]) {
-              if (INTER && V > 1) {
-                load<T, 2 * V>(p + lo[s], e[u][s]);
-                if (BWD) load<T, 2 * V>(q + lo[s], g[u][s]);
-              } else {
-                load<T, V>(p + lo[s], e[u][s]);
-                load<T, V>(p + hi[s], e[u][s] + V);
-                if (BWD) {
-                  load<T, V>(q + lo[s], g[u][s]);
-                  load<T, V>(q + hi[s], g[u][s] + V);
-                }
-              }
-            } else {
+          for (int s = 0; s < SL; ++s) from[s] = xr + at[u] + lo[s];
+          raw[u].get(from, hi);
+          if (BWD) {
 #pragma unroll
-              for (int i = 0; i < 2 * V; ++i) {
-                e[u][s][i] = 0.f;
-                if (BWD) g[u][s][i] = 0.f;
-              }
-            }
+            for (int s = 0; s < SL; ++s) from[s] = gr + at[u] + lo[s];
+            rdy[u].get(from, hi);
           }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          if (u > 0 && b + u >= b1) break;
+          const bool on = (b + u) * per_warp + seg < nh;
+          float2 xa[N2], xb[N2];
+          raw[u].split(xa, xb);
           float r = 1.f;
           if (NORM) {
-            float ss = 0.f;
+            float2 ss = both(0.f);
+            if (SL > 1) {  // slots beyond the head were loaded from its first
 #pragma unroll
-            for (int s = 0; s < SL; ++s)
+              for (int j = 0; j < NP; ++j)
+                if (!valid[j / V]) {
+                  (j & 1 ? xa[j / 2].y : xa[j / 2].x) = 0.f;
+                  (j & 1 ? xb[j / 2].y : xb[j / 2].x) = 0.f;
+                }
+            }
 #pragma unroll
-              for (int i = 0; i < 2 * V; ++i) ss = fmaf(e[u][s][i], e[u][s][i], ss);
-            r = rsqrtf(fmaf(head_sum(ss, L, in_head, first), P.inv_d, P.eps));
+            for (int j = 0; j < N2; ++j) ss = fma2(xb[j], xb[j], fma2(xa[j], xa[j], ss));
+            r = rsqrtf(fmaf(head_sum<LC>(ss.x + ss.y, L, in_head, first), P.inv_d, P.eps));
           }
           if (!BWD) {
 #pragma unroll
-            for (int s = 0; s < SL; ++s) {
-              float* const v = e[u][s];
-              if (NORM)
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) v[i] = v[i] * r * w[o][s][i];
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                float& a = v[INTER ? 2 * i : i];
-                float& c = v[INTER ? 2 * i + 1 : V + i];
-                const float ya = a * cs[s][i] - c * sn[s][i], yc = c * cs[s][i] + a * sn[s][i];
-                a = ya;
-                c = yc;
-              }
+            for (int j = 0; j < N2; ++j) {
+              float2 ya = fma2(xb[j], B[j], mul2(xa[j], A[j])), yb = fma2(xa[j], D[j], mul2(xb[j], C[j]));
+              if (NORM) { ya = mul2(ya, both(r)); yb = mul2(yb, both(r)); }
+              xa[j] = ya;
+              xb[j] = yb;
             }
           } else {
-            float dot = 0.f;
+            float2 da[N2], db[N2], dot = both(0.f);
+            const float2 rr = both(on ? r : 0.f);  // a head loaded twice counts once
+            rdy[u].split(da, db);
 #pragma unroll
-            for (int s = 0; s < SL; ++s) {
-              float* const v = g[u][s];
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                float& a = v[INTER ? 2 * i : i];
-                float& c = v[INTER ? 2 * i + 1 : V + i];
-                const float ya = a * cs[s][i] - c * sn[s][i], yc = c * cs[s][i] + a * sn[s][i];
-                a = ya;
-                c = yc;
-              }
-#pragma unroll
-              for (int i = 0; i < 2 * V; ++i) {
-                acc[o][s][i] = fmaf(v[i], e[u][s][i] * r, acc[o][s][i]);
-                v[i] *= w[o][s][i];
-                dot = fmaf(v[i], e[u][s][i], dot);
-              }
+            for (int j = 0; j < N2; ++j) {
+              const float2 na = fma2(db[j], B[j], mul2(da[j], A[j])), nb = fma2(da[j], D[j], mul2(db[j], A[j]));
+              ga[j] = fma2(na, mul2(xa[j], rr), ga[j]);
+              gb[j] = fma2(nb, mul2(xb[j], rr), gb[j]);
+              da[j] = mul2(na, wa[j]);
+              db[j] = mul2(nb, wb[j]);
+              dot = fma2(db[j], xb[j], fma2(da[j], xa[j], dot));
             }
-            const float m = head_sum(dot, L, in_head, first) * P.inv_d * r * r;
+            const float m = -head_sum<LC>(dot.x + dot.y, L, in_head, first) * P.inv_d * r * r;
 #pragma unroll
-            for (int s = 0; s < SL; ++s)
-#pragma unroll
-              for (int i = 0; i < 2 * V; ++i) e[u][s][i] = r * (g[u][s][i] - e[u][s][i] * m);
+            for (int j = 0; j < N2; ++j) {
+              xa[j] = mul2(fma2(xa[j], both(m), da[j]), both(r));
+              xb[j] = mul2(fma2(xb[j], both(m), db[j]), both(r));
+            }
           }
-          const int h = (b + u) * per_warp + seg;
-          T* const q = yr + static_cast<long long>(h) * P.d;
+          raw[u].join(xa, xb);
+          if (on) {
+            T* to[SL];
 #pragma unroll
-          for (int s = 0; s < SL; ++s) {
-            if (!on[u][s]) continue;
-            if (INTER && V > 1) {
-              store<T, 2 * V>(q + lo[s], e[u][s]);
-            } else {
-              store<T, V>(q + lo[s], e[u][s]);
-              store<T, V>(q + hi[s], e[u][s] + V);
-            }
+            for (int s = 0; s < SL; ++s) to[s] = yr + at[u] + lo[s];
+            raw[u].put(to, hi, valid);
           }
         }
       }
@@ -299,45 +399,43 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Params P) {
     // channel adds them in order
     extern __shared__ float sums[];  // [warps * per_warp][d]
     const int nw = blockDim.x >> 5, warp = threadIdx.x >> 5;
-    for (int o = 0; o < 2; ++o) {
-      __syncthreads();
+    if (mine) {
+      float* const to = sums + static_cast<size_t>(warp * per_warp + seg) * P.d;
 #pragma unroll
-      for (int s = 0; s < SL; ++s) {
-        if (!valid[s]) continue;
-        float* const to = sums + static_cast<size_t>(warp * per_warp + seg) * P.d;
-#pragma unroll
-        for (int i = 0; i < 2 * V; ++i) to[(i < V ? lo[s] : hi[s] - V) + i] = o == 0 ? acc[0][s][i] : acc[1][s][i];
+      for (int j = 0; j < NP; ++j) {
+        if (!valid[j / V]) continue;
+        to[channel(j, 0)] = j & 1 ? ga[BWD ? j / 2 : 0].y : ga[BWD ? j / 2 : 0].x;
+        to[channel(j, 1)] = j & 1 ? gb[BWD ? j / 2 : 0].y : gb[BWD ? j / 2 : 0].x;
       }
-      __syncthreads();
-      for (int c = threadIdx.x; c < P.d; c += blockDim.x) {
-        float t = 0.f;
-        for (int k = 0; k < nw * per_warp; ++k) t += sums[static_cast<size_t>(k) * P.d + c];
-        P.partial[(static_cast<size_t>(blockIdx.x) * 2 + o) * P.d + c] = t;
-      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < P.d; c += blockDim.x) {
+      float t = 0.f;
+      for (int k = 0; k < nw * per_warp; ++k) t += sums[static_cast<size_t>(k) * P.d + c];
+      P.partial[static_cast<size_t>(blockIdx.x) * P.d + c] = t;
     }
   }
 }
 
-// dg[o][c] = sum over blocks of partial[block][o][c]: 32 columns a block, 32 threads a column, joined in order
-__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int blocks, int d,
+// dg[c] = sum over the queries' or the keys' blocks of partial[block][c]: 32 columns a block, 32 threads a
+// column, joined in order
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int blocks0, int blocks, int d,
                                                            void* dq_weight, void* dk_weight, int bf16) {
   __shared__ float part[32][33];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), k0 = threadIdx.x >> 5;
+  const int first = blockIdx.y ? blocks0 : 0, last = blockIdx.y ? blocks : blocks0;
   float t = 0.f;
-  if (c < 2 * d)
-    for (int b = k0; b < blocks; b += 32) t += partial[static_cast<size_t>(b) * 2 * d + c];
+  if (c < d)
+    for (int b = first + k0; b < last; b += 32) t += partial[static_cast<size_t>(b) * d + c];
   part[k0][threadIdx.x & 31] = t;
   __syncthreads();
-  if (k0 == 0 && c < 2 * d) {
+  void* const out = blockIdx.y ? dk_weight : dq_weight;
+  if (k0 == 0 && c < d && out) {
     t = 0.f;
 #pragma unroll
     for (int k = 0; k < 32; ++k) t += part[k][threadIdx.x];
-    void* const out = c < d ? dq_weight : dk_weight;
-    const int i = c < d ? c : c - d;
-    if (out) {
-      if (bf16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(t);
-      else static_cast<float*>(out)[i] = t;
-    }
+    if (bf16) static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(t);
+    else static_cast<float*>(out)[c] = t;
   }
 }
 
@@ -384,6 +482,8 @@ int fill_positions(const msl_rotary_geometry* g, Params& P, const float* table, 
     return MSL_OK;
   }
   if (!multiple_of(table, 8)) return failf(MSL_ERR_INVALID, "table must be 8-byte aligned");
+  if (static_cast<long long>(g->frames) * P.npair[0] + static_cast<long long>(g->height) * P.npair[1] + static_cast<long long>(g->width) * P.npair[2] > (1LL << 30))
+    return failf(MSL_ERR_UNSUPPORTED, "the table has over 2^30 entries");
   P.table = reinterpret_cast<const float2*>(table);
   P.index = index;
   P.index_rows = index_rows;
@@ -402,12 +502,10 @@ int fill_positions(const msl_rotary_geometry* g, Params& P, const float* table, 
 
 // The widest slot that head_dim, the turning channels and the alignment of every row operand allow (V = 1 goes
 // element by element).  SL (slots of a lane)
-// follows from it: V = 8 and 4 need at most 32 lanes for 256 channels, V = 2 two slots, V = 1 four.
+// follows from it: V = 4 needs at most 32 lanes for 256 channels, V = 2 two slots, V = 1 four.
 int choose_v(const Params& P, bool inter, int dtype, bool bwd, int nops) {
   const int es = dtype == MSL_DTYPE_BF16 ? 2 : 4;
-  for (int v = 8; v > 1; v /= 2) {
-    // 8 pairs a lane only where it makes 16-byte loads out of 8-byte ones (split pairs of bf16)
-    if (v == 8 && (inter || es == 4)) continue;
+  for (int v = 4; v > 1; v /= 2) {
     if (P.d % (2 * v) || P.R % (2 * v)) continue;
     const int bytes = min((inter ? 2 * v : v) * es, 16);
     bool ok = true;
@@ -421,50 +519,65 @@ int choose_v(const Params& P, bool inter, int dtype, bool bwd, int nops) {
   return 1;
 }
 
-template <typename T, int V, int SL, bool INTER, bool NORM, bool BWD>
-cudaError_t launch(Params P, cudaStream_t s, int blocks_fixed) {
+// Blocks of a backward whose weights' gradients are wanted: resident ones only, each keeps its sums.  The
+// queries' share goes by the heads.
+int bwd_blocks(const msl_rotary_geometry* g, const msl_qk_norm_io* io, int* blocks0) {
+  const long long most = static_cast<long long>(sm_count()) * kBwdBlocksPerSm;
+  const long long need = (g->rows * io->heads + kWarps - 1) / kWarps, need1 = (g->rows * io->kv_heads + kWarps - 1) / kWarps;
+  if (need + need1 <= most) {
+    *blocks0 = static_cast<int>(need > 0 ? need : 1);
+    return *blocks0 + static_cast<int>(need1);
+  }
+  long long b0 = io->kv_heads ? most * io->heads / (io->heads + io->kv_heads) : most;
+  if (b0 < 1) b0 = 1;
+  if (io->kv_heads && b0 == most) b0 = most - 1;
+  *blocks0 = static_cast<int>(b0);
+  return static_cast<int>(most);
+}
+
+template <typename T, int V, int SL, bool INTER, int MODE, int LC>
+cudaError_t launch(Params P, cudaStream_t s, int blocks) {
   P.lanes = (P.d / (2 * V) + SL - 1) / SL;
   const int per_warp = 32 / P.lanes;
-  const int units = (P.heads[0] + per_warp - 1) / per_warp + (P.heads[1] + per_warp - 1) / per_warp;
+  const int units0 = (P.heads[0] + per_warp - 1) / per_warp, units1 = (P.heads[1] + per_warp - 1) / per_warp;
   // few tokens: several warps share a token's heads, until every SM has some
   const long long want = static_cast<long long>(sm_count()) * kWarps;
   long long splits = P.rows >= want ? 1 : (want + P.rows - 1) / P.rows;
-  if (splits > units) splits = units;
+  if (splits > (units0 > units1 ? units0 : units1)) splits = units0 > units1 ? units0 : units1;
   P.splits = static_cast<int>(splits);
-  long long blocks = (P.rows * splits + kWarps - 1) / kWarps;
-  if (blocks_fixed) blocks = blocks_fixed;
-  if (blocks > 0x7fffffffLL) blocks = 0x7fffffffLL;  // the kernel strides over the rest
-  const size_t smem = BWD && P.partial ? sizeof(float) * kWarps * per_warp * P.d : 0;
-  rotary_kernel<T, V, SL, INTER, NORM, BWD><<<static_cast<unsigned>(blocks), kWarps * 32, smem, s>>>(P);
+  // several tokens a warp once every SM has its warps: their places follow from one another
+  P.group = P.rows >= 16 * want ? 4 : P.rows >= 8 * want ? 2 : 1;
+  P.table_vec = SL == 1 && V % 2 == 0 && multiple_of(P.table, 16);
+  for (int a = 0; a < 3; ++a) P.table_vec = P.table_vec && P.npair[a] % V == 0;
+  if (blocks == 0) {
+    long long each = ((P.rows + P.group - 1) / P.group * splits + kWarps - 1) / kWarps;
+    if (each > 0x3fffffffLL) each = 0x3fffffffLL;  // the kernel strides over the rest
+    P.blocks0 = static_cast<int>(each);
+    blocks = static_cast<int>(P.heads[1] ? 2 * each : each);
+  }
+  const size_t smem = MODE == kBackward && P.partial ? sizeof(float) * kWarps * per_warp * P.d : 0;
+  rotary_kernel<T, V, SL, INTER, MODE, LC><<<static_cast<unsigned>(blocks), kWarps * 32, smem, s>>>(P);
   return cudaGetLastError();
 }
 
-template <typename T, bool INTER, bool NORM, bool BWD>
+template <typename T, bool INTER, int MODE>
 cudaError_t by_v(const Params& P, int v, cudaStream_t s, int blocks) {
   switch (v) {
-    case 8:
-      if constexpr (!INTER && sizeof(T) == 2) return launch<T, 8, 1, INTER, NORM, BWD>(P, s, blocks);
-      return cudaErrorInvalidValue;
-    case 4: return launch<T, 4, 1, INTER, NORM, BWD>(P, s, blocks);
-    case 2: return launch<T, 2, 2, INTER, NORM, BWD>(P, s, blocks);
-    default: return launch<T, 1, 4, INTER, NORM, BWD>(P, s, blocks);
+    case 4:
+      if (MODE != kRotate && P.d == 64) return launch<T, 4, 1, INTER, MODE, 8>(P, s, blocks);
+      if (MODE != kRotate && P.d == 128) return launch<T, 4, 1, INTER, MODE, 16>(P, s, blocks);
+      return launch<T, 4, 1, INTER, MODE, 0>(P, s, blocks);
+    case 2: return launch<T, 2, 2, INTER, MODE, 0>(P, s, blocks);
+    default: return launch<T, 1, 4, INTER, MODE, 0>(P, s, blocks);
   }
 }
 
-template <bool NORM, bool BWD>
+template <int MODE>
 cudaError_t dispatch(const Params& P, bool inter, int dtype, cudaStream_t s, int blocks) {
-  const int v = choose_v(P, inter, dtype, BWD, 2);
+  const int v = choose_v(P, inter, dtype, MODE == kBackward, 2);
   if (dtype == MSL_DTYPE_BF16)
-    return inter ? by_v<__nv_bfloat16, true, NORM, BWD>(P, v, s, blocks) : by_v<__nv_bfloat16, false, NORM, BWD>(P, v, s, blocks);
-  return inter ? by_v<float, true, NORM, BWD>(P, v, s, blocks) : by_v<float, false, NORM, BWD>(P, v, s, blocks);
-}
-
-// Blocks of a backward whose weights' gradients are wanted: resident ones only, each keeps its sums.
-int bwd_blocks(const msl_rotary_geometry* g, const msl_qk_norm_io* io) {
-  const long long most = static_cast<long long>(sm_count()) * kBwdBlocksPerSm;
-  const long long units = g->rows * (static_cast<long long>(io->heads) + io->kv_heads);  // at least as many as items
-  const long long need = (units + kWarps - 1) / kWarps;
-  return static_cast<int>(need < most ? (need > 0 ? need : 1) : most);
+    return inter ? by_v<__nv_bfloat16, true, MODE>(P, v, s, blocks) : by_v<__nv_bfloat16, false, MODE>(P, v, s, blocks);
+  return inter ? by_v<float, true, MODE>(P, v, s, blocks) : by_v<float, false, MODE>(P, v, s, blocks);
 }
 
 int fill_norm(const msl_rotary_geometry* g, const msl_qk_norm_io* io, Params& P) {
@@ -518,7 +631,7 @@ int msl_rope3d(const msl_rotary_geometry* geom, int32_t heads, const void* x, in
   P.x[0] = x; P.x_ld[0] = x_ld;
   P.y[0] = y; P.y_ld[0] = y_ld;
   P.sign = inverse ? -1.f : 1.f;
-  const cudaError_t e = rot::dispatch<false, false>(P, geom->interleaved != 0, geom->dtype, static_cast<cudaStream_t>(stream), 0);
+  const cudaError_t e = rot::dispatch<rot::kRotate>(P, geom->interleaved != 0, geom->dtype, static_cast<cudaStream_t>(stream), 0);
   if (e != cudaSuccess) return cuda_failf(e, "rotary_kernel launch");
   count_launches(1);
   return MSL_OK;
@@ -536,7 +649,7 @@ int msl_qk_norm_rope_fwd(const msl_rotary_geometry* geom, const msl_qk_norm_io* 
   if (rc) return rc;
   P.y[0] = io->q_out; P.y_ld[0] = io->q_out_ld;
   P.y[1] = io->k_out; P.y_ld[1] = io->k_out_ld;
-  const cudaError_t e = rot::dispatch<true, false>(P, geom->interleaved != 0, geom->dtype, static_cast<cudaStream_t>(stream), 0);
+  const cudaError_t e = rot::dispatch<rot::kForward>(P, geom->interleaved != 0, geom->dtype, static_cast<cudaStream_t>(stream), 0);
   if (e != cudaSuccess) return cuda_failf(e, "rotary_kernel launch");
   count_launches(1);
   return MSL_OK;
@@ -546,7 +659,8 @@ size_t msl_qk_norm_rope_bwd_workspace_bytes(const msl_rotary_geometry* geom, con
   rot::Params P;
   if (rot::fill_norm(geom, io, P)) return 0;
   if (!io->dq_weight && !io->dk_weight) return 0;
-  return sizeof(float) * 2 * P.d * rot::bwd_blocks(geom, io);
+  int blocks0 = 0;
+  return sizeof(float) * P.d * rot::bwd_blocks(geom, io, &blocks0);
 }
 
 int msl_qk_norm_rope_bwd(const msl_rotary_geometry* geom, const msl_qk_norm_io* io, void* workspace,
@@ -577,19 +691,21 @@ int msl_qk_norm_rope_bwd(const msl_rotary_geometry* geom, const msl_qk_norm_io* 
   P.y[0] = io->dq; P.y_ld[0] = io->dq_ld;
   P.y[1] = io->dk; P.y_ld[1] = io->dk_ld;
   P.sign = -1.f;
-  const int blocks = rot::bwd_blocks(geom, io);
+  int blocks0 = 0;
+  const int blocks = rot::bwd_blocks(geom, io, &blocks0);
   if (dw) {
-    const size_t need = sizeof(float) * 2 * P.d * blocks;
+    P.blocks0 = blocks0;
+    const size_t need = sizeof(float) * P.d * blocks;
     if (!workspace || workspace_bytes < need)
       return failf(MSL_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
     if (!multiple_of(workspace, 4)) return failf(MSL_ERR_INVALID, "workspace must be 4-byte aligned");
     P.partial = static_cast<float*>(workspace);
   }
-  cudaError_t e = rot::dispatch<true, true>(P, geom->interleaved != 0, geom->dtype, s, dw ? blocks : 0);
+  cudaError_t e = rot::dispatch<rot::kBackward>(P, geom->interleaved != 0, geom->dtype, s, dw ? blocks : 0);
   if (e != cudaSuccess) return cuda_failf(e, "rotary_kernel launch");
   if (dw) {
-    rot::weight_grad_kernel<<<(2 * P.d + 31) / 32, 1024, 0, s>>>(P.partial, blocks, P.d, io->dq_weight, io->dk_weight,
-                                                                io->weight_dtype == MSL_DTYPE_BF16);
+    rot::weight_grad_kernel<<<dim3((P.d + 31) / 32, io->kv_heads ? 2 : 1), 1024, 0, s>>>(P.partial, blocks0, blocks, P.d, io->dq_weight, io->dk_weight,
+                                                                                        io->weight_dtype == MSL_DTYPE_BF16);
     e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_failf(e, "weight_grad_kernel launch");
   }
