@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256) product_simt_kernel(const Product P) {
       } else if (EPI == kGate) {
         const float g = acc[0][i][j] + (bias ? to_f32<T>(bias[n]) : 0.f);
         const float u = acc[NB - 1][i][j] + (bias ? to_f32<T>(bias[P.N + n]) : 0.f);
-        out[m * P.ldo + n] = from_f32<T>(act_value<sizeof(T) == 2>(g, P.act) * u);
+        out[m * P.ldo + n] = from_f32<T>(act_value(g, P.act) * u);
         if (P.gu_out) {
           T* const gu = static_cast<T*>(P.gu_out) + m * 2 * P.N;
           gu[n] = from_f32<T>(g);
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(256) product_simt_kernel(const Product P) {
       } else {
         const T* const gu = static_cast<const T*>(P.gu) + m * 2 * P.N;
         float da;
-        const float a = act_value_grad<sizeof(T) == 2>(to_f32<T>(gu[n]), P.act, da);
+        const float a = act_value_grad(to_f32<T>(gu[n]), P.act, da);
         out[m * 2 * P.N + n] = from_f32<T>(acc[0][i][j] * to_f32<T>(gu[P.N + n]) * da);
         out[m * 2 * P.N + P.N + n] = from_f32<T>(acc[0][i][j] * a);
       }
@@ -110,23 +110,51 @@ cudaError_t launch_product_simt(const Product& p, cudaStream_t s) {
 
 // ------------------------------------------------------------------------------------------ column sums
 
-// partial[slice][c] = sum of the slice's rows; 32 columns x 8 rows of threads.
-template <typename T>
+// Bound by bytes (604 MB for the 32768 x 9216 gradients of the projections in bf16): every element is read
+// once, V adjacent columns a thread (16 bytes), 8 warps a block on alternate rows, four rows' loads in flight.
+// partial[slice][c] = sum of the slice's rows.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x, long long ld, long long rows, int cols, long long per,
                                                          float* __restrict__ partial) {
-  __shared__ float part[8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+  __shared__ float part[8][32 * V + 1];
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int c = (blockIdx.x * 32 + lane) * V;
   const long long r1 = min(rows, (blockIdx.y + 1LL) * per);
-  float t = 0.f;
-  if (c < cols)
-    for (long long r = blockIdx.y * per + y; r < r1; r += 8) t += to_f32<T>(x[r * ld + c]);
-  part[y][threadIdx.x & 31] = t;
-  __syncthreads();
-  if (y == 0 && c < cols) {
-    t = 0.f;
+  float t[V];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += part[i][threadIdx.x];
-    partial[static_cast<size_t>(blockIdx.y) * cols + c] = t;
+  for (int i = 0; i < V; ++i) t[i] = 0.f;
+  if (c < cols) {
+    const T* p = x + (blockIdx.y * per + y) * ld + c;
+    long long r = blockIdx.y * per + y;
+    if constexpr (V == 1) {
+      for (; r < r1; r += 8, p += 8 * ld) t[0] += to_f32<T>(p[0]);
+    } else {
+      for (; r + 24 < r1; r += 32, p += 32 * ld) {
+        uint4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = __ldg(reinterpret_cast<const uint4*>(p + u * 8 * ld));
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int i = 0; i < V; ++i) t[i] += to_f32<T>(reinterpret_cast<const T*>(&w[u])[i]);
+      }
+      for (; r < r1; r += 8, p += 8 * ld) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] += to_f32<T>(reinterpret_cast<const T*>(&w)[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) part[y][lane * V + i] = t[i];
+  __syncthreads();
+  for (int k = threadIdx.x; k < 32 * V; k += 256) {
+    const int col = blockIdx.x * 32 * V + k;
+    if (col >= cols) break;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += part[i][k];
+    partial[static_cast<size_t>(blockIdx.y) * cols + col] = sum;
   }
 }
 
@@ -135,25 +163,32 @@ __global__ void __launch_bounds__(256) column_join_kernel(const float* __restric
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
   float t = 0.f;
+#pragma unroll 8
   for (int s = 0; s < slices; ++s) t += partial[static_cast<size_t>(s) * cols + c];
   out[c] = from_f32<T>(t);
 }
 
 constexpr int kSlices = 64;
 
-static cudaError_t column_sums(int dtype, const void* x, long long ld, long long rows, int cols, void* out, float* partial, cudaStream_t s) {
-  const long long per = (rows + kSlices - 1) / kSlices;
+template <typename T>
+static cudaError_t column_sums_t(const T* x, long long ld, long long rows, int cols, T* out, float* partial, cudaStream_t s) {
+  constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  const long long per = rows > 64 * kSlices ? (rows + kSlices - 1) / kSlices : 64;
   const int slices = static_cast<int>((rows + per - 1) / per);
-  const dim3 grid((cols + 31) / 32, slices);
-  if (dtype == MSL_DTYPE_BF16) {
-    column_sum_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), ld, rows, cols, per, partial);
-    column_join_kernel<<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, static_cast<__nv_bfloat16*>(out));
-  } else {
-    column_sum_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(x), ld, rows, cols, per, partial);
-    column_join_kernel<<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, static_cast<float*>(out));
-  }
+  const bool vec = multiple_of(x, 16) && ld % kVec == 0 && cols % kVec == 0;
+  const int v = vec ? kVec : 1;
+  const dim3 grid((cols + 32 * v - 1) / (32 * v), slices);
+  if (vec) column_sum_kernel<T, kVec><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial);
+  else column_sum_kernel<T, 1><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial);
+  column_join_kernel<T><<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, out);
   count_launches(2);
   return cudaGetLastError();
+}
+
+static cudaError_t column_sums(int dtype, const void* x, long long ld, long long rows, int cols, void* out, float* partial, cudaStream_t s) {
+  if (dtype == MSL_DTYPE_BF16)
+    return column_sums_t(static_cast<const __nv_bfloat16*>(x), ld, rows, cols, static_cast<__nv_bfloat16*>(out), partial, s);
+  return column_sums_t(static_cast<const float*>(x), ld, rows, cols, static_cast<float*>(out), partial, s);
 }
 
 static int run(const Product& p, cudaStream_t s) {
@@ -175,11 +210,45 @@ static int check(const msl_ffn_geometry* g, const msl_ffn_io* io) {
   return MSL_OK;
 }
 
-static Product product(const msl_ffn_geometry* g, const msl_ffn_io* io) {
+// Workspace: the sums of parts of tiles of one product at a time, then the column sums' slices.
+struct Workspace {
+  size_t partial, columns, total;
+};
+static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
+  Workspace w{};
+  const long long M = g->rows, C = g->dim, F = g->hidden;
+  auto need = [&](long long m, long long n, long long k, int epilogue, bool b_major) {
+    const size_t b = M > 0 && g->dtype == MSL_DTYPE_BF16 ? tc_partial_bytes(m, n, k, epilogue, b_major) : 0;
+    if (b > w.partial) w.partial = b;
+  };
+  if (backward) {
+    need(M, F, C, kDgate, true);
+    need(M, C, 2 * F, kPlain, true);
+    need(2 * F, C, M, kPlain, true);
+    need(C, F, M, kPlain, true);
+    w.columns = sizeof(float) * kSlices * static_cast<size_t>(2 * F > C ? 2 * F : C);
+  } else {
+    need(M, F, C, kGate, false);
+    need(M, C, F, kPlain, false);
+  }
+  w.partial = (w.partial + 255) / 256 * 256;
+  w.total = w.partial + w.columns;
+  return w;
+}
+static int check_workspace(const Workspace& w, const void* p, size_t bytes) {
+  if (w.total == 0) return MSL_OK;
+  if (!p || bytes < w.total) return failf(MSL_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", w.total, p ? bytes : 0);
+  if (!multiple_of(p, 16)) return failf(MSL_ERR_INVALID, "workspace must be 16-byte aligned");
+  return MSL_OK;
+}
+
+static Product product(const msl_ffn_geometry* g, const msl_ffn_io* io, const Workspace& w, void* workspace) {
   Product p{};
   p.dtype = g->dtype;
   p.act = g->activation;
   p.status = io->status;
+  p.partial = static_cast<float*>(workspace);
+  p.partial_bytes = w.partial;
   return p;
 }
 
@@ -192,9 +261,7 @@ extern "C" {
 
 size_t msl_gated_ffn_workspace_bytes(const msl_ffn_geometry* geom, int32_t backward) {
   msl_ffn_io none{};
-  if (ffn::check(geom, &none) || !backward) return 0;
-  return sizeof(float) * ffn::kSlices * (2 * static_cast<size_t>(geom->hidden) > static_cast<size_t>(geom->dim) ? 2 * static_cast<size_t>(geom->hidden)
-                                                                                                              : static_cast<size_t>(geom->dim));
+  return ffn::check(geom, &none) ? 0 : ffn::workspace_of(geom, backward != 0).total;
 }
 
 int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,
@@ -206,8 +273,11 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   if (M == 0) return MSL_OK;
   if (!io->x || !io->h || !io->y) return failf(MSL_ERR_INVALID, "x, h and y are required");
   if (io->x_ld < C || io->y_ld < C) return failf(MSL_ERR_INVALID, "row strides must be >= dim = %lld", C);
+  const ffn::Workspace W = ffn::workspace_of(geom, false);
+  rc = ffn::check_workspace(W, workspace, workspace_bytes);
+  if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  ffn::Product p = ffn::product(geom, io);
+  ffn::Product p = ffn::product(geom, io, W, workspace);
   p.epilogue = ffn::kGate;
   p.a = io->x; p.lda = io->x_ld;
   p.b = io->w_in; p.ldb = C;
@@ -217,7 +287,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.M = M; p.N = F; p.K = C;
   rc = ffn::run(p, s);
   if (rc) return rc;
-  p = ffn::product(geom, io);
+  p = ffn::product(geom, io, W, workspace);
   p.epilogue = ffn::kPlain;
   p.a = io->h; p.lda = F;
   p.b = io->w_out; p.ldb = F;
@@ -248,15 +318,12 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   if (io->dx && (!io->w_in || io->dx_ld < C)) return failf(MSL_ERR_INVALID, "dx needs w_in and a row stride >= dim");
   if (io->dw_in && (!io->x || io->x_ld < C)) return failf(MSL_ERR_INVALID, "dw_in needs x");
   if (io->dw_out && !io->h) return failf(MSL_ERR_INVALID, "dw_out needs h");
-  if (io->db_in || io->db_out) {
-    const size_t need = msl_gated_ffn_workspace_bytes(geom, 1);
-    if (!workspace || workspace_bytes < need)
-      return failf(MSL_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
-    if (!multiple_of(workspace, 16)) return failf(MSL_ERR_INVALID, "workspace must be 16-byte aligned");
-  }
+  const ffn::Workspace W = ffn::workspace_of(geom, true);
+  rc = ffn::check_workspace(W, workspace, workspace_bytes);
+  if (rc) return rc;
   ffn::Product p;
   if (inner) {
-    p = ffn::product(geom, io);
+    p = ffn::product(geom, io, W, workspace);
     p.epilogue = ffn::kDgate;
     p.a = io->dy; p.lda = io->dy_ld;
     p.b = io->w_out; p.ldb = F; p.b_major = true;  // [K = dim, N = hidden]
@@ -267,7 +334,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     if (rc) return rc;
   }
   if (io->dx) {
-    p = ffn::product(geom, io);
+    p = ffn::product(geom, io, W, workspace);
     p.a = io->dgu; p.lda = 2 * F;
     p.b = io->w_in; p.ldb = C; p.b_major = true;  // [K = 2 hidden, N = dim]
     p.out = io->dx; p.ldo = io->dx_ld;
@@ -276,7 +343,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     if (rc) return rc;
   }
   if (io->dw_in) {
-    p = ffn::product(geom, io);
+    p = ffn::product(geom, io, W, workspace);
     p.a = io->dgu; p.lda = 2 * F; p.a_major = true;  // [K = rows, M = 2 hidden]
     p.b = io->x; p.ldb = io->x_ld; p.b_major = true;  // [K = rows, N = dim]
     p.out = io->dw_in; p.ldo = C;
@@ -285,7 +352,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     if (rc) return rc;
   }
   if (io->dw_out) {
-    p = ffn::product(geom, io);
+    p = ffn::product(geom, io, W, workspace);
     p.a = io->dy; p.lda = io->dy_ld; p.a_major = true;  // [K = rows, M = dim]
     p.b = io->h; p.ldb = F; p.b_major = true;           // [K = rows, N = hidden]
     p.out = io->dw_out; p.ldo = F;
@@ -293,7 +360,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     rc = ffn::run(p, s);
     if (rc) return rc;
   }
-  float* const partial = static_cast<float*>(workspace);
+  float* const partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + W.partial);
   if (io->db_in) {
     const cudaError_t e = ffn::column_sums(geom->dtype, io->dgu, 2 * F, M, static_cast<int>(2 * F), io->db_in, partial, s);
     if (e != cudaSuccess) return cuda_failf(e, "column_sum_kernel launch");

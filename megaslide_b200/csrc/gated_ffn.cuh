@@ -31,32 +31,71 @@ struct Product {
   int dtype, act, epilogue;
   bool a_major, b_major;
   uint32_t* status;
+  float* partial;  // workspace of tiles that are cut along k
+  size_t partial_bytes;
 };
 
-// act(g) and its derivative, in float32.  FAST: the exponential by __expf, whose error (about 2^-22 of the
-// result for the sizes that matter) is far below the rounding of a bf16 result.
-template <bool FAST>
-__device__ __forceinline__ float act_exp(float x) { return FAST ? __expf(x) : expf(x); }
-template <bool FAST>
+// act(g) and its derivative, in float32, for results in float32.
 __device__ __forceinline__ float act_value(float g, int act) {
-  if (act == MSL_ACT_SILU) return g / (1.f + act_exp<FAST>(-g));
+  if (act == MSL_ACT_SILU) return g / (1.f + expf(-g));
   return 0.5f * g * (1.f + erff(g * 0.7071067811865476f));
 }
-template <bool FAST>
 __device__ __forceinline__ float act_value_grad(float g, int act, float& da) {
   if (act == MSL_ACT_SILU) {
-    const float s = 1.f / (1.f + act_exp<FAST>(-g));
+    const float s = 1.f / (1.f + expf(-g));
     da = s * (1.f + g * (1.f - s));
     return g * s;
   }
   const float c = 0.5f * (1.f + erff(g * 0.7071067811865476f));
-  da = fmaf(g * 0.3989422804014327f, act_exp<FAST>(-0.5f * g * g), c);
+  da = fmaf(g * 0.3989422804014327f, expf(-0.5f * g * g), c);
+  return g * c;
+}
+
+// The same for results in bf16, in a third of the instructions: the epilogues of the tensor-core products have
+// about 150 clocks for a row of 32 elements before they hold up the multiplications.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid_fast(float g) { return __fdividef(1.f, 1.f + fast_exp2(-1.4426950408889634f * g)); }
+// Normal distribution function and, by e, exp(-g^2/2): for x = |g| the tail is exp(-x^2/2) q(t), t = 1/(1 + 0.38 x),
+// where q is a minimax polynomial (least largest relative error on [0, 14], by linear programming) of
+// exp(x^2/2) erfc(x/sqrt 2)/2: within 3.6e-5 of the tail, 2^-15.
+__device__ __forceinline__ float normal_cdf_fast(float g, float& e) {
+  const float x = fabsf(g);
+  const float t = __fdividef(1.f, fmaf(0.38f, x, 1.f));
+  e = fast_exp2(-0.7213475204444817f * g * g);
+  float q = fmaf(t, -0.08992771633985343f, 0.18887508919166987f);
+  q = fmaf(t, q, 0.09198074100439507f);
+  q = fmaf(t, q, 0.15782920020547297f);
+  q = fmaf(t, q, 0.15122516174542605f);
+  const float tail = q * t * e;
+  return g < 0.f ? tail : 1.f - tail;
+}
+template <int ACT>
+__device__ __forceinline__ float act_fast(float g) {
+  if (ACT == MSL_ACT_SILU) return g * sigmoid_fast(g);
+  float e;
+  return g * normal_cdf_fast(g, e);
+}
+template <int ACT>
+__device__ __forceinline__ float act_grad_fast(float g, float& da) {
+  if (ACT == MSL_ACT_SILU) {
+    const float s = sigmoid_fast(g), a = g * s;
+    da = fmaf(a, 1.f - s, s);
+    return a;
+  }
+  float e;
+  const float c = normal_cdf_fast(g, e);
+  da = fmaf(g * 0.3989422804014327f, e, c);
   return g * c;
 }
 
 cudaError_t launch_product_simt(const Product& p, cudaStream_t s);
 // Tensor-core form (gated_ffn_tc.cu), and whether the operands allow it.
 bool tc_applies(const Product& p);
+size_t tc_partial_bytes(long long M, long long N, long long K, int epilogue, bool b_major);
 cudaError_t launch_product_tc(const Product& p, cudaStream_t s);
 
 }  // namespace ffn

@@ -7,12 +7,22 @@
 // by TMA with the 128-byte swizzle that tcgen05.mma reads in either orientation; ragged edges are the TMA's zero
 // fill and clipping, no element is handled apart.
 //
-// One CTA per SM walks over 128 x BN tiles: one thread loads (a ring of stages), one thread issues the
-// multiplications (128 x BN x 16 each), eight warps turn finished accumulators into results while the next
-// tile is multiplied into the other half of the tensor memory.
-//   gate:  the tile's columns are 128 gate columns and the same 128 columns of the other projection, so g and u of an
-//          element meet in one epilogue thread: bias, activation, product, and the kept g, u leave from there
-//   dgate: the accumulator is the gradient of h; the epilogue reads the kept g, u and writes both their gradients
+// Two CTAs (a cluster) share a 256 x BN tile: each holds 128 rows of A, half of B and the sums of its 128 rows,
+// and every multiplication (256 x BN x 16) reads both halves of B, which each SM loads and stores only once.  In a
+// CTA one thread loads (a ring of stages), one thread of the first CTA issues the multiplications, eight warps turn
+// finished sums into results while the next tile is multiplied into the other half of the tensor memory.  The
+// pairs walk over the tiles, one pair per two SMs.
+//   gate:  the tile's columns are BN/2 gate columns (the first CTA's half of B) and the same columns of the other
+//          projection, so g and u of an element meet in one epilogue thread: bias, activation, product, and the
+//          kept g, u leave from there
+//   dgate: the sums are the gradient of h; the epilogue fetches the kept g, u by TMA, a step ahead, and
+//          writes both their gradients over them in shared memory, from where they leave
+//
+// Tiles that do not fill a last round of all pairs are cut along k among the pairs left over: their parts' sums
+// go to the workspace in float32 and a small kernel joins them, in order, and does the epilogue.
+//
+// What bounds it: the multiplications.  One CTA alone on 128 x 256 tiles fills its shared memory's bandwidth (48 KB
+// in and out for 512 clocks of multiplication); the pair needs 32 KB.
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -23,12 +33,15 @@ namespace msl {
 namespace ffn {
 namespace tc {
 
-constexpr int kBM = 128, kBK = 64;
+constexpr int kBM = 128, kBK = 64;  // of a CTA; a pair has 2 kBM rows
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kStageA = kBM * kBK * 2;
-constexpr int kStaging = 32 * 128;  // of an epilogue warp: 32 rows x 64 bf16
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr int kTile = 2048;           // a staging tile: 32 rows x 32 bf16
+constexpr int kStaging = 4 * kTile;   // of an epilogue warp
+constexpr int kRing = 5 * 2 * kStageA;  // shared memory of the stages
+constexpr int kMaxStages = 8;
+constexpr long long kWaitClocks = 4000000000ll;  // two seconds, at most four
 
 struct Maps {
   CUtensorMap a, b, out, gu;
@@ -36,9 +49,11 @@ struct Maps {
 
 struct Args {
   const __nv_bfloat16* bias;
-  const __nv_bfloat16* gu;
   long long M, N;
-  int kblocks, mt, nt, gm, act, keep;
+  int kblocks, mt, nt, gm, keep;  // mt: tiles of 256 rows
+  int bn, stages, stage_bytes, boxes;  // width of a tile, the ring, boxes of 64 that a CTA's half of B takes
+  int full, items, parts, kper;        // tiles done whole; with the parts of the others; parts of a tile, their k-blocks
+  float* partial;                      // [items - full][2 CTAs][4 x 32 rows][bn / 32][32 columns][32 rows]
   uint32_t* status;
 };
 
@@ -60,18 +75,14 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-// Waits for phase `parity` of a barrier, at most kWaitNs: then the CTA is marked dead and every role leaves.
+// Waits for phase `parity` of a barrier, at most kWaitClocks (counted on the SM's own clock: reading
+// the global timer takes longer than most waits): then the CTA is marked dead and every role leaves.
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* dead, uint32_t* status) {
   if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = now_ns();
+  const long long t0 = clock64();
   while (!mbar_try(bar, parity)) {
     if (*dead) return false;
-    if (now_ns() - t0 > kWaitNs) {
+    if (clock64() - t0 > kWaitClocks) {
       *dead = 1;
       if (status) atomicOr(status, MSL_STATUS_TIMEOUT);
       return false;
@@ -92,16 +103,39 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
                "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// arrives on the first CTA's barrier at the same place as `bar`.  Nothing that the thread itself wrote goes with
+// it (the operands are the TMA's, the sums were read), so the plain form will do: .release.cluster took a
+// microsecond, four times a block of 64 k.
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.shared::cluster.b64 _, [a];\n}" ::"r"(bar)
+               : "memory");
+}
+
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
                "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0) : "memory");
 }
+// arrives on the barrier at this place in both CTAs when the multiplications issued so far are done
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(static_cast<uint16_t>(3)) : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -139,19 +173,48 @@ __device__ __forceinline__ void tile_at(const Args& P, int t, int& m, int& n) {
   m = first + r - n * rows;
 }
 
+// What a pair does in a turn: a tile, its k-blocks [k0, k1), and its place in `partial` (-1: the whole tile).
+struct Item {
+  int m, n, k0, k1, part;
+};
+__device__ __forceinline__ Item item_at(const Args& P, int i) {
+  Item w;
+  w.k0 = 0;
+  w.k1 = P.kblocks;
+  w.part = -1;
+  int t = i;
+  if (i >= P.full) {
+    w.part = i - P.full;
+    t = P.full + w.part / P.parts;
+    w.k0 = w.part % P.parts * P.kper;
+    w.k1 = min(P.kblocks, w.k0 + P.kper);
+  }
+  tile_at(P, t, w.m, w.n);
+  return w;
+}
+
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&t);
 }
 
-// Half a row (32 columns) of a warp's staging tile: 16-byte chunk c of row r lies at c ^ (r & 7), as the TMA's
-// 128-byte swizzle has it (and no two lanes of a quarter meet in a bank).
-__device__ __forceinline__ void stage_half(uint32_t base, int row, int half, const uint32_t (&w)[16]) {
+// Chunk c (16 bytes) of row r of a staging tile lies at c ^ (r / 2 & 3), as the TMA's 64-byte swizzle has it (and no
+// two lanes of a quarter meet in a bank).
+__device__ __forceinline__ uint32_t chunk32(uint32_t base, int row, int c) { return base + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
+__device__ __forceinline__ uint4 lds(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts(uint32_t at, const uint32_t (&w)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+__device__ __forceinline__ void stage(uint32_t base, int row, const float (&v)[32]) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const uint32_t at = base + row * 128 + (((half * 4 + c) ^ (row & 7)) << 4);
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[c * 4]), "r"(w[c * 4 + 1]), "r"(w[c * 4 + 2]), "r"(w[c * 4 + 3])
-                 : "memory");
+    const uint32_t w[4] = {pack(v[c * 8], v[c * 8 + 1]), pack(v[c * 8 + 2], v[c * 8 + 3]), pack(v[c * 8 + 4], v[c * 8 + 5]), pack(v[c * 8 + 6], v[c * 8 + 7])};
+    sts(chunk32(base, row, c), w);
   }
 }
 
@@ -170,46 +233,45 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const __nv_bfloat16* bi
   }
 }
 
-__device__ __forceinline__ void load_half(uint4 (&w)[4], const __nv_bfloat16* p, bool row_in, long long n, long long N) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    w[c] = row_in && n + c * 8 + 8 <= N ? __ldg(reinterpret_cast<const uint4*>(p + n) + c) : make_uint4(0, 0, 0, 0);
-}
-
-template <int EPI, int BN, int STAGES, bool AM, bool BM>
+template <int EPI, bool AM, bool BM, int ACT>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args P) {
-  constexpr int kStageB = BN * kBK * 2, kStage = kStageA + kStageB;
-  constexpr int kBoxN = EPI == kGate ? BN / 2 : BN;      // columns of N that a tile covers
-  constexpr int kAcc = BN <= 128 ? 128 : 256;            // tensor memory columns of an accumulator
+  constexpr int kAcc = 256;  // tensor memory columns of a tile's sums
+  const int half = P.bn / 2;                              // rows of B that a CTA holds
+  const int width = EPI == kGate ? half : P.bn;           // columns of the result that a tile covers
+  const int stages = P.stages;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-  const uint32_t staging = base + STAGES * kStage;
+  const uint32_t staging = base + kRing;
   const uint32_t bars = staging + kEpiWarps * kStaging;
-  const uint32_t full = bars, empty = bars + 8 * STAGES, tfull = empty + 8 * STAGES, tempty = tfull + 16;
-  const uint32_t tmem_slot = tempty + 16;
+  const uint32_t full = bars, empty = bars + 8 * kMaxStages, peer = empty + 8 * kMaxStages, tfull = peer + 8 * kMaxStages, tempty = tfull + 16;
+  const uint32_t kept = tempty + 16, tmem_slot = kept + 16 * kEpiWarps;
   volatile int* const dead = reinterpret_cast<volatile int*>(raw + (tmem_slot + 4 - smem_u32(raw)));
   volatile uint32_t* const slot = reinterpret_cast<volatile uint32_t*>(raw + (tmem_slot - smem_u32(raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles = P.mt * P.nt;
+  const int rank = static_cast<int>(cluster_rank());
+  const int t0 = blockIdx.x >> 1, tstep = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
+    for (int i = 0; i < stages; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
+      mbar_init(peer + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull + 8 * i, 1);
-      mbar_init(tempty + 8 * i, kEpiWarps);
+      mbar_init(tempty + 8 * i, 2 * kEpiWarps);
     }
+    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(kept + 8 * i, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(2 * kAcc) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(2 * kAcc) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     fence_before();
   }
   __syncthreads();
+  cluster_sync();
   fence_after();
   const uint32_t tmem = *slot;
 
@@ -218,62 +280,77 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       int st = 0;
       uint32_t ph = 0;
       bool alive = true;
-      for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x) {
-        int m, n;
-        tile_at(P, t, m, n);
-        for (int kb = 0; kb < P.kblocks; ++kb) {
+      for (int t = t0; t < P.items && alive; t += tstep) {
+        const Item w = item_at(P, t);
+        const int m = w.m, n = w.n;
+        const int arow = (2 * m + rank) * kBM;
+        // rows of B: halves of the tile's columns; for the gate the first CTA has the gate's, the second the others
+        const int brow = EPI == kGate ? n * width + (rank ? static_cast<int>(P.N) : 0) : n * width + rank * half;
+        for (int kb = w.k0; kb < w.k1; ++kb) {
           if (!wait(empty + 8 * st, ph ^ 1, dead, P.status)) { alive = false; break; }
-          const uint32_t a = base + st * kStage, b = a + kStageA, bar = full + 8 * st;
-          mbar_expect(bar, kStage);
+          const uint32_t a = base + st * P.stage_bytes, b = a + kStageA, bar = full + 8 * st;
+          mbar_expect(bar, P.stage_bytes);
           if (AM) {
 #pragma unroll
-            for (int i = 0; i < kBM / 64; ++i) tma_load_2d(a + i * 8192, &maps.a, bar, m * kBM + i * 64, kb * kBK);
+            for (int i = 0; i < kBM / 64; ++i) tma_load_2d(a + i * 8192, &maps.a, bar, arow + i * 64, kb * kBK);
           } else {
-            tma_load_2d(a, &maps.a, bar, kb * kBK, m * kBM);
+            tma_load_2d(a, &maps.a, bar, kb * kBK, arow);
           }
           if (BM) {
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i) tma_load_2d(b + i * 8192, &maps.b, bar, n * BN + i * 64, kb * kBK);
+            for (int i = 0; i < P.boxes; ++i) tma_load_2d(b + i * 8192, &maps.b, bar, brow + i * 64, kb * kBK);
           } else {
-            tma_load_2d(b, &maps.b, bar, kb * kBK, n * kBoxN);
-            if (EPI == kGate) tma_load_2d(b + kStageB / 2, &maps.b, bar, kb * kBK, static_cast<int>(P.N) + n * kBoxN);
+            tma_load_2d(b, &maps.b, bar, kb * kBK, brow);
           }
-          if (++st == STAGES) { st = 0; ph ^= 1; }
+          if (++st == stages) { st = 0; ph ^= 1; }
         }
       }
       // the copies still in flight land before the CTA leaves
-      const unsigned long long t0 = now_ns();
+      const long long since = clock64();
       if (!alive)
-        for (int i = 0; i < STAGES; ++i)
-          while (!mbar_try(full + 8 * i, (i < st ? ph : ph ^ 1)) && now_ns() - t0 < kWaitNs) {
+        for (int i = 0; i < stages; ++i)
+          while (!mbar_try(full + 8 * i, (i < st ? ph : ph ^ 1)) && clock64() - since < kWaitClocks) {
           }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       // bf16 x bf16 -> float32, transpose bits where an operand's own axis is contiguous
-      constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (AM ? 1u << 15 : 0u) | (BM ? 1u << 16 : 0u) |
-                                 (static_cast<uint32_t>(BN >> 3) << 17) | (static_cast<uint32_t>(kBM >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (AM ? 1u << 15 : 0u) | (BM ? 1u << 16 : 0u) |
+                             (static_cast<uint32_t>(P.bn >> 3) << 17) | (static_cast<uint32_t>(2 * kBM >> 4) << 24);
       constexpr uint64_t a_step = (AM ? 2048 : 32) >> 4, b_step = (BM ? 2048 : 32) >> 4;
       int st = 0, buf = 0;
       uint32_t ph = 0, tph = 0;
       bool alive = true;
-      for (int t = blockIdx.x; t < tiles && alive; t += gridDim.x) {
+      for (int t = t0; t < P.items && alive; t += tstep) {
         if (!wait(tempty + 8 * buf, tph ^ 1, dead, P.status)) break;
         fence_after();
-        for (int kb = 0; kb < P.kblocks; ++kb) {
-          if (!wait(full + 8 * st, ph, dead, P.status)) { alive = false; break; }
+        const Item w = item_at(P, t);
+        for (int kb = w.k0; kb < w.k1; ++kb) {
+          if (!wait(full + 8 * st, ph, dead, P.status) || !wait(peer + 8 * st, ph, dead, P.status)) { alive = false; break; }
           fence_after();
-          const uint32_t a = base + st * kStage;
+          const uint32_t a = base + st * P.stage_bytes;
           const uint64_t da = operand<AM>(a), db = operand<BM>(a + kStageA);
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) mma(tmem + buf * kAcc, da + k * a_step, db + k * b_step, idesc, kb > 0 || k > 0);
+          for (int k = 0; k < kBK / 16; ++k) mma(tmem + buf * kAcc, da + k * a_step, db + k * b_step, idesc, kb > w.k0 || k > 0);
           mma_commit(empty + 8 * st);
-          if (++st == STAGES) { st = 0; ph ^= 1; }
+          if (++st == stages) { st = 0; ph ^= 1; }
         }
         if (alive) mma_commit(tfull + 8 * buf);
         buf ^= 1;
         if (buf == 0) tph ^= 1;
+      }
+    } else if (lane == 0) {
+      // the second CTA tells the first when its operands have landed
+      int st = 0;
+      uint32_t ph = 0;
+      bool alive = true;
+      for (int t = t0; t < P.items && alive; t += tstep) {
+        const Item w = item_at(P, t);
+        for (int kb = w.k0; kb < w.k1; ++kb) {
+          if (!wait(full + 8 * st, ph, dead, P.status)) { alive = false; break; }
+          arrive_first(peer + 8 * st);
+          if (++st == stages) { st = 0; ph ^= 1; }
+        }
       }
     }
     __syncwarp();
@@ -281,136 +358,235 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     const int ew = warp - 2, quad = warp & 3, set = ew >> 2;
     const uint32_t mine = staging + ew * kStaging;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t mykept = kept + 16 * ew;
     int buf = 0;
     uint32_t tph = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-      int m, n;
-      tile_at(P, t, m, n);
-      const long long row = static_cast<long long>(m) * kBM + quad * 32 + lane;
-      const int row0 = m * kBM + quad * 32;
-      const long long col0 = static_cast<long long>(n) * kBoxN;
+    uint32_t turn = 0;  // steps so far
+    // a tile goes in steps of 32 columns, the first half of them to set 0
+    const int steps = width / 32, first = set ? (steps + 1) / 2 : 0, last = set ? steps : (steps + 1) / 2;
+    for (int t = t0; t < P.items; t += tstep) {
+      const Item w = item_at(P, t);
+      const int m = w.m, n = w.n;
+      const int row0 = (2 * m + rank) * kBM + quad * 32;
+      const int col0 = n * width;
       const uint32_t acc = tmem + buf * kAcc + lanes;
-      uint4 kg[4], ku[4];
-      if (EPI == kDgate)  // the first kept values come while the tile is still multiplied
-      {
-        const __nv_bfloat16* const p = P.gu + row * 2 * P.N;
-        load_half(kg, p, row < P.M, col0 + set * 64, P.N);
-        load_half(ku, p + P.N, row < P.M, col0 + set * 64, P.N);
+      const bool rows_in = row0 < P.M;  // a box wholly outside is not started
+      // dgate: the staging buffer holds g and u of two steps
+      auto fetch = [&](uint32_t at, int i) {
+        const uint32_t to = mine + (at & 1) * 2 * kTile, bar = mykept + 8 * (at & 1);
+        mbar_expect(bar, 2 * kTile);
+        tma_load_3d(to, &maps.gu, bar, col0 + i * 32, 0, row0);
+        tma_load_3d(to + kTile, &maps.gu, bar, col0 + i * 32, 1, row0);
+      };
+      if (EPI == kDgate && lane == 0 && first < last && w.part < 0) {  // on their way while the tile is still multiplied
+        bulk_wait_read<0>();                             // the last tile's results have left
+        fetch(turn, first);
+        if (first + 1 < last) fetch(turn + 1, first + 1);
       }
+      __syncwarp();
       if (!wait(tfull + 8 * buf, tph, dead, P.status)) break;
       fence_after();
-      if (EPI == kGate) {
-        // 64 columns a set: h, then (kept) g and u, each a 32 x 64 tile through the staging buffer
-        if (set * 64 < kBoxN) {
-#pragma unroll
-          for (int what = 0; what < 3; ++what) {
-            if (what > 0 && !P.keep) break;
-            if (lane == 0) bulk_wait_read();
-            __syncwarp();
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int c = set * 64 + half * 32;
-              uint32_t w[16];
-              float g[32], u[32];
-              if (what != 2) {
-                tmem_ld32(acc + c, g);
-                if (P.bias) add_bias(g, P.bias, col0 + c, P.N);
-              }
-              if (what != 1) {
-                tmem_ld32(acc + kBoxN + c, u);
-                if (P.bias) add_bias(u, P.bias + P.N, col0 + c, P.N);
-              }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                if (what == 0) w[i] = pack(act_value<true>(g[2 * i], P.act) * u[2 * i], act_value<true>(g[2 * i + 1], P.act) * u[2 * i + 1]);
-                if (what == 1) w[i] = pack(g[2 * i], g[2 * i + 1]);
-                if (what == 2) w[i] = pack(u[2 * i], u[2 * i + 1]);
-              }
-              stage_half(mine, lane, half, w);
-            }
-            fence_async();
-            __syncwarp();
-            const int x = static_cast<int>(col0) + set * 64;
-            if (lane == 0 && x < P.N && row0 < P.M) {
-              if (what == 0) tma_store_2d(&maps.out, mine, x, row0);
-              else tma_store_3d(&maps.gu, mine, x, what - 1, row0);
-              bulk_commit();
-            }
-          }
-        }
-      } else {
+      bool alive = true;
+      if (w.part >= 0) {
+        const int blocks = P.bn / 32;
+        float* const to = P.partial + static_cast<size_t>((w.part * 2 + rank) * 4 + quad) * blocks * 1024 + lane;
 #pragma unroll 1
-        for (int c0 = set * 64; c0 < BN; c0 += 128) {
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
-          uint32_t later[2][16];
+        for (int i = set; i < blocks; i += 2) {
+          float v[32];
+          tmem_ld32(acc + i * 32, v);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int c = c0 + half * 32;
-            float v[32];
-            uint32_t w[16];
-            tmem_ld32(acc + c, v);
-            if (EPI == kPlain) {
-              if (P.bias) add_bias(v, P.bias, col0 + c, P.N);
+          for (int j = 0; j < 32; ++j) to[i * 1024 + j * 32] = v[j];
+        }
+      }
+#pragma unroll 1
+      for (int i = w.part < 0 ? first : last; i < last; ++i, ++turn) {
+        const int c = i * 32, x = col0 + c;
+        const bool store = lane == 0 && rows_in && x < P.N;
+        float v[32];
+        tmem_ld32(acc + c, v);
+        if (EPI == kDgate) {
+          const uint32_t g0 = mine + (turn & 1) * 2 * kTile, u0 = g0 + kTile;
+          if (!wait(mykept + 8 * (turn & 1), (turn >> 1) & 1, dead, P.status)) { alive = false; break; }
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = pack(v[2 * i], v[2 * i + 1]);
-            } else {
-              const uint4 cg[4] = {kg[0], kg[1], kg[2], kg[3]}, cu[4] = {ku[0], ku[1], ku[2], ku[3]};
-              const int next = half == 0 ? c + 32 : c0 + 128;
-              if (next < BN) {
-                const __nv_bfloat16* const p = P.gu + row * 2 * P.N;
-                load_half(kg, p, row < P.M, col0 + next, P.N);
-                load_half(ku, p + P.N, row < P.M, col0 + next, P.N);
-              }
-              const uint32_t* const gw = reinterpret_cast<const uint32_t*>(cg);
-              const uint32_t* const uw = reinterpret_cast<const uint32_t*>(cu);
+          for (int q = 0; q < 4; ++q) {
+            const uint4 gv = lds(chunk32(g0, lane, q)), uv = lds(chunk32(u0, lane, q));
+            const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+            uint32_t dg[4], du[4];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float d0, d1;
-                const float a0 = act_value_grad<true>(bf16_lo(gw[i]), P.act, d0), a1 = act_value_grad<true>(bf16_hi(gw[i]), P.act, d1);
-                w[i] = pack(v[2 * i] * bf16_lo(uw[i]) * d0, v[2 * i + 1] * bf16_hi(uw[i]) * d1);
-                later[half][i] = pack(v[2 * i] * a0, v[2 * i + 1] * a1);
-              }
+            for (int j = 0; j < 4; ++j) {
+              float d0, d1;
+              const float a0 = act_grad_fast<ACT>(bf16_lo(gw[j]), d0), a1 = act_grad_fast<ACT>(bf16_hi(gw[j]), d1);
+              const float h0 = v[q * 8 + 2 * j], h1 = v[q * 8 + 2 * j + 1];
+              dg[j] = pack(h0 * bf16_lo(uw[j]) * d0, h1 * bf16_hi(uw[j]) * d1);
+              du[j] = pack(h0 * a0, h1 * a1);
             }
-            stage_half(mine, lane, half, w);
+            sts(chunk32(g0, lane, q), dg);
+            sts(chunk32(u0, lane, q), du);
           }
           fence_async();
           __syncwarp();
-          const int x = static_cast<int>(col0) + c0;
-          const bool store = lane == 0 && x < P.N && row0 < P.M;  // a box wholly outside is not started
           if (store) {
-            if (EPI == kPlain) tma_store_2d(&maps.out, mine, x, row0);
-            else tma_store_3d(&maps.out, mine, x, 0, row0);
+            tma_store_3d(&maps.out, g0, x, 0, row0);
+            tma_store_3d(&maps.out, u0, x, 1, row0);
             bulk_commit();
           }
-          if (EPI == kDgate) {
-            if (lane == 0) bulk_wait_read();
-            __syncwarp();
-            stage_half(mine, lane, 0, later[0]);
-            stage_half(mine, lane, 1, later[1]);
-            fence_async();
-            __syncwarp();
-            if (store) {
-              tma_store_3d(&maps.out, mine, x, 1, row0);
-              bulk_commit();
-            }
+          if (i + 2 < last && lane == 0) {
+            bulk_wait_read<0>();
+            fetch(turn + 2, i + 2);
           }
+        } else if (EPI == kGate) {
+          // the staging tiles in turn: h, g, u of this step (kept), or h alone
+          float u[32];
+          tmem_ld32(acc + half + c, u);
+          if (P.bias) {
+            add_bias(v, P.bias, x, P.N);
+            add_bias(u, P.bias + P.N, x, P.N);
+          }
+          if (P.keep) {
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+            stage(mine, lane, v);
+            stage(mine + kTile, lane, u);
+          } else {
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = act_fast<ACT>(v[j]) * u[j];
+          const uint32_t to = mine + (2 + (turn & 1)) * kTile;
+          stage(to, lane, v);
+          fence_async();
+          __syncwarp();
+          if (store) {
+            if (P.keep) {
+              tma_store_3d(&maps.gu, mine, x, 0, row0);
+              tma_store_3d(&maps.gu, mine + kTile, x, 1, row0);
+            }
+            tma_store_2d(&maps.out, to, x, row0);
+          }
+          if (lane == 0) bulk_commit();
+        } else {
+          if (P.bias) add_bias(v, P.bias, x, P.N);
+          if (lane == 0) bulk_wait_read<3>();
+          __syncwarp();
+          const uint32_t to = mine + (turn & 3) * kTile;
+          stage(to, lane, v);
+          fence_async();
+          __syncwarp();
+          if (store) tma_store_2d(&maps.out, to, x, row0);
+          if (lane == 0) bulk_commit();
         }
       }
+      if (!alive) break;
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(tempty + 8 * buf);
+      if (lane == 0) arrive_first(tempty + 8 * buf);
       buf ^= 1;
       if (buf == 0) tph ^= 1;
     }
-    if (lane == 0) bulk_wait_all();
+    if (lane == 0) {
+      if (EPI == kDgate && *dead) {  // fetches may still be in flight: those of the next two steps
+        const long long since = clock64();
+        for (uint32_t i = turn; i < turn + 2; ++i)
+          while (!mbar_try(mykept + 8 * (i & 1), (i >> 1) & 1) && clock64() - since < kWaitClocks / 4) {
+          }
+      }
+      bulk_wait_all();
+    }
     __syncwarp();
   }
   fence_before();
   __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may still read its operands or arrive at its barriers
   if (warp == 1) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAcc));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kAcc));
+  }
+}
+
+// ------------------------------------------------------------------------------------------ join
+
+// Epilogue of the tiles that were cut along k: a warp adds up the parts of 32 rows x 8 columns, four parts' loads
+// in flight, always in their order.
+struct JoinArgs {
+  Args tc;
+  __nv_bfloat16* out;
+  const __nv_bfloat16* gu;
+  __nv_bfloat16* gu_out;
+  long long ldo;
+};
+
+__device__ __forceinline__ void add_parts(const Args& P, int tail, int rank, int quad, int block, int col, int lane, float (&v)[8]) {
+  const size_t hop = static_cast<size_t>(8) * (P.bn / 32) * 1024;  // from a part to the next
+  const float* from = P.partial + (static_cast<size_t>((tail * P.parts * 2 + rank) * 4 + quad) * (P.bn / 32) + block) * 1024 + col * 32 + lane;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  for (int s = 0; s < P.parts; s += 4) {
+    float t[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[u][j] = s + u < P.parts ? __ldg(from + (s + u) * hop + j * 32) : 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[u][j];
+  }
+}
+__device__ __forceinline__ void add_bias8(float (&v)[8], const __nv_bfloat16* bias) {
+  const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias));
+  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] += bf16_lo(w[i]);
+    v[2 * i + 1] += bf16_hi(w[i]);
+  }
+}
+__device__ __forceinline__ void put8(__nv_bfloat16* to, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(to) = make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
+}
+
+template <int EPI, int ACT>
+__global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ JoinArgs J) {
+  const Args& P = J.tc;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = P.bn / 2, width = EPI == kGate ? half : P.bn, steps = width / 32;
+  const int quad = warp & 3, col = (warp >> 2) * 8, rank = blockIdx.y, tail = blockIdx.x / steps, i = blockIdx.x - tail * steps;
+  int m, n;
+  tile_at(P, P.full + tail, m, n);
+  const long long row = (2LL * m + rank) * kBM + quad * 32 + lane;
+  const int x = n * width + i * 32 + col;
+  if (x >= P.N || (2LL * m + rank) * kBM + quad * 32 >= P.M) return;  // N is a multiple of 8
+  float v[8], u[8];
+  add_parts(P, tail, rank, quad, i, col, lane, v);
+  if (EPI == kGate) add_parts(P, tail, rank, quad, steps + i, col, lane, u);
+  if (EPI != kDgate && P.bias) add_bias8(v, P.bias + x);
+  if (EPI == kGate && P.bias) add_bias8(u, P.bias + P.N + x);
+  if (row >= P.M) return;
+  if (EPI == kGate) {
+    if (J.gu_out) {
+      put8(J.gu_out + row * 2 * P.N + x, v);
+      put8(J.gu_out + row * 2 * P.N + P.N + x, u);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act_fast<ACT>(v[j]) * u[j];
+  }
+  if (EPI == kDgate) {
+    const __nv_bfloat16* const kept = J.gu + row * 2 * P.N + x;
+    const uint4 gv = __ldg(reinterpret_cast<const uint4*>(kept)), uv = __ldg(reinterpret_cast<const uint4*>(kept + P.N));
+    const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float d0, d1;
+      const float a0 = act_grad_fast<ACT>(bf16_lo(gw[j]), d0), a1 = act_grad_fast<ACT>(bf16_hi(gw[j]), d1);
+      u[2 * j] = v[2 * j] * a0;
+      u[2 * j + 1] = v[2 * j + 1] * a1;
+      v[2 * j] = v[2 * j] * bf16_lo(uw[j]) * d0;
+      v[2 * j + 1] = v[2 * j + 1] * bf16_hi(uw[j]) * d1;
+    }
+    put8(J.out + row * 2 * P.N + x, v);
+    put8(J.out + row * 2 * P.N + P.N + x, u);
+  } else {
+    put8(J.out + row * J.ldo + x, v);
   }
 }
 
@@ -429,88 +605,122 @@ Encode encoder() {
   return encode;
 }
 
-// Map of a bf16 matrix [rows, cols] with row stride ld: boxes of 64 columns x `box` rows, 128-byte swizzle.
-bool matrix_map(CUtensorMap* map, const void* p, long long rows, long long cols, long long ld, int box) {
+// Map of a bf16 matrix [rows, cols] with row stride ld: boxes of `box` rows x 64 columns (128-byte swizzle) or 32 (64).
+bool matrix_map(CUtensorMap* map, const void* p, long long rows, long long cols, long long ld, int box, int width = 64) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-  const cuuint32_t boxes[2] = {64, static_cast<cuuint32_t>(box)}, steps[2] = {1, 1};
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(width), static_cast<cuuint32_t>(box)}, steps[2] = {1, 1};
   return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                   width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Map of two matrices side by side, [rows, 2, cols] contiguous, that clips each at its own columns.
-bool pair_map(CUtensorMap* map, const void* p, long long rows, long long cols, int box) {
+// Map of two matrices side by side, [rows, 2, cols] contiguous, that clips each at its own columns: boxes of 32 rows
+// x 32 columns (64-byte swizzle).
+bool pair_map(CUtensorMap* map, const void* p, long long rows, long long cols) {
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), 2, static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols) * 2, static_cast<cuuint64_t>(cols) * 4};
-  const cuuint32_t boxes[3] = {64, 1, static_cast<cuuint32_t>(box)}, steps[3] = {1, 1, 1};
+  const cuuint32_t boxes[3] = {32, 1, 32}, steps[3] = {1, 1, 1};
   return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                   CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int EPI, int BN, int STAGES, bool AM, bool BM>
-cudaError_t launch(const Product& p, cudaStream_t s) {
-  constexpr int kBoxN = EPI == kGate ? BN / 2 : BN;
-  Maps maps;
-  bool ok = AM ? matrix_map(&maps.a, p.a, p.K, p.M, p.lda, kBK) : matrix_map(&maps.a, p.a, p.M, p.K, p.lda, kBM);
-  const long long brows = EPI == kGate ? 2 * p.N : p.N;
-  ok = ok && (BM ? matrix_map(&maps.b, p.b, p.K, p.N, p.ldb, kBK) : matrix_map(&maps.b, p.b, brows, p.K, p.ldb, kBoxN));
-  if (EPI == kDgate) ok = ok && pair_map(&maps.out, p.out, p.M, p.N, 32);
-  else ok = ok && matrix_map(&maps.out, p.out, p.M, p.N, p.ldo, 32);
-  maps.gu = maps.out;
-  if (EPI == kGate && p.gu_out) ok = ok && pair_map(&maps.gu, p.gu_out, p.M, p.N, 32);
-  if (!ok) return cudaErrorInvalidValue;
-  Args a{};
-  a.bias = static_cast<const __nv_bfloat16*>(p.bias);
-  a.gu = static_cast<const __nv_bfloat16*>(p.gu);
-  a.M = p.M;
-  a.N = p.N;
-  a.kblocks = static_cast<int>((p.K + kBK - 1) / kBK);
-  a.mt = static_cast<int>((p.M + kBM - 1) / kBM);
-  a.nt = static_cast<int>((p.N + kBoxN - 1) / kBoxN);
-  a.gm = a.mt <= 32 ? a.mt : 16;  // rows of tiles that go together: their operands stay in the L2 cache
-  a.act = p.act;
-  a.keep = p.gu_out != nullptr;
-  a.status = p.status;
-  constexpr int smem = 1024 + STAGES * (kStageA + BN * kBK * 2) + kEpiWarps * kStaging + 16 * STAGES + 64;
-  static_assert(smem <= 232448, "shared memory of a block");
-  auto* const kernel = product_kernel<EPI, BN, STAGES, AM, BM>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  const long long tiles = static_cast<long long>(a.mt) * a.nt;
-  const int grid = static_cast<int>(tiles < sm_count() ? tiles : sm_count());
-  kernel<<<grid, kThreads, smem, s>>>(maps, a);
-  return cudaGetLastError();
-}
+// How a product is cut: tiles of bn columns, `full` of them whole, the others in `parts` along k.
+struct Plan {
+  int bn, parts, kper;
+  long long mt, nt, full, items;
+  size_t bytes;
+};
 
-// Width of the tiles: the one whose rounds of all SMs cover the result with the least columns (a tile's time
-// goes by its columns, plus about 32 for what does not).
-int choose_bn(long long M, long long N, bool gate, std::initializer_list<int> widths) {
-  int best = 0;
+// The cheapest cut by what was measured (microseconds): a block of 64 k of a 256 x bn tile takes 0.23 + 0.00066
+// bn (B by boxes of 64 where its own axis is contiguous) whatever its neighbours do, the end of a round about 3
+// more, joining parts 7; a part has at least 4 blocks.
+Plan plan(long long M, long long N, long long K, bool gate, bool boxed) {
+  const long long pairs = sm_count() / 2, kblocks = (K + kBK - 1) / kBK;
+  Plan best{};
   double least = 0;
-  for (int bn : widths) {
-    const long long box = gate ? bn / 2 : bn;
-    const long long tiles = (M + kBM - 1) / kBM * ((N + box - 1) / box);
-    const double cost = static_cast<double>((tiles + sm_count() - 1) / sm_count()) * (bn + 32);
-    if (best == 0 || cost < least) {
-      best = bn;
+  for (int bn = 256; bn >= 64; bn -= gate ? 64 : 32) {
+    Plan p{};
+    const long long width = gate ? bn / 2 : bn;
+    p.bn = bn;
+    p.mt = (M + 2 * kBM - 1) / (2 * kBM);
+    p.nt = (N + width - 1) / width;
+    const long long tiles = p.mt * p.nt, tail = tiles % pairs;
+    const double block = 0.23 + 0.00066 * (boxed ? (bn / 2 + 63) / 64 * 128 : bn) + 0.0001 * bn;
+    for (long long parts = 1; parts == 1 || (tail > 0 && parts <= pairs / tail && parts <= 32); ++parts) {
+      const long long kper = (kblocks + parts - 1) / parts;
+      if (parts > 1 && (kper < 4 || (kblocks + kper - 1) / kper != parts)) continue;
+      const double rounds = static_cast<double>(tiles / pairs) + (tail == 0 ? 0.0 : parts == 1 ? 1.0 : static_cast<double>(kper) / kblocks);
+      const double cost = rounds * kblocks * block + 3.0 + (parts > 1 ? 7.0 : 0.0);
+      if (least != 0 && cost >= least) continue;
       least = cost;
+      p.parts = static_cast<int>(parts);
+      p.kper = static_cast<int>(kper);
+      p.full = parts == 1 ? tiles : tiles - tail;
+      p.items = p.full + (parts == 1 ? 0 : tail * parts);
+      p.bytes = sizeof(float) * static_cast<size_t>(p.items - p.full) * 2 * kBM * bn;
+      best = p;
     }
   }
   return best;
 }
 
-template <int EPI, bool AM, bool BM>
-cudaError_t by_width(const Product& p, cudaStream_t s) {
-  if constexpr (EPI == kGate) {
-    if (choose_bn(p.M, p.N, true, {256, 128}) == 256) return launch<EPI, 256, 4, AM, BM>(p, s);
-    return launch<EPI, 128, 6, AM, BM>(p, s);
-  } else {
-    switch (choose_bn(p.M, p.N, false, {256, 192, 128})) {
-      case 256: return launch<EPI, 256, 4, AM, BM>(p, s);
-      case 192: return launch<EPI, 192, 4, AM, BM>(p, s);
-      default: return launch<EPI, 128, 6, AM, BM>(p, s);
-    }
-  }
+template <int EPI, bool AM, bool BM, int ACT>
+cudaError_t launch(const Product& p, cudaStream_t s) {
+  const Plan cut = plan(p.M, p.N, p.K, EPI == kGate, BM);
+  if (cut.bytes > p.partial_bytes) return cudaErrorInvalidValue;
+  Args a{};
+  a.bn = cut.bn;
+  a.full = static_cast<int>(cut.full);
+  a.items = static_cast<int>(cut.items);
+  a.parts = cut.parts;
+  a.kper = cut.kper;
+  a.partial = p.partial;
+  a.boxes = (a.bn / 2 + 63) / 64;
+  a.stage_bytes = kStageA + (BM ? a.boxes * 8192 : a.bn / 2 * kBK * 2);
+  // stages start on the swizzle's 1024 bytes: half of B is a multiple of 16 rows of 128 bytes
+  a.stages = kRing / a.stage_bytes < kMaxStages ? kRing / a.stage_bytes : kMaxStages;
+  Maps maps;
+  bool ok = AM ? matrix_map(&maps.a, p.a, p.K, p.M, p.lda, kBK) : matrix_map(&maps.a, p.a, p.M, p.K, p.lda, kBM);
+  const long long brows = EPI == kGate ? 2 * p.N : p.N;
+  ok = ok && (BM ? matrix_map(&maps.b, p.b, p.K, p.N, p.ldb, kBK) : matrix_map(&maps.b, p.b, brows, p.K, p.ldb, a.bn / 2));
+  if (EPI == kDgate) ok = ok && pair_map(&maps.out, p.out, p.M, p.N) && pair_map(&maps.gu, p.gu, p.M, p.N);
+  else ok = ok && matrix_map(&maps.out, p.out, p.M, p.N, p.ldo, 32, 32);
+  if (EPI == kGate && p.gu_out) ok = ok && pair_map(&maps.gu, p.gu_out, p.M, p.N);
+  else if (EPI != kDgate) maps.gu = maps.out;
+  if (!ok) return cudaErrorInvalidValue;
+  a.bias = static_cast<const __nv_bfloat16*>(p.bias);
+  a.M = p.M;
+  a.N = p.N;
+  a.kblocks = static_cast<int>((p.K + kBK - 1) / kBK);
+  a.mt = static_cast<int>(cut.mt);
+  a.nt = static_cast<int>(cut.nt);
+  a.gm = a.mt <= 16 ? a.mt : 8;  // rows of tiles that go together: their operands stay in the L2 cache
+  a.keep = p.gu_out != nullptr;
+  a.status = p.status;
+  constexpr int smem = 1024 + kRing + kEpiWarps * kStaging + 24 * kMaxStages + 16 * kEpiWarps + 64;
+  static_assert(smem <= 232448, "shared memory of a block");
+  auto* const kernel = product_kernel<EPI, AM, BM, ACT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int pairs = sm_count() / 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * (a.items < pairs ? a.items : pairs)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, maps, a);
+  if (e != cudaSuccess || a.items == a.full) return e;
+  JoinArgs j{a, static_cast<__nv_bfloat16*>(p.out), static_cast<const __nv_bfloat16*>(p.gu), static_cast<__nv_bfloat16*>(p.gu_out), p.ldo};
+  const int steps = (EPI == kGate ? a.bn / 2 : a.bn) / 32;
+  join_kernel<EPI, ACT><<<dim3((a.mt * a.nt - a.full) * steps, 2), 512, 0, s>>>(j);
+  count_launches(1);
+  return cudaGetLastError();
 }
 
 }  // namespace tc
@@ -526,13 +736,20 @@ bool tc_applies(const Product& p) {
   return true;
 }
 
+size_t tc_partial_bytes(long long M, long long N, long long K, int epilogue, bool b_major) {
+  return tc::plan(M, N, K, epilogue == kGate, b_major).bytes;
+}
+
 cudaError_t launch_product_tc(const Product& p, cudaStream_t s) {
+  const bool silu = p.act == MSL_ACT_SILU;
   switch (p.epilogue) {
-    case kGate: return tc::by_width<kGate, false, false>(p, s);
-    case kDgate: return tc::by_width<kDgate, false, true>(p, s);
+    case kGate:
+      return silu ? tc::launch<kGate, false, false, MSL_ACT_SILU>(p, s) : tc::launch<kGate, false, false, MSL_ACT_GELU>(p, s);
+    case kDgate:
+      return silu ? tc::launch<kDgate, false, true, MSL_ACT_SILU>(p, s) : tc::launch<kDgate, false, true, MSL_ACT_GELU>(p, s);
     default:
-      if (p.a_major) return tc::by_width<kPlain, true, true>(p, s);
-      return p.b_major ? tc::by_width<kPlain, false, true>(p, s) : tc::by_width<kPlain, false, false>(p, s);
+      if (p.a_major) return tc::launch<kPlain, true, true, 0>(p, s);
+      return p.b_major ? tc::launch<kPlain, false, true, 0>(p, s) : tc::launch<kPlain, false, false, 0>(p, s);
   }
 }
 

@@ -61,24 +61,50 @@ __device__ __forceinline__ void sum_span(const T* p, int n, float& acc) {
 }
 
 template <typename T>
+__device__ __forceinline__ uint4 scaled(uint4 w, float c) {
+  T* const e = reinterpret_cast<T*>(&w);
+#pragma unroll
+  for (int j = 0; j < 16 / static_cast<int>(sizeof(T)); ++j) e[j] = from_f32<T>(to_f32<T>(e[j]) * c);
+  return w;
+}
+
+// 16 bytes from `shift` bytes into two adjacent aligned 16-byte words (shift a multiple of 2, 0 < shift < 16)
+__device__ __forceinline__ uint4 window(uint4 a, uint4 b, int shift) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t t[5], o[4];
+  const int words = shift >> 2, bits = (shift & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) t[i] = words == 0 ? w[i] : words == 1 ? w[i + 1] : words == 2 ? w[i + 2] : w[i + 3 < 8 ? i + 3 : 7];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(t[i], t[i + 1], bits);
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Stores are whole aligned 16-byte words.  Where the source is not aligned alike, each word comes out of two
+// aligned loads of the source (the second is the neighbour's first: it hits L1).
+template <typename T>
 __device__ __forceinline__ void scale_span(const T* p, T* o, int n, float c) {
   constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-  int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
+  const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(o) & 15)) & 15) / sizeof(T)));
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p + head) & 15);
+  // the two loads of a word stay inside the span: one word less where the last would reach past it, and the
+  // first is done apart where its loads would begin before it
+  const int before = shift != 0 && head * static_cast<int>(sizeof(T)) < shift ? 1 : 0;
   int nv = (n - head) / kPer;
-  if ((reinterpret_cast<uintptr_t>(o + head) & 15) != 0) nv = 0;  // source and result are not aligned alike
-  for (int i = threadIdx.x; i < head; i += kThreads) o[i] = from_f32<T>(to_f32<T>(p[i]) * c);
-  const uint4* const q = reinterpret_cast<const uint4*>(p + head);
-  uint4* const r = reinterpret_cast<uint4*>(o + head);
+  if (shift != 0 && nv > 0 && (n - head - nv * kPer) * static_cast<int>(sizeof(T)) < 16 - shift) --nv;
+  const int start = min(head + before * kPer, n);  // elements before the words
+  nv = max(nv - before, 0);
+  for (int i = threadIdx.x; i < start; i += kThreads) o[i] = from_f32<T>(to_f32<T>(p[i]) * c);
+  uint4* const r = reinterpret_cast<uint4*>(o + start);
+  const uint4* const q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p + start) - shift);
+  if (shift == 0) {
 #pragma unroll 4
-  for (int i = threadIdx.x; i < nv; i += kThreads) {
-    uint4 w = q[i];
-    T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) e[j] = from_f32<T>(to_f32<T>(e[j]) * c);
-    r[i] = w;
+    for (int i = threadIdx.x; i < nv; i += kThreads) r[i] = scaled<T>(q[i], c);
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += kThreads) r[i] = scaled<T>(window(q[i], q[i + 1], shift), c);
   }
-#pragma unroll 4
-  for (int i = head + nv * kPer + threadIdx.x; i < n; i += kThreads) o[i] = from_f32<T>(to_f32<T>(p[i]) * c);
+  for (int i = start + nv * kPer + threadIdx.x; i < n; i += kThreads) o[i] = from_f32<T>(to_f32<T>(p[i]) * c);
 }
 
 __device__ __forceinline__ double block_sum(double v) {
