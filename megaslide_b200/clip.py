@@ -16,9 +16,10 @@ Tensors = Union[Tensor, Iterable[Optional[Tensor]]]
 
 def _list(tensors: Tensors) -> List[Tensor]:
     """The tensors of a call; of parameters (which require gradients) their gradients, where they have one."""
-    ts = [tensors] if isinstance(tensors, Tensor) else [t for t in tensors if t is not None]
-    return [t.detach() if not isinstance(t, torch.nn.Parameter) else t.grad for t in ts
-            if not isinstance(t, torch.nn.Parameter) or t.grad is not None]
+    ts = [tensors] if isinstance(tensors, Tensor) else tensors
+    # plain tensors first: isinstance of Parameter runs a check in Python
+    ts = [t if type(t) is Tensor else t.grad if isinstance(t, torch.nn.Parameter) else t for t in ts if t is not None]
+    return [t for t in ts if t is not None]
 
 
 def _check(extra_sumsq: float) -> float:

@@ -21,37 +21,31 @@ from . import ops
 
 
 def _rows_of(x: Tensor) -> Tensor:
-    """[..., C] as a [rows, C] row view (a copy where the strides allow none)."""
+    """[..., C] whose rows lie at one stride: x, a row view of it, or a copy where its strides have none."""
+    if x.is_contiguous():
+        return x
     x2 = x.reshape(-1, x.shape[-1])
     if (x2.stride(1) != 1 and x2.shape[1] > 1) or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
         x2 = x2.contiguous()
     return x2
 
 
-def _status(dev: torch.device):
-    sw = ops.status_word(dev)
-    sw.poll()
-    return sw
-
-
 class GatedFFNFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, activation):
         x2 = _rows_of(x)
-        y, h, gu = ops.gated_ffn_fwd(x2, w_in, w_out, b_in, b_out, activation, keep=True, status=ops.status_word(x.device).word)
+        y, h, gu = ops.gated_ffn_fwd(x2, w_in, w_out, b_in, b_out, activation, keep=True)
         ctx.save_for_backward(x2, w_in, w_out, b_in, b_out, h, gu)
         ctx.activation = activation
         ctx.x_shape = x.shape
-        return y.view(x.shape)
+        return y if y.shape == x.shape else y.view(x.shape)
 
     @staticmethod
     def backward(ctx, dy):
         x2, w_in, w_out, b_in, b_out, h, gu = ctx.saved_tensors
-        sw = _status(x2.device)
         dx, dw_in, dw_out, db_in, db_out = ops.gated_ffn_bwd(x2, w_in, w_out, h, gu, _rows_of(dy), b_in, b_out, ctx.activation,
-                                                             needs=ctx.needs_input_grad[:5], status=sw.word)
-        sw.post()
-        return dx.view(ctx.x_shape) if dx is not None else None, dw_in, dw_out, db_in, db_out, None
+                                                             needs=ctx.needs_input_grad[:5])
+        return dx.view(ctx.x_shape) if dx is not None and dx.shape != ctx.x_shape else dx, dw_in, dw_out, db_in, db_out, None
 
 
 def gated_ffn(x: Tensor, w_in: Tensor, w_out: Tensor, b_in: Optional[Tensor] = None, b_out: Optional[Tensor] = None,
@@ -65,7 +59,8 @@ def gated_ffn(x: Tensor, w_in: Tensor, w_out: Tensor, b_in: Optional[Tensor] = N
     ops.dtype_code(x.dtype)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out)):
         return GatedFFNFunction.apply(x, w_in, w_out, b_in, b_out, activation)
-    return ops.gated_ffn_fwd(_rows_of(x), w_in, w_out, b_in, b_out, activation, status=ops.status_word(x.device).word)[0].view(x.shape)
+    y = ops.gated_ffn_fwd(_rows_of(x), w_in, w_out, b_in, b_out, activation)[0]
+    return y if y.shape == x.shape else y.view(x.shape)
 
 
 class GatedMLP(nn.Module):

@@ -11,6 +11,7 @@ import ctypes
 import math
 from contextlib import contextmanager, nullcontext
 from dataclasses import dataclass
+from operator import attrgetter
 from typing import List, Optional, Tuple
 
 import torch
@@ -76,11 +77,11 @@ class StatusWord:
     """The per-device status word the attention kernels OR their MSL_STATUS_* bits into (device int32),
     read back without stalling the host: after every call an asynchronous copy into pinned memory is
     enqueued with an event, and the next call (poll) reads that copy once its event has completed.  A
-    halo miss, a timed-out TMA wait or a position outside its axis (results not valid) raises MslError there, at most one call late;
+    halo miss or a timed-out TMA wait (results not valid) raises MslError there, at most one call late;
     check() reads the word synchronously.  MSL_STATUS_TC_RANGE is informational (the kernels computed
     such tiles with the CUDA-core gather)."""
 
-    BAD = _lib.MSL_STATUS_HALO_MISS | _lib.MSL_STATUS_TIMEOUT | _lib.MSL_STATUS_ROTARY_INDEX
+    BAD = _lib.MSL_STATUS_HALO_MISS | _lib.MSL_STATUS_TIMEOUT
 
     def __init__(self, device: torch.device):
         self.word = torch.zeros(1, dtype=torch.int32, device=device)
@@ -103,11 +104,6 @@ class StatusWord:
                 what.append("a sample corner fell outside the K/V frames the call was given (halo miss)")
             if v & _lib.MSL_STATUS_TIMEOUT:
                 what.append("a tensor-core CTA's TMA copies did not complete within a second")
-            if v & _lib.MSL_STATUS_ROTARY_INDEX:
-                what.append("a rotary position index was outside its axis")
-            if v & self.BAD == _lib.MSL_STATUS_ROTARY_INDEX:
-                raise _lib.MslError("msl_rope3d / msl_qk_norm_rope", _lib.MSL_ERR_CUDA,
-                                    "a previous call produced invalid results: " + "; ".join(what))
             raise _lib.MslError("msl_dsa_attn", _lib.MSL_ERR_CUDA,
                                 "a previous attention call produced invalid results: " + "; ".join(what))
 
@@ -137,10 +133,49 @@ def status_word(device: torch.device) -> StatusWord:
     return sw
 
 
+class HostFlag:
+    """The status word of the operators around the attention (rotary positions, feed-forward): one pinned host
+    word per device that their kernels write only when something went wrong, so a good call costs nothing.
+    The next call that finds a bit set raises MslError (the failed call's results are not valid)."""
+
+    def __init__(self):
+        self.word = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.ptr = self.word.data_ptr()
+        self._view = self.word.numpy()
+
+    def poll(self) -> None:
+        v = self._view[0]
+        if v:
+            self._view[0] = 0
+            what = []
+            if v & _lib.MSL_STATUS_ROTARY_INDEX:
+                what.append("a rotary position index was outside its axis (msl_rope3d, msl_qk_norm_rope)")
+            if v & _lib.MSL_STATUS_TIMEOUT:
+                what.append("operand copies of a matrix product did not complete within seconds (msl_gated_ffn)")
+            raise _lib.MslError("a previous call", _lib.MSL_ERR_CUDA, "its results are not valid: " + "; ".join(what))
+
+
+_FLAGS: dict = {}
+
+
+def host_flag(device: torch.device) -> HostFlag:
+    """The process-wide HostFlag of a CUDA device."""
+    f = _FLAGS.get(device.index)
+    if f is None:
+        f = _FLAGS[device.index] = HostFlag()
+    return f
+
+
 def check_status(device=None) -> int:
-    """Synchronously checks the attention kernels' status word of `device` (default: current): raises
-    MslError if a call produced invalid results, else returns the informational bits seen so far."""
-    return status_word(device if device is not None else torch.device("cuda", torch.cuda.current_device())).check()
+    """Synchronously checks the kernels' status words of `device` (default: current): raises MslError if a call
+    produced invalid results, else returns the attention kernels' informational bits seen so far."""
+    dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    bits = status_word(dev).check()
+    torch.cuda.synchronize(dev)
+    for index, flag in _FLAGS.items():
+        if index == (dev.index if dev.index is not None else torch.cuda.current_device()):
+            flag.poll()
+    return bits
 
 
 def _need_cuda(*ts):
@@ -473,6 +508,7 @@ def convert_f32(src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
 
 
 _HERE = nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: current_stream() builds an object, 2 us a call
 
 
 def _on(dev: torch.device):
@@ -480,34 +516,48 @@ def _on(dev: torch.device):
     return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-@dataclass(frozen=True)
-class RotaryShape:
-    """Geometry of a rotary call (mirrors ``msl_rotary_geometry``): `tokens` of each of `batch` samples, the
-    table's extents (frames, height, width), the channels each axis turns, the heads' width."""
+def _ld(t: torch.Tensor, name: str) -> int:
+    """Row stride (elements) of rows of t.shape[-1]: of contiguous tensors of any shape, of row views [rows, C] and of
+    [B, N, C] whose samples follow one another at the rows' stride."""
+    if t.is_contiguous():
+        return t.shape[-1]
+    if t.dim() == 3:
+        B, N, C = t.shape
+        sb, sn, sc = t.stride()
+        if (sc == 1 or C == 1) and (B == 1 or N == 1 or sb == N * sn):
+            ld = sn if N > 1 else sb
+            if ld >= C:
+                return ld
+        raise ValueError(f"{name} must be rows at one stride, got shape {tuple(t.shape)} strides {t.stride()}")
+    return _rows(t, name)
 
-    batch: int
-    tokens: int
-    video_shape: Tuple[int, int, int]
-    axes: Tuple[int, int, int]
-    head_dim: int
-    frame0: int = 0
-    interleaved: bool = True
+
+class RotaryShape:
+    """Geometry of a rotary call (``msl_rotary_geometry``): `tokens` of each of `batch` samples, the table's extents
+    (frames, height, width), the channels each axis turns, the heads' width."""
+
+    __slots__ = ("batch", "tokens", "video_shape", "axes", "head_dim", "table_pairs", "_geom")
+
+    def __init__(self, batch: int, tokens: int, video_shape: Tuple[int, int, int], axes: Tuple[int, int, int], head_dim: int,
+                 frame0: int = 0, interleaved: bool = True):
+        t, h, w = video_shape
+        at, ah, aw = axes
+        self.batch, self.tokens, self.video_shape, self.axes, self.head_dim = batch, tokens, video_shape, axes, head_dim
+        self.table_pairs = (t * at + h * ah + w * aw) // 2
+        self._geom = _lib.RotaryGeometry(batch * tokens, tokens or 1, t, h, w, frame0, at, ah, aw, head_dim, 1 if interleaved else 0, 0)
 
     def geometry(self, dtype: torch.dtype) -> "_lib.RotaryGeometry":
-        t, h, w = self.video_shape
-        at, ah, aw = self.axes
-        return _lib.RotaryGeometry(self.batch * self.tokens, max(self.tokens, 1), t, h, w, self.frame0, at, ah, aw, self.head_dim,
-                                   1 if self.interleaved else 0, dtype_code(dtype))
+        self._geom.dtype = dtype_code(dtype)
+        return self._geom
 
 
 def _check_positions(shape: RotaryShape, table: Optional[torch.Tensor], index: Optional[torch.Tensor], dev: torch.device) -> int:
     """Checks a rotary call's table and index; returns the rows of the index (0 without one)."""
     if table is None:
         return 0
-    (t, h, w), (at, ah, aw) = shape.video_shape, shape.axes
-    want = (t * at + h * ah + w * aw) // 2
-    if table.dtype != torch.float32 or table.numel() != 2 * want or not table.is_contiguous():
-        raise ValueError(f"table must be a contiguous float32 tensor of {want} (cos, sin) pairs (rotary_table), got {tuple(table.shape)} {table.dtype}")
+    if table.dtype != torch.float32 or table.numel() != 2 * shape.table_pairs or not table.is_contiguous():
+        raise ValueError(f"table must be a contiguous float32 tensor of {shape.table_pairs} (cos, sin) pairs (rotary_table), "
+                         f"got {tuple(table.shape)} {table.dtype}")
     if table.device != dev:
         raise RuntimeError("table must be on the tokens' CUDA device")
     if index is None:
@@ -522,25 +572,39 @@ def _check_positions(shape: RotaryShape, table: Optional[torch.Tensor], index: O
     return rows
 
 
+def _flag(dev: torch.device, status: Optional[torch.Tensor]) -> int:
+    """Address a kernel reports to: the caller's device word, or the device's HostFlag (which raises here if an
+    earlier call has reported)."""
+    if status is not None:
+        return status.data_ptr()
+    f = _FLAGS.get(dev.index) or host_flag(dev)
+    f.poll()
+    return f.ptr
+
+
 def rope3d(shape: RotaryShape, heads: int, x: torch.Tensor, table: torch.Tensor, index: Optional[torch.Tensor] = None,
            inverse: bool = False, out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Rotates the heads of x [rows, >= heads*head_dim] (row view) by their tokens' positions; ``inverse`` turns
-    back, which is the backward pass.  ``out`` may be x."""
+    """Rotates the heads of x [rows, >= heads*head_dim] (row view; or [B, N, C] at one row stride) by their tokens' positions; ``inverse`` turns
+    back, which is the backward pass.  ``out`` may be x.  status: a device word for MSL_STATUS_ROTARY_INDEX in
+    place of the device's HostFlag."""
     _need_cuda(x, table, index)
-    index_rows = _check_positions(shape, table, index, x.device)
+    dev = x.device
+    index_rows = _check_positions(shape, table, index, dev)
     if out is None:
-        out = torch.empty(x.shape[0], heads * shape.head_dim, device=x.device, dtype=x.dtype)
+        out = torch.empty(*x.shape[:-1], heads * shape.head_dim, device=dev, dtype=x.dtype)
     g = shape.geometry(x.dtype)
-    with _on(x.device):
-        rc = _call("msl_rope3d", x.device, lambda: _lib.load().msl_rope3d(
-            ctypes.byref(g), heads, _ptr(x), _rows(x, "x"), _ptr(table), _ptr(index), index_rows, 1 if inverse else 0,
-            _ptr(out), _rows(out, "out"), _ptr(status), _stream(x.device)))
+    flag = _flag(dev, status) if index is not None else None
+    with _on(dev):
+        rc = _call("msl_rope3d", dev, lambda: _lib.load().msl_rope3d(
+            ctypes.byref(g), heads, x.data_ptr(), _ld(x, "x"), table.data_ptr(), _ptr(index), index_rows, 1 if inverse else 0,
+            out.data_ptr(), _ld(out, "out"), flag, _raw_stream(dev.index)))
     _lib.check("msl_rope3d", rc)
     return out
 
 
 def _qk_io(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weight, k_weight, eps, table, index, status) -> "_lib.QkNormIO":
     _need_cuda(q, k, q_weight, k_weight, table, index)
+    dev = q.device
     if k is not None and k.dtype != q.dtype:
         raise TypeError(f"q and k must have the same dtype, got {q.dtype} and {k.dtype}")
     wdt = torch.float32
@@ -549,18 +613,15 @@ def _qk_io(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weight, k_weig
             continue
         if w.numel() != shape.head_dim or not w.is_contiguous():
             raise ValueError(f"{nm} must be a contiguous tensor of head_dim = {shape.head_dim} elements, got {tuple(w.shape)}")
+        if w.device != dev:
+            raise RuntimeError(f"{nm} must be on q's CUDA device")
         wdt = w.dtype
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise TypeError("q_weight and k_weight must have the same dtype")
-    io = _lib.QkNormIO()
-    io.index_rows = _check_positions(shape, table, index, q.device)
-    io.q, io.q_ld = _ptr(q), _rows(q, "q")
-    if kv_heads:
-        io.k, io.k_ld = _ptr(k), _rows(k, "k")
-    io.q_weight, io.k_weight = _ptr(q_weight), _ptr(k_weight)
-    io.table, io.index, io.status = _ptr(table), _ptr(index), _ptr(status)
-    io.heads, io.kv_heads, io.weight_dtype, io.eps = heads, kv_heads, dtype_code(wdt), eps
-    return io
+    return _lib.QkNormIO(
+        q.data_ptr(), _ld(q, "q"), _ptr(k) if kv_heads else None, _ld(k, "k") if kv_heads else 0, _ptr(q_weight), _ptr(k_weight),
+        None, 0, None, 0, _ptr(table), _ptr(index), _check_positions(shape, table, index, dev),
+        _flag(dev, status) if index is not None else None, heads, kv_heads, dtype_code(wdt), eps)
 
 
 def qk_norm_rope_fwd(shape: RotaryShape, heads: int, kv_heads: int, q: torch.Tensor, k: Optional[torch.Tensor],
@@ -570,19 +631,20 @@ def qk_norm_rope_fwd(shape: RotaryShape, heads: int, kv_heads: int, q: torch.Ten
                      status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """RMS norm of every head of q [rows, >= heads*head_dim] and k [rows, >= kv_heads*head_dim] (row views) times
     the weights (None = ones), then the rotation (none without a table).  q_out / k_out may be q / k; kv_heads = 0
-    takes q alone."""
+    takes q alone.  status as in rope3d."""
     io = _qk_io(shape, heads, kv_heads, q, k, q_weight, k_weight, eps, table, index, status)
+    dev = q.device
     if q_out is None:
-        q_out = torch.empty(q.shape[0], heads * shape.head_dim, device=q.device, dtype=q.dtype)
-    io.q_out, io.q_out_ld = _ptr(q_out), _rows(q_out, "q_out")
+        q_out = torch.empty(*q.shape[:-1], heads * shape.head_dim, device=dev, dtype=q.dtype)
+    io.q_out, io.q_out_ld = q_out.data_ptr(), _ld(q_out, "q_out")
     if kv_heads:
         if k_out is None:
-            k_out = torch.empty(k.shape[0], kv_heads * shape.head_dim, device=k.device, dtype=k.dtype)
-        io.k_out, io.k_out_ld = _ptr(k_out), _rows(k_out, "k_out")
+            k_out = torch.empty(*k.shape[:-1], kv_heads * shape.head_dim, device=dev, dtype=k.dtype)
+        io.k_out, io.k_out_ld = k_out.data_ptr(), _ld(k_out, "k_out")
     g = shape.geometry(q.dtype)
-    with _on(q.device):
-        rc = _call("msl_qk_norm_rope_fwd", q.device, lambda: _lib.load().msl_qk_norm_rope_fwd(
-            ctypes.byref(g), ctypes.byref(io), _stream(q.device)))
+    with _on(dev):
+        rc = _call("msl_qk_norm_rope_fwd", dev, lambda: _lib.load().msl_qk_norm_rope_fwd(
+            ctypes.byref(g), ctypes.byref(io), _raw_stream(dev.index)))
     _lib.check("msl_qk_norm_rope_fwd", rc)
     return q_out, k_out
 
@@ -593,23 +655,24 @@ def qk_norm_rope_bwd(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weig
     that are None and where ``weight_grads`` is false.  dq / dk may be dq_out / dk_out."""
     io = _qk_io(shape, heads, kv_heads, q, k, q_weight, k_weight, eps, table, index, status)
     _need_cuda(dq_out, dk_out)
+    dev = q.device
     if dq is None:
-        dq = torch.empty(q.shape[0], heads * shape.head_dim, device=q.device, dtype=q.dtype)
-    io.dq_out, io.dq_out_ld, io.dq, io.dq_ld = _ptr(dq_out), _rows(dq_out, "dq_out"), _ptr(dq), _rows(dq, "dq")
+        dq = torch.empty(*q.shape[:-1], heads * shape.head_dim, device=dev, dtype=q.dtype)
+    io.dq_out, io.dq_out_ld, io.dq, io.dq_ld = dq_out.data_ptr(), _ld(dq_out, "dq_out"), dq.data_ptr(), _ld(dq, "dq")
     if kv_heads:
         if dk is None:
-            dk = torch.empty(k.shape[0], kv_heads * shape.head_dim, device=k.device, dtype=k.dtype)
-        io.dk_out, io.dk_out_ld, io.dk, io.dk_ld = _ptr(dk_out), _rows(dk_out, "dk_out"), _ptr(dk), _rows(dk, "dk")
+            dk = torch.empty(*k.shape[:-1], kv_heads * shape.head_dim, device=dev, dtype=k.dtype)
+        io.dk_out, io.dk_out_ld, io.dk, io.dk_ld = dk_out.data_ptr(), _ld(dk_out, "dk_out"), dk.data_ptr(), _ld(dk, "dk")
     dgq = torch.empty_like(q_weight) if weight_grads and q_weight is not None else None
     dgk = torch.empty_like(k_weight) if weight_grads and k_weight is not None and kv_heads else None
     io.dq_weight, io.dk_weight = _ptr(dgq), _ptr(dgk)
     g = shape.geometry(q.dtype)
     lib = _lib.load()
-    with _on(q.device):
+    with _on(dev):
         need = int(lib.msl_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(g), ctypes.byref(io)))
-        ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
-        rc = _call("msl_qk_norm_rope_bwd", q.device, lambda: lib.msl_qk_norm_rope_bwd(
-            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _stream(q.device)))
+        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+        rc = _call("msl_qk_norm_rope_bwd", dev, lambda: lib.msl_qk_norm_rope_bwd(
+            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _raw_stream(dev.index)))
     _lib.check("msl_qk_norm_rope_bwd", rc)
     return dq, dk, dgq, dgk
 
@@ -627,23 +690,24 @@ def activation_code(name: str) -> int:
 def _ffn_check(x, w_in, w_out, b_in, b_out) -> Tuple[int, int, int]:
     """(rows, dim, hidden) of a gated feed-forward call, its operands checked."""
     _need_cuda(x, w_in, w_out, b_in, b_out)
-    M, C = x.shape
+    C = x.shape[-1]
+    M = x.numel() // C if C else 0
     if w_in.dim() != 2 or w_in.shape[0] % 2 or w_in.shape[1] != C:
         raise ValueError(f"w_in must be [2 * hidden, {C}], got {tuple(w_in.shape)}")
     F = w_in.shape[0] // 2
     if tuple(w_out.shape) != (C, F):
         raise ValueError(f"w_out must be {(C, F)}, got {tuple(w_out.shape)}")
-    for t, n, nm in ((b_in, 2 * F, "b_in"), (b_out, C, "b_out")):
-        if t is not None and (t.dim() != 1 or t.numel() != n):
-            raise ValueError(f"{nm} must be [{n}], got {tuple(t.shape)}")
-    for t, nm in ((w_in, "w_in"), (w_out, "w_out"), (b_in, "b_in"), (b_out, "b_out")):
+    dev, dt = x.device, x.dtype
+    for t, n, nm in ((w_in, 0, "w_in"), (w_out, 0, "w_out"), (b_in, 2 * F, "b_in"), (b_out, C, "b_out")):
         if t is None:
             continue
-        if t.dtype != x.dtype:
-            raise TypeError(f"{nm} must have x's dtype {x.dtype}, got {t.dtype}")
+        if n and (t.dim() != 1 or t.numel() != n):
+            raise ValueError(f"{nm} must be [{n}], got {tuple(t.shape)}")
+        if t.dtype != dt:
+            raise TypeError(f"{nm} must have x's dtype {dt}, got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{nm} must be contiguous")
-        if t.device != x.device:
+        if t.device != dev:
             raise RuntimeError(f"{nm} must be on x's CUDA device")
     return M, C, F
 
@@ -652,21 +716,24 @@ def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in
                   b_out: Optional[torch.Tensor] = None, activation: str = "silu", keep: bool = False,
                   status: Optional[torch.Tensor] = None):
     """Gated feed-forward block on x [rows, >= dim] (row view).  Returns (y, h, gu): h [rows, hidden] the gated
-    product, gu [rows, 2 * hidden] the two projections where ``keep`` (for the backward), else None."""
+    product, gu [rows, 2 * hidden] the two projections where ``keep`` (for the backward), else None.  status: a
+    device word for MSL_STATUS_TIMEOUT in place of the device's HostFlag."""
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
-    h = torch.empty(M, F, device=x.device, dtype=x.dtype)
-    gu = torch.empty(M, 2 * F, device=x.device, dtype=x.dtype) if keep else None
-    y = torch.empty(M, C, device=x.device, dtype=x.dtype)
-    g = _lib.FfnGeometry(M, C, F, dtype_code(x.dtype), activation_code(activation))
-    io = _lib.FfnIO()
-    io.x, io.x_ld, io.w_in, io.b_in, io.w_out, io.b_out = _ptr(x), _rows(x, "x"), _ptr(w_in), _ptr(b_in), _ptr(w_out), _ptr(b_out)
-    io.h, io.gu, io.y, io.y_ld, io.status = _ptr(h), _ptr(gu), _ptr(y), C, _ptr(status)
+    dev, dt = x.device, x.dtype
+    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation))
+    x_ld = _ld(x, "x")
+    h = torch.empty(M, F, device=dev, dtype=dt)
+    gu = torch.empty(M, 2 * F, device=dev, dtype=dt) if keep else None
+    y = torch.empty(x.shape, device=dev, dtype=dt)
+    io = _lib.FfnIO(x.data_ptr(), x_ld, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out), h.data_ptr(), _ptr(gu),
+                    y.data_ptr(), C)
+    io.status = _flag(dev, status)
     lib = _lib.load()
-    with _on(x.device):
+    with _on(dev):
         need = int(lib.msl_gated_ffn_workspace_bytes(ctypes.byref(g), 0))
-        ws = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
-        rc = _call("msl_gated_ffn_fwd", x.device, lambda: lib.msl_gated_ffn_fwd(
-            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _stream(x.device)))
+        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+        rc = _call("msl_gated_ffn_fwd", dev, lambda: lib.msl_gated_ffn_fwd(
+            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _raw_stream(dev.index)))
     _lib.check("msl_gated_ffn_fwd", rc)
     return y, h, gu
 
@@ -679,26 +746,35 @@ def gated_ffn_bwd(x, w_in, w_out, h, gu, dy, b_in=None, b_out=None, activation: 
     _need_cuda(h, gu, dy)
     dev, dt = x.device, x.dtype
     needs = (needs[0], needs[1], needs[2], needs[3] and b_in is not None, needs[4] and b_out is not None)
-    dx = torch.empty(M, C, device=dev, dtype=dt) if needs[0] else None
+    dx = torch.empty(x.shape, device=dev, dtype=dt) if needs[0] else None
     dw_in = torch.empty_like(w_in) if needs[1] else None
     dw_out = torch.empty_like(w_out) if needs[2] else None
     db_in = torch.empty_like(b_in) if needs[3] else None
     db_out = torch.empty_like(b_out) if needs[4] else None
     dgu = torch.empty(M, 2 * F, device=dev, dtype=dt) if needs[0] or needs[1] or needs[3] else None
     g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation))
-    io = _lib.FfnIO()
-    io.x, io.x_ld, io.w_in, io.w_out = _ptr(x), _rows(x, "x"), _ptr(w_in), _ptr(w_out)
-    io.h, io.gu, io.dy, io.dy_ld, io.dgu = _ptr(h), _ptr(gu), _ptr(dy), _rows(dy, "dy"), _ptr(dgu)
-    io.dx, io.dx_ld, io.dw_in, io.dw_out, io.db_in, io.db_out = _ptr(dx), C, _ptr(dw_in), _ptr(dw_out), _ptr(db_in), _ptr(db_out)
-    io.status = _ptr(status)
+    io = _lib.FfnIO(x.data_ptr(), _ld(x, "x"), w_in.data_ptr(), None, w_out.data_ptr(), None, h.data_ptr(), gu.data_ptr(), None, 0,
+                    dy.data_ptr(), _ld(dy, "dy"), _ptr(dgu), _ptr(dx), C, _ptr(dw_in), _ptr(dw_out), _ptr(db_in), _ptr(db_out),
+                    _flag(dev, status))
     lib = _lib.load()
     with _on(dev):
         need = int(lib.msl_gated_ffn_workspace_bytes(ctypes.byref(g), 1))
         ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
         rc = _call("msl_gated_ffn_bwd", dev, lambda: lib.msl_gated_ffn_bwd(
-            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _stream(dev)))
+            ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _raw_stream(dev.index)))
     _lib.check("msl_gated_ffn_bwd", rc)
     return dx, dw_in, dw_out, db_in, db_out
+
+
+_dtype_of, _device_of = attrgetter("dtype"), attrgetter("device")
+_numel_of, _ptr_of, _is_whole = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+
+
+def _one_device(ts: List[torch.Tensor], dev: torch.device, name: str) -> None:
+    if set(map(_device_of, ts)) != {dev} or dev.type != "cuda":
+        raise RuntimeError(f"every {name} must be on the same CUDA device (no CPU fallback)")
+    if not all(map(_is_whole, ts)):
+        raise ValueError(f"{name} {list(map(_is_whole, ts)).index(False)} must be contiguous")
 
 
 def grad_norm(src: List[torch.Tensor], dst: Optional[List[torch.Tensor]] = None, max_norm: float = 0.0,
@@ -707,23 +783,21 @@ def grad_norm(src: List[torch.Tensor], dst: Optional[List[torch.Tensor]] = None,
     float32 tensor; with ``dst`` also dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)) (dst[i] may be src[i])."""
     if not src:
         raise ValueError("no tensors")
-    dev = src[0].device
     n = len(src)
-    if dst is not None and len(dst) != n:
-        raise ValueError(f"{n} tensors, but {len(dst)} to write")
-    for ts, nm in ((src, "tensor"), (dst or (), "out")):
-        for i, t in enumerate(ts):
-            if not t.is_cuda or t.device != dev:
-                raise RuntimeError(f"{nm} {i} must be on the same CUDA device as the first tensor (no CPU fallback)")
-            if not t.is_contiguous():
-                raise ValueError(f"{nm} {i} must be contiguous")
-    if dst is not None:
-        for i, (a, b) in enumerate(zip(src, dst)):
-            if a.dtype != b.dtype or a.numel() != b.numel():
-                raise ValueError(f"out {i} must have the tensor's dtype and size, got {b.numel()} {b.dtype} for {a.numel()} {a.dtype}")
-    numel = (ctypes.c_int64 * n)(*[t.numel() for t in src])
-    dtypes = (ctypes.c_int32 * n)(*[dtype_code(t.dtype) for t in src])
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in src])
+    dev = src[0].device
+    _one_device(src, dev, "tensor")
+    dtypes = list(map(_dtype_of, src))
+    sizes = list(map(_numel_of, src))
+    if dst is not None and dst is not src:
+        if len(dst) != n:
+            raise ValueError(f"{n} tensors, but {len(dst)} to write")
+        _one_device(dst, dev, "out")
+        if list(map(_dtype_of, dst)) != dtypes or list(map(_numel_of, dst)) != sizes:
+            raise ValueError("every out must have its tensor's dtype and size")
+    codes = {d: dtype_code(d) for d in set(dtypes)}
+    numel = (ctypes.c_int64 * n)(*sizes)
+    codes_arr = (ctypes.c_int32 * n)(*[codes[d] for d in dtypes])
+    ptrs = (ctypes.c_void_p * n)(*map(_ptr_of, src))
     norm = torch.empty((), device=dev, dtype=torch.float32)
     lib = _lib.load()
     with _on(dev):
@@ -731,11 +805,12 @@ def grad_norm(src: List[torch.Tensor], dst: Optional[List[torch.Tensor]] = None,
         ws = torch.empty(need, device=dev, dtype=torch.uint8)
         if dst is None:
             name = "msl_grad_norm"
-            rc = _call(name, dev, lambda: lib.msl_grad_norm(ptrs, numel, dtypes, n, extra_sumsq, _ptr(norm), _ptr(ws), need, _stream(dev)))
+            rc = _call(name, dev, lambda: lib.msl_grad_norm(ptrs, numel, codes_arr, n, extra_sumsq, norm.data_ptr(), ws.data_ptr(),
+                                                            need, _raw_stream(dev.index)))
         else:
             name = "msl_grad_clip"
-            outs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst])
-            rc = _call(name, dev, lambda: lib.msl_grad_clip(ptrs, outs, numel, dtypes, n, extra_sumsq, max_norm, _ptr(norm),
-                                                            _ptr(ws), need, _stream(dev)))
+            outs = ptrs if dst is src else (ctypes.c_void_p * n)(*map(_ptr_of, dst))
+            rc = _call(name, dev, lambda: lib.msl_grad_clip(ptrs, outs, numel, codes_arr, n, extra_sumsq, max_norm,
+                                                            norm.data_ptr(), ws.data_ptr(), need, _raw_stream(dev.index)))
     _lib.check(name, rc)
     return norm

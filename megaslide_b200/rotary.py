@@ -8,7 +8,8 @@ queries and keys for each head, on the kernels of csrc/rotary.cu.
 Tokens are [B, N, heads * head_dim] in the order n = (t*H + h)*W + w, as everywhere in this package; q and k may
 be columns of one qkv buffer.  `frame0` places a call's first token at a later frame of the table (a rank's
 frames of a sharded volume, a streamed frame); `index` (int32 [B, N, 3] or [N, 3]) gives each token its
-own three positions instead (packed images and videos, single tokens).  float32 or bfloat16; the
+own three positions instead (packed images and videos, single tokens); a position outside its axis is reported by a
+later call or by check_status.  float32 or bfloat16; the
 statistics, the rotation and the weights' gradients are computed in float32 and rounded once.
 """
 
@@ -48,13 +49,14 @@ def rotary_table(video_shape: Int3, axes: Int3, theta: float = 10000.0, position
 
 
 def _as_rows(x: Tensor) -> Tensor:
-    """[B, N, C] tokens as a [B*N, C] row view (a copy where the strides allow none)."""
+    """[B, N, C] tokens whose rows lie at one stride: x, or a copy where its strides have none."""
+    if x.is_contiguous():
+        return x
     B, N, C = x.shape
-    if (x.stride(2) == 1 or C == 1) and (B == 1 or N == 1 or x.stride(0) == N * x.stride(1)):
-        ld = x.stride(1) if N > 1 else (x.stride(0) if B > 1 else C)
-        if ld >= C:
-            return x.as_strided((B * N, C), (ld, 1))
-    return x.reshape(B * N, C).contiguous()
+    sb, sn, sc = x.stride()
+    if (sc == 1 or C == 1) and (B == 1 or N == 1 or sb == N * sn) and (sn if N > 1 else sb) >= C:
+        return x
+    return x.contiguous()
 
 
 def _check_tokens(name: str, x: Tensor, heads: int) -> int:
@@ -76,22 +78,8 @@ class _Call:
         self.shape, self.heads, self.kv_heads, self.eps = shape, heads, kv_heads, eps
 
 
-def _status(index: Optional[Tensor], dev: torch.device):
-    """The device's status word for calls whose positions come from the user's index (raises if an earlier call
-    reported one out of range); none otherwise: the positions of a grid are checked on the host."""
-    if index is None:
-        return None
-    sw = ops.status_word(dev)
-    sw.poll()
-    return sw
-
-
 def _rotate(call: _Call, x: Tensor, table: Tensor, index: Optional[Tensor], inverse: bool) -> Tensor:
-    sw = _status(index, x.device)
-    y = ops.rope3d(call.shape, call.heads, _as_rows(x), table, index, inverse, status=sw.word if sw else None)
-    if sw:
-        sw.post()
-    return y.view(x.shape)
+    return ops.rope3d(call.shape, call.heads, _as_rows(x), table, index, inverse)
 
 
 class Rope3DFunction(torch.autograd.Function):
@@ -124,12 +112,8 @@ def rope3d(x: Tensor, table: Tensor, *, video_shape: Int3, axes: Int3, heads: in
 
 
 def _norm_rotate(call: _Call, q, k, q_weight, k_weight, table, index):
-    sw = _status(index, q.device)
-    q2, k2 = ops.qk_norm_rope_fwd(call.shape, call.heads, call.kv_heads, _as_rows(q), _as_rows(k), q_weight, k_weight, call.eps,
-                                  table, index, status=sw.word if sw else None)
-    if sw:
-        sw.post()
-    return q2.view(q.shape), k2.view(k.shape)
+    return ops.qk_norm_rope_fwd(call.shape, call.heads, call.kv_heads, _as_rows(q), _as_rows(k), q_weight, k_weight, call.eps,
+                                table, index)
 
 
 class QKNormRopeFunction(torch.autograd.Function):
@@ -145,14 +129,10 @@ class QKNormRopeFunction(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, table, index = ctx.saved_tensors
         c = ctx.call
-        sw = _status(index, q.device)
         dq, dk, dgq, dgk = ops.qk_norm_rope_bwd(c.shape, c.heads, c.kv_heads, _as_rows(q), _as_rows(k), q_weight, k_weight,
                                                 _as_rows(dq_out), _as_rows(dk_out), c.eps, table, index,
-                                                weight_grads=ctx.needs_input_grad[3] or ctx.needs_input_grad[4],
-                                                status=sw.word if sw else None)
-        if sw:
-            sw.post()
-        return None, dq.view(q.shape), dk.view(k.shape), dgq, dgk, None, None
+                                                weight_grads=ctx.needs_input_grad[3] or ctx.needs_input_grad[4])
+        return None, dq, dk, dgq, dgk, None, None
 
 
 def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], table: Optional[Tensor] = None, *,

@@ -78,14 +78,18 @@ def test_gated_mlp_parameters():
 
 
 def test_row_views():
+    """Tokens whose rows lie at one stride are used as they are, others are copied."""
     x = torch.zeros(2, 3, 10)
-    assert rotary._as_rows(x).data_ptr() == x.data_ptr()
+    assert rotary._as_rows(x) is x and ops._ld(x, "x") == 10
     cols = torch.zeros(2, 3, 30)[..., 10:20]
-    v = rotary._as_rows(cols)
-    assert v.data_ptr() == cols.data_ptr() and v.stride() == (30, 1) and v.shape == (6, 10)
-    assert rotary._as_rows(torch.zeros(3, 2, 10).transpose(0, 1)).is_contiguous()
-    assert rotary._as_rows(torch.zeros(2, 1, 10).expand(2, 4, 10)).stride(0) >= 10  # a broadcast sample is copied
-    assert rotary._as_rows(torch.zeros(1, 0, 10)).shape == (0, 10)
+    assert rotary._as_rows(cols) is cols and ops._ld(cols, "x") == 30
+    swapped = torch.zeros(3, 2, 10).transpose(0, 1)
+    assert rotary._as_rows(swapped).is_contiguous()
+    with pytest.raises(ValueError, match="one stride"):
+        ops._ld(swapped, "x")
+    spread = torch.zeros(2, 1, 10).expand(2, 4, 10)  # one row for every token of a sample
+    assert rotary._as_rows(spread).is_contiguous() and rotary._as_rows(torch.zeros(1, 1, 10).expand(1, 4, 10)).stride(1) == 10
+    assert ops._ld(rotary._as_rows(torch.zeros(1, 0, 10)), "x") == 10
 
 
 def _err():
