@@ -5,6 +5,8 @@
 //   dh = dy w_out;  dg = dh u act'(g);  du = dh act(g);  dx = [dg du] w_in;  dw_in = [dg du]^T x;
 //   dw_out = dy^T h;  db_in, db_out = column sums of [dg du], dy
 
+#include <initializer_list>
+
 #include "gated_ffn.cuh"
 
 namespace msl {
@@ -191,10 +193,37 @@ static cudaError_t column_sums(int dtype, const void* x, long long ld, long long
   return column_sums_t(static_cast<const float*>(x), ld, rows, cols, static_cast<float*>(out), partial, s);
 }
 
-static int run(const Product& p, cudaStream_t s) {
-  const bool tc = tc_applies(p);
-  const cudaError_t e = tc ? launch_product_tc(p, s) : launch_product_simt(p, s);
-  if (e != cudaSuccess) return cuda_failf(e, tc ? "product_kernel launch" : "product_simt_kernel launch");
+// The workspace's slots for planes, and whose planes they hold in this call.
+struct Slots {
+  char* at[3];
+  size_t bytes[3];
+  const void* of[3];
+};
+
+static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStream_t s) {
+  cudaError_t e;
+  if (tc_applies(p)) {
+    e = launch_product_tc(p, s);
+    if (e != cudaSuccess) return cuda_failf(e, "product_kernel launch");
+  } else if (slots.at[0] && planes_apply(p)) {
+    const long long rows[2] = {p.a_major ? p.K : p.M, p.b_major ? p.K : (p.epilogue == kGate ? 2 * p.N : p.N)};
+    const long long cols[2] = {p.a_major ? p.M : p.K, p.b_major ? p.N : p.K};
+    const void* const src[2] = {p.a, p.b};
+    const long long ld[2] = {p.lda, p.ldb};
+    const int slot[2] = {slot_a, slot_b};
+    for (int i = 0; i < 2; ++i) {
+      if (slots.of[slot[i]] == src[i]) continue;
+      if (planes_bytes(p.dtype, rows[i], cols[i]) > slots.bytes[slot[i]]) return failf(MSL_ERR_WORKSPACE, "planes beyond their slot");
+      e = launch_planes(p.dtype, src[i], ld[i], rows[i], cols[i], slots.at[slot[i]], s);
+      if (e != cudaSuccess) return cuda_failf(e, "split_kernel launch");
+      slots.of[slot[i]] = src[i];
+    }
+    e = launch_product_planes(p, slots.at[slot_a], slots.at[slot_b], s);
+    if (e != cudaSuccess) return cuda_failf(e, "planes_kernel launch");
+  } else {
+    e = launch_product_simt(p, s);
+    if (e != cudaSuccess) return cuda_failf(e, "product_simt_kernel launch");
+  }
   count_launches(1);
   return MSL_OK;
 }
@@ -210,30 +239,62 @@ static int check(const msl_ffn_geometry* g, const msl_ffn_io* io) {
   return MSL_OK;
 }
 
-// Workspace: the sums of parts of tiles of one product at a time, then the column sums' slices.
+// Workspace: the sums of parts of tiles of one product at a time, the column sums' slices, and planes of
+// operands: forward, x or h and one weight; backward, dy, the gradients of g and u, and the product's other operand.
 struct Workspace {
-  size_t partial, columns, total;
+  size_t partial, columns, planes[3], total;
 };
 static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
   Workspace w{};
   const long long M = g->rows, C = g->dim, F = g->hidden;
+  const bool planes = g->dtype == MSL_DTYPE_F32 || C % 8 || F % 8;
   auto need = [&](long long m, long long n, long long k, int epilogue, bool b_major) {
-    const size_t b = M > 0 && g->dtype == MSL_DTYPE_BF16 ? tc_partial_bytes(m, n, k, epilogue, b_major) : 0;
+    if (M == 0) return;
+    // one product of a bf16 block may be addressable though the others are not (hidden a multiple of 4)
+    const size_t b = planes ? planes_partial_bytes(g->dtype, m, n, k, epilogue) : 0;
+    const size_t t = g->dtype == MSL_DTYPE_BF16 ? tc_partial_bytes(m, n, k, epilogue, b_major) : 0;
     if (b > w.partial) w.partial = b;
+    if (t > w.partial) w.partial = t;
   };
+  auto most = [](std::initializer_list<size_t> v) {
+    size_t m = 0;
+    for (size_t x : v) m = x > m ? x : m;
+    return m;
+  };
+  auto size = [&](long long rows, long long cols) { return planes_bytes(g->dtype, rows, cols); };
   if (backward) {
     need(M, F, C, kDgate, true);
     need(M, C, 2 * F, kPlain, true);
     need(2 * F, C, M, kPlain, true);
     need(C, F, M, kPlain, true);
     w.columns = sizeof(float) * kSlices * static_cast<size_t>(2 * F > C ? 2 * F : C);
+    w.columns = (w.columns + 255) / 256 * 256;
+    if (planes && M > 0) {
+      w.planes[0] = size(M, C);
+      w.planes[1] = size(M, 2 * F);
+      w.planes[2] = most({size(C, F), size(2 * F, C), size(M, C), size(M, F)});
+    }
   } else {
     need(M, F, C, kGate, false);
     need(M, C, F, kPlain, false);
+    if (planes && M > 0) {
+      w.planes[0] = most({size(M, C), size(M, F)});
+      w.planes[1] = most({size(2 * F, C), size(C, F)});
+    }
   }
   w.partial = (w.partial + 255) / 256 * 256;
-  w.total = w.partial + w.columns;
+  w.total = w.partial + w.columns + w.planes[0] + w.planes[1] + w.planes[2];
   return w;
+}
+static Slots slots_of(const Workspace& w, void* workspace) {
+  Slots s{};
+  char* at = static_cast<char*>(workspace) + w.partial + w.columns;
+  for (int i = 0; i < 3; ++i) {
+    s.at[i] = w.planes[0] ? at : nullptr;
+    s.bytes[i] = w.planes[i];
+    at += w.planes[i];
+  }
+  return s;
 }
 static int check_workspace(const Workspace& w, const void* p, size_t bytes) {
   if (w.total == 0) return MSL_OK;
@@ -277,6 +338,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   rc = ffn::check_workspace(W, workspace, workspace_bytes);
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  ffn::Slots slots = ffn::slots_of(W, workspace);
   ffn::Product p = ffn::product(geom, io, W, workspace);
   p.epilogue = ffn::kGate;
   p.a = io->x; p.lda = io->x_ld;
@@ -285,7 +347,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.bias = io->b_in;
   p.gu_out = io->gu;
   p.M = M; p.N = F; p.K = C;
-  rc = ffn::run(p, s);
+  rc = ffn::run(p, slots, 0, 1, s);
   if (rc) return rc;
   p = ffn::product(geom, io, W, workspace);
   p.epilogue = ffn::kPlain;
@@ -294,7 +356,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.out = io->y; p.ldo = io->y_ld;
   p.bias = io->b_out;
   p.M = M; p.N = C; p.K = F;
-  return ffn::run(p, s);
+  return ffn::run(p, slots, 0, 1, s);
 }
 
 int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,
@@ -321,6 +383,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   const ffn::Workspace W = ffn::workspace_of(geom, true);
   rc = ffn::check_workspace(W, workspace, workspace_bytes);
   if (rc) return rc;
+  ffn::Slots slots = ffn::slots_of(W, workspace);
   ffn::Product p;
   if (inner) {
     p = ffn::product(geom, io, W, workspace);
@@ -330,7 +393,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     p.out = io->dgu; p.ldo = 2 * F;
     p.gu = io->gu;
     p.M = M; p.N = F; p.K = C;
-    rc = ffn::run(p, s);
+    rc = ffn::run(p, slots, 0, 2, s);
     if (rc) return rc;
   }
   if (io->dx) {
@@ -339,7 +402,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     p.b = io->w_in; p.ldb = C; p.b_major = true;  // [K = 2 hidden, N = dim]
     p.out = io->dx; p.ldo = io->dx_ld;
     p.M = M; p.N = C; p.K = 2 * F;
-    rc = ffn::run(p, s);
+    rc = ffn::run(p, slots, 1, 2, s);
     if (rc) return rc;
   }
   if (io->dw_in) {
@@ -348,7 +411,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     p.b = io->x; p.ldb = io->x_ld; p.b_major = true;  // [K = rows, N = dim]
     p.out = io->dw_in; p.ldo = C;
     p.M = 2 * F; p.N = C; p.K = M;
-    rc = ffn::run(p, s);
+    rc = ffn::run(p, slots, 1, 2, s);
     if (rc) return rc;
   }
   if (io->dw_out) {
@@ -357,7 +420,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     p.b = io->h; p.ldb = F; p.b_major = true;           // [K = rows, N = hidden]
     p.out = io->dw_out; p.ldo = F;
     p.M = C; p.N = F; p.K = M;
-    rc = ffn::run(p, s);
+    rc = ffn::run(p, slots, 0, 2, s);
     if (rc) return rc;
   }
   float* const partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + W.partial);

@@ -98,5 +98,13 @@ bool tc_applies(const Product& p);
 size_t tc_partial_bytes(long long M, long long N, long long K, int epilogue, bool b_major);
 cudaError_t launch_product_tc(const Product& p, cudaStream_t s);
 
+// Tensor-core form for float32 and for widths that are no multiple of 8 (gated_ffn_planes.cu): the operands as
+// planes [planes][rows][cols padded to 8] of planes_bytes, written by launch_planes from rows as they are stored.
+bool planes_apply(const Product& p);
+size_t planes_bytes(int dtype, long long rows, long long cols);
+size_t planes_partial_bytes(int dtype, long long M, long long N, long long K, int epilogue);
+cudaError_t launch_planes(int dtype, const void* x, long long ld, long long rows, long long cols, void* out, cudaStream_t s);
+cudaError_t launch_product_planes(const Product& p, const void* pa, const void* pb, cudaStream_t s);
+
 }  // namespace ffn
 }  // namespace msl

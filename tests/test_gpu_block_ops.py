@@ -380,6 +380,16 @@ def test_gated_ffn(M, C, F, dtype, act):
     _ffn_check_all(M, C, F, dtype, act, bias=act == "gelu")
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("M,C,F,bias", [(700, 1150, 2301, True), (333, 640, 1604, False), (2048, 256, 1024, True), (9249, 253, 1020, True),
+                                        (40, 1533, 6143, False), (1000, 1001, 1600, True)])
+def test_gated_ffn_widths_that_no_vector_divides(M, C, F, bias, dtype, act):
+    """Widths off any vector's or tile's multiple, large enough for the tensor cores: float32 as three planes, bf16 as
+    padded copies, sums of the last tiles cut along k."""
+    _ffn_check_all(M, C, F, dtype, act, bias)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("M,C,F,bias", [(1, 1152, 4608, True), (8, 1152, 2880, False), (1027, 1536, 3840, False), (2500, 640, 1600, True)])
 def test_gated_ffn_sizes(M, C, F, bias, dtype):
