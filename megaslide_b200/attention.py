@@ -15,7 +15,10 @@ per-parameter ``requires_grad`` toggling, as the trainer uses it):
   a    = deformable gather attention(q, k, v, off, extra)   msl_dsa_attn_fwd
   y    = a @ Wo^T + D                             cuBLAS GEMM accumulating into D
 
-and the backward mirrors it with msl_dsa_attn_bwd, msl_dwconv3d_bwd_data / _bwd_weight and the
+With ``qk_norm`` / ``rotary_axes`` (options this package adds; off by default) q and k first pass the per-head RMS
+norm and the rotation by the tokens' (time, row, column): msl_qk_norm_rope_fwd, or msl_rope3d alone.
+
+The backward mirrors it with msl_dsa_attn_bwd, msl_dwconv3d_bwd_data / _bwd_weight and the
 GELU'-epilogue conv.  Activations compute in the input's dtype (float32 or bfloat16; under CUDA
 autocast to bfloat16 the input is cast), every gather / softmax / stencil accumulates in float32.
 There is no CPU path: CPU tensors raise.
@@ -31,6 +34,7 @@ from torch import Tensor
 
 from . import ops
 from ._lib import MSL_EPI_GELU, MSL_EPI_GELU_GRAD, MSL_EPI_NONE, MSL_ERR_UNSUPPORTED, MslError
+from .rotary import rotary_table
 
 
 def _mm_f32(a: Tensor, b: Tensor) -> Tensor:
@@ -41,9 +45,9 @@ def _mm_f32(a: Tensor, b: Tensor) -> Tensor:
 
 
 class _Cfg:
-    __slots__ = ("shape", "conv_k", "conv_3", "dtype", "param_dtypes", "G", "kernel", "capture")
+    __slots__ = ("shape", "conv_k", "conv_3", "dtype", "param_dtypes", "G", "kernel", "capture", "rotary", "eps")
 
-    def __init__(self, shape, conv_k, conv_3, dtype, param_dtypes, G, kernel, capture=None):
+    def __init__(self, shape, conv_k, conv_3, dtype, param_dtypes, G, kernel, capture=None, rotary=None, eps=1e-6):
         self.shape = shape
         self.conv_k = conv_k
         self.conv_3 = conv_3
@@ -52,13 +56,55 @@ class _Cfg:
         self.G = G
         self.kernel = kernel
         self.capture = capture  # dict that receives the call's intermediates (parity checks), or None
+        self.rotary = rotary  # ops.RotaryShape of q and k where they are normalised or turned, or None
+        self.eps = eps
+
+
+def _turn_qk(cfg: _Cfg, qkv: Tensor, gq, gk, table) -> Tuple[Tensor, Tensor]:
+    """q and k as the attention reads them, from the columns of qkv [BN, 3C]: normalised (with weights), then turned."""
+    sh = cfg.shape
+    C = sh.heads * sh.head_dim
+    qk = torch.empty(qkv.shape[0], 2 * C, device=qkv.device, dtype=qkv.dtype)
+    if gq is None:  # both at once: their heads are adjacent columns
+        ops.rope3d(cfg.rotary, 2 * sh.heads, qkv[:, :2 * C], table, out=qk)
+        return qk[:, :C], qk[:, C:]
+    return ops.qk_norm_rope_fwd(cfg.rotary, sh.heads, sh.heads, qkv[:, :C], qkv[:, C:2 * C], gq, gk, cfg.eps, table,
+                                q_out=qk[:, :C], k_out=qk[:, C:])
+
+
+def _turn_back(cfg: _Cfg, qkv: Tensor, dqkv: Tensor, gq, gk, table):
+    """The gradients of q and k in dqkv's columns become those of the projections, in place; returns the weights'."""
+    sh = cfg.shape
+    C = sh.heads * sh.head_dim
+    if gq is None:
+        ops.rope3d(cfg.rotary, 2 * sh.heads, dqkv[:, :2 * C], table, inverse=True, out=dqkv[:, :2 * C])
+        return None, None
+    _, _, dgq, dgk = ops.qk_norm_rope_bwd(cfg.rotary, sh.heads, sh.heads, qkv[:, :C], qkv[:, C:2 * C], gq, gk, dqkv[:, :C],
+                                          dqkv[:, C:2 * C], cfg.eps, table, dq=dqkv[:, :C], dk=dqkv[:, C:2 * C])
+    return dgq, dgk
+
+
+def _norm_extra(cfg: _Cfg, ek: Tensor, gk: Tensor) -> Tensor:
+    """Extra keys have no position: they are normalised as keys are, and not turned."""
+    sh = cfg.shape
+    shape = ops.RotaryShape(1, ek.shape[0], (1, 1, 1), (0, 0, 0), sh.head_dim)
+    return ops.qk_norm_rope_fwd(shape, sh.heads, 0, ek, None, gk, None, cfg.eps)[0]
+
+
+def _norm_extra_back(cfg: _Cfg, ek: Tensor, gk: Tensor, dek: Tensor) -> Tuple[Tensor, Tensor]:
+    """float32 gradients of the extra keys before the norm and of the weight."""
+    sh = cfg.shape
+    shape = ops.RotaryShape(1, ek.shape[0], (1, 1, 1), (0, 0, 0), sh.head_dim)
+    dek, _, dg, _ = ops.qk_norm_rope_bwd(shape, sh.heads, 0, ek.float(), None, gk.float(), None, dek, None, cfg.eps)
+    return dek, dg
 
 
 class DSA3DFunction(torch.autograd.Function):
     """Forward/backward of DeformableSlideAttention3D (attention.py:82-192) on the B200 kernels."""
 
     @staticmethod
-    def forward(ctx, cfg: _Cfg, x, extra_kv, off_in, wq, bq, wk, bk, wv, bv, wo, bo, wd, bd, w1, b1, w2, b2):
+    def forward(ctx, cfg: _Cfg, x, extra_kv, off_in, wq, bq, wk, bk, wv, bv, wo, bo, wd, bd, w1, b1, w2, b2, gq=None, gk=None,
+                table=None):
         sh: ops.DsaShape = cfg.shape
         dt = cfg.dtype
         B, N, C = x.shape
@@ -68,6 +114,10 @@ class DSA3DFunction(torch.autograd.Function):
         bqkv = torch.cat([bq, bk, bv], 0).to(dt)
         qkv = torch.addmm(bqkv, x2, wqkv.t())  # [BN, 3C]
         q, k, v = qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:]
+        if cfg.rotary is not None:
+            gq = gq.detach().to(dt) if gq is not None else None
+            gk = gk.detach().to(dt) if gk is not None else None
+            q, k = _turn_qk(cfg, qkv, gq, gk, table)
         O = w2.shape[0]
         w2m = w2.reshape(O, C)
         w1_kc = ops.conv_weight_kc(w1)
@@ -86,11 +136,14 @@ class DSA3DFunction(torch.autograd.Function):
         wd_kc = ops.conv_weight_kc(wd)
         D = ops.dwconv_fwd(cfg.conv_k, x2, wd_kc, bd.detach().float().contiguous(), bo.detach().float().contiguous(),
                            epilogue=MSL_EPI_NONE)
-        ek = ev = e2 = None
+        ek = ev = e2 = ek_raw = None
         if G:
             e2 = extra_kv.reshape(B * G, C).to(dt).contiguous()
             ekv = torch.addmm(torch.cat([bk, bv], 0).to(dt), e2, torch.cat([wk, wv], 0).to(dt).t())
             ek, ev = ekv[:, :C], ekv[:, C:]
+            if gk is not None:
+                ek_raw, ek = ek, _norm_extra(cfg, ek, gk)
+                ev = ev.contiguous()  # both at one row stride
         train = any(ctx.needs_input_grad)
         sw = ops.status_word(x2.device)
         sw.poll()  # raises if an earlier call produced invalid results
@@ -112,8 +165,9 @@ class DSA3DFunction(torch.autograd.Function):
         if cfg.capture is not None:
             cfg.capture.update(x2=x2, qkv=qkv, hact=hact, off=off, offset_bias=b2f, attn=attn, lse=lse, y=y)
         if train:
+            turned = (q, k, gq, gk, table, ek_raw) if cfg.rotary is not None else (None,) * 6
             ctx.save_for_backward(x2, qkv, hact, off, b2f, attn, lse, e2, ek, ev, wqkv, wo, w2m, w1_kc, b1f, wd_kc, probs,
-                                  saved)
+                                  saved, *turned)
             ctx.cfg = cfg
             ctx.in_dtype = x.dtype
             ctx.off_dtype = off_in.dtype if off_in is not None else None
@@ -123,7 +177,7 @@ class DSA3DFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (x2, qkv, hact, off, b2f, attn, lse, e2, ek, ev, wqkv, wo, w2m, w1_kc, b1f, wd_kc, probs,
-         saved) = ctx.saved_tensors
+         saved, q_t, k_t, gq, gk, table, ek_raw) = ctx.saved_tensors
         cfg: _Cfg = ctx.cfg
         sh: ops.DsaShape = cfg.shape
         dt = cfg.dtype
@@ -142,12 +196,20 @@ class DSA3DFunction(torch.autograd.Function):
             # deformable attention core -> dq, dk, dv written straight into one [BN, 3C] buffer
             dqkv = torch.empty_like(qkv)
             q, k, v = qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:]
+            if cfg.rotary is not None:
+                q, k = q_t, k_t
             sw = ops.status_word(dy2.device)
             _, _, _, doff, dek, dev = ops.attn_bwd(
                 sh, q, k, v, off, attn, lse, dattn, ek=ek, ev=ev,
                 dq=dqkv[:, :C], dk=dqkv[:, C:2 * C], dv=dqkv[:, 2 * C:], probs=probs, saved=saved, doff_dtype=dt,
                 offset_bias=b2f, status=sw.word)
             sw.post()
+            dgq = dgk = None
+            if cfg.rotary is not None:
+                dgq, dgk = _turn_back(cfg, qkv, dqkv, gq, gk, table)
+                if ek_raw is not None:
+                    dek, dge = _norm_extra_back(cfg, ek_raw, gk, dek)
+                    dgk = dgk.float() + dge
             # q/k/v projections; dx accumulates in float32 across the three branches (the depthwise
             # convs add their transposed convolutions into it)
             dx = _mm_f32(dqkv, wqkv)
@@ -202,6 +264,8 @@ class DSA3DFunction(torch.autograd.Function):
             grads += (None, None, None, None)
         dx_out = dx.view(B, BN // B, C).to(ctx.in_dtype)
         de = d_extra.to(ctx.extra_dtype) if d_extra is not None else None
+        if len(ctx.needs_input_grad) > 18:
+            grads += (dgq.to(pd[14]) if dgq is not None else None, dgk.to(pd[15]) if dgk is not None else None, None)
         return (None, dx_out, de, d_off_in) + grads
 
 
@@ -216,13 +280,21 @@ class DeformableSlideAttention3D(nn.Module):
         offset_scale: scale of the learned offsets.
         dropout: dropout on the softmax weights (counter-based in-kernel mask in training mode).
 
+    Options beyond the reference, all off by default (the parameters and results are then the reference's):
+        qk_norm: RMS norm of queries and keys for each head, weights q_norm_weight / k_norm_weight [head_dim]
+            shared by the heads (extra keys are normalised too).
+        rotary_axes: (at, ah, aw), the channels of a head that turn with a token's time, row and column (rotary
+            positions; each even, at most head_dim together; extra keys do not turn).
+        rotary_theta: their base.
+
     ``capture`` (not a parameter; None by default): a dict set here receives references to the
     intermediates of the next forward / backward (q/k/v, offsets, attention output, lse and their
     gradients), which a checker compares with an independent implementation at sampled rows.
     """
 
     def __init__(self, hidden_size: int, num_heads: int, kernel_size: Tuple[int, int, int] = (3, 7, 7),
-                 offset_scale: float = 1.0, dropout: float = 0.0):
+                 offset_scale: float = 1.0, dropout: float = 0.0, qk_norm: bool = False,
+                 rotary_axes: Optional[Tuple[int, int, int]] = None, rotary_theta: float = 10000.0):
         super().__init__()
         assert hidden_size % num_heads == 0, "hidden_size must be divisible by num_heads"
         self.hidden_size = hidden_size
@@ -248,6 +320,32 @@ class DeformableSlideAttention3D(nn.Module):
         nn.init.zeros_(self.offset_net[-1].bias)
         self.dropout = nn.Dropout(dropout)
         self.capture: Optional[dict] = None
+        self.qk_norm = qk_norm
+        if qk_norm:
+            if self.head_dim % 2:
+                raise ValueError(f"qk_norm needs an even head_dim, got {self.head_dim}")
+            self.q_norm_weight = nn.Parameter(torch.ones(self.head_dim))
+            self.k_norm_weight = nn.Parameter(torch.ones(self.head_dim))
+        if rotary_axes is not None:
+            rotary_axes = tuple(rotary_axes)
+            if len(rotary_axes) != 3 or any(a < 0 or a % 2 for a in rotary_axes) or not 0 < sum(rotary_axes) <= self.head_dim:
+                raise ValueError(f"rotary_axes must be three even channel counts of at most head_dim = {self.head_dim} together, "
+                                 f"got {rotary_axes}")
+        self.rotary_axes = rotary_axes
+        self.rotary_theta = rotary_theta
+        self._tables: dict = {}  # (video shape, device) -> table of cosines and sines
+
+    def _table(self, video_shape: Tuple[int, int, int], device) -> Optional[Tensor]:
+        if self.rotary_axes is None:
+            return None
+        key = (tuple(video_shape), device)
+        t = self._tables.get(key)
+        if t is None:
+            t = self._tables[key] = rotary_table(video_shape, self.rotary_axes, self.rotary_theta, device=device)
+        return t
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "_tables": {}}
 
     def _params(self):
         return (self.q_proj.weight, self.q_proj.bias, self.k_proj.weight, self.k_proj.bias,
@@ -306,10 +404,17 @@ class DeformableSlideAttention3D(nn.Module):
         seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if p > 0 else 0
         shape = ops.DsaShape(B, T, H, W, self.num_heads, self.head_dim, (self.k_t, self.k_h, self.k_w), extra=G,
                              offset_scale=float(self.offset_scale), dropout_p=float(p), dropout_seed=seed)
+        turned = self.qk_norm or self.rotary_axes is not None
+        params = self._params()
+        if turned:
+            params += (self.q_norm_weight, self.k_norm_weight) if self.qk_norm else (None, None)
         cfg = _Cfg(shape,
                    ops.ConvShape(B, T, H, W, D, (self.k_t, self.k_h, self.k_w)),
                    ops.ConvShape(B, T, H, W, D, (3, 3, 3)),
-                   dt, tuple(t.dtype for t in self._params()), G, (self.k_t, self.k_h, self.k_w),
+                   dt, tuple(t.dtype if t is not None else None for t in params), G, (self.k_t, self.k_h, self.k_w),
                    capture=self.capture)
+        if turned:
+            cfg.rotary = ops.RotaryShape(B, N, (T, H, W), self.rotary_axes or (0, 0, 0), self.head_dim)
+            params += (self._table((T, H, W), x.device),)
         with torch.autocast("cuda", enabled=False):
-            return DSA3DFunction.apply(cfg, x, extra_kv, offsets, *self._params())
+            return DSA3DFunction.apply(cfg, x, extra_kv, offsets, *params)

@@ -4,7 +4,8 @@ Same module tree, parameter names / shapes and initialisation as the reference's
 (infinity/video/model.py:21-264: MLP, DiTBlock with pre-norm 3D-DSA + optional text cross-attention +
 MLP, spatial patchify, additive sinusoidal timestep embedding, unpatchify), so state dicts move
 between the two.  The attention is megaslide_b200.DeformableSlideAttention3D; the other layers are
-torch modules (cuBLAS GEMMs, torch LayerNorm / GELU).  `VideoDiTConfig` carries the fields of the
+torch modules (cuBLAS GEMMs, torch LayerNorm / GELU).  The config's qk_norm, rotary_axes and gated_mlp (off by default)
+put this package's norm of queries and keys, rotary positions and gated feed-forward block into every block.  `VideoDiTConfig` carries the fields of the
 reference's MegaSlideConfig (infinity/video/config.py) that the model and the trainer read, with the
 same names and defaults.
 """
@@ -20,6 +21,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from .attention import DeformableSlideAttention3D
+from .ffn import GatedMLP
 
 
 @dataclass
@@ -51,6 +53,13 @@ class VideoDiTConfig:
     force_cpu: bool = False
     log_interval: int = 10
     resident_blocks: Optional[bool] = None  # CPU-master trainer: None = decide from device memory
+    # options beyond the reference, off by default
+    qk_norm: bool = False  # RMS norm of queries and keys for each head
+    rotary_axes: Optional[Tuple[int, int, int]] = None  # channels of a head that turn with time, row and column
+    rotary_theta: float = 10000.0
+    gated_mlp: bool = False  # act(gate) * up feed-forward block (GatedMLP) in place of fc1 - GELU - fc2
+    gated_activation: str = "silu"
+    fused_clip: bool = False  # trainer: norm and clipping of the GPU-resident gradients in two kernels
 
     @property
     def num_patches(self) -> int:
@@ -96,9 +105,14 @@ class DiTBlock(nn.Module):
         super().__init__()
         self.norm1 = nn.LayerNorm(config.hidden_size, eps=1e-6)
         self.attn = DeformableSlideAttention3D(config.hidden_size, config.num_heads, tuple(config.dsa_kernel_size),
-                                               offset_scale=config.offset_scale, dropout=config.dropout)
+                                               offset_scale=config.offset_scale, dropout=config.dropout,
+                                               qk_norm=config.qk_norm, rotary_axes=config.rotary_axes,
+                                               rotary_theta=config.rotary_theta)
         self.norm2 = nn.LayerNorm(config.hidden_size, eps=1e-6)
-        self.mlp = MLP(config.hidden_size, config.mlp_hidden_size, config.dropout)
+        if config.gated_mlp:
+            self.mlp = GatedMLP(config.hidden_size, config.mlp_hidden_size, config.dropout, config.gated_activation)
+        else:
+            self.mlp = MLP(config.hidden_size, config.mlp_hidden_size, config.dropout)
         if config.use_text_conditioning:
             self.norm_cross = nn.LayerNorm(config.hidden_size, eps=1e-6)
             self.cross_attn = nn.MultiheadAttention(config.hidden_size, config.num_heads, dropout=config.dropout,

@@ -583,6 +583,8 @@ class TimeShardedDSA3D(nn.Module):
     def __init__(self, module: DeformableSlideAttention3D, group=None,
                  frame_ranges: Optional[Sequence[Range]] = None, speculative_window: bool = False):
         super().__init__()
+        if module.qk_norm or module.rotary_axes is not None:
+            raise NotImplementedError("TimeShardedDSA3D does not run modules with qk_norm or rotary_axes")
         self.module = module
         self.group = group
         self.frame_ranges = list(frame_ranges) if frame_ranges is not None else None

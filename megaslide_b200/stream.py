@@ -51,6 +51,7 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import _lib
+from .clip import clip_grad_norm_, grad_norm
 
 
 def _flat_params(module: nn.Module) -> List[nn.Parameter]:
@@ -490,14 +491,24 @@ class CPUMasterVideoDiT:
         cfg = self.config
         sq = sum(self.sumsq[i] for i in range(self.num_blocks) if self.has_grad[i])
         res_grads = [p.grad for p in self.res_params if p.grad is not None]
-        if res_grads:
+        fused = bool(getattr(cfg, "fused_clip", False)) and bool(res_grads)
+        if fused:
+            # norm over the blocks' host sums and the resident gradients, which are scaled by the same two kernels
+            for p in self.res_params:
+                if p.grad is not None and not p.grad.is_contiguous():
+                    p.grad = p.grad.contiguous()
+            res_grads = [p.grad for p in self.res_params if p.grad is not None]
+            clip = cfg.max_grad_norm > 0
+            norm = float(clip_grad_norm_(res_grads, cfg.max_grad_norm, extra_sumsq=sq) if clip else grad_norm(res_grads, extra_sumsq=sq))
+        elif res_grads:
             sq += float(torch.stack([g.float().square().sum() for g in res_grads]).sum())
-        norm = math.sqrt(sq)
+        if not fused:
+            norm = math.sqrt(sq)
         scale = 1.0
         if cfg.max_grad_norm > 0 and norm > cfg.max_grad_norm:
             scale = cfg.max_grad_norm / (norm + 1e-6)
         if res_grads:
-            if scale != 1.0:
+            if scale != 1.0 and not fused:
                 for g in res_grads:
                     g.mul_(scale)
             self.gpu_opt.step()
