@@ -329,14 +329,14 @@ typedef struct msl_ffn_geometry {
 } msl_ffn_geometry;
 
 /* Matrices are contiguous rows of their width except x, y, dy and dx (row strides given).  h [rows, hidden]
- * is the gated product that the second projection reads; gu [rows, 2*hidden] receives g and u, which the
- * backward reads (NULL = not kept).  Backward: dgu [rows, 2*hidden] is scratch (the gradients of g and u);
+ * is the gated product that the second projection reads; kept [rows, 2*hidden] receives u act'(g), then act(g),
+ * the factors the backward multiplies the gradient of h by (NULL = not kept).  Backward: dgu [rows, 2*hidden] is scratch (the gradients of g and u);
  * dx, dw_in, dw_out, db_in, db_out are written where they are not NULL. */
 typedef struct msl_ffn_io {
   const void* x; int64_t x_ld;
   const void* w_in; const void* b_in;
   const void* w_out; const void* b_out;
-  void* h; void* gu;
+  void* h; void* kept;
   void* y; int64_t y_ld;
   const void* dy; int64_t dy_ld;
   void* dgu;

@@ -2,7 +2,7 @@
 // widths that no 16-byte row allows), the bias gradients, and the entry points.
 //
 //   [g u] = x w_in^T + b_in;  h = act(g) u;  y = h w_out^T + b_out
-//   dh = dy w_out;  dg = dh u act'(g);  du = dh act(g);  dx = [dg du] w_in;  dw_in = [dg du]^T x;
+//   dh = dy w_out;  dg = dh (u act'(g));  du = dh act(g), of which the forward keeps the two factors;  dx = [dg du] w_in;  dw_in = [dg du]^T x;
 //   dw_out = dy^T h;  db_in, db_out = column sums of [dg du], dy
 
 #include <initializer_list>
@@ -74,18 +74,18 @@ __global__ void __launch_bounds__(256) product_simt_kernel(const Product P) {
       } else if (EPI == kGate) {
         const float g = acc[0][i][j] + (bias ? to_f32<T>(bias[n]) : 0.f);
         const float u = acc[NB - 1][i][j] + (bias ? to_f32<T>(bias[P.N + n]) : 0.f);
-        out[m * P.ldo + n] = from_f32<T>(act_value(g, P.act) * u);
-        if (P.gu_out) {
-          T* const gu = static_cast<T*>(P.gu_out) + m * 2 * P.N;
-          gu[n] = from_f32<T>(g);
-          gu[P.N + n] = from_f32<T>(u);
+        float da;
+        const float a = act_value_grad(g, P.act, da);
+        out[m * P.ldo + n] = from_f32<T>(a * u);
+        if (P.kept_out) {
+          T* const kept = static_cast<T*>(P.kept_out) + m * 2 * P.N;
+          kept[n] = from_f32<T>(u * da);
+          kept[P.N + n] = from_f32<T>(a);
         }
       } else {
-        const T* const gu = static_cast<const T*>(P.gu) + m * 2 * P.N;
-        float da;
-        const float a = act_value_grad(to_f32<T>(gu[n]), P.act, da);
-        out[m * 2 * P.N + n] = from_f32<T>(acc[0][i][j] * to_f32<T>(gu[P.N + n]) * da);
-        out[m * 2 * P.N + P.N + n] = from_f32<T>(acc[0][i][j] * a);
+        const T* const kept = static_cast<const T*>(P.kept) + m * 2 * P.N;
+        out[m * 2 * P.N + n] = from_f32<T>(acc[0][i][j] * to_f32<T>(kept[n]));
+        out[m * 2 * P.N + P.N + n] = from_f32<T>(acc[0][i][j] * to_f32<T>(kept[P.N + n]));
       }
     }
   }
@@ -345,7 +345,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.b = io->w_in; p.ldb = C;
   p.out = io->h; p.ldo = F;
   p.bias = io->b_in;
-  p.gu_out = io->gu;
+  p.kept_out = io->kept;
   p.M = M; p.N = F; p.K = C;
   rc = ffn::run(p, slots, 0, 1, s);
   if (rc) return rc;
@@ -376,7 +376,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   }
   const bool inner = io->dx || io->dw_in || io->db_in;  // wants the gradients of g and u
   if (!io->dy || io->dy_ld < C) return failf(MSL_ERR_INVALID, "dy (row stride >= dim) is required");
-  if (inner && (!io->w_out || !io->gu || !io->dgu)) return failf(MSL_ERR_INVALID, "w_out, gu and dgu are required");
+  if (inner && (!io->w_out || !io->kept || !io->dgu)) return failf(MSL_ERR_INVALID, "w_out, kept and dgu are required");
   if (io->dx && (!io->w_in || io->dx_ld < C)) return failf(MSL_ERR_INVALID, "dx needs w_in and a row stride >= dim");
   if (io->dw_in && (!io->x || io->x_ld < C)) return failf(MSL_ERR_INVALID, "dw_in needs x");
   if (io->dw_out && !io->h) return failf(MSL_ERR_INVALID, "dw_out needs h");
@@ -391,7 +391,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     p.a = io->dy; p.lda = io->dy_ld;
     p.b = io->w_out; p.ldb = F; p.b_major = true;  // [K = dim, N = hidden]
     p.out = io->dgu; p.ldo = 2 * F;
-    p.gu = io->gu;
+    p.kept = io->kept;
     p.M = M; p.N = F; p.K = C;
     rc = ffn::run(p, slots, 0, 2, s);
     if (rc) return rc;

@@ -13,8 +13,8 @@ namespace ffn {
 // What a product does with its result.
 enum Epilogue : int {
   kPlain = 0,  // out = acc + bias
-  kGate = 1,   // out = act(g) * u of the two accumulators g, u (bias added); gu receives g and u
-  kDgate = 2,  // acc is the gradient of h: dgu = [acc * u * act'(g), acc * act(g)] of the kept g, u
+  kGate = 1,   // out = act(g) * u of the two accumulators g, u (bias added); kept_out receives u act'(g) and act(g)
+  kDgate = 2,  // acc is the gradient of h: dgu = acc times each of the two kept values
 };
 
 // C[M, N] = sum_k A(m, k) B(n, k).  a_major / b_major: the contiguous axis is m / n instead of k (the operand
@@ -25,8 +25,8 @@ struct Product {
   long long lda, ldb, ldo;
   void* out;
   const void* bias;  // [N] (kGate: [2N]) or NULL
-  const void* gu;    // kDgate: kept g and u, [M, 2N]
-  void* gu_out;      // kGate: [M, 2N] or NULL
+  const void* kept;  // kDgate: u act'(g), then act(g), [M, 2N]
+  void* kept_out;    // kGate: [M, 2N] or NULL
   long long M, N, K;
   int dtype, act, epilogue;
   bool a_major, b_major;

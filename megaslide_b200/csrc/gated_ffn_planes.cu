@@ -39,9 +39,8 @@ struct Maps {
 
 struct Args {
   const void* bias;
-  const void* gu;
   void* out;
-  void* gu_out;
+  void* kept_out;
   long long M, N, ldo;
   int np, act;
   int kblocks, mt, nt, gm;
@@ -351,17 +350,33 @@ __global__ void __launch_bounds__(kThreads, 1) planes_kernel(const __grid_consta
                 acc[b][j] += bias_at<T>(P.bias, x + j);
                 acc[2 + b][j] += bias_at<T>(P.bias, P.N + x + j);
               }
-          if (P.gu_out) {
-            put_block<T>(tile, lane, acc[b], static_cast<T*>(P.gu_out), 2 * P.N, row0, x, P.M, P.N);
-            put_block<T>(tile, lane, acc[2 + b], static_cast<T*>(P.gu_out) + P.N, 2 * P.N, row0, x, P.M, P.N);
+          // g goes into the tile, the activation turns it into what the other projection is multiplied by
+          auto with_gate = [&](float (&v)[32], auto f) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) tile[lane * kPitch + j] = acc[b][j];
+            times_block(tile, lane, v, [&](int r) { return f(r, tile[r * kPitch + lane]); });
+          };
+          if (P.kept_out) {
+            T* const kept = static_cast<T*>(P.kept_out);
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = acc[2 + b][j];
+            with_gate(v, [&](int, float g) {
+              float da;
+              act_value_grad(g, P.act, da);
+              return da;
+            });
+            put_block<T>(tile, lane, v, kept, 2 * P.N, row0, x, P.M, P.N);
+            with_gate(acc[2 + b], [&](int r, float g) {
+              const float a = act_value(g, P.act);
+              if (row0 + r < P.M && x + lane < P.N) kept[(row0 + r) * 2 * P.N + P.N + x + lane] = from_f32<T>(a);
+              return a;
+            });
+          } else {
+            with_gate(acc[2 + b], [&](int, float g) { return act_value(g, P.act); });
           }
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) tile[lane * kPitch + j] = acc[b][j];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[b][j] = acc[2 + b][j];
-          times_block(tile, lane, acc[b], [&](int r) { return act_value(tile[r * kPitch + lane], P.act); });
-          put_block<T>(tile, lane, acc[b], static_cast<T*>(P.out), P.ldo, row0, x, P.M, P.N);
+          put_block<T>(tile, lane, acc[2 + b], static_cast<T*>(P.out), P.ldo, row0, x, P.M, P.N);
         }
       }
     }
@@ -403,30 +418,29 @@ __global__ void __launch_bounds__(256) planes_join_kernel(const __grid_constant_
     } else {
       v += bias_at<T>(P.bias, x);
       u += bias_at<T>(P.bias, P.N + x);
-      if (P.gu_out) {
-        static_cast<T*>(P.gu_out)[row * 2 * P.N + x] = from_f32<T>(v);
-        static_cast<T*>(P.gu_out)[row * 2 * P.N + P.N + x] = from_f32<T>(u);
+      float da;
+      const float a = act_value_grad(v, P.act, da);
+      if (P.kept_out) {
+        static_cast<T*>(P.kept_out)[row * 2 * P.N + x] = from_f32<T>(u * da);
+        static_cast<T*>(P.kept_out)[row * 2 * P.N + P.N + x] = from_f32<T>(a);
       }
-      static_cast<T*>(P.out)[row * P.ldo + x] = from_f32<T>(act_value(v, P.act) * u);
+      static_cast<T*>(P.out)[row * P.ldo + x] = from_f32<T>(a * u);
     }
   }
 }
 
-// The gradients of g and u from that of h, which the product has left in u's place: dgu [M, 2N], gu as kept.  Apart
-// from the product, whose epilogue holds up the sums that run through it (a kernel of its own costs one more
-// pass over the gradient of h; inside, 940 us instead of 350 at 4097 x 1152 x 4608 in float32).
+// The gradients of g and u from that of h, which the product has left in the second one's place: dgu [M, 2N], kept
+// likewise.  A kernel of its own: in the product's epilogue it would hold up the sums that run through there.
 template <typename T>
-__global__ void __launch_bounds__(256) dgate_kernel(const T* __restrict__ gu, T* dgu, long long M, long long N, int act) {
+__global__ void __launch_bounds__(256) dgate_kernel(const T* __restrict__ kept, T* dgu, long long M, long long N) {
   const long long row = blockIdx.x;
-  const T* const kept = gu + row * 2 * N;
+  const T* const by = kept + row * 2 * N;
   T* const out = dgu + row * 2 * N;
 #pragma unroll 4
   for (long long c = blockIdx.y * 256LL + threadIdx.x; c < N; c += gridDim.y * 256LL) {
     const float dh = to_f32<T>(out[N + c]);
-    float da;
-    const float a = act_value_grad(to_f32<T>(kept[c]), act, da);
-    out[c] = from_f32<T>(dh * to_f32<T>(kept[N + c]) * da);
-    out[N + c] = from_f32<T>(dh * a);
+    out[c] = from_f32<T>(dh * to_f32<T>(by[c]));
+    out[N + c] = from_f32<T>(dh * to_f32<T>(by[N + c]));
   }
 }
 
@@ -489,9 +503,8 @@ cudaError_t launch(const Product& p, const void* pa, const void* pb, cudaStream_
   if (cut.bytes > p.partial_bytes) return cudaErrorInvalidValue;
   Args a{};
   a.bias = p.bias;
-  a.gu = p.gu;
   a.out = p.out;
-  a.gu_out = p.gu_out;
+  a.kept_out = p.kept_out;
   a.M = p.M;
   a.N = p.N;
   a.ldo = p.ldo;
@@ -594,9 +607,9 @@ cudaError_t launch_product_planes(const Product& p0, const void* pa, const void*
     const long long cols = (p.N + 1023) / 1024;
     const dim3 grid(static_cast<unsigned>(p.M), static_cast<unsigned>(cols < 64 ? cols : 64));
     if (p.dtype == MSL_DTYPE_F32)
-      planes::dgate_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(p.gu), static_cast<float*>(p0.out), p.M, p.N, p.act);
+      planes::dgate_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(p.kept), static_cast<float*>(p0.out), p.M, p.N);
     else
-      planes::dgate_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(p.gu), static_cast<__nv_bfloat16*>(p0.out), p.M, p.N, p.act);
+      planes::dgate_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(p.kept), static_cast<__nv_bfloat16*>(p0.out), p.M, p.N);
     count_launches(1);
     return cudaGetLastError();
   }

@@ -13,16 +13,22 @@
 // finished sums into results while the next tile is multiplied into the other half of the tensor memory.  The
 // pairs walk over the tiles, one pair per two SMs.
 //   gate:  the tile's columns are BN/2 gate columns (the first CTA's half of B) and the same columns of the other
-//          projection, so g and u of an element meet in one epilogue thread: bias, activation, product, and the
-//          kept g, u leave from there
-//   dgate: the sums are the gradient of h; the epilogue fetches the kept g, u by TMA, a step ahead, and
-//          writes both their gradients over them in shared memory, from where they leave
+//          projection, so g and u of an element meet in one epilogue thread: bias, activation and product; for
+//          the backward it also keeps u act'(g) and act(g), rounded to bf16 once each (g and u themselves would
+//          be rounded before the activation's derivative, and cost the backward the activation again)
+//   dgate: the sums are the gradient of h; the epilogue fetches the two kept factors by TMA, a step ahead, and
+//          writes the gradients of g and u over them in shared memory, from where they leave
 //
 // Tiles that do not fill a last round of all pairs are cut along k among the pairs left over: their parts' sums
 // go to the workspace in float32 and a small kernel joins them, in order, and does the epilogue.
 //
-// What bounds it: the multiplications.  One CTA alone on 128 x 256 tiles fills its shared memory's bandwidth (48 KB
-// in and out for 512 clocks of multiplication); the pair needs 32 KB.
+// What bounds it: an SM takes in about 63 bytes a clock, 520 clocks for the 32 KB of a stage, whose multiplications
+// take 512; with both that near, a stage takes 620 to 680 clocks (82% of the tensor cores; 128 x 256 tiles of one CTA
+// alone need 48 KB).  Where k is short the epilogue's bytes share that path: with 18 stages a tile (k = 1152) the gate's
+// results are 17% more and its stage takes 900 clocks, dgate's kept factors and results 44% more.  16 epilogue warps
+// instead of 8, or a second loading thread, change nothing.  In long runs the power limit holds the clock near
+// 1.4 to 1.6 GHz.  4096 x 7168 x 28672: 1.25 to 1.31 PFLOP/s a product; 32768 x 1152 x 4608: 1.13 (gate), 0.92
+// (dgate), 1.25 (the others).
 
 #include "gated_ffn.cuh"
 #include "tcgen05.cuh"
@@ -43,7 +49,7 @@ constexpr int kRing = 5 * 2 * kStageA;  // shared memory of the stages
 constexpr int kMaxStages = 8;
 
 struct Maps {
-  CUtensorMap a, b, out, gu;
+  CUtensorMap a, b, out, kept;
 };
 
 struct Args {
@@ -263,12 +269,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const int col0 = n * width;
       const uint32_t acc = tmem + buf * kAcc + lanes;
       const bool rows_in = row0 < P.M;  // a box wholly outside is not started
-      // dgate: the staging buffer holds g and u of two steps
+      // dgate: the staging buffer holds the kept factors of two steps
       auto fetch = [&](uint32_t at, int i) {
         const uint32_t to = mine + (at & 1) * 2 * kTile, bar = mykept + 8 * (at & 1);
         mbar_expect(bar, 2 * kTile);
-        tma_load_3d(to, &maps.gu, bar, col0 + i * 32, 0, row0);
-        tma_load_3d(to + kTile, &maps.gu, bar, col0 + i * 32, 1, row0);
+        tma_load_3d(to, &maps.kept, bar, col0 + i * 32, 0, row0);
+        tma_load_3d(to + kTile, &maps.kept, bar, col0 + i * 32, 1, row0);
       };
       if (EPI == kDgate && lane == 0 && first < last && w.part < 0) {  // on their way while the tile is still multiplied
         bulk_wait_read<0>();                             // the last tile's results have left
@@ -306,11 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             uint32_t dg[4], du[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float d0, d1;
-              const float a0 = act_grad_fast<ACT>(bf16_lo(gw[j]), d0), a1 = act_grad_fast<ACT>(bf16_hi(gw[j]), d1);
               const float h0 = v[q * 8 + 2 * j], h1 = v[q * 8 + 2 * j + 1];
-              dg[j] = pack(h0 * bf16_lo(uw[j]) * d0, h1 * bf16_hi(uw[j]) * d1);
-              du[j] = pack(h0 * a0, h1 * a1);
+              dg[j] = pack(h0 * bf16_lo(gw[j]), h1 * bf16_hi(gw[j]));
+              du[j] = pack(h0 * bf16_lo(uw[j]), h1 * bf16_hi(uw[j]));
             }
             sts(chunk32(g0, lane, q), dg);
             sts(chunk32(u0, lane, q), du);
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             fetch(turn + 2, i + 2);
           }
         } else if (EPI == kGate) {
-          // the staging tiles in turn: h, g, u of this step (kept), or h alone
+          // staging tiles: the two kept factors, and h in turn in the two others
           float u[32];
           tmem_ld32(acc + half + c, u);
           if (P.bias) {
@@ -335,24 +339,33 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             add_bias(u, P.bias + P.N, x, P.N);
           }
           if (P.keep) {
+            float d[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float da;
+              v[j] = act_grad_fast<ACT>(v[j], da);
+              d[j] = u[j] * da;
+            }
             if (lane == 0) bulk_wait_read<0>();
             __syncwarp();
-            stage(mine, lane, v);
-            stage(mine + kTile, lane, u);
+            stage(mine, lane, d);
+            stage(mine + kTile, lane, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= u[j];
           } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_fast<ACT>(v[j]) * u[j];
             if (lane == 0) bulk_wait_read<1>();
             __syncwarp();
           }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = act_fast<ACT>(v[j]) * u[j];
           const uint32_t to = mine + (2 + (turn & 1)) * kTile;
           stage(to, lane, v);
           fence_async();
           __syncwarp();
           if (store) {
             if (P.keep) {
-              tma_store_3d(&maps.gu, mine, x, 0, row0);
-              tma_store_3d(&maps.gu, mine + kTile, x, 1, row0);
+              tma_store_3d(&maps.kept, mine, x, 0, row0);
+              tma_store_3d(&maps.kept, mine + kTile, x, 1, row0);
             }
             tma_store_2d(&maps.out, to, x, row0);
           }
@@ -403,8 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 struct JoinArgs {
   Args tc;
   __nv_bfloat16* out;
-  const __nv_bfloat16* gu;
-  __nv_bfloat16* gu_out;
+  const __nv_bfloat16* kept;
+  __nv_bfloat16* kept_out;
   long long ldo;
 };
 
@@ -455,25 +468,30 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ JoinA
   if (EPI == kGate && P.bias) add_bias8(u, P.bias + P.N + x);
   if (row >= P.M) return;
   if (EPI == kGate) {
-    if (J.gu_out) {
-      put8(J.gu_out + row * 2 * P.N + x, v);
-      put8(J.gu_out + row * 2 * P.N + P.N + x, u);
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float da;
+      v[j] = act_grad_fast<ACT>(v[j], da);
+      d[j] = u[j] * da;
+    }
+    if (J.kept_out) {
+      put8(J.kept_out + row * 2 * P.N + x, d);
+      put8(J.kept_out + row * 2 * P.N + P.N + x, v);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = act_fast<ACT>(v[j]) * u[j];
+    for (int j = 0; j < 8; ++j) v[j] *= u[j];
   }
   if (EPI == kDgate) {
-    const __nv_bfloat16* const kept = J.gu + row * 2 * P.N + x;
+    const __nv_bfloat16* const kept = J.kept + row * 2 * P.N + x;
     const uint4 gv = __ldg(reinterpret_cast<const uint4*>(kept)), uv = __ldg(reinterpret_cast<const uint4*>(kept + P.N));
     const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float d0, d1;
-      const float a0 = act_grad_fast<ACT>(bf16_lo(gw[j]), d0), a1 = act_grad_fast<ACT>(bf16_hi(gw[j]), d1);
-      u[2 * j] = v[2 * j] * a0;
-      u[2 * j + 1] = v[2 * j + 1] * a1;
-      v[2 * j] = v[2 * j] * bf16_lo(uw[j]) * d0;
-      v[2 * j + 1] = v[2 * j + 1] * bf16_hi(uw[j]) * d1;
+      u[2 * j] = v[2 * j] * bf16_lo(uw[j]);
+      u[2 * j + 1] = v[2 * j + 1] * bf16_hi(uw[j]);
+      v[2 * j] *= bf16_lo(gw[j]);
+      v[2 * j + 1] *= bf16_hi(gw[j]);
     }
     put8(J.out + row * 2 * P.N + x, v);
     put8(J.out + row * 2 * P.N + P.N + x, u);
@@ -562,10 +580,10 @@ cudaError_t launch(const Product& p, cudaStream_t s) {
   bool ok = AM ? matrix_map(&maps.a, p.a, p.K, p.M, p.lda, kBK) : matrix_map(&maps.a, p.a, p.M, p.K, p.lda, kBM);
   const long long brows = EPI == kGate ? 2 * p.N : p.N;
   ok = ok && (BM ? matrix_map(&maps.b, p.b, p.K, p.N, p.ldb, kBK) : matrix_map(&maps.b, p.b, brows, p.K, p.ldb, a.bn / 2));
-  if (EPI == kDgate) ok = ok && pair_map(&maps.out, p.out, p.M, p.N) && pair_map(&maps.gu, p.gu, p.M, p.N);
+  if (EPI == kDgate) ok = ok && pair_map(&maps.out, p.out, p.M, p.N) && pair_map(&maps.kept, p.kept, p.M, p.N);
   else ok = ok && matrix_map(&maps.out, p.out, p.M, p.N, p.ldo, 32, 32);
-  if (EPI == kGate && p.gu_out) ok = ok && pair_map(&maps.gu, p.gu_out, p.M, p.N);
-  else if (EPI != kDgate) maps.gu = maps.out;
+  if (EPI == kGate && p.kept_out) ok = ok && pair_map(&maps.kept, p.kept_out, p.M, p.N);
+  else if (EPI != kDgate) maps.kept = maps.out;
   if (!ok) return cudaErrorInvalidValue;
   a.bias = static_cast<const __nv_bfloat16*>(p.bias);
   a.M = p.M;
@@ -574,7 +592,7 @@ cudaError_t launch(const Product& p, cudaStream_t s) {
   a.mt = static_cast<int>(cut.mt);
   a.nt = static_cast<int>(cut.nt);
   a.gm = a.mt <= 16 ? a.mt : 8;  // rows of tiles that go together: their operands stay in the L2 cache
-  a.keep = p.gu_out != nullptr;
+  a.keep = p.kept_out != nullptr;
   a.status = p.status;
   constexpr int smem = 1024 + kRing + kEpiWarps * kStaging + 24 * kMaxStages + 16 * kEpiWarps + 64;
   static_assert(smem <= 232448, "shared memory of a block");
@@ -595,7 +613,7 @@ cudaError_t launch(const Product& p, cudaStream_t s) {
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kernel, maps, a);
   if (e != cudaSuccess || a.items == a.full) return e;
-  JoinArgs j{a, static_cast<__nv_bfloat16*>(p.out), static_cast<const __nv_bfloat16*>(p.gu), static_cast<__nv_bfloat16*>(p.gu_out), p.ldo};
+  JoinArgs j{a, static_cast<__nv_bfloat16*>(p.out), static_cast<const __nv_bfloat16*>(p.kept), static_cast<__nv_bfloat16*>(p.kept_out), p.ldo};
   const int steps = (EPI == kGate ? a.bn / 2 : a.bn) / 32;
   join_kernel<EPI, ACT><<<dim3((a.mt * a.nt - a.full) * steps, 2), 512, 0, s>>>(j);
   count_launches(1);
@@ -609,7 +627,7 @@ bool tc_applies(const Product& p) {
   if (p.dtype != MSL_DTYPE_BF16 || !t5::encoder()) return false;
   if (!multiple_of(p.a, 16) || !multiple_of(p.b, 16) || !multiple_of(p.out, 16) || p.lda % 8 || p.ldb % 8 || p.ldo % 8 || p.N % 8) return false;
   if (p.bias && !multiple_of(p.bias, 16)) return false;
-  if ((p.gu && !multiple_of(p.gu, 16)) || (p.gu_out && !multiple_of(p.gu_out, 16))) return false;
+  if ((p.kept && !multiple_of(p.kept, 16)) || (p.kept_out && !multiple_of(p.kept_out, 16))) return false;
   if (p.M > (1LL << 31) - 256 || p.N > (1LL << 30) || p.K > (1LL << 31) - 256) return false;
   if ((p.M + 127) / 128 * ((p.N + 63) / 64) > (1LL << 30)) return false;
   return true;
@@ -625,7 +643,7 @@ cudaError_t launch_product_tc(const Product& p, cudaStream_t s) {
     case kGate:
       return silu ? tc::launch<kGate, false, false, MSL_ACT_SILU>(p, s) : tc::launch<kGate, false, false, MSL_ACT_GELU>(p, s);
     case kDgate:
-      return silu ? tc::launch<kDgate, false, true, MSL_ACT_SILU>(p, s) : tc::launch<kDgate, false, true, MSL_ACT_GELU>(p, s);
+      return tc::launch<kDgate, false, true, 0>(p, s);
     default:
       if (p.a_major) return tc::launch<kPlain, true, true, 0>(p, s);
       return p.b_major ? tc::launch<kPlain, false, true, 0>(p, s) : tc::launch<kPlain, false, false, 0>(p, s);

@@ -3,10 +3,10 @@
     y = (act(x Wg^T + bg) * (x Wu^T + bu)) w_out^T + b_out,   w_in = [Wg; Wu]
 
 Both projections, their biases, the activation and the product are one kernel; the second projection is another.
-The backward keeps the two projections and the gated product, and is one kernel for the gradients of the
-projections (product with w_out, the activation's derivative and the products) and one for each of dx, dw_in and
+For the backward the first also writes two factors of every hidden element, u act'(g) and act(g); the backward is one
+kernel for the gradients of the projections (dy w_out, times the two factors) and one for each of dx, dw_in and
 dw_out.  float32 or bfloat16 operands, float32 sums; the intermediate results are rounded to the operands' type,
-in which the next product reads them.
+in which the next product reads them.  (float32, and widths that are no multiple of 8, take a few more kernels.)
 """
 
 from __future__ import annotations
@@ -34,16 +34,16 @@ class GatedFFNFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, activation):
         x2 = _rows_of(x)
-        y, h, gu = ops.gated_ffn_fwd(x2, w_in, w_out, b_in, b_out, activation, keep=True)
-        ctx.save_for_backward(x2, w_in, w_out, b_in, b_out, h, gu)
+        y, h, kept = ops.gated_ffn_fwd(x2, w_in, w_out, b_in, b_out, activation, keep=True)
+        ctx.save_for_backward(x2, w_in, w_out, b_in, b_out, h, kept)
         ctx.activation = activation
         ctx.x_shape = x.shape
         return y if y.shape == x.shape else y.view(x.shape)
 
     @staticmethod
     def backward(ctx, dy):
-        x2, w_in, w_out, b_in, b_out, h, gu = ctx.saved_tensors
-        dx, dw_in, dw_out, db_in, db_out = ops.gated_ffn_bwd(x2, w_in, w_out, h, gu, _rows_of(dy), b_in, b_out, ctx.activation,
+        x2, w_in, w_out, b_in, b_out, h, kept = ctx.saved_tensors
+        dx, dw_in, dw_out, db_in, db_out = ops.gated_ffn_bwd(x2, w_in, w_out, h, kept, _rows_of(dy), b_in, b_out, ctx.activation,
                                                              needs=ctx.needs_input_grad[:5])
         return dx.view(ctx.x_shape) if dx is not None and dx.shape != ctx.x_shape else dx, dw_in, dw_out, db_in, db_out, None
 

@@ -715,17 +715,17 @@ def _ffn_check(x, w_in, w_out, b_in, b_out) -> Tuple[int, int, int]:
 def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
                   b_out: Optional[torch.Tensor] = None, activation: str = "silu", keep: bool = False,
                   status: Optional[torch.Tensor] = None):
-    """Gated feed-forward block on x [rows, >= dim] (row view).  Returns (y, h, gu): h [rows, hidden] the gated
-    product, gu [rows, 2 * hidden] the two projections where ``keep`` (for the backward), else None.  status: a
+    """Gated feed-forward block on x [rows, >= dim] (row view).  Returns (y, h, kept): h [rows, hidden] the gated
+    product, kept [rows, 2 * hidden] what the backward needs (u act'(g), then act(g)) where ``keep``, else None.  status: a
     device word for MSL_STATUS_TIMEOUT in place of the device's HostFlag."""
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
     dev, dt = x.device, x.dtype
     g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation))
     x_ld = _ld(x, "x")
     h = torch.empty(M, F, device=dev, dtype=dt)
-    gu = torch.empty(M, 2 * F, device=dev, dtype=dt) if keep else None
+    kept = torch.empty(M, 2 * F, device=dev, dtype=dt) if keep else None
     y = torch.empty(x.shape, device=dev, dtype=dt)
-    io = _lib.FfnIO(x.data_ptr(), x_ld, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out), h.data_ptr(), _ptr(gu),
+    io = _lib.FfnIO(x.data_ptr(), x_ld, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out), h.data_ptr(), _ptr(kept),
                     y.data_ptr(), C)
     io.status = _flag(dev, status)
     lib = _lib.load()
@@ -735,15 +735,15 @@ def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in
         rc = _call("msl_gated_ffn_fwd", dev, lambda: lib.msl_gated_ffn_fwd(
             ctypes.byref(g), ctypes.byref(io), _ptr(ws), need, _raw_stream(dev.index)))
     _lib.check("msl_gated_ffn_fwd", rc)
-    return y, h, gu
+    return y, h, kept
 
 
-def gated_ffn_bwd(x, w_in, w_out, h, gu, dy, b_in=None, b_out=None, activation: str = "silu",
+def gated_ffn_bwd(x, w_in, w_out, h, kept, dy, b_in=None, b_out=None, activation: str = "silu",
                   needs=(True, True, True, True, True), status: Optional[torch.Tensor] = None):
     """Backward of gated_ffn_fwd(keep=True): (dx, dw_in, dw_out, db_in, db_out); ``needs`` says which are computed
     (the others, and those of biases that are None, are None)."""
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
-    _need_cuda(h, gu, dy)
+    _need_cuda(h, kept, dy)
     dev, dt = x.device, x.dtype
     needs = (needs[0], needs[1], needs[2], needs[3] and b_in is not None, needs[4] and b_out is not None)
     dx = torch.empty(x.shape, device=dev, dtype=dt) if needs[0] else None
@@ -753,7 +753,7 @@ def gated_ffn_bwd(x, w_in, w_out, h, gu, dy, b_in=None, b_out=None, activation: 
     db_out = torch.empty_like(b_out) if needs[4] else None
     dgu = torch.empty(M, 2 * F, device=dev, dtype=dt) if needs[0] or needs[1] or needs[3] else None
     g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation))
-    io = _lib.FfnIO(x.data_ptr(), _ld(x, "x"), w_in.data_ptr(), None, w_out.data_ptr(), None, h.data_ptr(), gu.data_ptr(), None, 0,
+    io = _lib.FfnIO(x.data_ptr(), _ld(x, "x"), w_in.data_ptr(), None, w_out.data_ptr(), None, h.data_ptr(), kept.data_ptr(), None, 0,
                     dy.data_ptr(), _ld(dy, "dy"), _ptr(dgu), _ptr(dx), C, _ptr(dw_in), _ptr(dw_out), _ptr(db_in), _ptr(db_out),
                     _flag(dev, status))
     lib = _lib.load()
