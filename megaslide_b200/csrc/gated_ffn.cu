@@ -200,9 +200,12 @@ struct Slots {
   const void* of[3];
 };
 
-static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStream_t s) {
+static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStream_t s, bool rows = false) {
   cudaError_t e;
-  if (tc_applies(p)) {
+  if (rows) {
+    e = launch_product_rows(p, s);
+    if (e != cudaSuccess) return cuda_failf(e, "rows_kernel launch");
+  } else if (tc_applies(p)) {
     e = launch_product_tc(p, s);
     if (e != cudaSuccess) return cuda_failf(e, "product_kernel launch");
   } else if (slots.at[0] && planes_apply(p)) {
@@ -347,7 +350,10 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.bias = io->b_in;
   p.kept_out = io->kept;
   p.M = M; p.N = F; p.K = C;
-  rc = ffn::run(p, slots, 0, 1, s);
+  // both products by rows, or neither: the second is launched into the first
+  const bool rows = ffn::rows_apply(p) && multiple_of(io->h, 16) && multiple_of(io->w_out, 16) &&
+                    F * (geom->dtype == MSL_DTYPE_BF16 ? 2 : 4) % 16 == 0;
+  rc = ffn::run(p, slots, 0, 1, s, rows);
   if (rc) return rc;
   p = ffn::product(geom, io, W, workspace);
   p.epilogue = ffn::kPlain;
@@ -356,7 +362,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.out = io->y; p.ldo = io->y_ld;
   p.bias = io->b_out;
   p.M = M; p.N = C; p.K = F;
-  return ffn::run(p, slots, 0, 1, s);
+  return ffn::run(p, slots, 0, 1, s, rows);
 }
 
 int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,

@@ -98,6 +98,10 @@ bool tc_applies(const Product& p);
 size_t tc_partial_bytes(long long M, long long N, long long K, int epilogue, bool b_major);
 cudaError_t launch_product_tc(const Product& p, cudaStream_t s);
 
+// Form for a few rows (gated_ffn_rows.cu): the forward's two products, launched one after the other.
+constexpr int kMostRows = 16, kMostRowsF32 = 8;
+bool rows_apply(const Product& p);
+cudaError_t launch_product_rows(const Product& p, cudaStream_t s);
 // Tensor-core form for float32 and for widths that are no multiple of 8 (gated_ffn_planes.cu): the operands as
 // planes [planes][rows][cols padded to 8] of planes_bytes, written by launch_planes from rows as they are stored.
 bool planes_apply(const Product& p);

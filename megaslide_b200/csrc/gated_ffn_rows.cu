@@ -1,0 +1,302 @@
+// The gated feed-forward block's forward products for a few rows (single tokens up to kMostRows): the weights are
+// read once, at the speed of the memory, and the rows of x stay in the caches.
+//
+// One row of bf16, or up to 8 of float32: a warp takes two rows of the weights (the gate's and the other
+// projection's of one hidden element, or two of the second projection) and all rows of x; its lanes split k in
+// 16-byte loads, four of each weight row in flight before the first is used.  More rows of bf16: mma.sync, below.
+// Where there are fewer pairs of rows than warps the GPU holds, several warps share a pair's k.  Sums are float32,
+// joined in a fixed order.  The second projection is launched so that it may start while the first still
+// runs: it loads weights first and waits for h only then.
+//
+// What bounds it: 1 x 1152 x 4608 in bf16 (32 MB of weights, which the L2 cache holds) 6.8 and 6.2 us, 8 rows 7.4 and
+// 8.0: the launches and one trip to the cache; 1 x 7168 x 28672 (1.23 GB) the memory, 131 us for the first
+// projection's 822 MB, 6.3 TB/s (by mma.sync 165 us, so one row does without; at the small size they are
+// even).  The tensor cores' own form takes 24 us and 260 us for 17 rows.
+
+#include "gated_ffn.cuh"
+
+namespace msl {
+namespace ffn {
+namespace rows {
+
+constexpr int kWarps = 8;
+
+struct Args {
+  const void* a;
+  const void* b;
+  const void* bias;
+  void* out;
+  void* kept_out;
+  long long lda, ldb, ldo, N;
+  int M, K, act, share;  // warps that share a pair of weight rows
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void dot(float& acc, const uint4& w, const uint4& x) {
+  const T* const a = reinterpret_cast<const T*>(&w);
+  const T* const b = reinterpret_cast<const T*>(&x);
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc = fmaf(to_f32<T>(a[i]), to_f32<T>(b[i]), acc);
+}
+
+template <typename T, int MR, int EPI>
+__global__ void __launch_bounds__(32 * kWarps) rows_kernel(const __grid_constant__ Args P) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), U = MR > 4 ? 2 : 4;
+  __shared__ float part[kWarps][2 * MR];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int slot = warp % P.share;
+  const long long pair = static_cast<long long>(blockIdx.x) * (kWarps / P.share) + warp / P.share;
+  const long long n0 = EPI == kGate ? pair : 2 * pair, n1 = EPI == kGate ? P.N + pair : 2 * pair + 1;
+  const bool in = n0 < P.N, in1 = EPI == kGate ? in : n1 < P.N;
+  const uint4* const w0 = reinterpret_cast<const uint4*>(static_cast<const T*>(P.b) + (in ? n0 : 0) * P.ldb);
+  const uint4* const w1 = reinterpret_cast<const uint4*>(static_cast<const T*>(P.b) + (in1 ? n1 : 0) * P.ldb);
+  const int words = P.K / V, step = 32 * P.share;
+  float acc[2][MR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) acc[0][m] = acc[1][m] = 0.f;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  bool waited = EPI == kGate;
+  for (int c = slot * 32 + lane; c - lane < words; c += U * step) {
+    uint4 w[2][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool have = in && c + u * step < words;
+      w[0][u] = have ? __ldg(w0 + c + u * step) : zero;
+      w[1][u] = have ? __ldg(w1 + c + u * step) : zero;
+    }
+    if (!waited) {  // h is the kernel's before
+      cudaGridDependencySynchronize();
+      waited = true;
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      if (m >= P.M) break;
+      const uint4* const x = reinterpret_cast<const uint4*>(static_cast<const T*>(P.a) + m * P.lda);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c + u * step >= words) continue;
+        const uint4 v = x[c + u * step];
+        dot<T, V>(acc[0][m], w[0][u], v);
+        dot<T, V>(acc[1][m], w[1][u], v);
+      }
+    }
+  }
+  if (EPI == kGate) cudaTriggerProgrammaticLaunchCompletion();
+  else if (!waited) cudaGridDependencySynchronize();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      float t = acc[i][m];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kFull, t, o);
+      if (lane == 0) part[warp][i * MR + m] = t;
+    }
+  __syncthreads();
+  if (slot != 0 || !in || lane >= P.M) return;
+  float s[2] = {0.f, 0.f};
+  for (int k = 0; k < P.share; ++k) {
+    s[0] += part[warp + k][lane];
+    s[1] += part[warp + k][MR + lane];
+  }
+  const T* const bias = static_cast<const T*>(P.bias);
+  if (bias) {
+    s[0] += to_f32<T>(bias[n0]);
+    if (in1) s[1] += to_f32<T>(bias[n1]);
+  }
+  T* const out = static_cast<T*>(P.out) + lane * P.ldo;
+  if (EPI == kGate) {
+    float da;
+    const float a = act_value_grad(s[0], P.act, da);
+    out[n0] = from_f32<T>(a * s[1]);
+    if (P.kept_out) {
+      T* const kept = static_cast<T*>(P.kept_out) + lane * 2 * P.N;
+      kept[n0] = from_f32<T>(s[1] * da);
+      kept[P.N + n0] = from_f32<T>(a);
+    }
+  } else {
+    out[n0] = from_f32<T>(s[0]);
+    if (in1) out[n1] = from_f32<T>(s[1]);
+  }
+}
+
+template <typename T, int MR, int EPI>
+cudaError_t launch(const Args& a, cudaStream_t s) {
+  const long long pairs = EPI == kGate ? a.N : (a.N + 1) / 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((pairs + kWarps / a.share - 1) / (kWarps / a.share)));
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = EPI == kGate ? 0 : 1;
+  return cudaLaunchKernelEx(&cfg, rows_kernel<T, MR, EPI>, a);
+}
+
+template <typename T, int EPI>
+cudaError_t by_rows(const Args& a, cudaStream_t s) {
+  if (a.M == 1) return launch<T, 1, EPI>(a, s);
+  if (a.M == 2) return launch<T, 2, EPI>(a, s);
+  return a.M <= 4 ? launch<T, 4, EPI>(a, s) : launch<T, 8, EPI>(a, s);
+}
+
+// bf16, up to 8 * NT rows: 16 rows of the weights a warp (the gate: 8 hidden elements, rows 0-7 the gate's and 8-15
+// the other projection's, so both end in one thread) against the rows of x, by mma.sync.  A thread's fragments
+// are 16 adjacent bytes of a row: the same 8 k of the weights and of x, in whatever place the instruction's own
+// order of k has them, so nothing is shuffled or converted.  (tcgen05 would need 128 rows of operands in shared
+// memory for this; here the memory is the limit.)
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kMmaWarps = 16;
+
+template <int NT, int EPI>
+__global__ void __launch_bounds__(32 * kMmaWarps) rows_mma_kernel(const __grid_constant__ Args P) {
+  using T = __nv_bfloat16;
+  constexpr int U = 4;
+  __shared__ float part[kMmaWarps][NT * 4][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int slot = warp % P.share;
+  const long long group = static_cast<long long>(blockIdx.x) * (kMmaWarps / P.share) + warp / P.share;
+  const long long n0 = EPI == kGate ? group * 8 + g : group * 16 + g, n1 = EPI == kGate ? P.N + n0 : n0 + 8;
+  const bool in0 = n0 < P.N, in1 = EPI == kGate ? in0 : n1 < P.N;
+  const T* const w0 = static_cast<const T*>(P.b) + (in0 ? n0 : 0) * P.ldb + t * 8;
+  const T* const w1 = static_cast<const T*>(P.b) + (in1 ? n1 : 0) * P.ldb + t * 8;
+  const T* const x = static_cast<const T*>(P.a) + t * 8;
+  float acc[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  bool waited = EPI == kGate;
+  const int hop = 32 * P.share;
+  for (int k = slot * 32; k < P.K; k += U * hop) {
+    uint4 a[2][U], b[NT][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = k + u * hop;
+      const bool have = at + t * 8 < P.K;
+      a[0][u] = have && in0 ? __ldg(reinterpret_cast<const uint4*>(w0 + at)) : zero;
+      a[1][u] = have && in1 ? __ldg(reinterpret_cast<const uint4*>(w1 + at)) : zero;
+    }
+    if (!waited) {  // h is the kernel's before
+      cudaGridDependencySynchronize();
+      waited = true;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int at = k + u * hop;
+        b[i][u] = at + t * 8 < P.K && i * 8 + g < P.M ? *reinterpret_cast<const uint4*>(x + (i * 8 + g) * P.lda + at) : zero;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        mma16816(acc[i], a[0][u].x, a[1][u].x, a[0][u].y, a[1][u].y, b[i][u].x, b[i][u].y);
+        mma16816(acc[i], a[0][u].z, a[1][u].z, a[0][u].w, a[1][u].w, b[i][u].z, b[i][u].w);
+      }
+  }
+  if (EPI == kGate) cudaTriggerProgrammaticLaunchCompletion();
+  else if (!waited) cudaGridDependencySynchronize();
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[warp][i * 4 + j][lane] = acc[i][j];
+  __syncthreads();
+  if (slot != 0) return;
+  const T* const bias = static_cast<const T*>(P.bias);
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int m = i * 8 + t * 2 + j;
+      if (m >= P.M) continue;
+      float v0 = 0.f, v1 = 0.f;  // weight rows g and g + 8
+      for (int k = 0; k < P.share; ++k) {
+        v0 += part[warp + k][i * 4 + j][lane];
+        v1 += part[warp + k][i * 4 + 2 + j][lane];
+      }
+      if (bias) {
+        v0 += in0 ? to_f32<T>(bias[n0]) : 0.f;
+        v1 += in1 ? to_f32<T>(bias[n1]) : 0.f;
+      }
+      T* const out = static_cast<T*>(P.out) + m * P.ldo;
+      if (EPI == kGate) {
+        if (!in0) continue;
+        float da;
+        const float a = P.act == MSL_ACT_SILU ? act_grad_fast<MSL_ACT_SILU>(v0, da) : act_grad_fast<MSL_ACT_GELU>(v0, da);
+        out[n0] = from_f32<T>(a * v1);
+        if (P.kept_out) {
+          T* const kept = static_cast<T*>(P.kept_out) + m * 2LL * P.N;
+          kept[n0] = from_f32<T>(v1 * da);
+          kept[P.N + n0] = from_f32<T>(a);
+        }
+      } else {
+        if (in0) out[n0] = from_f32<T>(v0);
+        if (in1) out[n1] = from_f32<T>(v1);
+      }
+    }
+}
+
+template <int NT, int EPI>
+cudaError_t launch_mma(Args a, cudaStream_t s) {
+  const long long per = EPI == kGate ? 8 : 16, groups = (a.N + per - 1) / per;
+  a.share = 1;
+  while (a.share < kMmaWarps && groups * a.share < 24LL * sm_count() && a.K > 64 * a.share) a.share *= 2;
+  const int each = kMmaWarps / a.share;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((groups + each - 1) / each));
+  cfg.blockDim = dim3(32 * kMmaWarps);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = EPI == kGate ? 0 : 1;
+  return cudaLaunchKernelEx(&cfg, rows_mma_kernel<NT, EPI>, a);
+}
+
+}  // namespace rows
+
+bool rows_apply(const Product& p) {
+  const long long es = p.dtype == MSL_DTYPE_BF16 ? 2 : 4;
+  // 9 to 16 rows only while the caches hold the weights (7168 x 28672: 390 us for 16, against 260 on the tensor cores)
+  const long long most = p.dtype == MSL_DTYPE_F32 ? kMostRowsF32 : p.N * p.K * (p.epilogue == kGate ? 2 : 1) < (1LL << 25) ? kMostRows : kMostRows / 2;
+  return p.M <= most && !p.a_major && !p.b_major && p.epilogue != kDgate && p.K * es % 16 == 0 && p.lda * es % 16 == 0 &&
+         p.ldb * es % 16 == 0 && multiple_of(p.a, 16) && multiple_of(p.b, 16) && p.K <= (1 << 30) && p.N <= (1 << 30);
+}
+
+cudaError_t launch_product_rows(const Product& p, cudaStream_t s) {
+  rows::Args a{};
+  a.a = p.a; a.lda = p.lda;
+  a.b = p.b; a.ldb = p.ldb;
+  a.bias = p.bias;
+  a.out = p.out; a.ldo = p.ldo;
+  a.kept_out = p.kept_out;
+  a.N = p.N;
+  a.M = static_cast<int>(p.M);
+  a.K = static_cast<int>(p.K);
+  a.act = p.act;
+  // warps enough for every SM to hold two dozen, as long as each still has a few loads of its own
+  const long long pairs = p.epilogue == kGate ? p.N : (p.N + 1) / 2, es = p.dtype == MSL_DTYPE_BF16 ? 2 : 4;
+  a.share = 1;
+  while (a.share < rows::kWarps && pairs * a.share < 24LL * sm_count() && p.K * es / 16 > 64LL * a.share) a.share *= 2;
+  if (p.dtype == MSL_DTYPE_BF16 && a.M > 1) {
+    if (a.M <= 8) return p.epilogue == kGate ? rows::launch_mma<1, kGate>(a, s) : rows::launch_mma<1, kPlain>(a, s);
+    return p.epilogue == kGate ? rows::launch_mma<2, kGate>(a, s) : rows::launch_mma<2, kPlain>(a, s);
+  }
+  if (p.dtype == MSL_DTYPE_BF16)
+    return p.epilogue == kGate ? rows::launch<__nv_bfloat16, 1, kGate>(a, s) : rows::launch<__nv_bfloat16, 1, kPlain>(a, s);
+  return p.epilogue == kGate ? rows::by_rows<float, kGate>(a, s) : rows::by_rows<float, kPlain>(a, s);
+}
+
+}  // namespace ffn
+}  // namespace msl
