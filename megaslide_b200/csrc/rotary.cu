@@ -13,9 +13,14 @@
 // slot (SL of them where V is small) for the whole call, so the cosines and sines of a token are loaded once and
 // serve all its heads, and the gradients of the weights add up in registers.  32 / (lanes of a head) heads go
 // through together, whole rows of adjacent loads; the sums of a head are shuffles among its lanes.
-// With that the limit is the instructions of an element, not the bytes, so the arithmetic goes two pairs at
-// a time (fma.rn.f32x2), the weights are multiplied into the cosines and sines once per token, and lanes
-// without a head load a neighbour's instead of branching (they only never store).
+// The loads run three stages ahead through shared memory, each lane copying its own bytes to its own place
+// (cp.async: no registers hold them and no lane waits for another), over a warp's tokens.  The arithmetic goes
+// two pairs at a time (fma.rn.f32x2), the weights are multiplied into the cosines and sines once per token, and
+// lanes without a head load a neighbour's instead of branching (they only never store).
+//
+// Measured, bf16 (of the measured copy bandwidth): rotation of 131072 x 16 x 72, 604 MB, 110 us, 5.5 TB/s (84%); norm
+// and rotation of 262144 x 24 x 64 queries and keys, 3.2 GB, 578 us, 5.6 TB/s (85%); their backward, 4.8 GB, 825 us,
+// 5.9 TB/s (89%).  With loads straight to registers 145, 740 and 1035 us.
 
 #include "msl_abi.cuh"
 #include "msl_common.cuh"
@@ -155,15 +160,30 @@ __device__ __forceinline__ float head_sum(float v, int lanes, int in_head, int f
   return __shfl_sync(kFull, v, first);
 }
 
+// Copies of a lane's own bytes to its own place in shared memory: the loads ahead, without registers to hold them.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// Stages of a warp's ring and units (steps of 32 / lanes heads) of a stage, where a lane's unit is whole 16- or two
+// 8-byte words (V = 4).  Stages 6: as fast; one unit a stage and 8 stages: forward 671 us instead of 598.
+constexpr int kStages = 4;
+constexpr int units_of(bool bwd, int element) { return bwd && element == 4 ? 1 : 2; }
+
 enum Mode : int { kRotate = 0, kForward = 1, kBackward = 2 };
 
 template <typename T, int V, int SL, bool INTER, int MODE, int LC>
 __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1) rotary_kernel(const __grid_constant__ Params P) {
   constexpr int NP = V * SL, N2 = NP / 2;         // pairs of a lane
-  // heads in flight, and blocks a SM (the launch bounds): measured together on 262144 x 24 x 64 and 131072 x 16 x 72 in
-  // bf16; forward 3 and 3 blocks 850 us, 2 and 3 740, 1 and 4 830; backward 2 and 2 1035, 1 and 3 1700, 1 and 4 1270;
-  // rotation alone 3 and 3 145 us, 2 and 3 211, 1 and 4 174
-  constexpr int U = MODE == kRotate ? 3 : 2;
+  constexpr int UU = units_of(MODE == kBackward, sizeof(T)), OPS = MODE == kBackward ? 2 : 1;
+  // pieces of a lane's unit: 16 bytes of adjacent pairs, or the two halves of split ones
+  constexpr int kPiece = INTER ? 16 : V * static_cast<int>(sizeof(T)), kPieces = 2 * V * static_cast<int>(sizeof(T)) / kPiece;
+  extern __shared__ __align__(16) uint8_t ring[];  // [warps][stages][units][operands][pieces][32 lanes]
   constexpr bool NORM = MODE != kRotate, BWD = MODE == kBackward;
   using R = Raw<T, V, SL, INTER>;
   const int lane = threadIdx.x & 31;
@@ -172,6 +192,8 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
   const int per_warp = 32 / L;  // heads of one step
   const int nslots = P.d / (2 * V), turning = P.R / (2 * V);
   const bool mine = seg < per_warp;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  const uint32_t mine_at = ring_at + (threadIdx.x >> 5) * (kStages * UU * OPS * kPieces * 32 * kPiece) + lane * kPiece;
   const int first = min(seg, per_warp - 1) * L;
   // queries or keys
   const int o = static_cast<int>(blockIdx.x) >= P.blocks0 ? 1 : 0;
@@ -255,6 +277,40 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
       pos[1] = rest / P.W;
       pos[2] = rest - pos[1] * P.W;
     }
+    // the item's units in their order, a few stages ahead
+    long long ahead = row0;
+    int ahead_unit = b0, slot = 0;
+    auto issue = [&](int to) {
+      if (ahead < row1) {
+#pragma unroll
+        for (int u = 0; u < UU; ++u) {
+          const int at = min(min(ahead_unit + u, b1 - 1) * per_warp + seg, nh - 1) * P.d + lo[0];
+#pragma unroll
+          for (int k = 0; k < OPS; ++k) {
+            const T* const from = (k ? static_cast<const T*>(P.dy[o]) + ahead * P.dy_ld[o] : static_cast<const T*>(P.x[o]) + ahead * P.x_ld[o]) + at;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+              copy_async<kPiece>(mine_at + (((to * UU + u) * OPS + k) * kPieces + i) * 32 * kPiece, from + i * (INTER ? kPiece / static_cast<int>(sizeof(T)) : hi[0]));
+          }
+        }
+        ahead_unit += UU;
+        if (ahead_unit >= b1) {
+          ahead_unit = b0;
+          ++ahead;
+        }
+      }
+      copy_commit();
+    };
+    auto take = [&](int from, int u, int k, R& r) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        load<T, kPiece / static_cast<int>(sizeof(T))>(
+            reinterpret_cast<const T*>(ring + (mine_at - ring_at) + (((from * UU + u) * OPS + k) * kPieces + i) * 32 * kPiece), &r.e[0][i * (kPiece / static_cast<int>(sizeof(T)))]);
+    };
+    if constexpr (V == 4) {
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) issue(i);
+    }
     for (long long row = row0; row < row1; ++row) {
       float2 cs[N2], sn[N2];
 #pragma unroll
@@ -313,82 +369,93 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
         C[j] = MODE == kForward ? mul2(cs[j], wb[j]) : cs[j];
         D[j] = MODE == kForward ? mul2(s, wa[j]) : s;
       }
-      const T* const xr = static_cast<const T*>(P.x[o]) + row * P.x_ld[o];
-      const T* const gr = BWD ? static_cast<const T*>(P.dy[o]) + row * P.dy_ld[o] : nullptr;
       T* const yr = static_cast<T*>(P.y[o]) + row * P.y_ld[o];
-      for (int b = b0; b < b1; b += U) {
-        R raw[U], rdy[BWD ? U : 1];
-        int at[U];
+      auto finish = [&](R& raw, const R& rdy, int b) {
+        const bool on = b * per_warp + seg < nh;
+        float2 xa[N2], xb[N2];
+        raw.split(xa, xb);
+        float r = 1.f;
+        if (NORM) {
+          float2 ss = both(0.f);
+          if (SL > 1) {  // slots beyond the head were loaded from its first
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (u > 0 && b + u >= b1) break;
-          at[u] = min((b + u) * per_warp + seg, nh - 1) * P.d;
-          const T* from[SL];
+            for (int j = 0; j < NP; ++j)
+              if (!valid[j / V]) {
+                (j & 1 ? xa[j / 2].y : xa[j / 2].x) = 0.f;
+                (j & 1 ? xb[j / 2].y : xb[j / 2].x) = 0.f;
+              }
+          }
 #pragma unroll
-          for (int s = 0; s < SL; ++s) from[s] = xr + at[u] + lo[s];
-          raw[u].get(from, hi);
-          if (BWD) {
+          for (int j = 0; j < N2; ++j) ss = fma2(xb[j], xb[j], fma2(xa[j], xa[j], ss));
+          r = rsqrtf(fmaf(head_sum<LC>(ss.x + ss.y, L, in_head, first), P.inv_d, P.eps));
+        }
+        if (!BWD) {
 #pragma unroll
-            for (int s = 0; s < SL; ++s) from[s] = gr + at[u] + lo[s];
-            rdy[u].get(from, hi);
+          for (int j = 0; j < N2; ++j) {
+            float2 ya = fma2(xb[j], B[j], mul2(xa[j], A[j])), yb = fma2(xa[j], D[j], mul2(xb[j], C[j]));
+            if (NORM) { ya = mul2(ya, both(r)); yb = mul2(yb, both(r)); }
+            xa[j] = ya;
+            xb[j] = yb;
+          }
+        } else {
+          float2 da[N2], db[N2], dot = both(0.f);
+          const float2 rr = both(on ? r : 0.f);  // a head loaded twice counts once
+          rdy.split(da, db);
+#pragma unroll
+          for (int j = 0; j < N2; ++j) {
+            const float2 na = fma2(db[j], B[j], mul2(da[j], A[j])), nb = fma2(da[j], D[j], mul2(db[j], A[j]));
+            ga[j] = fma2(na, mul2(xa[j], rr), ga[j]);
+            gb[j] = fma2(nb, mul2(xb[j], rr), gb[j]);
+            da[j] = mul2(na, wa[j]);
+            db[j] = mul2(nb, wb[j]);
+            dot = fma2(db[j], xb[j], fma2(da[j], xa[j], dot));
+          }
+          const float m = -head_sum<LC>(dot.x + dot.y, L, in_head, first) * P.inv_d * r * r;
+#pragma unroll
+          for (int j = 0; j < N2; ++j) {
+            xa[j] = mul2(fma2(xa[j], both(m), da[j]), both(r));
+            xb[j] = mul2(fma2(xb[j], both(m), db[j]), both(r));
           }
         }
+        raw.join(xa, xb);
+        if (on) {
+          T* to[SL];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (u > 0 && b + u >= b1) break;
-          const bool on = (b + u) * per_warp + seg < nh;
-          float2 xa[N2], xb[N2];
-          raw[u].split(xa, xb);
-          float r = 1.f;
-          if (NORM) {
-            float2 ss = both(0.f);
-            if (SL > 1) {  // slots beyond the head were loaded from its first
+          for (int s = 0; s < SL; ++s) to[s] = yr + min(b * per_warp + seg, nh - 1) * P.d + lo[s];
+          raw.put(to, hi, valid);
+        }
+      };
+      if constexpr (V == 4) {
+        for (int b = b0; b < b1; b += UU) {
+          copy_wait<kStages - 2>();
+          issue(slot == 0 ? kStages - 1 : slot - 1);  // the stage that was used last
+          R raw[UU], rdy[UU];
 #pragma unroll
-              for (int j = 0; j < NP; ++j)
-                if (!valid[j / V]) {
-                  (j & 1 ? xa[j / 2].y : xa[j / 2].x) = 0.f;
-                  (j & 1 ? xb[j / 2].y : xb[j / 2].x) = 0.f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < N2; ++j) ss = fma2(xb[j], xb[j], fma2(xa[j], xa[j], ss));
-            r = rsqrtf(fmaf(head_sum<LC>(ss.x + ss.y, L, in_head, first), P.inv_d, P.eps));
+          for (int u = 0; u < UU; ++u) {
+            take(slot, u, 0, raw[u]);
+            if (BWD) take(slot, u, 1, rdy[u]);
           }
-          if (!BWD) {
+          slot = slot == kStages - 1 ? 0 : slot + 1;
 #pragma unroll
-            for (int j = 0; j < N2; ++j) {
-              float2 ya = fma2(xb[j], B[j], mul2(xa[j], A[j])), yb = fma2(xa[j], D[j], mul2(xb[j], C[j]));
-              if (NORM) { ya = mul2(ya, both(r)); yb = mul2(yb, both(r)); }
-              xa[j] = ya;
-              xb[j] = yb;
-            }
-          } else {
-            float2 da[N2], db[N2], dot = both(0.f);
-            const float2 rr = both(on ? r : 0.f);  // a head loaded twice counts once
-            rdy[u].split(da, db);
+          for (int u = 0; u < UU; ++u)
+            if (u == 0 || b + u < b1) finish(raw[u], rdy[u], b + u);
+        }
+      } else {
+        const T* const xr = static_cast<const T*>(P.x[o]) + row * P.x_ld[o];
+        const T* const gr = BWD ? static_cast<const T*>(P.dy[o]) + row * P.dy_ld[o] : nullptr;
+        for (int b = b0; b < b1; ++b) {
+          R raw, rdy;
+          const int at = min(b * per_warp + seg, nh - 1) * P.d;
+          const T* from[SL];
 #pragma unroll
-            for (int j = 0; j < N2; ++j) {
-              const float2 na = fma2(db[j], B[j], mul2(da[j], A[j])), nb = fma2(da[j], D[j], mul2(db[j], A[j]));
-              ga[j] = fma2(na, mul2(xa[j], rr), ga[j]);
-              gb[j] = fma2(nb, mul2(xb[j], rr), gb[j]);
-              da[j] = mul2(na, wa[j]);
-              db[j] = mul2(nb, wb[j]);
-              dot = fma2(db[j], xb[j], fma2(da[j], xa[j], dot));
-            }
-            const float m = -head_sum<LC>(dot.x + dot.y, L, in_head, first) * P.inv_d * r * r;
+          for (int s = 0; s < SL; ++s) from[s] = xr + at + lo[s];
+          raw.get(from, hi);
+          if (BWD) {
 #pragma unroll
-            for (int j = 0; j < N2; ++j) {
-              xa[j] = mul2(fma2(xa[j], both(m), da[j]), both(r));
-              xb[j] = mul2(fma2(xb[j], both(m), db[j]), both(r));
-            }
+            for (int s = 0; s < SL; ++s) from[s] = gr + at + lo[s];
+            rdy.get(from, hi);
           }
-          raw[u].join(xa, xb);
-          if (on) {
-            T* to[SL];
-#pragma unroll
-            for (int s = 0; s < SL; ++s) to[s] = yr + at[u] + lo[s];
-            raw[u].put(to, hi, valid);
-          }
+          finish(raw, rdy, b);
         }
       }
     }
@@ -397,8 +464,9 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
   if (BWD && P.partial) {
     // the block's sums: every warp and head position of a warp writes its channels, then one thread per
     // channel adds them in order
-    extern __shared__ float sums[];  // [warps * per_warp][d]
+    float* const sums = reinterpret_cast<float*>(ring);  // [warps * per_warp][d]
     const int nw = blockDim.x >> 5, warp = threadIdx.x >> 5;
+    __syncthreads();
     if (mine) {
       float* const to = sums + static_cast<size_t>(warp * per_warp + seg) * P.d;
 #pragma unroll
@@ -442,6 +510,7 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restri
 // ------------------------------------------------------------------------------------------ host
 
 constexpr int kWarps = 8;
+constexpr int kMostGroup = 8;  // tokens of a warp's turn; 4: forward 599 us instead of 578, 16: rotation 122 us instead of 110
 constexpr int kBwdBlocksPerSm = 4;
 
 int fill(const msl_rotary_geometry* g, Params& P) {
@@ -545,8 +614,9 @@ cudaError_t launch(Params P, cudaStream_t s, int blocks) {
   long long splits = P.rows >= want ? 1 : (want + P.rows - 1) / P.rows;
   if (splits > (units0 > units1 ? units0 : units1)) splits = units0 > units1 ? units0 : units1;
   P.splits = static_cast<int>(splits);
-  // several tokens a warp once every SM has its warps: their places follow from one another
-  P.group = P.rows >= 16 * want ? 4 : P.rows >= 8 * want ? 2 : 1;
+  // several tokens a warp once every SM has its warps: their loads run ahead over them, their places follow
+  const long long each_warp = (P.rows + 3 * want - 1) / (3 * want);
+  P.group = static_cast<int>(splits > 1 ? 1 : each_warp < kMostGroup ? each_warp : kMostGroup);
   P.table_vec = SL == 1 && V % 2 == 0 && multiple_of(P.table, 16);
   for (int a = 0; a < 3; ++a) P.table_vec = P.table_vec && P.npair[a] % V == 0;
   if (blocks == 0) {
@@ -555,7 +625,13 @@ cudaError_t launch(Params P, cudaStream_t s, int blocks) {
     P.blocks0 = static_cast<int>(each);
     blocks = static_cast<int>(P.heads[1] ? 2 * each : each);
   }
-  const size_t smem = MODE == kBackward && P.partial ? sizeof(float) * kWarps * per_warp * P.d : 0;
+  constexpr size_t kRing = V == 4 ? kWarps * kStages * units_of(MODE == kBackward, sizeof(T)) * (MODE == kBackward ? 2 : 1) * 32 * 2 * V * sizeof(T) : 0;
+  const size_t sums = MODE == kBackward && P.partial ? sizeof(float) * kWarps * per_warp * P.d : 0;
+  const size_t smem = sums > kRing ? sums : kRing;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(rotary_kernel<T, V, SL, INTER, MODE, LC>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
   rotary_kernel<T, V, SL, INTER, MODE, LC><<<static_cast<unsigned>(blocks), kWarps * 32, smem, s>>>(P);
   return cudaGetLastError();
 }
