@@ -115,7 +115,7 @@ class QkNormIO(ctypes.Structure):
 class FfnGeometry(ctypes.Structure):
     """Mirror of ``msl_ffn_geometry``."""
 
-    _fields_ = [("rows", _i64), ("dim", _i32), ("hidden", _i32), ("dtype", _i32), ("activation", _i32)]
+    _fields_ = [("rows", _i64), ("dim", _i32), ("hidden", _i32), ("dtype", _i32), ("activation", _i32), ("unaligned", _i32)]
 
 
 class FfnIO(ctypes.Structure):

@@ -114,10 +114,10 @@ cudaError_t launch_product_simt(const Product& p, cudaStream_t s) {
 
 // Bound by bytes (604 MB for the 32768 x 9216 gradients of the projections in bf16): every element is read
 // once, V adjacent columns a thread (16 bytes), 8 warps a block on alternate rows, four rows' loads in flight.
-// partial[slice][c] = sum of the slice's rows.
+// partial[slice][c] = sum of the slice's rows, or out[c] where there is one slice.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x, long long ld, long long rows, int cols, long long per,
-                                                         float* __restrict__ partial) {
+                                                         float* __restrict__ partial, T* __restrict__ out) {
   __shared__ float part[8][32 * V + 1];
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + lane) * V;
@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += part[i][k];
-    partial[static_cast<size_t>(blockIdx.y) * cols + col] = sum;
+    if (gridDim.y == 1) out[col] = from_f32<T>(sum);
+    else partial[static_cast<size_t>(blockIdx.y) * cols + col] = sum;
   }
 }
 
@@ -175,15 +176,15 @@ constexpr int kSlices = 64;
 template <typename T>
 static cudaError_t column_sums_t(const T* x, long long ld, long long rows, int cols, T* out, float* partial, cudaStream_t s) {
   constexpr int kVec = 16 / static_cast<int>(sizeof(T));
-  const long long per = rows > 64 * kSlices ? (rows + kSlices - 1) / kSlices : 64;
+  const long long per = rows > 128 * kSlices ? (rows + kSlices - 1) / kSlices : 128;
   const int slices = static_cast<int>((rows + per - 1) / per);
   const bool vec = multiple_of(x, 16) && ld % kVec == 0 && cols % kVec == 0;
   const int v = vec ? kVec : 1;
   const dim3 grid((cols + 32 * v - 1) / (32 * v), slices);
-  if (vec) column_sum_kernel<T, kVec><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial);
-  else column_sum_kernel<T, 1><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial);
-  column_join_kernel<T><<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, out);
-  count_launches(2);
+  if (vec) column_sum_kernel<T, kVec><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial, out);
+  else column_sum_kernel<T, 1><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial, out);
+  if (slices > 1) column_join_kernel<T><<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, out);
+  count_launches(slices > 1 ? 2 : 1);
   return cudaGetLastError();
 }
 
@@ -250,10 +251,10 @@ struct Workspace {
 static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
   Workspace w{};
   const long long M = g->rows, C = g->dim, F = g->hidden;
-  const bool planes = g->dtype == MSL_DTYPE_F32 || C % 8 || F % 8;
+  const bool planes = g->dtype == MSL_DTYPE_F32 || C % 8 || F % 8 || g->unaligned;
   auto need = [&](long long m, long long n, long long k, int epilogue, bool b_major) {
     if (M == 0) return;
-    // one product of a bf16 block may be addressable though the others are not (hidden a multiple of 4)
+    // some products of a bf16 block may be addressable though others are not
     const size_t b = planes ? planes_partial_bytes(g->dtype, m, n, k, epilogue) : 0;
     const size_t t = g->dtype == MSL_DTYPE_BF16 ? tc_partial_bytes(m, n, k, epilogue, b_major) : 0;
     if (b > w.partial) w.partial = b;

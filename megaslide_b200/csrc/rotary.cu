@@ -677,6 +677,7 @@ int fill_norm(const msl_rotary_geometry* g, const msl_qk_norm_io* io, Params& P)
 
 int check_rows(const char* what, const void* p, long long ld, long long heads, int d, int dtype) {
   if (!p) return failf(MSL_ERR_INVALID, "%s is required", what);
+  if (heads > (1 << 20)) return failf(MSL_ERR_UNSUPPORTED, "%s: over 2^20 heads", what);
   if (!multiple_of(p, dtype == MSL_DTYPE_BF16 ? 2 : 4)) return failf(MSL_ERR_INVALID, "%s is not aligned to its elements", what);
   if (ld < heads * d) return failf(MSL_ERR_INVALID, "%s: row stride %lld is under heads * head_dim = %lld", what, ld, heads * d);
   return MSL_OK;

@@ -712,6 +712,11 @@ def _ffn_check(x, w_in, w_out, b_in, b_out) -> Tuple[int, int, int]:
     return M, C, F
 
 
+def _unaligned(*operands) -> int:
+    """1 where an operand's address is no multiple of 16 bytes (views into packed buffers, say)."""
+    return 1 if any(t is not None and t.data_ptr() & 15 for t in operands) else 0
+
+
 def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
                   b_out: Optional[torch.Tensor] = None, activation: str = "silu", keep: bool = False,
                   status: Optional[torch.Tensor] = None):
@@ -720,8 +725,8 @@ def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in
     device word for MSL_STATUS_TIMEOUT in place of the device's HostFlag."""
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
     dev, dt = x.device, x.dtype
-    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation))
     x_ld = _ld(x, "x")
+    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation), _unaligned(x, w_in, w_out, b_in, b_out) or int(x_ld % 8 != 0))
     h = torch.empty(M, F, device=dev, dtype=dt)
     kept = torch.empty(M, 2 * F, device=dev, dtype=dt) if keep else None
     y = torch.empty(x.shape, device=dev, dtype=dt)
@@ -752,9 +757,10 @@ def gated_ffn_bwd(x, w_in, w_out, h, kept, dy, b_in=None, b_out=None, activation
     db_in = torch.empty_like(b_in) if needs[3] else None
     db_out = torch.empty_like(b_out) if needs[4] else None
     dgu = torch.empty(M, 2 * F, device=dev, dtype=dt) if needs[0] or needs[1] or needs[3] else None
-    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation))
-    io = _lib.FfnIO(x.data_ptr(), _ld(x, "x"), w_in.data_ptr(), None, w_out.data_ptr(), None, h.data_ptr(), kept.data_ptr(), None, 0,
-                    dy.data_ptr(), _ld(dy, "dy"), _ptr(dgu), _ptr(dx), C, _ptr(dw_in), _ptr(dw_out), _ptr(db_in), _ptr(db_out),
+    x_ld, dy_ld = _ld(x, "x"), _ld(dy, "dy")
+    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation), _unaligned(x, w_in, w_out, dy, h, kept) or int((x_ld | dy_ld) % 8 != 0))
+    io = _lib.FfnIO(x.data_ptr(), x_ld, w_in.data_ptr(), None, w_out.data_ptr(), None, h.data_ptr(), kept.data_ptr(), None, 0,
+                    dy.data_ptr(), dy_ld, _ptr(dgu), _ptr(dx), C, _ptr(dw_in), _ptr(dw_out), _ptr(db_in), _ptr(db_out),
                     _flag(dev, status))
     lib = _lib.load()
     with _on(dev):

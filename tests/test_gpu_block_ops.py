@@ -439,6 +439,29 @@ def test_gated_ffn_some_gradients_and_strides(dtype):
         _close(got[1], full[1].double(), 2 * tol, "dw_in")
 
 
+def test_gated_ffn_weights_inside_a_packed_buffer():
+    """Weights at any element of a flat buffer, as the CPU-master trainer packs them: results as from weights of
+    their own, within the rounding of sums in another order."""
+    M, C, F = 700, 256, 512
+    x, w_in, w_out, b_in, b_out = (t.detach() for t in _ffn_case(M, C, F, torch.bfloat16, "silu", True))
+    dy = _rand(9, M, C, dtype=torch.bfloat16)
+
+    def run(*ws):
+        leaves = [x.clone().requires_grad_(), *(w.requires_grad_() for w in ws)]
+        y = msl.gated_ffn(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = run(w_in.clone(), w_out.clone(), b_in.clone(), b_out.clone())
+    for first in (1, 2, 4):
+        flat = torch.cat([torch.zeros(first, dtype=torch.bfloat16, device=_dev())] + [t.reshape(-1) for t in (w_in, w_out, b_in, b_out)])
+        views, at = [], first
+        for t in (w_in, w_out, b_in, b_out):
+            views.append(flat[at:at + t.numel()].view(t.shape).detach())
+            at += t.numel()
+        for name, a, b in zip(("y", "dx", "dw_in", "dw_out", "db_in", "db_out"), run(*views), want):
+            _close(a, b.double(), 2 * RMS, name)
+
+
 def test_gated_ffn_gradient_against_differences():
     M, C, F = 6, 16, 24
     args = [t.detach() for t in _ffn_case(M, C, F, torch.float32, "gelu", True)]
