@@ -4,12 +4,13 @@
 //
 // Bound by bytes: the norm reads everything once, the scaling reads it again (the factor is known only
 // when the last element has been read; backwards, so that it begins with what the caches still hold) and writes
-// it.  The tensors are cut into chunks; a block takes an equal share of consecutive chunks, whatever the tensors'
-// sizes, so two launches serve any number of tensors up to kMaxTensors (more take further launches).  Chunks
-// grow with the total from 2048 elements (a few megabytes still reach every SM) to 32768 (1.63 GB of bf16 in 504
-// tensors, results not aligned with their sources: norm 254 us, 6.4 TB/s, scaling 650 us, 5.0 TB/s; with 8192 260
-// and 720 us; with 4 instead of 8 blocks a SM 880 us).  The table of
-// tensors travels in the kernel's parameters: no copy to the device, nothing to keep alive.
+// it.  The tensors are cut into chunks, which the blocks take in turn, whatever the tensors' sizes, so two
+// launches serve any number of tensors up to kMaxTensors (more take further launches).  Chunks grow with the
+// total from 2048 elements (a few megabytes still reach every SM) to 32768.  Measured with 504 bf16 tensors of
+// 1.63 GB, results not aligned with their sources: norm 260 us, 6.3 TB/s, scaling 588 us, 5.5 TB/s (a
+// contiguous share of the chunks for every block: 650 us; chunks of 8192: 284 and 641; 4 blocks a SM instead
+// of 8: 880 us).
+// The table of tensors travels in the kernel's parameters: no copy to the device, nothing to keep alive.
 // Sums: float32 in a thread's part of a chunk, double from there on, joined in a fixed order (the same result on
 // every run on the same kind of GPU).
 
@@ -122,29 +123,19 @@ __device__ __forceinline__ double block_sum(double v) {
   return v;
 }
 
-// the chunks of this block: an equal share of `total`
-__device__ __forceinline__ void share(unsigned total, unsigned& c0, unsigned& c1) {
-  c0 = static_cast<unsigned>(static_cast<unsigned long long>(total) * blockIdx.x / gridDim.x);
-  c1 = static_cast<unsigned>(static_cast<unsigned long long>(total) * (blockIdx.x + 1) / gridDim.x);
-}
-
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) sumsq_kernel(const __grid_constant__ Table t, double* __restrict__ partial) {
-  unsigned c0, c1;
-  share(t.first[t.count], c0, c1);
-  // a chunk's squares of a thread (128 at most) add up in float32, the chunks in double: thousands of squares of bf16
-  // numbers, whose few bits leave many ties, drift by 5e-6 in one float32 sum
+  // a chunk's squares of a thread (128 at most) add up in float32, the chunks in double: thousands of squares of
+  // bf16 numbers, whose few bits leave many ties, drift by 5e-6 in one float32 sum
   double sum = 0.0;
-  if (c0 < c1) {
-    int k = tensor_of(t, c0);
-    for (unsigned c = c0; c < c1; ++c) {
-      while (c >= t.first[k + 1]) ++k;
-      const long long at = static_cast<long long>(c - t.first[k]) * t.chunk;
-      const int n = static_cast<int>(min(static_cast<long long>(t.chunk), t.numel[k] - at));
-      float acc = 0.f;
-      if (t.bf16[k]) sum_span(static_cast<const __nv_bfloat16*>(t.src[k]) + at, n, acc);
-      else sum_span(static_cast<const float*>(t.src[k]) + at, n, acc);
-      sum += static_cast<double>(acc);
-    }
+  const unsigned all = t.first[t.count];
+  for (unsigned c = blockIdx.x; c < all; c += gridDim.x) {
+    const int k = tensor_of(t, c);
+    const long long at = static_cast<long long>(c - t.first[k]) * t.chunk;
+    const int n = static_cast<int>(min(static_cast<long long>(t.chunk), t.numel[k] - at));
+    float acc = 0.f;
+    if (t.bf16[k]) sum_span(static_cast<const __nv_bfloat16*>(t.src[k]) + at, n, acc);
+    else sum_span(static_cast<const float*>(t.src[k]) + at, n, acc);
+    sum += static_cast<double>(acc);
   }
   const double s = block_sum(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -168,12 +159,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
   float f = max_norm / (v + 1e-6f);
   f = f > 1.f ? 1.f : f;  // a NaN stays a NaN
-  unsigned c0, c1;
-  share(t.first[t.count], c0, c1);
-  if (c0 >= c1) return;
-  int k = tensor_of(t, c1 - 1);
-  for (unsigned c = c1; c-- > c0;) {
-    while (c < t.first[k]) --k;
+  const unsigned all = t.first[t.count];
+  for (unsigned i = blockIdx.x; i < all; i += gridDim.x) {
+    const unsigned c = all - 1 - i;
+    const int k = tensor_of(t, c);
     const long long at = static_cast<long long>(c - t.first[k]) * t.chunk;
     const int m = static_cast<int>(min(static_cast<long long>(t.chunk), t.numel[k] - at));
     if (t.bf16[k]) scale_span(static_cast<const __nv_bfloat16*>(t.src[k]) + at, static_cast<__nv_bfloat16*>(t.dst[k]) + at, m, f);
