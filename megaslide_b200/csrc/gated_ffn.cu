@@ -224,6 +224,9 @@ static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStrea
     }
     e = launch_product_planes(p, slots.at[slot_a], slots.at[slot_b], s);
     if (e != cudaSuccess) return cuda_failf(e, "planes_kernel launch");
+  } else if (skinny_apply(p)) {
+    e = launch_product_skinny(p, s);
+    if (e != cudaSuccess) return cuda_failf(e, "skinny_kernel launch");
   } else {
     e = launch_product_simt(p, s);
     if (e != cudaSuccess) return cuda_failf(e, "product_simt_kernel launch");
@@ -251,12 +254,25 @@ struct Workspace {
 static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
   Workspace w{};
   const long long M = g->rows, C = g->dim, F = g->hidden;
-  const bool planes = g->dtype == MSL_DTYPE_F32 || C % 8 || F % 8 || g->unaligned;
-  auto need = [&](long long m, long long n, long long k, int epilogue, bool b_major) {
+  const bool f32 = g->dtype == MSL_DTYPE_F32, copies = !f32 && (C % 8 || F % 8 || g->unaligned);
+  bool planes = false;  // some product takes planes
+  auto need = [&](long long m, long long n, long long k, int epilogue, bool b_major, bool a_major = false) {
     if (M == 0) return;
+    Product p{};
+    p.dtype = g->dtype;
+    p.epilogue = epilogue;
+    p.M = m;
+    p.N = n;
+    p.K = k;
+    size_t b = 0;
+    if ((f32 || copies) && planes_apply(p)) {
+      planes = true;
+      b = planes_partial_bytes(g->dtype, m, n, k, epilogue);
+    } else if (f32) {
+      b = skinny_bytes(m, n, k, epilogue, a_major);
+    }
     // some products of a bf16 block may be addressable though others are not
-    const size_t b = planes ? planes_partial_bytes(g->dtype, m, n, k, epilogue) : 0;
-    const size_t t = g->dtype == MSL_DTYPE_BF16 ? tc_partial_bytes(m, n, k, epilogue, b_major) : 0;
+    const size_t t = f32 ? 0 : tc_partial_bytes(m, n, k, epilogue, b_major);
     if (b > w.partial) w.partial = b;
     if (t > w.partial) w.partial = t;
   };
@@ -269,8 +285,8 @@ static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
   if (backward) {
     need(M, F, C, kDgate, true);
     need(M, C, 2 * F, kPlain, true);
-    need(2 * F, C, M, kPlain, true);
-    need(C, F, M, kPlain, true);
+    need(2 * F, C, M, kPlain, true, true);
+    need(C, F, M, kPlain, true, true);
     w.columns = sizeof(float) * kSlices * static_cast<size_t>(2 * F > C ? 2 * F : C);
     w.columns = (w.columns + 255) / 256 * 256;
     if (planes && M > 0) {

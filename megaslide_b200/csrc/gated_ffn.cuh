@@ -102,6 +102,10 @@ cudaError_t launch_product_tc(const Product& p, cudaStream_t s);
 constexpr int kMostRows = 16, kMostRowsF32 = 8;
 bool rows_apply(const Product& p);
 cudaError_t launch_product_rows(const Product& p, cudaStream_t s);
+// CUDA-core form for float32, few rows or small products (gated_ffn_skinny.cu).
+bool skinny_apply(const Product& p);
+size_t skinny_bytes(long long M, long long N, long long K, int epilogue, bool a_major);
+cudaError_t launch_product_skinny(const Product& p, cudaStream_t s);
 // Tensor-core form for float32 and for widths that are no multiple of 8 (gated_ffn_planes.cu): the operands as
 // planes [planes][rows][cols padded to 8] of planes_bytes, written by launch_planes from rows as they are stored.
 bool planes_apply(const Product& p);

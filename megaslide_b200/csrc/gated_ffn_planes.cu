@@ -15,6 +15,8 @@
 // What bounds it: six times the multiplications, so about 220 TFLOP/s of float32 products; the CUDA cores' limit
 // is 75.
 
+#include <algorithm>
+
 #include "gated_ffn.cuh"
 #include "tcgen05.cuh"
 
@@ -586,9 +588,22 @@ cudaError_t launch_planes(int dtype, const void* x, long long ld, long long rows
 }
 
 bool planes_apply(const Product& p) {
-  // below this the CUDA cores are done before the planes are made (about 12 us of launches against 25 TFLOP/s)
-  return t5::encoder() && 2.0 * p.M * p.N * p.K * (p.epilogue == kGate ? 2 : 1) >= 3e8 && p.M <= (1LL << 31) - 256 &&
-         p.N <= (1LL << 30) && p.K <= (1LL << 31) - 256 && (p.M + 255) / 256 * ((p.N + 63) / 64) <= (1LL << 30);
+  if (!t5::encoder() || p.M > (1LL << 31) - 256 || p.N > (1LL << 30) || p.K > (1LL << 31) - 256 ||
+      (p.M + 255) / 256 * ((p.N + 63) / 64) > (1LL << 30))
+    return false;
+  const double cols = p.epilogue == kGate ? 2.0 * p.N : p.N, macs = 1.0 * p.M * cols * p.K;
+  // bf16: the CUDA cores are done before the copies are made only where k is short and the result small (they take
+  // 0.6 us for 16 k of a tile)
+  if (p.dtype != MSL_DTYPE_F32) return macs >= 1.5e8 || p.K >= 192;
+  // microseconds.  Planes: 10 bytes an element of both operands at 5 TB/s, rows in tiles of 256, 95 G multiplications a
+  // millisecond, 3 for every round of tiles, some launches.  CUDA cores: rows in their tiles, 15 G multiplications
+  // a millisecond (7.5 up to 16 rows, where the operands bound them), operands and result once.
+  const double elements = 1.0 * p.M * p.K + cols * p.K;
+  const double rows = (p.M + 255) / 256 * 256.0, rounds = rows * cols / 65536.0 / 74.0;
+  const double tile = p.M <= 8 ? 8 : p.M <= 16 ? 16 : p.M <= 32 ? 32 : (p.M + 63) / 64 * 64.0;
+  const double planes = elements * 10 / 5e6 + rows * cols * p.K / 95e6 + 3 * rounds + 12;
+  const double cores = std::max(tile * cols * p.K / (p.M <= 16 ? 7.5e6 : 15e6), (elements + p.M * cols) * 4 / 4e6) + 6;
+  return planes < cores;
 }
 
 size_t planes_partial_bytes(int dtype, long long M, long long N, long long K, int epilogue) {

@@ -39,31 +39,45 @@ __device__ __forceinline__ void dot(float& acc, const uint4& w, const uint4& x) 
   for (int i = 0; i < V; ++i) acc = fmaf(to_f32<T>(a[i]), to_f32<T>(b[i]), acc);
 }
 
+// Pairs of weight rows a warp takes: with more rows of x, more, so that a word of x serves several of them.
+constexpr int pairs_of(int mr) { return mr >= 8 ? 4 : mr >= 4 ? 2 : 1; }
+
 template <typename T, int MR, int EPI>
 __global__ void __launch_bounds__(32 * kWarps) rows_kernel(const __grid_constant__ Args P) {
-  constexpr int V = 16 / static_cast<int>(sizeof(T)), U = MR > 4 ? 2 : 4;
-  __shared__ float part[kWarps][2 * MR];
+  constexpr int V = 16 / static_cast<int>(sizeof(T)), NP = pairs_of(MR), U = MR >= 8 ? 1 : MR >= 4 ? 2 : 4;
+  __shared__ float part[kWarps][2 * NP * MR];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slot = warp % P.share;
-  const long long pair = static_cast<long long>(blockIdx.x) * (kWarps / P.share) + warp / P.share;
-  const long long n0 = EPI == kGate ? pair : 2 * pair, n1 = EPI == kGate ? P.N + pair : 2 * pair + 1;
-  const bool in = n0 < P.N, in1 = EPI == kGate ? in : n1 < P.N;
-  const uint4* const w0 = reinterpret_cast<const uint4*>(static_cast<const T*>(P.b) + (in ? n0 : 0) * P.ldb);
-  const uint4* const w1 = reinterpret_cast<const uint4*>(static_cast<const T*>(P.b) + (in1 ? n1 : 0) * P.ldb);
-  const int words = P.K / V, step = 32 * P.share;
-  float acc[2][MR];
+  const long long group = static_cast<long long>(blockIdx.x) * (kWarps / P.share) + warp / P.share;
+  long long n[NP][2];
+  bool in[NP][2];
+  const uint4* w_at[NP][2];
 #pragma unroll
-  for (int m = 0; m < MR; ++m) acc[0][m] = acc[1][m] = 0.f;
+  for (int p = 0; p < NP; ++p) {
+    const long long pair = group * NP + p;
+    n[p][0] = EPI == kGate ? pair : 2 * pair;
+    n[p][1] = EPI == kGate ? P.N + pair : 2 * pair + 1;
+    in[p][0] = n[p][0] < P.N;
+    in[p][1] = EPI == kGate ? in[p][0] : n[p][1] < P.N;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w_at[p][i] = reinterpret_cast<const uint4*>(static_cast<const T*>(P.b) + (in[p][i] ? n[p][i] : 0) * P.ldb);
+  }
+  const int words = P.K / V, step = 32 * P.share;
+  float acc[NP][2][MR];
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[p][0][m] = acc[p][1][m] = 0.f;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   bool waited = EPI == kGate;
   for (int c = slot * 32 + lane; c - lane < words; c += U * step) {
-    uint4 w[2][U];
+    uint4 w[U][NP][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool have = in && c + u * step < words;
-      w[0][u] = have ? __ldg(w0 + c + u * step) : zero;
-      w[1][u] = have ? __ldg(w1 + c + u * step) : zero;
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[u][p][i] = in[p][i] && c + u * step < words ? __ldg(w_at[p][i] + c + u * step) : zero;
     if (!waited) {  // h is the kernel's before
       cudaGridDependencySynchronize();
       waited = true;
@@ -76,41 +90,51 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(const __grid_constant
       for (int u = 0; u < U; ++u) {
         if (c + u * step >= words) continue;
         const uint4 v = x[c + u * step];
-        dot<T, V>(acc[0][m], w[0][u], v);
-        dot<T, V>(acc[1][m], w[1][u], v);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          dot<T, V>(acc[p][0][m], w[u][p][0], v);
+          dot<T, V>(acc[p][1][m], w[u][p][1], v);
+        }
       }
     }
   }
   if (EPI == kGate) cudaTriggerProgrammaticLaunchCompletion();
   else if (!waited) cudaGridDependencySynchronize();
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int p = 0; p < NP; ++p)
 #pragma unroll
-    for (int m = 0; m < MR; ++m) {
-      float t = acc[i][m];
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kFull, t, o);
-      if (lane == 0) part[warp][i * MR + m] = t;
-    }
+      for (int m = 0; m < MR; ++m) {
+        float t = acc[p][i][m];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(kFull, t, o);
+        if (lane == 0) part[warp][(p * 2 + i) * MR + m] = t;
+      }
   __syncthreads();
-  if (slot != 0 || !in || lane >= P.M) return;
+  // lane: a pair and a row of x
+  const int p = lane / MR, m = lane - p * MR;
+  if (slot != 0 || p >= NP || m >= P.M) return;
+  const long long pair = group * NP + p, n0 = EPI == kGate ? pair : 2 * pair, n1 = EPI == kGate ? P.N + pair : 2 * pair + 1;
+  if (n0 >= P.N) return;
+  const bool in1 = EPI == kGate || n1 < P.N;
   float s[2] = {0.f, 0.f};
   for (int k = 0; k < P.share; ++k) {
-    s[0] += part[warp + k][lane];
-    s[1] += part[warp + k][MR + lane];
+    s[0] += part[warp + k][p * 2 * MR + m];
+    s[1] += part[warp + k][(p * 2 + 1) * MR + m];
   }
   const T* const bias = static_cast<const T*>(P.bias);
   if (bias) {
     s[0] += to_f32<T>(bias[n0]);
     if (in1) s[1] += to_f32<T>(bias[n1]);
   }
-  T* const out = static_cast<T*>(P.out) + lane * P.ldo;
+  T* const out = static_cast<T*>(P.out) + m * P.ldo;
   if (EPI == kGate) {
     float da;
     const float a = act_value_grad(s[0], P.act, da);
     out[n0] = from_f32<T>(a * s[1]);
     if (P.kept_out) {
-      T* const kept = static_cast<T*>(P.kept_out) + lane * 2 * P.N;
+      T* const kept = static_cast<T*>(P.kept_out) + m * 2 * P.N;
       kept[n0] = from_f32<T>(s[1] * da);
       kept[P.N + n0] = from_f32<T>(a);
     }
@@ -121,10 +145,13 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(const __grid_constant
 }
 
 template <typename T, int MR, int EPI>
-cudaError_t launch(const Args& a, cudaStream_t s) {
-  const long long pairs = EPI == kGate ? a.N : (a.N + 1) / 2;
+cudaError_t launch(Args a, cudaStream_t s) {
+  const long long pairs = EPI == kGate ? a.N : (a.N + 1) / 2, groups = (pairs + pairs_of(MR) - 1) / pairs_of(MR);
+  // warps enough for every SM to hold two dozen, as long as each still has a few loads of its own
+  a.share = 1;
+  while (a.share < kWarps && groups * a.share < 24LL * sm_count() && a.K * static_cast<long long>(sizeof(T)) / 16 > 64LL * a.share) a.share *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((pairs + kWarps / a.share - 1) / (kWarps / a.share)));
+  cfg.gridDim = dim3(static_cast<unsigned>((groups + kWarps / a.share - 1) / (kWarps / a.share)));
   cfg.blockDim = dim3(32 * kWarps);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -285,10 +312,6 @@ cudaError_t launch_product_rows(const Product& p, cudaStream_t s) {
   a.M = static_cast<int>(p.M);
   a.K = static_cast<int>(p.K);
   a.act = p.act;
-  // warps enough for every SM to hold two dozen, as long as each still has a few loads of its own
-  const long long pairs = p.epilogue == kGate ? p.N : (p.N + 1) / 2, es = p.dtype == MSL_DTYPE_BF16 ? 2 : 4;
-  a.share = 1;
-  while (a.share < rows::kWarps && pairs * a.share < 24LL * sm_count() && p.K * es / 16 > 64LL * a.share) a.share *= 2;
   if (p.dtype == MSL_DTYPE_BF16 && a.M > 1) {
     if (a.M <= 8) return p.epilogue == kGate ? rows::launch_mma<1, kGate>(a, s) : rows::launch_mma<1, kPlain>(a, s);
     return p.epilogue == kGate ? rows::launch_mma<2, kGate>(a, s) : rows::launch_mma<2, kPlain>(a, s);

@@ -404,6 +404,13 @@ def test_gated_ffn_few_rows(M, dtype):
         _ffn_check_all(M, C, F, dtype, "gelu", bias)
 
 
+@pytest.mark.parametrize("M,C,F", [(1, 1152, 4608), (6, 2560, 1000), (13, 640, 2240), (16, 100, 70), (17, 250, 639), (30, 1152, 2880), (65, 640, 1600),
+                                   (100, 77, 1531)])
+def test_gated_ffn_float32_few_rows(M, C, F):
+    """The CUDA-core form: 16 and 64 rows a tile, shares of k, widths off its vectors."""
+    _ffn_check_all(M, C, F, torch.float32, "silu", True)
+
+
 def test_gated_ffn_without_rows():
     x, w_in, w_out, b_in, b_out = _ffn_case(0, 64, 96, torch.bfloat16, "silu", True)
     y = msl.gated_ffn(x, w_in, w_out, b_in, b_out)
