@@ -327,7 +327,7 @@ typedef struct msl_ffn_geometry {
   int32_t dtype;      /* MSL_DTYPE_* of every operand */
   int32_t activation; /* MSL_ACT_* */
   int32_t unaligned;  /* != 0: the workspace gets room for copies of bf16 operands whose address or row stride is no
-                         multiple of 16 bytes (without it such a call takes the CUDA cores) */
+                         multiple of 16 bytes (without it such a call is refused) */
 } msl_ffn_geometry;
 
 /* Matrices are contiguous rows of their width except x, y, dy and dx (row strides given).  h [rows, hidden]

@@ -1,9 +1,8 @@
-// Gated feed-forward block, forward and backward: the products on the CUDA cores (float32, and bf16
-// widths that no 16-byte row allows), the bias gradients, and the entry points.
+// Gated feed-forward block, forward and backward: which kernel takes a product, the bias gradients, and the entry points.
 //
 //   [g u] = x w_in^T + b_in;  h = act(g) u;  y = h w_out^T + b_out
-//   dh = dy w_out;  dg = dh (u act'(g));  du = dh act(g), of which the forward keeps the two factors;  dx = [dg du] w_in;  dw_in = [dg du]^T x;
-//   dw_out = dy^T h;  db_in, db_out = column sums of [dg du], dy
+//   dh = dy w_out;  dg = dh (u act'(g));  du = dh act(g), of which the forward keeps the two factors;
+//   dx = [dg du] w_in;  dw_in = [dg du]^T x;  dw_out = dy^T h;  db_in, db_out = column sums of [dg du], dy
 
 #include <initializer_list>
 
@@ -11,104 +10,6 @@
 
 namespace msl {
 namespace ffn {
-
-constexpr int kTM = 64, kTN = 64, kTK = 16;
-
-// One 64 x 64 tile per block, 4 x 4 results per thread (twice as many for the gate).
-template <typename T, int EPI, bool AM, bool BM>
-__global__ void __launch_bounds__(256) product_simt_kernel(const Product P) {
-  constexpr int NB = EPI == kGate ? 2 : 1;
-  __shared__ float As[kTK][kTM + 4], Bs[NB][kTK][kTN + 4];
-  const T* const A = static_cast<const T*>(P.a);
-  const T* const B = static_cast<const T*>(P.b);
-  const long long m0 = static_cast<long long>(blockIdx.x) * kTM, n0 = static_cast<long long>(blockIdx.y) * kTN;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[NB][4][4] = {};
-  for (long long k0 = 0; k0 < P.K; k0 += kTK) {
-#pragma unroll
-    for (int i = 0; i < kTM * kTK / 256; ++i) {
-      const int e = i * 256 + threadIdx.x;
-      const int m = AM ? e % kTM : e / kTK, k = AM ? e / kTM : e % kTK;
-      const bool in = m0 + m < P.M && k0 + k < P.K;
-      As[k][m] = in ? to_f32<T>(A[AM ? (k0 + k) * P.lda + m0 + m : (m0 + m) * P.lda + k0 + k]) : 0.f;
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < kTN * kTK / 256; ++i) {
-        const int e = i * 256 + threadIdx.x;
-        const int n = BM ? e % kTN : e / kTK, k = BM ? e / kTN : e % kTK;
-        const bool in = n0 + n < P.N && k0 + k < P.K;
-        const long long row = n0 + n + (b ? P.N : 0);
-        Bs[b][k][n] = in ? to_f32<T>(B[BM ? (k0 + k) * P.ldb + row : row * P.ldb + k0 + k]) : 0.f;
-      }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kTK; ++k) {
-      const float4 a = *reinterpret_cast<const float4*>(&As[k][ty * 4]);
-      const float av[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const float4 v = *reinterpret_cast<const float4*>(&Bs[b][k][tx * 4]);
-        const float bv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[b][i][j] = fmaf(av[i], bv[j], acc[b][i][j]);
-      }
-    }
-    __syncthreads();
-  }
-  const T* const bias = static_cast<const T*>(P.bias);
-  T* const out = static_cast<T*>(P.out);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long m = m0 + ty * 4 + i;
-    if (m >= P.M) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long long n = n0 + tx * 4 + j;
-      if (n >= P.N) continue;
-      if (EPI == kPlain) {
-        out[m * P.ldo + n] = from_f32<T>(acc[0][i][j] + (bias ? to_f32<T>(bias[n]) : 0.f));
-      } else if (EPI == kGate) {
-        const float g = acc[0][i][j] + (bias ? to_f32<T>(bias[n]) : 0.f);
-        const float u = acc[NB - 1][i][j] + (bias ? to_f32<T>(bias[P.N + n]) : 0.f);
-        float da;
-        const float a = act_value_grad(g, P.act, da);
-        out[m * P.ldo + n] = from_f32<T>(a * u);
-        if (P.kept_out) {
-          T* const kept = static_cast<T*>(P.kept_out) + m * 2 * P.N;
-          kept[n] = from_f32<T>(u * da);
-          kept[P.N + n] = from_f32<T>(a);
-        }
-      } else {
-        const T* const kept = static_cast<const T*>(P.kept) + m * 2 * P.N;
-        out[m * 2 * P.N + n] = from_f32<T>(acc[0][i][j] * to_f32<T>(kept[n]));
-        out[m * 2 * P.N + P.N + n] = from_f32<T>(acc[0][i][j] * to_f32<T>(kept[P.N + n]));
-      }
-    }
-  }
-}
-
-template <typename T, int EPI>
-static cudaError_t launch_simt(const Product& p, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((p.M + kTM - 1) / kTM), static_cast<unsigned>((p.N + kTN - 1) / kTN));
-  if (p.a_major && p.b_major) product_simt_kernel<T, EPI, true, true><<<grid, 256, 0, s>>>(p);
-  else if (p.a_major) return cudaErrorInvalidValue;
-  else if (p.b_major) product_simt_kernel<T, EPI, false, true><<<grid, 256, 0, s>>>(p);
-  else product_simt_kernel<T, EPI, false, false><<<grid, 256, 0, s>>>(p);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_product_simt(const Product& p, cudaStream_t s) {
-  const bool bf = p.dtype == MSL_DTYPE_BF16;
-  switch (p.epilogue) {
-    case kPlain: return bf ? launch_simt<__nv_bfloat16, kPlain>(p, s) : launch_simt<float, kPlain>(p, s);
-    case kGate: return bf ? launch_simt<__nv_bfloat16, kGate>(p, s) : launch_simt<float, kGate>(p, s);
-    default: return bf ? launch_simt<__nv_bfloat16, kDgate>(p, s) : launch_simt<float, kDgate>(p, s);
-  }
-}
 
 // ------------------------------------------------------------------------------------------ column sums
 
@@ -224,12 +125,13 @@ static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStrea
     }
     e = launch_product_planes(p, slots.at[slot_a], slots.at[slot_b], s);
     if (e != cudaSuccess) return cuda_failf(e, "planes_kernel launch");
-  } else if (skinny_apply(p)) {
+  } else if (p.dtype == MSL_DTYPE_F32) {
     e = launch_product_skinny(p, s);
     if (e != cudaSuccess) return cuda_failf(e, "skinny_kernel launch");
+  } else if (!slots.at[0]) {
+    return failf(MSL_ERR_INVALID, "an address or a row stride is no multiple of 16 bytes and the geometry's unaligned is 0");
   } else {
-    e = launch_product_simt(p, s);
-    if (e != cudaSuccess) return cuda_failf(e, "product_simt_kernel launch");
+    return failf(MSL_ERR_UNSUPPORTED, "the driver encodes no tensor maps, or the product has over 2^30 tiles");
   }
   count_launches(1);
   return MSL_OK;
@@ -241,7 +143,7 @@ static int check(const msl_ffn_geometry* g, const msl_ffn_io* io) {
   if (g->dtype != MSL_DTYPE_F32 && g->dtype != MSL_DTYPE_BF16) return failf(MSL_ERR_INVALID, "unknown dtype %d", g->dtype);
   if (g->activation != MSL_ACT_SILU && g->activation != MSL_ACT_GELU) return failf(MSL_ERR_INVALID, "unknown activation %d", g->activation);
   if (g->dim > (1 << 21) || g->hidden > (1 << 20)) return failf(MSL_ERR_UNSUPPORTED, "dim or hidden is over 2^20");
-  if (g->rows > (1LL << 31)) return failf(MSL_ERR_UNSUPPORTED, "rows is over 2^31");
+  if (g->rows > (1LL << 31) - 256) return failf(MSL_ERR_UNSUPPORTED, "rows is over 2^31 - 256");
   if (!io) return failf(MSL_ERR_INVALID, "io is NULL");
   return MSL_OK;
 }

@@ -92,7 +92,6 @@ __device__ __forceinline__ float act_grad_fast(float g, float& da) {
   return g * c;
 }
 
-cudaError_t launch_product_simt(const Product& p, cudaStream_t s);
 // Tensor-core form (gated_ffn_tc.cu), and whether the operands allow it.
 bool tc_applies(const Product& p);
 size_t tc_partial_bytes(long long M, long long N, long long K, int epilogue, bool b_major);
@@ -103,7 +102,6 @@ constexpr int kMostRows = 16, kMostRowsF32 = 8;
 bool rows_apply(const Product& p);
 cudaError_t launch_product_rows(const Product& p, cudaStream_t s);
 // CUDA-core form for float32, few rows or small products (gated_ffn_skinny.cu).
-bool skinny_apply(const Product& p);
 size_t skinny_bytes(long long M, long long N, long long K, int epilogue, bool a_major);
 cudaError_t launch_product_skinny(const Product& p, cudaStream_t s);
 // Tensor-core form for float32 and for widths that are no multiple of 8 (gated_ffn_planes.cu): the operands as

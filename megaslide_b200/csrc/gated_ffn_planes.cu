@@ -591,10 +591,8 @@ bool planes_apply(const Product& p) {
   if (!t5::encoder() || p.M > (1LL << 31) - 256 || p.N > (1LL << 30) || p.K > (1LL << 31) - 256 ||
       (p.M + 255) / 256 * ((p.N + 63) / 64) > (1LL << 30))
     return false;
-  const double cols = p.epilogue == kGate ? 2.0 * p.N : p.N, macs = 1.0 * p.M * cols * p.K;
-  // bf16: the CUDA cores are done before the copies are made only where k is short and the result small (they take
-  // 0.6 us for 16 k of a tile)
-  if (p.dtype != MSL_DTYPE_F32) return macs >= 1.5e8 || p.K >= 192;
+  if (p.dtype != MSL_DTYPE_F32) return true;
+  const double cols = p.epilogue == kGate ? 2.0 * p.N : p.N;
   // microseconds.  Planes: 10 bytes an element of both operands at 5 TB/s, rows in tiles of 256, 95 G multiplications a
   // millisecond, 3 for every round of tiles, some launches.  CUDA cores: rows in their tiles, 15 G multiplications
   // a millisecond (7.5 up to 16 rows, where the operands bound them), operands and result once.

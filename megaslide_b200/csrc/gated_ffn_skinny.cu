@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256, TM == 64 ? 2 : 3) skinny_kernel(const __g
   constexpr int kPitchA = TM + 4;
   constexpr int kTile = kTK * (kPitchA + kPitchB);
   extern __shared__ __align__(16) float sm[];
-  const long long n0 = static_cast<long long>(blockIdx.x) * kTN, m0 = static_cast<long long>(blockIdx.y) * TM;
+  const long long m0 = static_cast<long long>(blockIdx.x) * TM, n0 = static_cast<long long>(blockIdx.y) * kTN;
   const long long k0 = blockIdx.z * P.kper, k1 = min(P.K, k0 + P.kper);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   constexpr bool FEW = TM <= 16;
@@ -265,7 +265,7 @@ cudaError_t launch(const Args& a, int shares, cudaStream_t s) {
     const cudaError_t e = cudaFuncSetAttribute(skinny_kernel<TM, AM, BM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  const dim3 grid(static_cast<unsigned>((a.N + kTN - 1) / kTN), static_cast<unsigned>((a.M + TM - 1) / TM), static_cast<unsigned>(shares));
+  const dim3 grid(static_cast<unsigned>((a.M + TM - 1) / TM), static_cast<unsigned>((a.N + kTN - 1) / kTN), static_cast<unsigned>(shares));
   skinny_kernel<TM, AM, BM><<<grid, 256, smem, s>>>(a);
   return cudaGetLastError();
 }
@@ -280,10 +280,6 @@ cudaError_t by_order(const Product& p, const Args& a, int shares, cudaStream_t s
 
 size_t skinny_bytes(long long M, long long N, long long K, int epilogue, bool a_major) {
   return skinny::plan(M, epilogue == kGate ? 2 * N : N, K, a_major).bytes;
-}
-
-bool skinny_apply(const Product& p) {
-  return p.dtype == MSL_DTYPE_F32 && (p.M + 15) / 16 <= 65535 && (p.N + 63) / 64 <= (1LL << 30);
 }
 
 cudaError_t launch_product_skinny(const Product& p, cudaStream_t s) {
@@ -306,6 +302,7 @@ cudaError_t launch_product_skinny(const Product& p, cudaStream_t s) {
   a.va = multiple_of(p.a, 16) && p.lda % 4 == 0;
   a.vb = multiple_of(p.b, 16) && p.ldb % 4 == 0;
   cudaError_t e;
+  // rows on the grid's x, the axis that may be long (columns: at most 2^21 / 128)
   switch (cut.tm) {
     case 8: e = skinny::by_order<8>(p, a, cut.shares, s); break;
     case 16: e = skinny::by_order<16>(p, a, cut.shares, s); break;

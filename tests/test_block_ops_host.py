@@ -135,6 +135,7 @@ def test_rotary_entry_refuses_operands():
 @pytest.mark.parametrize("kw,code,text", [
     (dict(rows=-1), _lib.MSL_ERR_INVALID, "rows"), (dict(dim=0), _lib.MSL_ERR_INVALID, "dim"), (dict(dtype=3), _lib.MSL_ERR_INVALID, "dtype"),
     (dict(activation=7), _lib.MSL_ERR_INVALID, "activation"), (dict(hidden=1 << 21), _lib.MSL_ERR_UNSUPPORTED, "2^20"),
+    (dict(rows=2**31 - 255), _lib.MSL_ERR_UNSUPPORTED, "2^31"),
 ])
 def test_ffn_entry_refuses(kw, code, text):
     g = _lib.FfnGeometry(**{**dict(rows=4, dim=8, hidden=16, dtype=0, activation=0), **kw})

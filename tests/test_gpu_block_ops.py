@@ -10,13 +10,14 @@ roundings in float32; in bfloat16 RMS for each rounded intermediate and the resu
 kept projections, h, their gradients, the result).
 """
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import megaslide_b200 as msl
-from megaslide_b200 import ops
+from megaslide_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -467,6 +468,27 @@ def test_gated_ffn_weights_inside_a_packed_buffer():
             at += t.numel()
         for name, a, b in zip(("y", "dx", "dw_in", "dw_out", "db_in", "db_out"), run(*views), want):
             _close(a, b.double(), 2 * RMS, name)
+
+
+@pytest.mark.parametrize("C,F,x_ld", [(16, 32, 17), (15, 32, 16)])
+def test_gated_ffn_entry_refuses_rows_off_16_bytes_without_room(C, F, x_ld):
+    """A C caller that leaves unaligned at 0 gets an error for such rows, and nothing is written; odd widths say
+    it by themselves."""
+    lib, M = _lib.load(), 40
+    x = torch.zeros(M, x_ld, device=_dev(), dtype=torch.bfloat16)
+    w_in, w_out = (torch.zeros(n, device=_dev(), dtype=torch.bfloat16) for n in (2 * F * C, C * F))
+    h, y = (torch.full((M, n), 7.0, device=_dev(), dtype=torch.bfloat16) for n in (F, C))
+    g = _lib.FfnGeometry(M, C, F, _lib.MSL_DTYPE_BF16, 0, 0)
+    io = _lib.FfnIO(x=x.data_ptr(), x_ld=x_ld, w_in=w_in.data_ptr(), w_out=w_out.data_ptr(), h=h.data_ptr(), y=y.data_ptr(), y_ld=C)
+    need = lib.msl_gated_ffn_workspace_bytes(ctypes.byref(g), 0)
+    ws = torch.empty(max(need, 1), device=_dev(), dtype=torch.uint8)
+    rc = lib.msl_gated_ffn_fwd(ctypes.byref(g), ctypes.byref(io), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    if C % 8:
+        assert rc == _lib.MSL_OK and not bool(y.any())
+    else:
+        assert rc == _lib.MSL_ERR_INVALID and b"unaligned" in lib.msl_last_error()
+        assert bool((y == 7).all()) and bool((h == 7).all())
 
 
 def test_gated_ffn_gradient_against_differences():
