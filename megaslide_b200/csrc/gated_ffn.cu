@@ -13,35 +13,50 @@ namespace ffn {
 
 // ------------------------------------------------------------------------------------------ column sums
 
-// Bound by bytes (604 MB for the 32768 x 9216 gradients of the projections in bf16): every element is read
-// once, V adjacent columns a thread (16 bytes), 8 warps a block on alternate rows, four rows' loads in flight.
-// partial[slice][c] = sum of the slice's rows, or out[c] where there is one slice.
+// The sums of up to two matrices' columns in one launch.  Bound by bytes (604 MB for the 32768 x 9216 gradients of
+// the projections in bf16): every element is read once, V adjacent columns a thread (16 bytes), 8 warps a block on
+// alternate rows, four rows' loads in flight.  partial[slice][c] = sum of the slice's rows, or out[c] where there
+// is one slice.
+struct Columns {
+  const void* x;
+  void* out;
+  float* partial;
+  long long ld;
+  int cols, blocks;
+};
+struct ColumnArgs {
+  Columns of[2];
+  long long rows, per;
+};
+
 template <typename T, int V>
-__global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x, long long ld, long long rows, int cols, long long per,
-                                                         float* __restrict__ partial, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ ColumnArgs A) {
   __shared__ float part[8][32 * V + 1];
+  const int second = static_cast<int>(blockIdx.x) >= A.of[0].blocks;
+  const Columns& C = A.of[second];
+  const int block = static_cast<int>(blockIdx.x) - (second ? A.of[0].blocks : 0);
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int c = (blockIdx.x * 32 + lane) * V;
-  const long long r1 = min(rows, (blockIdx.y + 1LL) * per);
+  const int c = (block * 32 + lane) * V;
+  const long long r1 = min(A.rows, (blockIdx.y + 1LL) * A.per);
   float t[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) t[i] = 0.f;
-  if (c < cols) {
-    const T* p = x + (blockIdx.y * per + y) * ld + c;
-    long long r = blockIdx.y * per + y;
+  if (c < C.cols) {
+    const T* p = static_cast<const T*>(C.x) + (blockIdx.y * A.per + y) * C.ld + c;
+    long long r = blockIdx.y * A.per + y;
     if constexpr (V == 1) {
-      for (; r < r1; r += 8, p += 8 * ld) t[0] += to_f32<T>(p[0]);
+      for (; r < r1; r += 8, p += 8 * C.ld) t[0] += to_f32<T>(p[0]);
     } else {
-      for (; r + 24 < r1; r += 32, p += 32 * ld) {
+      for (; r + 24 < r1; r += 32, p += 32 * C.ld) {
         uint4 w[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) w[u] = __ldg(reinterpret_cast<const uint4*>(p + u * 8 * ld));
+        for (int u = 0; u < 4; ++u) w[u] = __ldg(reinterpret_cast<const uint4*>(p + u * 8 * C.ld));
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int i = 0; i < V; ++i) t[i] += to_f32<T>(reinterpret_cast<const T*>(&w[u])[i]);
       }
-      for (; r < r1; r += 8, p += 8 * ld) {
+      for (; r < r1; r += 8, p += 8 * C.ld) {
         const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
 #pragma unroll
         for (int i = 0; i < V; ++i) t[i] += to_f32<T>(reinterpret_cast<const T*>(&w)[i]);
@@ -52,47 +67,50 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ x
   for (int i = 0; i < V; ++i) part[y][lane * V + i] = t[i];
   __syncthreads();
   for (int k = threadIdx.x; k < 32 * V; k += 256) {
-    const int col = blockIdx.x * 32 * V + k;
-    if (col >= cols) break;
+    const int col = block * 32 * V + k;
+    if (col >= C.cols) break;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += part[i][k];
-    if (gridDim.y == 1) out[col] = from_f32<T>(sum);
-    else partial[static_cast<size_t>(blockIdx.y) * cols + col] = sum;
+    if (gridDim.y == 1) static_cast<T*>(C.out)[col] = from_f32<T>(sum);
+    else C.partial[static_cast<size_t>(blockIdx.y) * C.cols + col] = sum;
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) column_join_kernel(const float* __restrict__ partial, int slices, int cols, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) column_join_kernel(const __grid_constant__ ColumnArgs A, int slices) {
+  const Columns& C = A.of[blockIdx.y];
   const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+  if (c >= C.cols) return;
   float t = 0.f;
 #pragma unroll 8
-  for (int s = 0; s < slices; ++s) t += partial[static_cast<size_t>(s) * cols + c];
-  out[c] = from_f32<T>(t);
+  for (int s = 0; s < slices; ++s) t += C.partial[static_cast<size_t>(s) * C.cols + c];
+  static_cast<T*>(C.out)[c] = from_f32<T>(t);
 }
 
 constexpr int kSlices = 64;
 
 template <typename T>
-static cudaError_t column_sums_t(const T* x, long long ld, long long rows, int cols, T* out, float* partial, cudaStream_t s) {
+static cudaError_t column_sums_t(ColumnArgs a, cudaStream_t s) {
   constexpr int kVec = 16 / static_cast<int>(sizeof(T));
-  const long long per = rows > 128 * kSlices ? (rows + kSlices - 1) / kSlices : 128;
-  const int slices = static_cast<int>((rows + per - 1) / per);
-  const bool vec = multiple_of(x, 16) && ld % kVec == 0 && cols % kVec == 0;
+  const int count = a.of[1].out ? 2 : 1;
+  a.per = a.rows > 128 * kSlices ? (a.rows + kSlices - 1) / kSlices : 128;
+  const int slices = static_cast<int>((a.rows + a.per - 1) / a.per);
+  bool vec = true;
+  for (int i = 0; i < count; ++i) vec = vec && multiple_of(a.of[i].x, 16) && a.of[i].ld % kVec == 0 && a.of[i].cols % kVec == 0;
   const int v = vec ? kVec : 1;
-  const dim3 grid((cols + 32 * v - 1) / (32 * v), slices);
-  if (vec) column_sum_kernel<T, kVec><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial, out);
-  else column_sum_kernel<T, 1><<<grid, 256, 0, s>>>(x, ld, rows, cols, per, partial, out);
-  if (slices > 1) column_join_kernel<T><<<(cols + 255) / 256, 256, 0, s>>>(partial, slices, cols, out);
+  int blocks = 0, widest = 0;
+  for (int i = 0; i < count; ++i) {
+    a.of[i].blocks = (a.of[i].cols + 32 * v - 1) / (32 * v);
+    blocks += a.of[i].blocks;
+    widest = a.of[i].cols > widest ? a.of[i].cols : widest;
+  }
+  const dim3 grid(blocks, slices);
+  if (vec) column_sum_kernel<T, kVec><<<grid, 256, 0, s>>>(a);
+  else column_sum_kernel<T, 1><<<grid, 256, 0, s>>>(a);
+  if (slices > 1) column_join_kernel<T><<<dim3((widest + 255) / 256, count), 256, 0, s>>>(a, slices);
   count_launches(slices > 1 ? 2 : 1);
   return cudaGetLastError();
-}
-
-static cudaError_t column_sums(int dtype, const void* x, long long ld, long long rows, int cols, void* out, float* partial, cudaStream_t s) {
-  if (dtype == MSL_DTYPE_BF16)
-    return column_sums_t(static_cast<const __nv_bfloat16*>(x), ld, rows, cols, static_cast<__nv_bfloat16*>(out), partial, s);
-  return column_sums_t(static_cast<const float*>(x), ld, rows, cols, static_cast<float*>(out), partial, s);
 }
 
 // The workspace's slots for planes, and whose planes they hold in this call.
@@ -116,12 +134,17 @@ static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStrea
     const void* const src[2] = {p.a, p.b};
     const long long ld[2] = {p.lda, p.ldb};
     const int slot[2] = {slot_a, slot_b};
+    PlaneJob jobs[2];
+    int count = 0;
     for (int i = 0; i < 2; ++i) {
       if (slots.of[slot[i]] == src[i]) continue;
       if (planes_bytes(p.dtype, rows[i], cols[i]) > slots.bytes[slot[i]]) return failf(MSL_ERR_WORKSPACE, "planes beyond their slot");
-      e = launch_planes(p.dtype, src[i], ld[i], rows[i], cols[i], slots.at[slot[i]], s);
-      if (e != cudaSuccess) return cuda_failf(e, "split_kernel launch");
+      jobs[count++] = {src[i], ld[i], rows[i], cols[i], slots.at[slot[i]]};
       slots.of[slot[i]] = src[i];
+    }
+    if (count) {
+      e = launch_planes(p.dtype, jobs, count, s);
+      if (e != cudaSuccess) return cuda_failf(e, "split_kernel launch");
     }
     e = launch_product_planes(p, slots.at[slot_a], slots.at[slot_b], s);
     if (e != cudaSuccess) return cuda_failf(e, "planes_kernel launch");
@@ -189,7 +212,7 @@ static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
     need(M, C, 2 * F, kPlain, true);
     need(2 * F, C, M, kPlain, true, true);
     need(C, F, M, kPlain, true, true);
-    w.columns = sizeof(float) * kSlices * static_cast<size_t>(2 * F > C ? 2 * F : C);
+    w.columns = sizeof(float) * kSlices * static_cast<size_t>(2 * F + C);
     w.columns = (w.columns + 255) / 256 * 256;
     if (planes && M > 0) {
       w.planes[0] = size(M, C);
@@ -348,13 +371,14 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     rc = ffn::run(p, slots, 0, 2, s);
     if (rc) return rc;
   }
-  float* const partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + W.partial);
-  if (io->db_in) {
-    const cudaError_t e = ffn::column_sums(geom->dtype, io->dgu, 2 * F, M, static_cast<int>(2 * F), io->db_in, partial, s);
-    if (e != cudaSuccess) return cuda_failf(e, "column_sum_kernel launch");
-  }
-  if (io->db_out) {
-    const cudaError_t e = ffn::column_sums(geom->dtype, io->dy, io->dy_ld, M, static_cast<int>(C), io->db_out, partial, s);
+  if (io->db_in || io->db_out) {
+    float* const partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + W.partial);
+    ffn::ColumnArgs a{};
+    a.rows = M;
+    int i = 0;
+    if (io->db_in) a.of[i++] = {io->dgu, io->db_in, partial, 2 * F, static_cast<int>(2 * F), 0};
+    if (io->db_out) a.of[i] = {io->dy, io->db_out, partial + 2 * F * ffn::kSlices, io->dy_ld, static_cast<int>(C), 0};
+    const cudaError_t e = geom->dtype == MSL_DTYPE_BF16 ? ffn::column_sums_t<__nv_bfloat16>(a, s) : ffn::column_sums_t<float>(a, s);
     if (e != cudaSuccess) return cuda_failf(e, "column_sum_kernel launch");
   }
   return MSL_OK;

@@ -109,7 +109,12 @@ cudaError_t launch_product_skinny(const Product& p, cudaStream_t s);
 bool planes_apply(const Product& p);
 size_t planes_bytes(int dtype, long long rows, long long cols);
 size_t planes_partial_bytes(int dtype, long long M, long long N, long long K, int epilogue);
-cudaError_t launch_planes(int dtype, const void* x, long long ld, long long rows, long long cols, void* out, cudaStream_t s);
+struct PlaneJob {
+  const void* x;
+  long long ld, rows, cols;
+  void* out;
+};
+cudaError_t launch_planes(int dtype, const PlaneJob* jobs, int count, cudaStream_t s);  // one or two
 cudaError_t launch_product_planes(const Product& p, const void* pa, const void* pb, cudaStream_t s);
 
 }  // namespace ffn
