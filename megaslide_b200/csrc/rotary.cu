@@ -122,23 +122,48 @@ struct alignas(16) Raw {
       }
     }
   }
-  // pair j = (first, second); two pairs a float2
+  // pair j = (first, second); two pairs a float2.  bf16 goes by words of two elements: a shift or a mask each way out, one
+  // conversion for both on the way back.
+  static constexpr bool kWords = sizeof(T) == 2 && V > 1;
   __device__ __forceinline__ void split(float2 (&a)[V * SL / 2], float2 (&b)[V * SL / 2]) const {
 #pragma unroll
     for (int j = 0; j < V * SL; ++j) {
       const int s = j / V, i = j % V;
-      const float x = to_f32<T>(e[s][INTER ? 2 * i : i]), y = to_f32<T>(e[s][INTER ? 2 * i + 1 : V + i]);
+      float x, y;
+      if constexpr (kWords) {
+        const uint32_t* const w = reinterpret_cast<const uint32_t*>(e[s]);
+        x = INTER ? bf16_lo(w[i]) : i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
+        y = INTER ? bf16_hi(w[i]) : i & 1 ? bf16_hi(w[(V + i) / 2]) : bf16_lo(w[(V + i) / 2]);
+      } else {
+        x = to_f32<T>(e[s][INTER ? 2 * i : i]);
+        y = to_f32<T>(e[s][INTER ? 2 * i + 1 : V + i]);
+      }
       (j & 1 ? a[j / 2].y : a[j / 2].x) = x;
       (j & 1 ? b[j / 2].y : b[j / 2].x) = y;
     }
   }
   __device__ __forceinline__ void join(const float2 (&a)[V * SL / 2], const float2 (&b)[V * SL / 2]) {
+    if constexpr (kWords) {
+#pragma unroll
+      for (int j = 0; j < V * SL; j += 2) {
+        const int s = j / V, i = j % V;
+        uint32_t* const w = reinterpret_cast<uint32_t*>(e[s]);
+        const float2 p = a[j / 2], q = b[j / 2];
+        w[INTER ? i : i / 2] = INTER ? pack(p.x, q.x) : pack(p.x, p.y);
+        w[INTER ? i + 1 : (V + i) / 2] = INTER ? pack(p.y, q.y) : pack(q.x, q.y);
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < V * SL; ++j) {
       const int s = j / V, i = j % V;
       e[s][INTER ? 2 * i : i] = from_f32<T>(j & 1 ? a[j / 2].y : a[j / 2].x);
       e[s][INTER ? 2 * i + 1 : V + i] = from_f32<T>(j & 1 ? b[j / 2].y : b[j / 2].x);
     }
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(t);
   }
 };
 
@@ -277,26 +302,33 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
       pos[1] = rest / P.W;
       pos[2] = rest - pos[1] * P.W;
     }
-    // the item's units in their order, a few stages ahead
+    // The item's units in their order, a few stages ahead.  A unit's place in its row is min(unit's first, last head's)
+    // + lo, kept up from unit to unit.
+    const int step_at = per_warp * P.d, last_at = (nh - 1) * P.d, first_at = (b0 * per_warp + seg) * P.d;
     long long ahead = row0;
-    int ahead_unit = b0, slot = 0;
+    int ahead_unit = b0, ahead_at = first_at, slot = 0;
+    const T* src[OPS];
+    src[0] = static_cast<const T*>(P.x[o]) + row0 * P.x_ld[o] + lo[0];
+    if (BWD) src[OPS - 1] = static_cast<const T*>(P.dy[o]) + row0 * P.dy_ld[o] + lo[0];
     auto issue = [&](int to) {
       if (ahead < row1) {
 #pragma unroll
-        for (int u = 0; u < UU; ++u) {
-          const int at = min(min(ahead_unit + u, b1 - 1) * per_warp + seg, nh - 1) * P.d + lo[0];
+        for (int u = 0; u < UU; ++u) {  // units beyond b1 (another warp's, or the last head again) only fill the stage
+          const int at = min(ahead_at, last_at);
+          ahead_at += step_at;
 #pragma unroll
-          for (int k = 0; k < OPS; ++k) {
-            const T* const from = (k ? static_cast<const T*>(P.dy[o]) + ahead * P.dy_ld[o] : static_cast<const T*>(P.x[o]) + ahead * P.x_ld[o]) + at;
+          for (int k = 0; k < OPS; ++k)
 #pragma unroll
             for (int i = 0; i < kPieces; ++i)
-              copy_async<kPiece>(mine_at + (((to * UU + u) * OPS + k) * kPieces + i) * 32 * kPiece, from + i * (INTER ? kPiece / static_cast<int>(sizeof(T)) : hi[0]));
-          }
+              copy_async<kPiece>(mine_at + (((to * UU + u) * OPS + k) * kPieces + i) * 32 * kPiece, src[k] + (at + i * (INTER ? kPiece / static_cast<int>(sizeof(T)) : hi[0])));
         }
         ahead_unit += UU;
         if (ahead_unit >= b1) {
           ahead_unit = b0;
+          ahead_at = first_at;
           ++ahead;
+#pragma unroll
+          for (int k = 0; k < OPS; ++k) src[k] += k ? P.dy_ld[o] : P.x_ld[o];
         }
       }
       copy_commit();
@@ -371,7 +403,8 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
       }
       T* const yr = static_cast<T*>(P.y[o]) + row * P.y_ld[o];
       auto finish = [&](R& raw, const R& rdy, int b) {
-        const bool on = b * per_warp + seg < nh;
+        const int at = first_at + (b - b0) * step_at;
+        const bool on = at <= last_at;
         float2 xa[N2], xb[N2];
         raw.split(xa, xb);
         float r = 1.f;
@@ -421,7 +454,7 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
         if (on) {
           T* to[SL];
 #pragma unroll
-          for (int s = 0; s < SL; ++s) to[s] = yr + min(b * per_warp + seg, nh - 1) * P.d + lo[s];
+          for (int s = 0; s < SL; ++s) to[s] = yr + (at + lo[s]);
           raw.put(to, hi, valid);
         }
       };
@@ -445,7 +478,7 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
         const T* const gr = BWD ? static_cast<const T*>(P.dy[o]) + row * P.dy_ld[o] : nullptr;
         for (int b = b0; b < b1; ++b) {
           R raw, rdy;
-          const int at = min(b * per_warp + seg, nh - 1) * P.d;
+          const int at = min(first_at + (b - b0) * step_at, last_at);
           const T* from[SL];
 #pragma unroll
           for (int s = 0; s < SL; ++s) from[s] = xr + at + lo[s];
