@@ -18,9 +18,11 @@
 // two pairs at a time (fma.rn.f32x2), the weights are multiplied into the cosines and sines once per token, and
 // lanes without a head load a neighbour's instead of branching (they only never store).
 //
-// Measured, bf16 (of the measured copy bandwidth): rotation of 131072 x 16 x 72, 604 MB, 110 us, 5.5 TB/s (84%); norm
-// and rotation of 262144 x 24 x 64 queries and keys, 3.2 GB, 578 us, 5.6 TB/s (85%); their backward, 4.8 GB, 825 us,
-// 5.9 TB/s (89%).  With loads straight to registers 145, 740 and 1035 us.
+// Measured in a steady loop, bf16 (of the measured copy bandwidth): rotation of 131072 x 16 x 72, 604 MB, 107 us, 5.6
+// TB/s (86%); norm and rotation of 262144 x 24 x 64 queries and keys, 3.2 GB, 593 us, 5.4 TB/s (83%); their backward,
+// 4.8 GB, 859 us, 5.6 TB/s (86%).  At these rates the GPU is at its 1000 W (a plain copy takes 770) and the clock falls
+// to 1.7 GHz, so instructions count beside bytes; in the first milliseconds the forward and backward take 570 and 810 us.
+// With loads straight to registers 145, 740 and 1035 us.
 
 #include "msl_abi.cuh"
 #include "msl_common.cuh"
@@ -543,7 +545,6 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restri
 // ------------------------------------------------------------------------------------------ host
 
 constexpr int kWarps = 8;
-constexpr int kMostGroup = 8;  // tokens of a warp's turn; 4: forward 599 us instead of 578, 16: rotation 122 us instead of 110
 constexpr int kBwdBlocksPerSm = 4;
 
 int fill(const msl_rotary_geometry* g, Params& P) {
@@ -647,9 +648,12 @@ cudaError_t launch(Params P, cudaStream_t s, int blocks) {
   long long splits = P.rows >= want ? 1 : (want + P.rows - 1) / P.rows;
   if (splits > (units0 > units1 ? units0 : units1)) splits = units0 > units1 ? units0 : units1;
   P.splits = static_cast<int>(splits);
-  // several tokens a warp once every SM has its warps: their loads run ahead over them, their places follow
-  const long long each_warp = (P.rows + 3 * want - 1) / (3 * want);
-  P.group = static_cast<int>(splits > 1 ? 1 : each_warp < kMostGroup ? each_warp : kMostGroup);
+  // Several tokens a warp once every SM has its warps: their loads run ahead over them, their places follow.  Up to 8,
+  // and more where the GPU has its blocks four times over all the same (norm and rotation of 262144 x 24 x 64 queries
+  // and keys: 8 600 us, 37 582, 148 586; rotation of 131072 x 16 x 72: 8 114 us, 10 115, 37 122).
+  const long long resident = 3 * want, tokens = P.rows * (P.heads[1] ? 2 : 1);
+  const long long few = (P.rows + resident - 1) / resident, four = (tokens + 4 * resident - 1) / (4 * resident);
+  P.group = static_cast<int>(splits > 1 ? 1 : few <= 8 ? few : four > 8 ? four : 8);
   P.table_vec = SL == 1 && V % 2 == 0 && multiple_of(P.table, 16);
   for (int a = 0; a < 3; ++a) P.table_vec = P.table_vec && P.npair[a] % V == 0;
   if (blocks == 0) {
