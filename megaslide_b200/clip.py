@@ -8,6 +8,7 @@ from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import ops
 
@@ -52,4 +53,7 @@ def clip_grad_norm_(tensors: Tensors, max_norm: float, *, out: Optional[Sequence
     extra = _check(extra_sumsq)
     if not ts:
         return torch.tensor(math.sqrt(extra))
-    return ops.grad_norm(ts, ts if out is None else list(out), float(max_norm), extra)
+    out = ts if out is None else list(out)
+    norm = ops.grad_norm(ts, out, float(max_norm), extra)
+    increment_version(out)  # the kernel wrote them behind autograd's back
+    return norm

@@ -154,13 +154,13 @@ struct alignas(16) Raw {
         w[INTER ? i : i / 2] = INTER ? pack(p.x, q.x) : pack(p.x, p.y);
         w[INTER ? i + 1 : (V + i) / 2] = INTER ? pack(p.y, q.y) : pack(q.x, q.y);
       }
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int j = 0; j < V * SL; ++j) {
-      const int s = j / V, i = j % V;
-      e[s][INTER ? 2 * i : i] = from_f32<T>(j & 1 ? a[j / 2].y : a[j / 2].x);
-      e[s][INTER ? 2 * i + 1 : V + i] = from_f32<T>(j & 1 ? b[j / 2].y : b[j / 2].x);
+      for (int j = 0; j < V * SL; ++j) {
+        const int s = j / V, i = j % V;
+        e[s][INTER ? 2 * i : i] = from_f32<T>(j & 1 ? a[j / 2].y : a[j / 2].x);
+        e[s][INTER ? 2 * i + 1 : V + i] = from_f32<T>(j & 1 ? b[j / 2].y : b[j / 2].x);
+      }
     }
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -177,14 +177,15 @@ __device__ __forceinline__ float head_sum(float v, int lanes, int in_head, int f
 #pragma unroll
     for (int o = LC >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     return v;
-  }
+  } else {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    if (o >= lanes) break;
-    const float t = __shfl_down_sync(kFull, v, o);
-    if (in_head + o < lanes) v += t;
+    for (int o = 1; o < 32; o <<= 1) {
+      if (o >= lanes) break;
+      const float t = __shfl_down_sync(kFull, v, o);
+      if (in_head + o < lanes) v += t;
+    }
+    return __shfl_sync(kFull, v, first);
   }
-  return __shfl_sync(kFull, v, first);
 }
 
 // Copies of a lane's own bytes to its own place in shared memory: the loads ahead, without registers to hold them.

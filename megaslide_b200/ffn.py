@@ -41,6 +41,7 @@ class GatedFFNFunction(torch.autograd.Function):
         return y if y.shape == x.shape else y.view(x.shape)
 
     @staticmethod
+    @ops.once_only
     def backward(ctx, dy):
         x2, w_in, w_out, b_in, b_out, h, kept = ctx.saved_tensors
         dx, dw_in, dw_out, db_in, db_out = ops.gated_ffn_bwd(x2, w_in, w_out, h, kept, _rows_of(dy), b_in, b_out, ctx.activation,

@@ -15,6 +15,7 @@ from operator import attrgetter
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import DsaBwdIO, DsaFwdIO, DsaGeometry, DwconvGeometry
@@ -27,6 +28,17 @@ def dtype_code(dt: torch.dtype) -> int:
         return _DTYPES[dt]
     except KeyError:
         raise TypeError(f"megaslide_b200 supports float32 and bfloat16 activations, got {dt}") from None
+
+
+def once_only(backward):
+    """torch's once_differentiable, an error where a second derivative is taken, at its cost (a few microseconds) only
+    where a graph of the backward is recorded."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -92,6 +92,7 @@ class Rope3DFunction(torch.autograd.Function):
         return _rotate(call, x, table, index, False)
 
     @staticmethod
+    @ops.once_only
     def backward(ctx, dy):
         table, index = ctx.saved_tensors
         return None, _rotate(ctx.call, dy, table, index, True), None, None
@@ -126,6 +127,7 @@ class QKNormRopeFunction(torch.autograd.Function):
         return _norm_rotate(call, q, k, q_weight, k_weight, table, index)
 
     @staticmethod
+    @ops.once_only
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, table, index = ctx.saved_tensors
         c = ctx.call

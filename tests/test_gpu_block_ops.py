@@ -632,3 +632,34 @@ def test_norm_beyond_2_31_elements_and_on_another_stream():
     s.synchronize()
     want = 0.5 * math.sqrt(2 ** 31 + 5)
     assert abs(float(norm) - want) <= 4 * EPS * want
+
+
+# ------------------------------------------------------------------------------------------ with autograd
+
+def test_second_derivatives_are_refused():
+    """The backward passes are kernels without a derivative of their own: asking for one is an error, not a term that
+    is silently missing."""
+    x = _rand(1, 1, 6, 16).requires_grad_()
+    table = msl.rotary_table((1, 2, 3), (2, 2, 4), device=_dev())
+    w = torch.ones(8, device=_dev(), requires_grad=True)
+    w_in, w_out = _rand(2, 16, 16).requires_grad_(), _rand(3, 16, 8).requires_grad_()
+    for y in (msl.rope3d(x, table, video_shape=(1, 2, 3), axes=(2, 2, 4), heads=2),
+              msl.qk_norm_rope(x, x, w, w, heads=2)[0], msl.gated_ffn(x, w_in, w_out)):
+        dx, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (dx * dx).sum().backward()
+
+
+def test_clipping_counts_as_a_write():
+    """A tensor that autograd has saved and the clipping then scales is noticed by autograd."""
+    a = torch.ones(64, device=_dev(), requires_grad=True)
+    g = torch.full((64,), 2.0, device=_dev())
+    y = (a * g).sum()
+    msl.clip_grad_norm_([g], 1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    b, c = torch.ones(64, device=_dev()), torch.empty(64, device=_dev())
+    y = (a * b).sum() + (a * c).sum()
+    msl.clip_grad_norm_([b], 1.0, out=[c])
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
