@@ -21,8 +21,8 @@
 // Measured in a steady loop, bf16 (of the measured copy bandwidth): rotation of 131072 x 16 x 72, 604 MB, 107 us, 5.6
 // TB/s (86%); norm and rotation of 262144 x 24 x 64 queries and keys, 3.2 GB, 593 us, 5.4 TB/s (83%); their backward,
 // 4.8 GB, 859 us, 5.6 TB/s (86%).  At these rates the GPU is at its 1000 W (a plain copy takes 770) and the clock falls
-// to 1.7 GHz, so instructions count beside bytes; in the first milliseconds the forward and backward take 570 and 810 us.
-// With loads straight to registers 145, 740 and 1035 us.
+// to 1.7 GHz, so instructions count beside bytes; a GPU that kept its clock took 518 and 807 us (95 and 91%).  With
+// loads straight to registers 145, 740 and 1035 us.
 
 #include "msl_abi.cuh"
 #include "msl_common.cuh"
@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
   const unsigned block = blockIdx.x - (o ? P.blocks0 : 0), nblocks = o ? gridDim.x - P.blocks0 : P.blocks0;
   const int nh = P.heads[o];
   const int units = (nh + per_warp - 1) / per_warp;
+  const bool ragged = units * per_warp != nh;
 
   int lo[SL], hi[SL];  // the slot's first channel, and from there to its second half
   bool valid[SL];
@@ -437,6 +438,11 @@ __global__ void __launch_bounds__(256, V == 4 ? (MODE == kBackward ? 2 : 3) : 1)
           float2 da[N2], db[N2], dot = both(0.f);
           const float2 rr = both(on ? r : 0.f);  // a head loaded twice counts once
           rdy.split(da, db);
+          if (ragged && b == units - 1) {  // what a lane without a head has loaded may be another's result by now (dx over dy)
+#pragma unroll
+            for (int j = 0; j < N2; ++j)
+              if (!on) xa[j] = xb[j] = da[j] = db[j] = both(0.f);
+          }
 #pragma unroll
           for (int j = 0; j < N2; ++j) {
             const float2 na = fma2(db[j], B[j], mul2(da[j], A[j])), nb = fma2(da[j], D[j], mul2(db[j], A[j]));

@@ -663,3 +663,36 @@ def test_clipping_counts_as_a_write():
     msl.clip_grad_norm_([b], 1.0, out=[c])
     with pytest.raises(RuntimeError, match="inplace"):
         y.backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_calls_in_a_cuda_graph(dtype):
+    """A step over all operators, forward and backward, captured once and replayed on other inputs, equals the calls."""
+    M, C, F, vs, axes = 60, 64, 96, (3, 4, 5), (4, 4, 8)
+    x = _rand(1, 1, M, C, dtype=dtype).requires_grad_()
+    w_in, w_out = _rand(2, 2 * F, C, dtype=dtype, std=0.1).requires_grad_(), _rand(3, C, F, dtype=dtype, std=0.1).requires_grad_()
+    weight = _rand(4, 16).add_(2).requires_grad_()
+    table = msl.rotary_table(vs, axes, device=_dev())
+
+    def step():
+        kw = dict(video_shape=vs, axes=axes, heads=4)
+        q, k = msl.qk_norm_rope(x, msl.rope3d(x, table, **kw), weight, weight, table, **kw)
+        grads = torch.autograd.grad(msl.gated_ffn(q + k, w_in, w_out), (x, w_in, w_out, weight), torch.ones_like(x))
+        grads = [g.clone() for g in grads]
+        return [msl.clip_grad_norm_(grads, 0.5), *grads, msl.gated_ffn(x[:, :1].detach(), w_in.detach(), w_out.detach())]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (5, 6):
+        with torch.no_grad():
+            x.copy_(_rand(seed, 1, M, C, dtype=dtype))
+        graph.replay()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
