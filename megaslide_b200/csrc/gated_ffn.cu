@@ -120,6 +120,8 @@ struct Slots {
   const void* of[3];
 };
 
+static const char* const kOff16 = "an address or a row stride is no multiple of 16 bytes and the geometry's unaligned is 0";
+
 static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStream_t s, bool rows = false) {
   cudaError_t e;
   if (rows) {
@@ -152,7 +154,7 @@ static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStrea
     e = launch_product_skinny(p, s);
     if (e != cudaSuccess) return cuda_failf(e, "skinny_kernel launch");
   } else if (!slots.at[0]) {
-    return failf(MSL_ERR_INVALID, "an address or a row stride is no multiple of 16 bytes and the geometry's unaligned is 0");
+    return failf(MSL_ERR_INVALID, kOff16);
   } else {
     return failf(MSL_ERR_UNSUPPORTED, "the driver encodes no tensor maps, or the product has over 2^30 tiles");
   }
@@ -176,10 +178,16 @@ static int check(const msl_ffn_geometry* g, const msl_ffn_io* io) {
 struct Workspace {
   size_t partial, columns, planes[3], total;
 };
+// A bf16 forward that the kernels for few rows do whole, if the operands lie on 16 bytes as the geometry says.
+static bool few_rows(const msl_ffn_geometry* g, bool backward) {
+  return !backward && g->dtype == MSL_DTYPE_BF16 && g->rows <= rows_most(g->dtype, 2LL * g->hidden * g->dim) && g->dim % 8 == 0 &&
+         g->hidden % 8 == 0 && !g->unaligned;
+}
 static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
   Workspace w{};
   const long long M = g->rows, C = g->dim, F = g->hidden;
   const bool f32 = g->dtype == MSL_DTYPE_F32, copies = !f32 && (C % 8 || F % 8 || g->unaligned);
+  if (few_rows(g, backward)) return w;
   bool planes = false;  // some product takes planes
   auto need = [&](long long m, long long n, long long k, int epilogue, bool b_major, bool a_major = false) {
     if (M == 0) return;
@@ -295,6 +303,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   // both products by rows, or neither: the second is launched into the first
   const bool rows = ffn::rows_apply(p) && multiple_of(io->h, 16) && multiple_of(io->w_out, 16) &&
                     F * (geom->dtype == MSL_DTYPE_BF16 ? 2 : 4) % 16 == 0;
+  if (!rows && ffn::few_rows(geom, false)) return failf(MSL_ERR_INVALID, ffn::kOff16);
   rc = ffn::run(p, slots, 0, 1, s, rows);
   if (rc) return rc;
   p = ffn::product(geom, io, W, workspace);

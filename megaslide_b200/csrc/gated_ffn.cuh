@@ -99,6 +99,7 @@ cudaError_t launch_product_tc(const Product& p, cudaStream_t s);
 
 // Form for a few rows (gated_ffn_rows.cu): the forward's two products, launched one after the other.
 constexpr int kMostRows = 16, kMostRowsF32 = 8;
+long long rows_most(int dtype, long long weights);  // rows up to which it is taken, by the elements of the first product's weights
 bool rows_apply(const Product& p);
 cudaError_t launch_product_rows(const Product& p, cudaStream_t s);
 // CUDA-core form for float32, few rows or small products (gated_ffn_skinny.cu).

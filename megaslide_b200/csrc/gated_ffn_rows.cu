@@ -293,12 +293,17 @@ cudaError_t launch_mma(Args a, cudaStream_t s) {
 
 }  // namespace rows
 
+// 9 to 16 rows of bf16 only while the caches hold the weights (7168 x 28672: 390 us for 16, against 260 on the tensor
+// cores)
+long long rows_most(int dtype, long long weights) {
+  return dtype == MSL_DTYPE_F32 ? kMostRowsF32 : weights < (1LL << 25) ? kMostRows : kMostRows / 2;
+}
+
 bool rows_apply(const Product& p) {
   const long long es = p.dtype == MSL_DTYPE_BF16 ? 2 : 4;
-  // 9 to 16 rows only while the caches hold the weights (7168 x 28672: 390 us for 16, against 260 on the tensor cores)
-  const long long most = p.dtype == MSL_DTYPE_F32 ? kMostRowsF32 : p.N * p.K * (p.epilogue == kGate ? 2 : 1) < (1LL << 25) ? kMostRows : kMostRows / 2;
-  return p.M <= most && !p.a_major && !p.b_major && p.epilogue != kDgate && p.K * es % 16 == 0 && p.lda * es % 16 == 0 &&
-         p.ldb * es % 16 == 0 && multiple_of(p.a, 16) && multiple_of(p.b, 16) && p.K <= (1 << 30) && p.N <= (1 << 30);
+  return p.M <= rows_most(p.dtype, p.N * p.K * (p.epilogue == kGate ? 2 : 1)) && !p.a_major && !p.b_major && p.epilogue != kDgate &&
+         p.K * es % 16 == 0 && p.lda * es % 16 == 0 && p.ldb * es % 16 == 0 && multiple_of(p.a, 16) && multiple_of(p.b, 16) &&
+         p.K <= (1 << 30) && p.N <= (1 << 30);
 }
 
 cudaError_t launch_product_rows(const Product& p, cudaStream_t s) {

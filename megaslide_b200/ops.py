@@ -520,12 +520,13 @@ def convert_f32(src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
 
 
 _HERE = nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: current_stream() builds an object, 2 us a call
+# the handle alone (current_stream() builds an object, 2 us a call), and the device without asking whether CUDA has started
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _on(dev: torch.device):
     """Context that makes `dev` current; nothing to do where it is."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == _current() else torch.cuda.device(dev)
 
 
 def _ld(t: torch.Tensor, name: str) -> int:
@@ -738,12 +739,13 @@ def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
     dev, dt = x.device, x.dtype
     x_ld = _ld(x, "x")
-    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation), _unaligned(x, w_in, w_out, b_in, b_out) or int(x_ld % 8 != 0))
+    px, pi, po, pbi, pbo = x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), _ptr(b_in), _ptr(b_out)
+    off = (px | pi | po | (pbi or 0) | (pbo or 0)) & 15 or x_ld % 8
+    g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation), 1 if off else 0)
     h = torch.empty(M, F, device=dev, dtype=dt)
     kept = torch.empty(M, 2 * F, device=dev, dtype=dt) if keep else None
     y = torch.empty(x.shape, device=dev, dtype=dt)
-    io = _lib.FfnIO(x.data_ptr(), x_ld, w_in.data_ptr(), _ptr(b_in), w_out.data_ptr(), _ptr(b_out), h.data_ptr(), _ptr(kept),
-                    y.data_ptr(), C)
+    io = _lib.FfnIO(px, x_ld, pi, pbi, po, pbo, h.data_ptr(), _ptr(kept), y.data_ptr(), C)
     io.status = _flag(dev, status)
     lib = _lib.load()
     with _on(dev):
