@@ -525,6 +525,8 @@ cudaError_t launch(const Product& p, const void* pa, const void* pb, cudaStream_
   a.kper = cut.kper;
   a.partial = p.partial;
   a.status = p.status;
+  cudaError_t e = bind_context();
+  if (e != cudaSuccess) return e;
   Maps maps;
   const long long brows = EPI == kGate ? 2 * p.N : p.N;
   const bool ok = (AM ? plane_map(&maps.a, pa, np, p.K, p.M, padded(p.M), kBK) : plane_map(&maps.a, pa, np, p.M, p.K, padded(p.K), kBM)) &&
@@ -533,7 +535,7 @@ cudaError_t launch(const Product& p, const void* pa, const void* pb, cudaStream_
   constexpr int smem = 1024 + kRing + kEpiWarps * kTileBytes + 24 * kMaxStages + 64;
   static_assert(smem <= 232448, "shared memory of a block");
   auto* const kernel = planes_kernel<T, EPI, AM, BM>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int pairs = sm_count() / 2;
   cudaLaunchConfig_t cfg{};

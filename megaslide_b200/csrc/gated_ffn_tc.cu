@@ -576,6 +576,8 @@ cudaError_t launch(const Product& p, cudaStream_t s) {
   a.stage_bytes = kStageA + (BM ? a.boxes * 8192 : a.bn / 2 * kBK * 2);
   // stages start on the swizzle's 1024 bytes: half of B is a multiple of 16 rows of 128 bytes
   a.stages = kRing / a.stage_bytes < kMaxStages ? kRing / a.stage_bytes : kMaxStages;
+  cudaError_t e = bind_context();
+  if (e != cudaSuccess) return e;
   Maps maps;
   bool ok = AM ? matrix_map(&maps.a, p.a, p.K, p.M, p.lda, kBK) : matrix_map(&maps.a, p.a, p.M, p.K, p.lda, kBM);
   const long long brows = EPI == kGate ? 2 * p.N : p.N;
@@ -597,7 +599,7 @@ cudaError_t launch(const Product& p, cudaStream_t s) {
   constexpr int smem = 1024 + kRing + kEpiWarps * kStaging + 24 * kMaxStages + 16 * kEpiWarps + 64;
   static_assert(smem <= 232448, "shared memory of a block");
   auto* const kernel = product_kernel<EPI, AM, BM, ACT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int pairs = sm_count() / 2;
   cudaLaunchConfig_t cfg{};

@@ -131,5 +131,13 @@ inline Encode encoder() {
   return encode;
 }
 
+// The encoder is a driver call and works only with the device's context current on the calling thread.  A thread that has
+// made no runtime call of its own has none yet: autograd's, say, where its memory came out of torch's cache.
+inline cudaError_t bind_context() {
+  int device = 0;
+  const cudaError_t e = cudaGetDevice(&device);
+  return e != cudaSuccess ? e : cudaSetDevice(device);
+}
+
 }  // namespace t5
 }  // namespace msl

@@ -12,6 +12,7 @@ kept projections, h, their gradients, the result).
 
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -405,6 +406,12 @@ def test_gated_ffn_few_rows(M, dtype):
         _ffn_check_all(M, C, F, dtype, "gelu", bias)
 
 
+@pytest.mark.parametrize("M", [8, 9, 16])
+def test_gated_ffn_few_rows_of_wide_weights(M):
+    """Weights beyond the size up to which 9 to 16 rows go by rows."""
+    _ffn_check_all(M, 4104, 4096, torch.bfloat16, "silu", True)
+
+
 @pytest.mark.parametrize("M,C,F", [(1, 1152, 4608), (6, 2560, 1000), (13, 640, 2240), (16, 100, 70), (17, 250, 639), (30, 1152, 2880), (65, 640, 1600),
                                    (100, 77, 1531)])
 def test_gated_ffn_float32_few_rows(M, C, F):
@@ -470,11 +477,11 @@ def test_gated_ffn_weights_inside_a_packed_buffer():
             _close(a, b.double(), 2 * RMS, name)
 
 
-@pytest.mark.parametrize("C,F,x_ld", [(16, 32, 17), (15, 32, 16)])
-def test_gated_ffn_entry_refuses_rows_off_16_bytes_without_room(C, F, x_ld):
+@pytest.mark.parametrize("M,C,F,x_ld", [(40, 16, 32, 17), (40, 15, 32, 16), (3, 16, 32, 17), (3, 15, 32, 16)])
+def test_gated_ffn_entry_refuses_rows_off_16_bytes_without_room(M, C, F, x_ld):
     """A C caller that leaves unaligned at 0 gets an error for such rows, and nothing is written; odd widths say
     it by themselves."""
-    lib, M = _lib.load(), 40
+    lib = _lib.load()
     x = torch.zeros(M, x_ld, device=_dev(), dtype=torch.bfloat16)
     w_in, w_out = (torch.zeros(n, device=_dev(), dtype=torch.bfloat16) for n in (2 * F * C, C * F))
     h, y = (torch.full((M, n), 7.0, device=_dev(), dtype=torch.bfloat16) for n in (F, C))
@@ -634,7 +641,44 @@ def test_norm_beyond_2_31_elements_and_on_another_stream():
     assert abs(float(norm) - want) <= 4 * EPS * want
 
 
-# ------------------------------------------------------------------------------------------ with autograd
+# ------------------------------------------------------------------------------------------ with threads and autograd
+
+@pytest.mark.parametrize("C", [64, 61])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_first_call_of_a_thread(dtype, C):
+    """A thread whose first contact with the GPU is a call of the gated block, all its memory from torch's cache (as
+    autograd's thread may be), gets the same results."""
+    M, F = 300, 128
+    x, w_in, w_out, b_in, b_out = (t.detach() for t in _ffn_case(M, C, F, dtype, "silu", True))
+    dy = _rand(9, M, C, dtype=dtype)
+    y, h, kept = ops.gated_ffn_fwd(x, w_in, w_out, b_in, b_out, keep=True)
+
+    def forward():
+        return ops.gated_ffn_fwd(x, w_in, w_out, b_in, b_out, keep=True)
+
+    def backward():
+        return ops.gated_ffn_bwd(x, w_in, w_out, h, kept, dy, b_in, b_out)
+
+    for call in (forward, backward):
+        want = [t.clone() for t in call()]
+        torch.cuda.synchronize()
+        got, errors = [], []
+
+        def run():
+            try:
+                got.extend(call())
+            except Exception as e:  # raised again where pytest sees it
+                errors.append(e)
+
+        thread = threading.Thread(target=run)
+        thread.start()
+        thread.join()
+        assert not errors, errors
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 
 def test_second_derivatives_are_refused():
     """The backward passes are kernels without a derivative of their own: asking for one is an error, not a term that
