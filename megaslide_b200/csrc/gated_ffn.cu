@@ -130,6 +130,9 @@ static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStrea
   } else if (tc_applies(p)) {
     e = launch_product_tc(p, s);
     if (e != cudaSuccess) return cuda_failf(e, "product_kernel launch");
+  } else if (few_apply(p)) {
+    e = launch_product_few(p, s);
+    if (e != cudaSuccess) return cuda_failf(e, "few_kernel launch");
   } else if (slots.at[0] && planes_apply(p)) {
     const long long rows[2] = {p.a_major ? p.K : p.M, p.b_major ? p.K : (p.epilogue == kGate ? 2 * p.N : p.N)};
     const long long cols[2] = {p.a_major ? p.M : p.K, p.b_major ? p.N : p.K};
@@ -203,6 +206,10 @@ static Workspace workspace_of(const msl_ffn_geometry* g, bool backward) {
       b = planes_partial_bytes(g->dtype, m, n, k, epilogue);
     } else if (f32) {
       b = skinny_bytes(m, n, k, epilogue, a_major);
+    }
+    if (f32 && few_shape(m, epilogue == kGate ? 2 * n : n, k, a_major, b_major)) {
+      const size_t few = few_bytes(m, n, k, epilogue);
+      b = few > b ? few : b;
     }
     // some products of a bf16 block may be addressable though others are not
     const size_t t = f32 ? 0 : tc_partial_bytes(m, n, k, epilogue, b_major);

@@ -105,6 +105,13 @@ cudaError_t launch_product_rows(const Product& p, cudaStream_t s);
 // CUDA-core form for float32, few rows or small products (gated_ffn_skinny.cu).
 size_t skinny_bytes(long long M, long long N, long long K, int epilogue, bool a_major);
 cudaError_t launch_product_skinny(const Product& p, cudaStream_t s);
+cudaError_t launch_skinny_join(const Product& p, int shares, cudaStream_t s);  // shares of k in p.partial, and the epilogue
+// Tensor-core form for few rows of float32 (gated_ffn_few.cu), and the shapes it takes where the operands lie on 16 bytes.
+constexpr int kMostRowsFew = 64;
+bool few_shape(long long M, long long cols, long long K, bool a_major, bool b_major);
+bool few_apply(const Product& p);
+size_t few_bytes(long long M, long long N, long long K, int epilogue);
+cudaError_t launch_product_few(const Product& p, cudaStream_t s);
 // Tensor-core form for float32 and for widths that are no multiple of 8 (gated_ffn_planes.cu): the operands as
 // planes [planes][rows][cols padded to 8] of planes_bytes, written by launch_planes from rows as they are stored.
 bool planes_apply(const Product& p);

@@ -601,13 +601,13 @@ bool planes_apply(const Product& p) {
     return false;
   if (p.dtype != MSL_DTYPE_F32) return true;
   const double cols = p.epilogue == kGate ? 2.0 * p.N : p.N;
-  // microseconds.  Planes: 10 bytes an element of both operands at 5 TB/s, rows in tiles of 256, 95 G multiplications a
-  // millisecond, 3 for every round of tiles, some launches.  CUDA cores: rows in their tiles, 15 G multiplications
+  // microseconds.  Planes: 10 bytes an element of both operands at 5 TB/s, rows in tiles of 256 and k in blocks of 64,
+  // 95 G multiplications a millisecond, 7 for every round of tiles, some launches.  CUDA cores: rows in their tiles, 15 G multiplications
   // a millisecond (7.5 up to 16 rows, where the operands bound them), operands and result once.
   const double elements = 1.0 * p.M * p.K + cols * p.K;
   const double rows = (p.M + 255) / 256 * 256.0, rounds = rows * cols / 65536.0 / 74.0;
   const double tile = p.M <= 8 ? 8 : p.M <= 16 ? 16 : p.M <= 32 ? 32 : (p.M + 63) / 64 * 64.0;
-  const double planes = elements * 10 / 5e6 + rows * cols * p.K / 95e6 + 3 * rounds + 12;
+  const double planes = elements * 10 / 5e6 + rows * cols * ((p.K + 63) / 64 * 64.0) / 95e6 + 7 * rounds + 12;
   const double cores = std::max(tile * cols * p.K / (p.M <= 16 ? 7.5e6 : 15e6), (elements + p.M * cols) * 4 / 4e6) + 6;
   return planes < cores;
 }

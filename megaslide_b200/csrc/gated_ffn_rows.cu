@@ -293,10 +293,12 @@ cudaError_t launch_mma(Args a, cudaStream_t s) {
 
 }  // namespace rows
 
-// 9 to 16 rows of bf16 only while the caches hold the weights (7168 x 28672: 390 us for 16, against 260 on the tensor
-// cores)
+// More rows only while the caches hold the weights: bf16, 7168 x 28672, 390 us for 16, against 260 on the tensor cores;
+// float32, 4 and 8 rows a call, 1152 x 4608: 27 and 40 us, against 48 by few_kernel, 7168 x 28672: 1064 and 1545
+// against 732 and 741.
 long long rows_most(int dtype, long long weights) {
-  return dtype == MSL_DTYPE_F32 ? kMostRowsF32 : weights < (1LL << 25) ? kMostRows : kMostRows / 2;
+  const bool cached = weights < (1LL << 25);
+  return dtype == MSL_DTYPE_F32 ? (cached ? kMostRowsF32 : 2) : cached ? kMostRows : kMostRows / 2;
 }
 
 bool rows_apply(const Product& p) {

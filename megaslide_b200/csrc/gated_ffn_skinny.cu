@@ -1,6 +1,6 @@
 // The gated feed-forward block's float32 products on the CUDA cores, where making planes for the tensor cores
 // (10 bytes an element of each operand, gated_ffn_planes.cu) would cost more than it saves: up to about a hundred
-// rows, and small products.
+// rows, and small products (few rows of wide weights on 16 bytes: gated_ffn_few.cu).
 //
 // A block has 128 columns and 8 to 64 rows of the result and a share of k; the operands come through registers
 // into shared memory ([k][row], [k][column]) while the last tile is multiplied, two columns an instruction
@@ -235,6 +235,46 @@ __global__ void __launch_bounds__(256) skinny_join_kernel(const float* __restric
   }
 }
 
+// The weights' gradients of up to KM rows, out[m][n] = sum_k a[k][m] b[k][n]: bound by the bytes of the result.  A thread
+// has 4 columns, whose b stays in registers, and writes them for kOuterRows rows; a comes through shared memory.
+// 7168 x 25088, both gradients on average (0.72 GB): 1 row 159 us (4.5 TB/s of writes alone), 13 rows 215, 30 rows 528; by skinny_kernel
+// 421, 437, and by planes 586.
+constexpr int kOuterRows = 32;
+
+template <int KM>
+__global__ void __launch_bounds__(256) outer_kernel(const __grid_constant__ Args P) {
+  __shared__ __align__(16) float as[kOuterRows][KM];
+  const long long m0 = static_cast<long long>(blockIdx.x) * kOuterRows, n = (blockIdx.y * 256LL + threadIdx.x) * 4;
+  const int K = static_cast<int>(P.K);
+  for (int e = threadIdx.x; e < kOuterRows * KM; e += 256) {
+    const int k = e / kOuterRows, m = e % kOuterRows;
+    as[m][k] = k < K && m0 + m < P.M ? __ldg(P.a + k * P.lda + m0 + m) : 0.f;
+  }
+  const bool in = n < P.N;
+  float2 b[KM][2];
+#pragma unroll
+  for (int k = 0; k < KM; ++k) {
+    const float4 v = in && k < K ? __ldg(reinterpret_cast<const float4*>(P.b + k * P.ldb + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    b[k][0] = make_float2(v.x, v.y);
+    b[k][1] = make_float2(v.z, v.w);
+  }
+  __syncthreads();
+  if (!in) return;
+  const int rows = static_cast<int>(min(static_cast<long long>(kOuterRows), P.M - m0));
+  float* out = P.out + m0 * P.ldo + n;
+#pragma unroll 4
+  for (int m = 0; m < rows; ++m, out += P.ldo) {
+    float2 s = make_float2(0.f, 0.f), t = s;
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      const float2 v = make_float2(as[m][k], as[m][k]);
+      s = fma2(v, b[k][0], s);
+      t = fma2(v, b[k][1], t);
+    }
+    *reinterpret_cast<float4*>(out) = make_float4(s.x, s.y, t.x, t.y);
+  }
+}
+
 struct Plan {
   int tm, shares;
   long long kper;
@@ -282,6 +322,22 @@ size_t skinny_bytes(long long M, long long N, long long K, int epilogue, bool a_
   return skinny::plan(M, epilogue == kGate ? 2 * N : N, K, a_major).bytes;
 }
 
+cudaError_t launch_skinny_join(const Product& p, int shares, cudaStream_t s) {
+  const unsigned blocks = static_cast<unsigned>((p.M * p.N + 255) / 256);
+  const float* const bias = static_cast<const float*>(p.bias);
+  const float* const kept = static_cast<const float*>(p.kept);
+  float* const kept_out = static_cast<float*>(p.kept_out);
+  float* const out = static_cast<float*>(p.out);
+  if (p.epilogue == kGate)
+    skinny::skinny_join_kernel<kGate><<<blocks, 256, 0, s>>>(p.partial, shares, p.M, p.N, bias, kept, kept_out, out, p.ldo, p.act);
+  else if (p.epilogue == kDgate)
+    skinny::skinny_join_kernel<kDgate><<<blocks, 256, 0, s>>>(p.partial, shares, p.M, p.N, bias, kept, kept_out, out, p.ldo, p.act);
+  else
+    skinny::skinny_join_kernel<kPlain><<<blocks, 256, 0, s>>>(p.partial, shares, p.M, p.N, bias, kept, kept_out, out, p.ldo, p.act);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_product_skinny(const Product& p, cudaStream_t s) {
   const long long cols = p.epilogue == kGate ? 2 * p.N : p.N;
   const bool direct = p.a_major;
@@ -302,6 +358,14 @@ cudaError_t launch_product_skinny(const Product& p, cudaStream_t s) {
   a.va = multiple_of(p.a, 16) && p.lda % 4 == 0;
   a.vb = multiple_of(p.b, 16) && p.ldb % 4 == 0;
   cudaError_t e;
+  if (direct && p.K <= 32 && p.N % 4 == 0 && a.vb && multiple_of(p.out, 16) && p.ldo % 4 == 0) {
+    const dim3 grid(static_cast<unsigned>((p.M + skinny::kOuterRows - 1) / skinny::kOuterRows), static_cast<unsigned>((p.N + 1023) / 1024));
+    if (p.K <= 4) skinny::outer_kernel<4><<<grid, 256, 0, s>>>(a);
+    else if (p.K <= 8) skinny::outer_kernel<8><<<grid, 256, 0, s>>>(a);
+    else if (p.K <= 16) skinny::outer_kernel<16><<<grid, 256, 0, s>>>(a);
+    else skinny::outer_kernel<32><<<grid, 256, 0, s>>>(a);
+    return cudaGetLastError();
+  }
   // rows on the grid's x, the axis that may be long (columns: at most 2^21 / 128)
   switch (cut.tm) {
     case 8: e = skinny::by_order<8>(p, a, cut.shares, s); break;
@@ -309,20 +373,7 @@ cudaError_t launch_product_skinny(const Product& p, cudaStream_t s) {
     case 32: e = skinny::by_order<32>(p, a, cut.shares, s); break;
     default: e = skinny::by_order<64>(p, a, cut.shares, s); break;
   }
-  if (e != cudaSuccess || direct) return e;
-  const unsigned blocks = static_cast<unsigned>((p.M * p.N + 255) / 256);
-  const float* const bias = static_cast<const float*>(p.bias);
-  const float* const kept = static_cast<const float*>(p.kept);
-  float* const kept_out = static_cast<float*>(p.kept_out);
-  float* const out = static_cast<float*>(p.out);
-  if (p.epilogue == kGate)
-    skinny::skinny_join_kernel<kGate><<<blocks, 256, 0, s>>>(p.partial, cut.shares, p.M, p.N, bias, kept, kept_out, out, p.ldo, p.act);
-  else if (p.epilogue == kDgate)
-    skinny::skinny_join_kernel<kDgate><<<blocks, 256, 0, s>>>(p.partial, cut.shares, p.M, p.N, bias, kept, kept_out, out, p.ldo, p.act);
-  else
-    skinny::skinny_join_kernel<kPlain><<<blocks, 256, 0, s>>>(p.partial, cut.shares, p.M, p.N, bias, kept, kept_out, out, p.ldo, p.act);
-  count_launches(1);
-  return cudaGetLastError();
+  return e != cudaSuccess || direct ? e : launch_skinny_join(p, cut.shares, s);
 }
 
 }  // namespace ffn

@@ -419,6 +419,25 @@ def test_gated_ffn_float32_few_rows(M, C, F):
     _ffn_check_all(M, C, F, torch.float32, "silu", True)
 
 
+@pytest.mark.parametrize("M", [1, 3, 12, 30, 50, 64, 65])
+def test_gated_ffn_float32_few_rows_of_wide_weights(M):
+    """Weights of 64 MB: split on the way to the tensor cores, up to 64 rows; columns and k off the blocks' multiples."""
+    _ffn_check_all(M, 4100, 4108, torch.float32, "gelu", True)
+
+
+def test_gated_ffn_float32_wide_weights_off_16_bytes():
+    """The same weights with rows of x that no 16-byte copy reads, and with weights at an odd address, go another way."""
+    M, C, F = 12, 4100, 4108
+    x, w_in, w_out, b_in, b_out = (t.detach() for t in _ffn_case(M, C, F, torch.float32, "silu", True))
+    want = msl.gated_ffn(x, w_in, w_out, b_in, b_out)
+    padded = torch.zeros(M, C + 1, device=_dev())
+    padded[:, :C] = x.reshape(M, C)
+    flat = torch.cat([torch.zeros(1, device=_dev()), w_in.reshape(-1)])
+    tol = 2 * (2 * math.sqrt(F) + 16) * EPS
+    _close(msl.gated_ffn(padded[:, :C], w_in, w_out, b_in, b_out), want.reshape(M, C).double(), tol, "x")
+    _close(msl.gated_ffn(x, flat[1:].view(2 * F, C), w_out, b_in, b_out), want.double(), tol, "w_in")
+
+
 def test_gated_ffn_without_rows():
     x, w_in, w_out, b_in, b_out = _ffn_case(0, 64, 96, torch.bfloat16, "silu", True)
     y = msl.gated_ffn(x, w_in, w_out, b_in, b_out)
