@@ -307,20 +307,18 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.bias = io->b_in;
   p.kept_out = io->kept;
   p.M = M; p.N = F; p.K = C;
-  // both products by rows, or neither: the second is launched into the first
-  const bool rows = ffn::rows_apply(p) && multiple_of(io->h, 16) && multiple_of(io->w_out, 16) &&
-                    F * (geom->dtype == MSL_DTYPE_BF16 ? 2 : 4) % 16 == 0;
-  if (!rows && ffn::few_rows(geom, false)) return failf(MSL_ERR_INVALID, ffn::kOff16);
-  rc = ffn::run(p, slots, 0, 1, s, rows);
-  if (rc) return rc;
-  p = ffn::product(geom, io, W, workspace);
-  p.epilogue = ffn::kPlain;
-  p.a = io->h; p.lda = F;
-  p.b = io->w_out; p.ldb = F;
-  p.out = io->y; p.ldo = io->y_ld;
-  p.bias = io->b_out;
-  p.M = M; p.N = C; p.K = F;
-  return ffn::run(p, slots, 0, 1, s, rows);
+  ffn::Product q = ffn::product(geom, io, W, workspace);
+  q.epilogue = ffn::kPlain;
+  q.a = io->h; q.lda = F;
+  q.b = io->w_out; q.ldb = F;
+  q.out = io->y; q.ldo = io->y_ld;
+  q.bias = io->b_out;
+  q.M = M; q.N = C; q.K = F;
+  // by rows, where each one's operands allow it (the second is launched into what comes before it)
+  const bool few = M <= ffn::rows_most(geom->dtype, 2 * F * C), first = few && ffn::rows_apply(p), second = few && ffn::rows_apply(q);
+  if (!(first && second) && ffn::few_rows(geom, false)) return failf(MSL_ERR_INVALID, ffn::kOff16);
+  rc = ffn::run(p, slots, 0, 1, s, first);
+  return rc ? rc : ffn::run(q, slots, 0, 1, s, second);
 }
 
 int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* workspace, size_t workspace_bytes,

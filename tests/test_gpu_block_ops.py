@@ -402,7 +402,7 @@ def test_gated_ffn_sizes(M, C, F, bias, dtype):
 @pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 7, 8, 9, 13, 16, 17])
 def test_gated_ffn_few_rows(M, dtype):
     """Single tokens up to the first size beyond their form, k that no warp's loads divide, and a long k."""
-    for C, F, bias in ((72, 200, True), (1160, 392, False), (64, 9000, True), (8, 8, False), (1152, 1228, True)):
+    for C, F, bias in ((72, 200, True), (1160, 392, False), (64, 9000, True), (8, 8, False), (1152, 1228, True), (64, 75, True), (77, 64, True)):
         _ffn_check_all(M, C, F, dtype, "gelu", bias)
 
 
