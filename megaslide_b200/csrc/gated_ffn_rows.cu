@@ -1,7 +1,7 @@
 // The gated feed-forward block's forward products for a few rows (single tokens up to kMostRows): the weights are
 // read once, at the speed of the memory, and the rows of x stay in the caches.
 //
-// One row of bf16, or up to 8 of float32: a warp takes two rows of the weights (the gate's and the other
+// One row of bf16, or up to 8 of float32 (rows_most): a warp takes two rows of the weights (the gate's and the other
 // projection's of one hidden element, or two of the second projection) and all rows of x; its lanes split k in
 // 16-byte loads, four of each weight row in flight before the first is used.  More rows of bf16: mma.sync, below.
 // Where there are fewer pairs of rows than warps the GPU holds, several warps share a pair's k.  Sums are float32,
