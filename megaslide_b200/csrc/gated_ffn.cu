@@ -113,11 +113,16 @@ static cudaError_t column_sums_t(ColumnArgs a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// The workspace's slots for planes, and whose planes they hold in this call.
+// The workspace's slots for planes, and the matrix whose planes each holds in this call.  Two operands may begin at one
+// address (w_out or x as the first rows of w_in, say), so a matrix is its shape and row stride as well.
+struct Held {
+  const void* src;
+  long long rows, cols, ld;
+};
 struct Slots {
   char* at[3];
   size_t bytes[3];
-  const void* of[3];
+  Held of[3];
 };
 
 static const char* const kOff16 = "an address or a row stride is no multiple of 16 bytes and the geometry's unaligned is 0";
@@ -142,10 +147,11 @@ static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStrea
     PlaneJob jobs[2];
     int count = 0;
     for (int i = 0; i < 2; ++i) {
-      if (slots.of[slot[i]] == src[i]) continue;
+      Held& held = slots.of[slot[i]];
+      if (held.src == src[i] && held.rows == rows[i] && held.cols == cols[i] && held.ld == ld[i]) continue;
       if (planes_bytes(p.dtype, rows[i], cols[i]) > slots.bytes[slot[i]]) return failf(MSL_ERR_WORKSPACE, "planes beyond their slot");
       jobs[count++] = {src[i], ld[i], rows[i], cols[i], slots.at[slot[i]]};
-      slots.of[slot[i]] = src[i];
+      held = {src[i], rows[i], cols[i], ld[i]};
     }
     if (count) {
       e = launch_planes(p.dtype, jobs, count, s);

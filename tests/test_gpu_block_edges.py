@@ -1,0 +1,46 @@
+"""The operators around the attention on the GPU where operands share memory, tensors come from inference mode, another
+memory order or another default device, and where a trainer's gradients are not finite.  Tolerances as in
+test_gpu_block_ops.py: (2 sqrt(K) + 16) roundings of float32 for a product of K terms in the 2-norm, RMS for every rounding
+to bfloat16."""
+
+import copy
+import math
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import megaslide_b200 as msl
+from megaslide_b200 import ops
+from megaslide_b200.dit import MegaSlideDiT, VideoDiTConfig
+from megaslide_b200.stream import CPUMasterVideoDiT, _HostAdamW
+from test_gpu_block_ops import DTYPES, EPS, HALF, IDS, RMS, _close, _dev, _ffn_case, _ffn_ref, _rand, _within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("shared", ["w_out", "x"])
+@pytest.mark.parametrize("dtype,M,D", [(torch.float32, 1000, 512), (torch.float32, 700, 509), (torch.bfloat16, 700, 253)], ids=["fp32", "fp32-odd", "bf16-odd"])
+def test_gated_ffn_operands_that_begin_at_one_address(dtype, M, D, shared):
+    """w_out or x as the first rows of w_in: the same address, another shape.  The gradient of the shared matrix is the sum
+    of two, each within its own tolerance (4 RMS in bf16), rounded once more."""
+    w = _rand(1, 2 * D, D, dtype=dtype, std=D ** -0.5).requires_grad_()
+    other = _rand(2, D, D, dtype=dtype, std=D ** -0.5).requires_grad_()
+    if shared == "w_out":
+        x, w_out = _rand(3, M, D, dtype=dtype).requires_grad_(), w[:D]
+    else:
+        x, w_out = w[:M], other
+    dy = _rand(4, x.shape[0], D, dtype=dtype)
+    want = list(_ffn_ref(x, w, w_out, None, None, "silu", dy)[:4])
+    y = msl.gated_ffn(x, w, w_out)
+    got = [y.detach(), *torch.autograd.grad(y, [w, x if shared == "w_out" else other], dy)]
+    dw = want[2].clone()
+    if shared == "w_out":
+        dw[:D] += want[3]
+        want = [want[0], dw, want[1]]
+    else:
+        dw[:M] += want[1]
+        want = [want[0], dw, want[3]]
+    K = max(2 * D, M)
+    for name, a, b, roundings in zip(("y", "shared", "alone"), got, want, (2, 5, 4)):
+        _close(a, b, (2 * math.sqrt(K) + 16) * EPS if dtype == torch.float32 else roundings * RMS, name)
