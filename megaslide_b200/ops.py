@@ -96,8 +96,9 @@ class StatusWord:
     BAD = _lib.MSL_STATUS_HALO_MISS | _lib.MSL_STATUS_TIMEOUT
 
     def __init__(self, device: torch.device):
-        self.word = torch.zeros(1, dtype=torch.int32, device=device)
-        self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
+        with torch.inference_mode(False):  # both outlive the call that makes them, which may be in inference mode
+            self.word = torch.zeros(1, dtype=torch.int32, device=device)
+            self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
         self.event: Optional[torch.cuda.Event] = None
         self.seen = 0  # every bit observed so far (TC_RANGE included)
 

@@ -44,3 +44,27 @@ def test_gated_ffn_operands_that_begin_at_one_address(dtype, M, D, shared):
     K = max(2 * D, M)
     for name, a, b, roundings in zip(("y", "shared", "alone"), got, want, (2, 5, 4)):
         _close(a, b, (2 * math.sqrt(K) + 16) * EPS if dtype == torch.float32 else roundings * RMS, name)
+
+
+@pytest.fixture
+def fresh_status():
+    """A process that has made no call yet: no status words."""
+    kept = [(d, dict(d)) for d in (ops._STATUS, ops._FLAGS)]
+    for d, _ in kept:
+        d.clear()
+    yield
+    for d, old in kept:
+        d.clear()
+        d.update(old)
+
+
+def test_attention_trains_after_a_first_call_in_inference_mode(fresh_status):
+    torch.manual_seed(0)
+    m = msl.DeformableSlideAttention3D(64, 4, (3, 3, 3)).cuda()
+    x = _rand(1, 2, 24, 64)
+    with torch.inference_mode():
+        first = m(x, (2, 3, 4)).clone()
+    y = m(x.requires_grad_(), (2, 3, 4))
+    y.sum().backward()
+    assert torch.equal(y.detach(), first) and torch.isfinite(x.grad).all()
+    torch.cuda.synchronize()
