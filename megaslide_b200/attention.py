@@ -341,7 +341,8 @@ class DeformableSlideAttention3D(nn.Module):
         key = (tuple(video_shape), device)
         t = self._tables.get(key)
         if t is None:
-            t = self._tables[key] = rotary_table(video_shape, self.rotary_axes, self.rotary_theta, device=device)
+            with torch.inference_mode(False):  # a first call in inference mode must leave a table that training can save
+                t = self._tables[key] = rotary_table(video_shape, self.rotary_axes, self.rotary_theta, device=device)
         return t
 
     def __getstate__(self):

@@ -1,0 +1,19 @@
+"""The operators around the attention without a GPU: what the module keeps between calls, host-side buffers, and refusals
+that come before any CUDA call."""
+
+import torch
+
+import megaslide_b200 as msl
+
+
+def _module(**kw):
+    return msl.DeformableSlideAttention3D(64, 4, (3, 3, 3), **{**dict(qk_norm=True, rotary_axes=(4, 6, 6)), **kw})
+
+
+def test_table_made_in_inference_mode_serves_training():
+    m, cpu = _module(), torch.device("cpu")
+    with torch.inference_mode():
+        first = m._table((2, 3, 4), cpu)
+    t = m._table((2, 3, 4), cpu)
+    assert t is first and not t.is_inference()
+    assert torch.equal(t, msl.rotary_table((2, 3, 4), (4, 6, 6)))

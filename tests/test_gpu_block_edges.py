@@ -68,3 +68,14 @@ def test_attention_trains_after_a_first_call_in_inference_mode(fresh_status):
     y.sum().backward()
     assert torch.equal(y.detach(), first) and torch.isfinite(x.grad).all()
     torch.cuda.synchronize()
+
+
+def test_module_with_rotary_positions_trains_after_a_first_call_in_inference_mode(fresh_status):
+    torch.manual_seed(0)
+    m = msl.DeformableSlideAttention3D(64, 4, (3, 3, 3), qk_norm=True, rotary_axes=(4, 6, 6)).cuda()
+    x = _rand(1, 2, 24, 64)
+    with torch.inference_mode():
+        first = m(x, (2, 3, 4)).clone()
+    y = m(x.requires_grad_(), (2, 3, 4))
+    y.sum().backward()
+    assert torch.equal(y.detach(), first) and torch.isfinite(x.grad).all()
