@@ -333,12 +333,12 @@ class DeformableSlideAttention3D(nn.Module):
                                  f"got {rotary_axes}")
         self.rotary_axes = rotary_axes
         self.rotary_theta = rotary_theta
-        self._tables: dict = {}  # (video shape, device) -> table of cosines and sines
+        self._tables: dict = {}  # (video shape, axes, theta, device) -> table of cosines and sines
 
     def _table(self, video_shape: Tuple[int, int, int], device) -> Optional[Tensor]:
         if self.rotary_axes is None:
             return None
-        key = (tuple(video_shape), device)
+        key = (tuple(video_shape), tuple(self.rotary_axes), self.rotary_theta, device)
         t = self._tables.get(key)
         if t is None:
             with torch.inference_mode(False):  # a first call in inference mode must leave a table that training can save

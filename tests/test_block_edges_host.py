@@ -17,3 +17,14 @@ def test_table_made_in_inference_mode_serves_training():
     t = m._table((2, 3, 4), cpu)
     assert t is first and not t.is_inference()
     assert torch.equal(t, msl.rotary_table((2, 3, 4), (4, 6, 6)))
+
+
+def test_table_follows_the_module_attributes():
+    m, cpu = _module(), torch.device("cpu")
+    before = m._table((2, 3, 4), cpu)
+    m.rotary_theta = 5.0
+    assert torch.equal(m._table((2, 3, 4), cpu), msl.rotary_table((2, 3, 4), (4, 6, 6), 5.0))
+    m.rotary_axes = (2, 4, 4)
+    assert torch.equal(m._table((2, 3, 4), cpu), msl.rotary_table((2, 3, 4), (2, 4, 4), 5.0))
+    m.rotary_axes, m.rotary_theta = (4, 6, 6), 10000.0
+    assert torch.equal(m._table((2, 3, 4), cpu), before)
