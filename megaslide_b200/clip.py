@@ -37,7 +37,7 @@ def grad_norm(tensors: Tensors, extra_sumsq: float = 0.0) -> Tensor:
     ts = _list(tensors)
     extra = _check(extra_sumsq)
     if not ts:
-        return torch.tensor(math.sqrt(extra))
+        return torch.tensor(math.sqrt(extra), device="cpu")
     return ops.grad_norm(ts, extra_sumsq=extra)
 
 
@@ -52,7 +52,7 @@ def clip_grad_norm_(tensors: Tensors, max_norm: float, *, out: Optional[Sequence
     ts = _list(tensors)
     extra = _check(extra_sumsq)
     if not ts:
-        return torch.tensor(math.sqrt(extra))
+        return torch.tensor(math.sqrt(extra), device="cpu")
     out = ts if out is None else list(out)
     norm = ops.grad_norm(ts, out, float(max_norm), extra)
     increment_version(out)  # the kernel wrote them behind autograd's back

@@ -98,7 +98,7 @@ class StatusWord:
     def __init__(self, device: torch.device):
         with torch.inference_mode(False):  # both outlive the call that makes them, which may be in inference mode
             self.word = torch.zeros(1, dtype=torch.int32, device=device)
-            self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
+            self.host = torch.zeros(1, dtype=torch.int32, device="cpu").pin_memory()
         self.event: Optional[torch.cuda.Event] = None
         self.seen = 0  # every bit observed so far (TC_RANGE included)
 
@@ -152,7 +152,7 @@ class HostFlag:
     The next call that finds a bit set raises MslError (the failed call's results are not valid)."""
 
     def __init__(self):
-        self.word = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.word = torch.zeros(1, dtype=torch.int32, device="cpu").pin_memory()
         self.ptr = self.word.data_ptr()
         self._view = self.word.numpy()
 

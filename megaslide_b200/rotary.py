@@ -37,12 +37,12 @@ def rotary_table(video_shape: Int3, axes: Int3, theta: float = 10000.0, position
         if size < 1 or ch < 0 or ch % 2:
             raise ValueError(f"extents must be >= 1 and axes even, got {tuple(video_shape)} and {tuple(axes)}")
         if positions is None:
-            pos = torch.arange(size, dtype=torch.float64)
+            pos = torch.arange(size, dtype=torch.float64, device="cpu")
         else:
             pos = positions[i].detach().to("cpu", torch.float64)
             if tuple(pos.shape) != (size,):
                 raise ValueError(f"positions[{i}] must be [{size}], got {tuple(pos.shape)}")
-        freq = theta ** (-torch.arange(0, ch, 2, dtype=torch.float64) / max(ch, 1))
+        freq = theta ** (-torch.arange(0, ch, 2, dtype=torch.float64, device="cpu") / max(ch, 1))
         angle = pos[:, None] * freq[None]
         parts.append(torch.stack([angle.cos(), angle.sin()], -1).reshape(-1, 2))
     return torch.cat(parts).float().to(device if device is not None else "cpu").contiguous()

@@ -28,3 +28,13 @@ def test_table_follows_the_module_attributes():
     assert torch.equal(m._table((2, 3, 4), cpu), msl.rotary_table((2, 3, 4), (2, 4, 4), 5.0))
     m.rotary_axes, m.rotary_theta = (4, 6, 6), 10000.0
     assert torch.equal(m._table((2, 3, 4), cpu), before)
+
+
+def test_table_under_another_default_device():
+    """torch.set_default_device does not reach the table's own arithmetic."""
+    half = [torch.tensor([0.0, 0.5]), torch.zeros(1), torch.zeros(1)]
+    want = msl.rotary_table((2, 1, 1), (2, 0, 0), positions=half), msl.rotary_table((2, 3, 4), (4, 6, 6))
+    with torch.device("meta"):
+        got = msl.rotary_table((2, 1, 1), (2, 0, 0), positions=half), msl.rotary_table((2, 3, 4), (4, 6, 6))
+    for a, b in zip(got, want):
+        assert a.device.type == "cpu" and torch.equal(a, b)

@@ -79,3 +79,19 @@ def test_module_with_rotary_positions_trains_after_a_first_call_in_inference_mod
     y = m(x.requires_grad_(), (2, 3, 4))
     y.sum().backward()
     assert torch.equal(y.detach(), first) and torch.isfinite(x.grad).all()
+
+
+def test_calls_under_another_default_device(fresh_status):
+    """torch.set_default_device does not reach into the host-side buffers of the package."""
+    x, w_in, w_out = _rand(1, 3, 16), _rand(2, 16, 16), _rand(3, 16, 8)
+    m = msl.DeformableSlideAttention3D(64, 4, (3, 3, 3)).cuda()
+    v = _rand(4, 2, 24, 64)
+    torch.set_default_device("cuda")
+    try:
+        y = msl.gated_ffn(x, w_in, w_out)
+        z = m(v, (2, 3, 4))
+        assert msl.grad_norm([], extra_sumsq=4.0).device.type == "cpu"
+    finally:
+        torch.set_default_device(None)
+    assert torch.equal(msl.gated_ffn(x, w_in, w_out), y) and torch.equal(m(v, (2, 3, 4)), z)
+    torch.cuda.synchronize()
