@@ -33,7 +33,7 @@ def grad_norm(tensors: Tensors, extra_sumsq: float = 0.0) -> Tensor:
     """2-norm of all elements of the tensors together (float32 or bfloat16, contiguous, on one CUDA device; parameters
     stand for their gradients), as a 0-dim float32 tensor on their device.  extra_sumsq: a sum of squares held
     elsewhere (on the host, on other ranks) that belongs to the norm.  Without tensors the norm of extra_sumsq
-    alone, on the CPU."""
+    alone, on the CPU.  Like torch's, it records no derivative."""
     ts = _list(tensors)
     extra = _check(extra_sumsq)
     if not ts:

@@ -58,7 +58,7 @@ def gated_ffn(x: Tensor, w_in: Tensor, w_out: Tensor, b_in: Optional[Tensor] = N
     if x.dim() < 1:
         raise ValueError("x must be [..., dim]")
     ops.dtype_code(x.dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out)):
+    if ops.takes_derivatives(x, w_in, w_out, b_in, b_out):
         return GatedFFNFunction.apply(x, w_in, w_out, b_in, b_out, activation)
     y = ops.gated_ffn_fwd(_rows_of(x), w_in, w_out, b_in, b_out, activation)[0]
     return y if y.shape == x.shape else y.view(x.shape)

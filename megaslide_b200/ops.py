@@ -15,6 +15,7 @@ from operator import attrgetter
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -28,6 +29,12 @@ def dtype_code(dt: torch.dtype) -> int:
         return _DTYPES[dt]
     except KeyError:
         raise TypeError(f"megaslide_b200 supports float32 and bfloat16 activations, got {dt}") from None
+
+
+def takes_derivatives(*ts) -> bool:
+    """Whether a call goes through its autograd function: an operand requires a gradient, or a level of forward mode is
+    open (a tangent asks for no gradient; the function refuses it, where the kernel alone would lose it)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)) or forward_ad._current_level >= 0
 
 
 def once_only(backward):

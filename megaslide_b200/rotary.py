@@ -107,7 +107,7 @@ def rope3d(x: Tensor, table: Tensor, *, video_shape: Int3, axes: Int3, heads: in
     Differentiable in x."""
     d = _check_tokens("x", x, heads)
     call = _Call(ops.RotaryShape(x.shape[0], x.shape[1], tuple(video_shape), tuple(axes), d, frame0, interleaved), heads)
-    if x.requires_grad and torch.is_grad_enabled():
+    if ops.takes_derivatives(x):
         return Rope3DFunction.apply(call, x, table, index)
     return _rotate(call, x, table, index, False)
 
@@ -156,6 +156,6 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Opt
         video_shape, axes, index, frame0 = (1, 1, 1), (0, 0, 0), None, 0
     call = _Call(ops.RotaryShape(q.shape[0], q.shape[1], tuple(video_shape), tuple(axes), d, frame0, interleaved), heads, kv_heads,
                  float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if ops.takes_derivatives(q, k, q_weight, k_weight):
         return QKNormRopeFunction.apply(call, q, k, q_weight, k_weight, table, index)
     return _norm_rotate(call, q, k, q_weight, k_weight, table, index)

@@ -95,3 +95,24 @@ def test_calls_under_another_default_device(fresh_status):
         torch.set_default_device(None)
     assert torch.equal(msl.gated_ffn(x, w_in, w_out), y) and torch.equal(m(v, (2, 3, 4)), z)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("op", ["rope3d", "qk_norm_rope", "gated_ffn"])
+def test_forward_mode_derivatives_are_refused(op):
+    """No operator has a forward-mode derivative: a tangent is an error, not a result without one.  Without a tangent the
+    calls inside a level are the same as outside."""
+    x, t = _rand(1, 1, 6, 16), _rand(2, 1, 6, 16)
+    table = msl.rotary_table((1, 2, 3), (2, 2, 4), device=_dev())
+    w_in, w_out = _rand(3, 16, 16), _rand(4, 16, 8)
+    call = {"rope3d": lambda v: msl.rope3d(v, table, video_shape=(1, 2, 3), axes=(2, 2, 4), heads=2),
+            "qk_norm_rope": lambda v: msl.qk_norm_rope(v, x, None, None, heads=2)[0],
+            "gated_ffn": lambda v: msl.gated_ffn(v, w_in, w_out)}[op]
+    want = call(x)
+    with forward_ad.dual_level():
+        assert torch.equal(call(x), want)
+        dual = forward_ad.make_dual(x, t)
+        with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
+            call(dual)
+        with torch.no_grad():
+            with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
+                call(dual)
