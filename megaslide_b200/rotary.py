@@ -69,6 +69,11 @@ def _check_tokens(name: str, x: Tensor, heads: int) -> int:
     return x.shape[2] // heads
 
 
+def _check_table(table: Optional[Tensor]) -> None:
+    if table is not None and table.requires_grad and torch.is_grad_enabled():
+        raise ValueError("table requires a gradient, which the rotation does not compute: detach it")
+
+
 class _Call:
     """What a call's backward needs besides its tensors."""
 
@@ -105,6 +110,7 @@ def rope3d(x: Tensor, table: Tensor, *, video_shape: Int3, axes: Int3, heads: in
     The first at/2 pairs of a head turn with the time, the next ah/2 with the row, the last aw/2 with the column;
     channels beyond at + ah + aw pass.  Pair p is channels (2p, 2p+1) (interleaved) or (p, p + (at+ah+aw)/2).
     Differentiable in x."""
+    _check_table(table)
     d = _check_tokens("x", x, heads)
     call = _Call(ops.RotaryShape(x.shape[0], x.shape[1], tuple(video_shape), tuple(axes), d, frame0, interleaved), heads)
     if ops.takes_derivatives(x):
@@ -144,6 +150,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Opt
     """RMS norm of every head of q [B, N, heads * head_dim] and k [B, N, kv_heads * head_dim] (kv_heads: heads by
     default, fewer for grouped heads), times the weights [head_dim] that the heads share (None = ones), then the
     rotation of rope3d (none without a table), in one pass.  Differentiable in q, k and the weights."""
+    _check_table(table)
     kv_heads = heads if kv_heads is None else kv_heads
     d = _check_tokens("q", q, heads)
     if _check_tokens("k", k, kv_heads) != d or k.shape[:2] != q.shape[:2]:

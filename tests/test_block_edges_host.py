@@ -1,6 +1,7 @@
 """The operators around the attention without a GPU: what the module keeps between calls, host-side buffers, and refusals
 that come before any CUDA call."""
 
+import pytest
 import torch
 
 import megaslide_b200 as msl
@@ -38,3 +39,17 @@ def test_table_under_another_default_device():
         got = msl.rotary_table((2, 1, 1), (2, 0, 0), positions=half), msl.rotary_table((2, 3, 4), (4, 6, 6))
     for a, b in zip(got, want):
         assert a.device.type == "cpu" and torch.equal(a, b)
+
+
+def test_table_that_requires_a_gradient_is_refused():
+    """The operators give no gradient of the table: a learned one must not be left without, silently."""
+    x = torch.zeros(1, 24, 64)
+    kw = dict(video_shape=(2, 3, 4), axes=(4, 6, 6), heads=4)
+    table = msl.rotary_table((2, 3, 4), (4, 6, 6)).requires_grad_()
+    for call in (lambda t: msl.rope3d(x, t, **kw), lambda t: msl.qk_norm_rope(x, x, None, None, t, **kw)):
+        with pytest.raises(ValueError, match="gradient"):
+            call(table)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            call(table)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(table.detach())
