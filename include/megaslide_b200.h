@@ -363,7 +363,8 @@ size_t msl_grad_norm_workspace_bytes(const int64_t* numel, int32_t count);
  * and joined in double, in a fixed order. */
 int msl_grad_norm(const void* const* src, const int64_t* numel, const int32_t* dtype, int32_t count,
                   double extra_sumsq, float* norm, void* workspace, size_t workspace_bytes, void* stream);
-/* msl_grad_norm, then dst = src * min(1, max_norm / (norm + 1e-6)) (dst of src's type; may be src). */
+/* msl_grad_norm, then dst = src * min(1, max_norm / (norm + 1e-6)) (dst of src's type; may be src).  A dst that overlaps
+ * another dst, or a src other than its own from the same address on, is refused (MSL_ERR_INVALID). */
 int msl_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int32_t count,
                   double extra_sumsq, float max_norm, float* norm, void* workspace, size_t workspace_bytes,
                   void* stream);

@@ -45,7 +45,8 @@ def clip_grad_norm_(tensors: Tensors, max_norm: float, *, out: Optional[Sequence
                     extra_sumsq: float = 0.0) -> Tensor:
     """Scales the tensors (parameters: their gradients) by min(1, max_norm / (norm + 1e-6)) and returns the norm
     before that, as grad_norm does; nothing waits for the GPU.  out: tensors of the same dtypes and sizes that
-    receive the result in place of the tensors themselves (slices of one flat buffer, say).  A norm that is not finite
+    receive the result in place of the tensors themselves (slices of one flat buffer, say).  Results share memory with
+    nothing but their own tensor, in place: a tensor twice in the list is refused (MslError).  A norm that is not finite
     reaches the results as the formula says (an infinite norm: zeros, and NaN for its infinite elements)."""
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")

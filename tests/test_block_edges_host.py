@@ -1,10 +1,13 @@
 """The operators around the attention without a GPU: what the module keeps between calls, host-side buffers, and refusals
 that come before any CUDA call."""
 
+import ctypes
+
 import pytest
 import torch
 
 import megaslide_b200 as msl
+from megaslide_b200 import _lib
 
 
 def _module(**kw):
@@ -53,3 +56,26 @@ def test_table_that_requires_a_gradient_is_refused():
             call(table)
         with pytest.raises(RuntimeError, match="CUDA"):
             call(table.detach())
+
+
+@pytest.mark.parametrize("src,dst,numel,bf16,text", [
+    ([4096, 4096], [4096, 4096], [10, 10], 0, "result of tensor"),  # the same tensor twice, in place
+    ([4096, 8192], [4096, 4100], [10, 10], 0, "result of tensor"),
+    ([4096, 8192], [4132, 8192], [10, 10], 0, "source of tensor 0"),  # its own source, shifted
+    ([4096, 4136], [4136, 4096], [10, 10], 0, "source of tensor"),  # exchanged
+    ([4096, 4116], [4096, 8192], [10, 10], 1, None),  # neighbours in bf16, one in place
+    ([4096, 4136], [4096, 4136], [10, 10], 0, None),
+    ([4096, 4096, 4100], [8192, 9000, 16384], [10, 0, 10], 0, None),  # sources may share, a tensor without elements is nowhere
+    ([4096, 4136], [4056, 4176], [10, 10], 0, None),  # a result on either side of the sources
+], ids=str)
+def test_clip_entry_refuses_overlapping_results(src, dst, numel, bf16, text):
+    """Checked before any launch: too small a workspace stops the calls that pass."""
+    n = len(src)
+    vp, i64, i32 = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int32 * n
+    lib = _lib.load()
+    rc = lib.msl_grad_clip(vp(*src), vp(*dst), i64(*numel), i32(*[bf16] * n), n, 0.0, 1.0, 16, 16, 0, None)
+    if text is None:
+        assert rc == _lib.MSL_ERR_WORKSPACE
+    else:
+        assert rc == _lib.MSL_ERR_INVALID and text in lib.msl_last_error().decode()
+    assert lib.msl_grad_norm(vp(*src), i64(*numel), i32(*[bf16] * n), n, 0.0, 16, 16, 0, None) == _lib.MSL_ERR_WORKSPACE

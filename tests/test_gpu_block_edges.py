@@ -116,3 +116,25 @@ def test_forward_mode_derivatives_are_refused(op):
         with torch.no_grad():
             with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
                 call(dual)
+
+
+def test_clip_refuses_results_that_overlap():
+    """Blocks write the results in no order: memory that belongs to two of them would be scaled once or twice by chance."""
+    t = _rand(1, 400)
+    want = t.clone()
+    for ts, out in (([t, t], None), ([t[:300], t[100:]], None), ([t[:200]], [t[50:250]]), ([t[:200], t[200:]], [t[200:], t[:200]])):
+        with pytest.raises(msl.MslError, match="overlap"):
+            msl.clip_grad_norm_(ts, 0.1, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(t, want)
+    norm = float(msl.grad_norm([t, t]))  # reading twice is no conflict
+    assert abs(norm - math.sqrt(2) * float(t.double().norm())) <= 1e-6 * norm
+    a, b = torch.empty(400, device=_dev()), torch.empty(400, device=_dev())
+    msl.clip_grad_norm_([t, t], 0.1, out=[a, b])
+    assert torch.equal(a, b)
+    msl.clip_grad_norm_([t[:200], t[200:]], 0.1, out=[t[:200], t[200:]])  # in place, piece by piece
+    # neighbours in one buffer, and sources that lie before the results
+    flat = torch.zeros(801, device=_dev())
+    flat[:400] = want
+    msl.clip_grad_norm_([flat[:100], flat[100:400]], 0.1, out=[flat[401:501], flat[501:801]])
+    assert torch.equal(flat[:400], want)
