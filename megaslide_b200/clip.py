@@ -30,8 +30,8 @@ def _check(extra_sumsq: float) -> float:
 
 
 def grad_norm(tensors: Tensors, extra_sumsq: float = 0.0) -> Tensor:
-    """2-norm of all elements of the tensors together (float32 or bfloat16, contiguous, on one CUDA device; parameters
-    stand for their gradients), as a 0-dim float32 tensor on their device.  extra_sumsq: a sum of squares held
+    """2-norm of all elements of the tensors together (float32 or bfloat16, dense in any order of the axes, on one CUDA
+    device; parameters stand for their gradients), as a 0-dim float32 tensor on their device.  extra_sumsq: a sum of squares held
     elsewhere (on the host, on other ranks) that belongs to the norm.  Without tensors the norm of extra_sumsq
     alone, on the CPU.  Like torch's, it records no derivative."""
     ts = _list(tensors)
@@ -44,8 +44,8 @@ def grad_norm(tensors: Tensors, extra_sumsq: float = 0.0) -> Tensor:
 def clip_grad_norm_(tensors: Tensors, max_norm: float, *, out: Optional[Sequence[Tensor]] = None,
                     extra_sumsq: float = 0.0) -> Tensor:
     """Scales the tensors (parameters: their gradients) by min(1, max_norm / (norm + 1e-6)) and returns the norm
-    before that, as grad_norm does; nothing waits for the GPU.  out: tensors of the same dtypes and sizes that
-    receive the result in place of the tensors themselves (slices of one flat buffer, say).  Results share memory with
+    before that, as grad_norm does; nothing waits for the GPU.  out: tensors of the same dtypes, sizes and
+    order that receive the result in place of the tensors themselves (slices of one flat buffer, say).  Results share memory with
     nothing but their own tensor, in place: a tensor twice in the list is refused (MslError).  A norm that is not finite
     reaches the results as the formula says (an infinite norm: zeros, and NaN for its infinite elements)."""
     if not max_norm >= 0:

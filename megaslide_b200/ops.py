@@ -798,30 +798,50 @@ _dtype_of, _device_of = attrgetter("dtype"), attrgetter("device")
 _numel_of, _ptr_of, _is_whole = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 
 
-def _one_device(ts: List[torch.Tensor], dev: torch.device, name: str) -> None:
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill their memory without gaps and none twice, in whatever order of the axes."""
+    n = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _one_device(ts: List[torch.Tensor], dev: torch.device, name: str) -> bool:
+    """Checks device and density of the tensors of a list; whether all lie in the order of their axes."""
     if set(map(_device_of, ts)) != {dev} or dev.type != "cuda":
         raise RuntimeError(f"every {name} must be on the same CUDA device (no CPU fallback)")
-    if not all(map(_is_whole, ts)):
-        raise ValueError(f"{name} {list(map(_is_whole, ts)).index(False)} must be contiguous")
+    whole = all(map(_is_whole, ts))
+    if not whole:
+        for i, t in enumerate(ts):
+            if not (_is_whole(t) or _dense(t)):
+                raise ValueError(f"{name} {i} must be dense, got shape {tuple(t.shape)} strides {t.stride()}")
+    return whole
 
 
 def grad_norm(src: List[torch.Tensor], dst: Optional[List[torch.Tensor]] = None, max_norm: float = 0.0,
               extra_sumsq: float = 0.0) -> torch.Tensor:
-    """sqrt(extra_sumsq + the sum of squares of every element of the contiguous CUDA tensors `src`), a 0-dim
-    float32 tensor; with ``dst`` also dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)) (dst[i] may be src[i])."""
+    """sqrt(extra_sumsq + the sum of squares of every element of the CUDA tensors `src`, each dense in any order of its
+    axes), a 0-dim float32 tensor; with ``dst`` also dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)) (dst[i] in src[i]'s
+    order; it may be src[i])."""
     if not src:
         raise ValueError("no tensors")
     n = len(src)
     dev = src[0].device
-    _one_device(src, dev, "tensor")
+    whole = _one_device(src, dev, "tensor")
     dtypes = list(map(_dtype_of, src))
     sizes = list(map(_numel_of, src))
     if dst is not None and dst is not src:
         if len(dst) != n:
             raise ValueError(f"{n} tensors, but {len(dst)} to write")
-        _one_device(dst, dev, "out")
+        whole = _one_device(dst, dev, "out") and whole
         if list(map(_dtype_of, dst)) != dtypes or list(map(_numel_of, dst)) != sizes:
             raise ValueError("every out must have its tensor's dtype and size")
+        if not whole:
+            for i, (a, b) in enumerate(zip(src, dst)):
+                if not (_is_whole(a) and _is_whole(b)) and (a.shape != b.shape or a.stride() != b.stride()):
+                    raise ValueError(f"out {i} must lie in its tensor's order: strides {a.stride()}, got {b.stride()}")
     codes = {d: dtype_code(d) for d in set(dtypes)}
     numel = (ctypes.c_int64 * n)(*sizes)
     codes_arr = (ctypes.c_int32 * n)(*[codes[d] for d in dtypes])

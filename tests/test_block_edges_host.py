@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import megaslide_b200 as msl
-from megaslide_b200 import _lib
+from megaslide_b200 import _lib, ops
 
 
 def _module(**kw):
@@ -79,3 +79,11 @@ def test_clip_entry_refuses_overlapping_results(src, dst, numel, bf16, text):
     else:
         assert rc == _lib.MSL_ERR_INVALID and text in lib.msl_last_error().decode()
     assert lib.msl_grad_norm(vp(*src), i64(*numel), i32(*[bf16] * n), n, 0.0, 16, 16, 0, None) == _lib.MSL_ERR_WORKSPACE
+
+
+def test_dense_in_any_order():
+    t = torch.zeros(2, 3, 4, 5)
+    for d in (t, t.permute(2, 0, 3, 1), t.transpose(0, 3), t[:1], t[:, :, :1, :1].contiguous().transpose(1, 2), torch.zeros(()), torch.zeros(3, 0).t()):
+        assert ops._dense(d)
+    for d in (t[:, 1:], t[..., ::2], t[:1, :, :, :1], torch.zeros(1, 5).expand(3, 5), torch.zeros(20).as_strided((4, 5), (3, 1))):
+        assert not ops._dense(d)

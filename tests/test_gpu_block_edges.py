@@ -138,3 +138,42 @@ def test_clip_refuses_results_that_overlap():
     flat[:400] = want
     msl.clip_grad_norm_([flat[:100], flat[100:400]], 0.1, out=[flat[401:501], flat[501:801]])
     assert torch.equal(flat[:400], want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_clip_tensors_in_another_memory_order(dtype):
+    """Gradients that are dense in an order other than their rows' (a channels-last convolution, a transposed matrix): norm and
+    scaling see every element once, whatever the order."""
+    conv = _rand(1, 8, 4, 1, 2, 2, dtype=dtype).to(memory_format=torch.channels_last_3d)
+    turned = _rand(2, 30, 50, dtype=dtype).t()
+    plain = _rand(3, 70, dtype=dtype)
+    ts = [conv, turned, plain]
+    assert not conv.is_contiguous() and not turned.is_contiguous()
+    want = math.sqrt(math.fsum(float(t.double().square().sum()) for t in ts))
+    assert abs(float(msl.grad_norm(ts)) - want) <= 1e-6 * want
+    before = [t.double().clone() for t in ts]
+    limit = want / 4
+    outs = [torch.empty_like(t) for t in ts]
+    msl.clip_grad_norm_(ts, limit, out=outs)
+    norm = msl.clip_grad_norm_(ts, limit)
+    assert abs(float(norm) - want) <= 1e-6 * want
+    for t, o, b in zip(ts, outs, before):
+        ref = b * (limit / (want + 1e-6))
+        assert torch.equal(t, o) and torch.all((t.double() - ref).abs() <= (HALF * (dtype == torch.bfloat16) + 2e-6) * ref.abs())
+    p = torch.nn.Parameter(torch.zeros(8, 4, 1, 2, 2, device=_dev(), dtype=dtype))
+    p.grad = conv
+    assert torch.allclose(msl.clip_grad_norm_([p], 1e9), conv.double().norm().float(), rtol=1e-6)
+
+
+def test_clip_refuses_what_has_no_order():
+    base = _rand(1, 6, 10)
+    with pytest.raises(ValueError, match="dense"):
+        msl.grad_norm([base[:, :5]])  # gaps
+    with pytest.raises(ValueError, match="dense"):
+        msl.grad_norm([base[:1].expand(6, 10)])  # one row six times
+    with pytest.raises(ValueError, match="dense"):
+        msl.clip_grad_norm_([base], 1.0, out=[torch.zeros(6, 20, device=_dev())[:, ::2]])
+    with pytest.raises(ValueError, match="order"):
+        msl.clip_grad_norm_([base], 1.0, out=[torch.zeros(10, 6, device=_dev()).t()])
+    with pytest.raises(ValueError, match="order"):
+        msl.clip_grad_norm_([base.t()], 1.0, out=[torch.zeros(60, device=_dev())])
