@@ -553,17 +553,30 @@ def _ld(t: torch.Tensor, name: str) -> int:
     return _rows(t, name)
 
 
+def _operand(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype, dev: torch.device) -> None:
+    """Refuses an operand that is not `rows` rows of at least `width` elements of the call's type, on its device: the
+    kernels go by the call's geometry and would read or write beyond it."""
+    c = t.shape[-1] if t.dim() else 0
+    if c < width or t.numel() != rows * c:
+        raise ValueError(f"{name} must be {rows} rows of {width} elements, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must have the call's dtype {dtype}, got {t.dtype}")
+    if t.device != dev:
+        raise RuntimeError(f"{name} must be on the call's CUDA device {dev}, got {t.device}")
+
+
 class RotaryShape:
     """Geometry of a rotary call (``msl_rotary_geometry``): `tokens` of each of `batch` samples, the table's extents
     (frames, height, width), the channels each axis turns, the heads' width."""
 
-    __slots__ = ("batch", "tokens", "video_shape", "axes", "head_dim", "table_pairs", "_geom")
+    __slots__ = ("batch", "tokens", "rows", "video_shape", "axes", "head_dim", "table_pairs", "_geom")
 
     def __init__(self, batch: int, tokens: int, video_shape: Tuple[int, int, int], axes: Tuple[int, int, int], head_dim: int,
                  frame0: int = 0, interleaved: bool = True):
         t, h, w = video_shape
         at, ah, aw = axes
         self.batch, self.tokens, self.video_shape, self.axes, self.head_dim = batch, tokens, video_shape, axes, head_dim
+        self.rows = batch * tokens
         self.table_pairs = (t * at + h * ah + w * aw) // 2
         self._geom = _lib.RotaryGeometry(batch * tokens, tokens or 1, t, h, w, frame0, at, ah, aw, head_dim, 1 if interleaved else 0, 0)
 
@@ -597,6 +610,8 @@ def _flag(dev: torch.device, status: Optional[torch.Tensor]) -> int:
     """Address a kernel reports to: the caller's device word, or the device's HostFlag (which raises here if an
     earlier call has reported)."""
     if status is not None:
+        if status.dtype != torch.int32 or status.numel() < 1 or status.device != dev:
+            raise ValueError(f"status must be an int32 word on {dev}, got {status.numel()} of {status.dtype} on {status.device}")
         return status.data_ptr()
     f = _FLAGS.get(dev.index) or host_flag(dev)
     f.poll()
@@ -611,8 +626,11 @@ def rope3d(shape: RotaryShape, heads: int, x: torch.Tensor, table: torch.Tensor,
     _need_cuda(x, table, index)
     dev = x.device
     index_rows = _check_positions(shape, table, index, dev)
+    _operand(x, "x", shape.rows, heads * shape.head_dim, x.dtype, dev)
     if out is None:
         out = torch.empty(*x.shape[:-1], heads * shape.head_dim, device=dev, dtype=x.dtype)
+    else:
+        _operand(out, "out", shape.rows, heads * shape.head_dim, x.dtype, dev)
     g = shape.geometry(x.dtype)
     flag = _flag(dev, status) if index is not None else None
     with _on(dev):
@@ -628,6 +646,9 @@ def _qk_io(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weight, k_weig
     dev = q.device
     if k is not None and k.dtype != q.dtype:
         raise TypeError(f"q and k must have the same dtype, got {q.dtype} and {k.dtype}")
+    _operand(q, "q", shape.rows, heads * shape.head_dim, q.dtype, dev)
+    if kv_heads:
+        _operand(k, "k", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
     wdt = torch.float32
     for w, nm in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is None:
@@ -657,10 +678,14 @@ def qk_norm_rope_fwd(shape: RotaryShape, heads: int, kv_heads: int, q: torch.Ten
     dev = q.device
     if q_out is None:
         q_out = torch.empty(*q.shape[:-1], heads * shape.head_dim, device=dev, dtype=q.dtype)
+    else:
+        _operand(q_out, "q_out", shape.rows, heads * shape.head_dim, q.dtype, dev)
     io.q_out, io.q_out_ld = q_out.data_ptr(), _ld(q_out, "q_out")
     if kv_heads:
         if k_out is None:
             k_out = torch.empty(*k.shape[:-1], kv_heads * shape.head_dim, device=dev, dtype=k.dtype)
+        else:
+            _operand(k_out, "k_out", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
         io.k_out, io.k_out_ld = k_out.data_ptr(), _ld(k_out, "k_out")
     g = shape.geometry(q.dtype)
     with _on(dev):
@@ -677,12 +702,18 @@ def qk_norm_rope_bwd(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weig
     io = _qk_io(shape, heads, kv_heads, q, k, q_weight, k_weight, eps, table, index, status)
     _need_cuda(dq_out, dk_out)
     dev = q.device
+    _operand(dq_out, "dq_out", shape.rows, heads * shape.head_dim, q.dtype, dev)
     if dq is None:
         dq = torch.empty(*q.shape[:-1], heads * shape.head_dim, device=dev, dtype=q.dtype)
+    else:
+        _operand(dq, "dq", shape.rows, heads * shape.head_dim, q.dtype, dev)
     io.dq_out, io.dq_out_ld, io.dq, io.dq_ld = dq_out.data_ptr(), _ld(dq_out, "dq_out"), dq.data_ptr(), _ld(dq, "dq")
     if kv_heads:
+        _operand(dk_out, "dk_out", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
         if dk is None:
             dk = torch.empty(*k.shape[:-1], kv_heads * shape.head_dim, device=dev, dtype=k.dtype)
+        else:
+            _operand(dk, "dk", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
         io.dk_out, io.dk_out_ld, io.dk, io.dk_ld = dk_out.data_ptr(), _ld(dk_out, "dk_out"), dk.data_ptr(), _ld(dk, "dk")
     dgq = torch.empty_like(q_weight) if weight_grads and q_weight is not None else None
     dgk = torch.empty_like(k_weight) if weight_grads and k_weight is not None and kv_heads else None
@@ -772,6 +803,12 @@ def gated_ffn_bwd(x, w_in, w_out, h, kept, dy, b_in=None, b_out=None, activation
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
     _need_cuda(h, kept, dy)
     dev, dt = x.device, x.dtype
+    for t, nm, width in ((h, "h", F), (kept, "kept", 2 * F), (dy, "dy", C)):
+        _operand(t, nm, M, width, dt, dev)
+        if nm != "dy" and (t.shape[-1] != width or not t.is_contiguous()):
+            raise ValueError(f"{nm} must be contiguous rows of {width} elements, got shape {tuple(t.shape)} strides {t.stride()}")
+    if dy.shape[-1] != C:
+        raise ValueError(f"dy must have rows of {C} elements, got {tuple(dy.shape)}")
     needs = (needs[0], needs[1], needs[2], needs[3] and b_in is not None, needs[4] and b_out is not None)
     dx = torch.empty(x.shape, device=dev, dtype=dt) if needs[0] else None
     dw_in = torch.empty_like(w_in) if needs[1] else None

@@ -2,6 +2,7 @@
 that come before any CUDA call."""
 
 import ctypes
+from contextlib import nullcontext
 
 import pytest
 import torch
@@ -87,3 +88,76 @@ def test_dense_in_any_order():
         assert ops._dense(d)
     for d in (t[:, 1:], t[..., ::2], t[:1, :, :, :1], torch.zeros(1, 5).expand(3, 5), torch.zeros(20).as_strided((4, 5), (3, 1))):
         assert not ops._dense(d)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The functions of ops on CPU tensors, up to the point of the launch: what they would have launched."""
+    seen = []
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "_on", lambda dev: nullcontext())
+    monkeypatch.setattr(ops, "_call", lambda name, dev, fn: seen.append(name) or 0)
+    monkeypatch.setattr(ops, "_flag", lambda dev, status: None)
+    return seen
+
+
+def test_rotary_functions_refuse_operands_beyond_the_geometry(launches):
+    sh, table = ops.RotaryShape(2, 24, (2, 3, 4), (4, 6, 6), 16), msl.rotary_table((2, 3, 4), (4, 6, 6))
+    x, few, narrow, half = torch.zeros(48, 64), torch.zeros(47, 64), torch.zeros(48, 63), torch.zeros(48, 64, dtype=torch.bfloat16)
+    wide = torch.zeros(48, 200)[:, :64]
+    w = torch.ones(16)
+
+    def forward(q=x, k=x, **kw):
+        return ops.qk_norm_rope_fwd(sh, 4, 4, q, k, w, w, 1e-6, table, **kw)
+
+    def backward(q=x, k=x, dq_out=x, dk_out=x, **kw):
+        return ops.qk_norm_rope_bwd(sh, 4, 4, q, k, w, w, dq_out, dk_out, 1e-6, table, **kw)
+
+    for good in (lambda: ops.rope3d(sh, 4, x, table), lambda: ops.rope3d(sh, 4, wide, table, out=wide), lambda: ops.rope3d(sh, 3, x, table),
+                 forward, lambda: forward(wide, wide, q_out=wide, k_out=x), backward, lambda: backward(dq=wide, dk=wide),
+                 lambda: forward(x.view(2, 24, 64), x.view(2, 24, 64))):
+        good()
+    assert len(launches) == 8
+    for bad, error in ((few, ValueError), (narrow, ValueError), (half, TypeError)):
+        calls = [lambda: ops.rope3d(sh, 4, x, table, out=bad)]
+        calls += [lambda nm=nm: forward(**{nm: bad}) for nm in ("k", "q_out", "k_out")]
+        calls += [lambda nm=nm: backward(**{nm: bad}) for nm in ("k", "dq_out", "dk_out", "dq", "dk")]
+        if bad is not half:
+            calls += [lambda: ops.rope3d(sh, 4, bad, table), lambda: forward(q=bad, k=bad)]
+        for call in calls:
+            with pytest.raises(error):
+                call()
+    with pytest.raises(ValueError):
+        ops.rope3d(sh, 5, x, table)
+    assert len(launches) == 8
+
+
+def test_gated_backward_refuses_operands_beyond_the_geometry(launches):
+    M, C, F = 6, 16, 24
+    x, w_in, w_out, dy = torch.zeros(M, C), torch.zeros(2 * F, C), torch.zeros(C, F), torch.zeros(M, C)
+    h, kept = torch.zeros(M, F), torch.zeros(M, 2 * F)
+
+    def call(**kw):
+        a = {**dict(h=h, kept=kept, dy=dy), **kw}
+        return ops.gated_ffn_bwd(x, w_in, w_out, a["h"], a["kept"], a["dy"])
+
+    call()
+    call(dy=torch.zeros(M, 40)[:, :C])
+    assert len(launches) == 2
+    for nm, t in (("h", h), ("kept", kept), ("dy", dy)):
+        for bad in (t[:-1], t[:, :-1].contiguous(), torch.zeros(M, t.shape[1] + 1)):
+            with pytest.raises(ValueError, match=nm):
+                call(**{nm: bad})
+        with pytest.raises(TypeError, match=nm):
+            call(**{nm: t.bfloat16()})
+    with pytest.raises(ValueError, match="h must"):
+        call(h=torch.zeros(M, F + 8)[:, :F])
+    assert len(launches) == 2
+
+
+def test_status_word_of_a_caller_is_checked():
+    dev = torch.device("cpu")
+    assert ops._flag(dev, torch.zeros(1, dtype=torch.int32)) != 0
+    for bad in (torch.zeros(1), torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int32, device="meta")):
+        with pytest.raises(ValueError, match="status"):
+            ops._flag(dev, bad)
