@@ -177,3 +177,52 @@ def test_clip_refuses_what_has_no_order():
         msl.clip_grad_norm_([base], 1.0, out=[torch.zeros(10, 6, device=_dev()).t()])
     with pytest.raises(ValueError, match="order"):
         msl.clip_grad_norm_([base.t()], 1.0, out=[torch.zeros(60, device=_dev())])
+
+
+def _trainer(fused, max_norm=0.05):
+    """A small trainer with gradients put into its buffers: the same for every call."""
+    torch.manual_seed(5)
+    cfg = VideoDiTConfig(frames=2, in_channels=4, height=8, width=8, patch_size=2, hidden_size=64, num_heads=2, num_layers=3,
+                         dsa_kernel_size=(3, 3, 3), checkpoint_interval=2, num_grad_slabs=3, learning_rate=1e-3, weight_decay=0.01,
+                         max_grad_norm=max_norm, dtype="float32", device=0, log_interval=0, gated_mlp=True, fused_clip=fused)
+    tr = CPUMasterVideoDiT(MegaSlideDiT(cfg), cfg)
+    for i in range(tr.num_blocks):
+        tr.hgrad[i].normal_(std=1e-2)
+        tr.has_grad[i] = True
+    for p in tr.res_params:
+        p.grad = torch.randn(p.shape).mul_(1e-2).to(p.device)
+    return tr
+
+
+def _step(tr, monkeypatch):
+    """(norm, scale handed to the host's updates, resident gradients, parameters) of one optimizer step."""
+    scales = []
+    update = _HostAdamW.update
+
+    def spy(self, p, g, scale, stage=None):
+        scales.append(scale)
+        return update(self, p, g, scale, stage=stage)
+
+    monkeypatch.setattr(_HostAdamW, "update", spy)
+    for i in range(tr.num_blocks):
+        tr.sumsq[i] = float(tr.hgrad[i].double().square().sum())
+    norm = tr.optimizer_step()
+    params = [p.detach().cpu().clone() for p in tr.get_parameters()]
+    assert len(scales) == tr.num_blocks
+    return norm, scales, [p.grad.cpu() for p in tr.res_params], params
+
+
+def test_fused_clip_scales_host_and_resident_gradients_alike(monkeypatch):
+    """The norm lies far above its limit: every gradient, on the host and on the GPU, is scaled by the same factor, once."""
+    tr = _trainer(True)
+    try:
+        before = [p.grad.double().cpu() for p in tr.res_params]
+        want = math.sqrt(sum(float(g.double().square().sum()) for g in tr.hgrad) + sum(float(g.square().sum()) for g in before))
+        assert want > 10 * tr.config.max_grad_norm
+        norm, scales, grads, _ = _step(tr, monkeypatch)
+        f = tr.config.max_grad_norm / (want + 1e-6)
+        assert abs(norm - want) <= 1e-5 * want and all(abs(s - f) <= 1e-5 * f for s in scales)
+        for g, b in zip(grads, before):
+            assert torch.all((g.double() - b * f).abs() <= 1e-5 * (b * f).abs())
+    finally:
+        tr.cleanup()
