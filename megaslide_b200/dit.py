@@ -59,7 +59,7 @@ class VideoDiTConfig:
     rotary_theta: float = 10000.0
     gated_mlp: bool = False  # act(gate) * up feed-forward block (GatedMLP) in place of fc1 - GELU - fc2
     gated_activation: str = "silu"
-    fused_clip: bool = False  # trainer: norm and clipping of the GPU-resident gradients in two kernels
+    fused_clip: bool = False  # trainer: norm and clipping of the GPU-resident gradients by grad_norm and clip_grad_norm_
 
     @property
     def num_patches(self) -> int:

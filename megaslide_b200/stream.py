@@ -493,13 +493,13 @@ class CPUMasterVideoDiT:
         res_grads = [p.grad for p in self.res_params if p.grad is not None]
         fused = bool(getattr(cfg, "fused_clip", False)) and bool(res_grads)
         if fused:
-            # norm over the blocks' host sums and the resident gradients, which are scaled by the same two kernels
+            # norm over the blocks' host sums and the resident gradients, read before anything is scaled: by the rule below
+            # a norm that is NaN scales nothing, neither on the host nor here
             for p in self.res_params:
                 if p.grad is not None and not p.grad.is_contiguous():
                     p.grad = p.grad.contiguous()
             res_grads = [p.grad for p in self.res_params if p.grad is not None]
-            clip = cfg.max_grad_norm > 0
-            norm = float(clip_grad_norm_(res_grads, cfg.max_grad_norm, extra_sumsq=sq) if clip else grad_norm(res_grads, extra_sumsq=sq))
+            norm = sq if math.isnan(sq) else float(grad_norm(res_grads, extra_sumsq=sq))
         elif res_grads:
             sq += float(torch.stack([g.float().square().sum() for g in res_grads]).sum())
         if not fused:
@@ -508,7 +508,9 @@ class CPUMasterVideoDiT:
         if cfg.max_grad_norm > 0 and norm > cfg.max_grad_norm:
             scale = cfg.max_grad_norm / (norm + 1e-6)
         if res_grads:
-            if scale != 1.0 and not fused:
+            if scale != 1.0 and fused:
+                clip_grad_norm_(res_grads, cfg.max_grad_norm, extra_sumsq=sq)
+            elif scale != 1.0:
                 for g in res_grads:
                     g.mul_(scale)
             self.gpu_opt.step()

@@ -226,3 +226,26 @@ def test_fused_clip_scales_host_and_resident_gradients_alike(monkeypatch):
             assert torch.all((g.double() - b * f).abs() <= 1e-5 * (b * f).abs())
     finally:
         tr.cleanup()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("where", ["block", "resident"])
+def test_fused_clip_with_a_gradient_that_is_not_finite(where, value, monkeypatch):
+    """One bad gradient has the same outcome with and without fused_clip, wherever it lies."""
+    got = []
+    for fused in (False, True):
+        tr = _trainer(fused)
+        try:
+            if where == "block":
+                tr.hgrad[1][7] = value
+            else:
+                tr.res_params[0].grad.view(-1)[3] = value
+            got.append(_step(tr, monkeypatch))
+            monkeypatch.undo()
+        finally:
+            tr.cleanup()
+    (n0, s0, g0, p0), (n1, s1, g1, p1) = got
+    assert (math.isnan(n0) and math.isnan(n1)) or n0 == n1
+    assert s0 == s1
+    for a, b in zip(g0 + p0, g1 + p1):
+        assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
