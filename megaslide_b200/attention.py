@@ -95,7 +95,7 @@ def _norm_extra_back(cfg: _Cfg, ek: Tensor, gk: Tensor, dek: Tensor) -> Tuple[Te
     """float32 gradients of the extra keys before the norm and of the weight."""
     sh = cfg.shape
     shape = ops.RotaryShape(1, ek.shape[0], (1, 1, 1), (0, 0, 0), sh.head_dim)
-    dek, _, dg, _ = ops.qk_norm_rope_bwd(shape, sh.heads, 0, ek.float(), None, gk.float(), None, dek, None, cfg.eps)
+    dek, _, dg, _ = ops.qk_norm_rope_bwd(shape, sh.heads, 0, ek.float(), None, gk, None, dek, None, cfg.eps)
     return dek, dg
 
 
@@ -115,8 +115,8 @@ class DSA3DFunction(torch.autograd.Function):
         qkv = torch.addmm(bqkv, x2, wqkv.t())  # [BN, 3C]
         q, k, v = qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:]
         if cfg.rotary is not None:
-            gq = gq.detach().to(dt) if gq is not None else None
-            gk = gk.detach().to(dt) if gk is not None else None
+            gq = gq.detach().float() if gq is not None else None  # the kernels take float32 weights beside any tokens
+            gk = gk.detach().float() if gk is not None else None
             q, k = _turn_qk(cfg, qkv, gq, gk, table)
         O = w2.shape[0]
         w2m = w2.reshape(O, C)
@@ -209,7 +209,7 @@ class DSA3DFunction(torch.autograd.Function):
                 dgq, dgk = _turn_back(cfg, qkv, dqkv, gq, gk, table)
                 if ek_raw is not None:
                     dek, dge = _norm_extra_back(cfg, ek_raw, gk, dek)
-                    dgk = dgk.float() + dge
+                    dgk = dgk + dge
             # q/k/v projections; dx accumulates in float32 across the three branches (the depthwise
             # convs add their transposed convolutions into it)
             dx = _mm_f32(dqkv, wqkv)

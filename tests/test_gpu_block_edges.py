@@ -249,3 +249,42 @@ def test_fused_clip_with_a_gradient_that_is_not_finite(where, value, monkeypatch
     assert s0 == s1
     for a, b in zip(g0 + p0, g1 + p1):
         assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.nan_to_num(a), torch.nan_to_num(b))
+
+
+@pytest.mark.parametrize("G", [0, 3], ids=["", "extra"])
+def test_norm_weights_stay_float32_under_autocast(G, monkeypatch):
+    """float32 norm weights reach the kernels beside bf16 tokens as they are, and their gradients, sums in float32, come back
+    without a rounding to bf16 on the way."""
+    torch.manual_seed(0)
+    m = msl.DeformableSlideAttention3D(64, 4, (3, 3, 3), qk_norm=True, rotary_axes=(4, 6, 6)).cuda()
+    with torch.no_grad():
+        m.q_norm_weight.normal_(1, 0.2)
+        m.k_norm_weight.normal_(1, 0.2)
+    seen, sums = [], {"q": 0.0, "k": 0.0}
+    forward, backward = ops.qk_norm_rope_fwd, ops.qk_norm_rope_bwd
+
+    def fwd(shape, heads, kv, q, k, gq, gk, *a, **kw):
+        seen.extend(w for w in (gq, gk) if w is not None)
+        return forward(shape, heads, kv, q, k, gq, gk, *a, **kw)
+
+    def bwd(shape, heads, kv, q, k, gq, gk, *a, **kw):
+        r = backward(shape, heads, kv, q, k, gq, gk, *a, **kw)
+        if kv:
+            sums["q"], sums["k"] = sums["q"] + r[2].float(), sums["k"] + r[3].float()
+        else:  # the extra keys
+            sums["k"] = sums["k"] + r[2].float()
+        return r
+
+    monkeypatch.setattr(ops, "qk_norm_rope_fwd", fwd)
+    monkeypatch.setattr(ops, "qk_norm_rope_bwd", bwd)
+    x = _rand(1, 2, 60, 64).requires_grad_()
+    extra = _rand(2, 2, G, 64).requires_grad_() if G else None
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = m(x, (3, 4, 5), extra)
+    y.float().square().sum().backward()
+    assert len(seen) == (3 if G else 2)
+    for w in seen:
+        assert any(torch.equal(w.float(), p.detach()) for p in (m.q_norm_weight, m.k_norm_weight))
+    for p, s in ((m.q_norm_weight, sums["q"]), (m.k_norm_weight, sums["k"])):
+        assert torch.equal(p.grad, s)
+        assert not torch.equal(p.grad, p.grad.bfloat16().float())
