@@ -157,7 +157,10 @@ static int run(const Product& p, Slots& slots, int slot_a, int slot_b, cudaStrea
       e = launch_planes(p.dtype, jobs, count, s);
       if (e != cudaSuccess) return cuda_failf(e, "split_kernel launch");
     }
-    e = launch_product_planes(p, slots.at[slot_a], slots.at[slot_b], s);
+    // the gradient of h passes through slot 1, as wide and not yet used: the gradients of g and u come after it
+    if (p.epilogue == kDgate && p.dtype == MSL_DTYPE_BF16 && sizeof(float) * p.M * p.N > slots.bytes[1])
+      return failf(MSL_ERR_WORKSPACE, "the gradient of h beyond its slot");
+    e = launch_product_planes(p, slots.at[slot_a], slots.at[slot_b], reinterpret_cast<float*>(slots.at[1]), s);
     if (e != cudaSuccess) return cuda_failf(e, "planes_kernel launch");
   } else if (p.dtype == MSL_DTYPE_F32) {
     e = launch_product_skinny(p, s);

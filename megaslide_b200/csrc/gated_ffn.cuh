@@ -123,7 +123,8 @@ struct PlaneJob {
   void* out;
 };
 cudaError_t launch_planes(int dtype, const PlaneJob* jobs, int count, cudaStream_t s);  // one or two
-cudaError_t launch_product_planes(const Product& p, const void* pa, const void* pb, cudaStream_t s);
+// dh: float32 [M, N] for the gradient of h of a kDgate product in bf16
+cudaError_t launch_product_planes(const Product& p, const void* pa, const void* pb, float* dh, cudaStream_t s);
 
 }  // namespace ffn
 }  // namespace msl

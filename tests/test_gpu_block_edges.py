@@ -288,3 +288,25 @@ def test_norm_weights_stay_float32_under_autocast(G, monkeypatch):
     for p, s in ((m.q_norm_weight, sums["q"]), (m.k_norm_weight, sums["k"])):
         assert torch.equal(p.grad, s)
         assert not torch.equal(p.grad, p.grad.bfloat16().float())
+
+
+@pytest.mark.parametrize("M,C,F", [(1, 9, 30), (40, 77, 203), (130, 253, 635), (200, 1533, 2047)])
+def test_gated_ffn_widths_off_vectors_round_the_inner_gradients_once(M, C, F):
+    """With one-hot rows of x, dw_in's columns are the gradients of g and u as the kernels hold them: the exact gradient
+    of h (a product of C terms) times the kept factor, rounded to bf16 once."""
+    x = torch.zeros(M, C, dtype=torch.bfloat16, device=_dev())
+    _, w_in, w_out, _, _ = (t.detach() if t is not None else None for t in _ffn_case(M, C, F, torch.bfloat16, "gelu", False))
+    rows = min(M, C)
+    x[torch.arange(rows), torch.arange(rows)] = 1
+    dy = _rand(9, M, C, dtype=torch.bfloat16)
+    _, h, kept = ops.gated_ffn_fwd(x, w_in, w_out, activation="gelu", keep=True)
+    dw_in = ops.gated_ffn_bwd(x, w_in, w_out, h, kept, dy, activation="gelu", needs=(False, True, False, False, False))[1]
+    got = dw_in.t()[:rows].double()
+    dh = dy.double() @ w_out.double()
+    mag = dy.double().abs() @ w_out.double().abs()
+    kd = kept.double()
+    want = torch.cat([dh * kd[:, :F], dh * kd[:, F:]], 1)[:rows]
+    bound = torch.cat([mag * kd[:, :F].abs(), mag * kd[:, F:].abs()], 1)[:rows] * (C + 2) * EPS
+    err = (got - want).abs()
+    # a result that is nearly halfway between two bf16 numbers may go either way by the sums' own roundings
+    assert torch.all(err <= HALF * want.abs() + 2 * bound + 1e-38), float((err / (HALF * want.abs() + 2 * bound + 1e-38)).max())
