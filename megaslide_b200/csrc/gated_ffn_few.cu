@@ -2,9 +2,11 @@
 // weights are read once, split into bf16 planes in registers and multiplied on the tensor cores by mma.sync.
 //
 // An element is hi + mid + lo, eight bits each: hi its upper half, cut off (so no finite value becomes infinite), the
-// others rounded to nearest; the six products that reach 2^-24 of a product, the small ones first.  Sums of 64 k
-// stay in the instruction's accumulators (which cut off what does not fit), then go into sums of their own, rounded.
-// An operand that is infinite gives NaN.
+// others rounded to nearest; the six products that reach 2^-24 of a product, the small ones of 32 k first.  Sums of 32 k
+// stay in the instruction's accumulators, which cut off what does not fit, two full-sized additions that way; then they
+// go into sums of their own, rounded.  Error of the whole block, 2560 to 7168 x 4108 to 25088, in the 2-norm: 2.7e-7
+// to 4.4e-7, plain float32 products 3.7e-7 to 3.7e-6; with 64 k that were not small ones first 1.2e-6, in the same time to
+// 10%.  Sums of 16 k 3.1e-7 to 6e-7 and, from 9 rows on, 5 to 10% slower.  An operand that is infinite gives NaN.
 //
 // A warp has 32 columns of the result (rows or columns of the weights) and all rows of x, a block 8 warps and a share
 // of k.  A lane copies its own 8 x 16 bytes of 32 k of the weights to its own place in shared memory, two such stages
@@ -12,10 +14,10 @@
 // operand whatever order that has k and columns in, as long as x uses the same.  x goes through registers
 // into planes in shared memory, kChunk k at a time, once for the block.  Shares of k are joined by skinny_join_kernel.
 //
-// Measured, 7168 x 25088 (the four products that read weights, 1.08 GB each on average): 5, 13, 30 and 60 rows 345, 375, 480
-// and 657 us, where skinny_kernel took 309 (1 row), 430, 850 and about 1300.  What bounds it: up to 8 rows the
-// splitting and the weights' bytes (3.1 TB/s), then the multiplications, 53 us for every 8 rows (2.4 clocks an
-// instruction).  12 or 16 warps a block are as fast; x by 64 k at a time and five stages 5% slower than by 128 and three.
+// Measured, 7168 x 25088 (the four products that read weights, 1.08 GB each on average, joins included): 5, 13, 30 and 60
+// rows 338, 403, 470 and 683 us, where skinny_kernel took 309 (1 row), 430, 850 and about 1300.  What bounds it: up to 8
+// rows the splitting and the weights' bytes (3.2 TB/s), then the multiplications, 50 us for every 8 rows (2.4 clocks
+// an instruction).  12 or 16 warps a block are as fast; x by 64 k at a time and five stages 5% slower than by 128 and three.
 
 #include "gated_ffn.cuh"
 
@@ -116,24 +118,13 @@ __global__ void __launch_bounds__(32 * kWarps, 1) few_kernel(const __grid_consta
   };
   fetch(k0);
 
-  float acc[2][NT][4], sum[2][NT][4];
+  float sum[2][NT][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][j][c] = sum[i][j][c] = 0.f;
-  auto drain = [&]() {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          sum[i][j][c] += acc[i][j][c];
-          acc[i][j][c] = 0.f;
-        }
-  };
+      for (int c = 0; c < 4; ++c) sum[i][j][c] = 0.f;
   int slot = 0, buf = 0;
   for (int first = 0; first < groups; first += kParts, buf ^= 1) {
     uint8_t* const planes = xs + buf * 3 * kPlane;
@@ -183,19 +174,20 @@ __global__ void __launch_bounds__(32 * kWarps, 1) few_kernel(const __grid_consta
         uint4 x[3];
 #pragma unroll
         for (int p = 0; p < 3; ++p) x[p] = *reinterpret_cast<const uint4*>(planes + p * kPlane + (part * kRows + j * 8 + g) * 64 + t * 16);
+        float acc[2][4] = {};
 #pragma unroll
         for (int c = 0; c < 6; ++c)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) mma16816(acc[i][j], wp[0][i][kOf[c][0]], x[kOf[c][1]].x, x[kOf[c][1]].y);
+          for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int c = 0; c < 6; ++c)
+            for (int i = 0; i < 2; ++i) mma16816(acc[i], wp[s][i][kOf[c][0]], s ? x[kOf[c][1]].z : x[kOf[c][1]].x, s ? x[kOf[c][1]].w : x[kOf[c][1]].y);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) mma16816(acc[i][j], wp[1][i][kOf[c][0]], x[kOf[c][1]].z, x[kOf[c][1]].w);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[i][j][c] += acc[i][c];
       }
-      if (part & 1) drain();
     }
   }
-  drain();
   float* const out = P.out + static_cast<long long>(blockIdx.y) * P.M * P.N;
 #pragma unroll
   for (int j = 0; j < NT; ++j)

@@ -310,3 +310,35 @@ def test_gated_ffn_widths_off_vectors_round_the_inner_gradients_once(M, C, F):
     err = (got - want).abs()
     # a result that is nearly halfway between two bf16 numbers may go either way by the sums' own roundings
     assert torch.all(err <= HALF * want.abs() + 2 * bound + 1e-38), float((err / (HALF * want.abs() + 2 * bound + 1e-38)).max())
+
+
+def _check_product(got, a, b):
+    """A product of K terms may be off by 4 EPS of its 2-norm for what the splitting and the accumulators of 32 terms cut
+    off, and by the random walk of K / 32 rounded additions to a sum that grows like one (EPS / sqrt(3) each):
+    EPS sqrt(K / 192).  What is cut off always pulls a sum towards zero: at most EPS of it, on average, for each of
+    the two full-sized additions of an accumulator."""
+    want = a.double() @ b.double()
+    err = got.double() - want
+    assert float(err.norm() / want.norm()) <= (4 + math.sqrt(a.shape[1] / 192)) * EPS
+    assert float((err * want.sign()).mean().abs() / want.abs().mean()) <= 2 * EPS
+
+
+@pytest.mark.parametrize("M", [3, 8, 12, 30, 40, 64])
+def test_gated_ffn_float32_few_rows_of_wide_weights_keep_float32(M):
+    """Single products of the form that splits the weights on their way."""
+    C, F = 4100, 4108
+    x, w_in, w_out, b_in, _ = (t.detach() for t in _ffn_case(M, C, F, torch.float32, "silu", True))
+    w_in[:F], b_in[:F], b_in[F:] = 0, 40, 0  # silu(40) = 40 and its derivative is 1: the first kept factor is u
+    kept = ops.gated_ffn_fwd(x, w_in, w_out, b_in, None, keep=True)[2]
+    assert torch.all(kept[:, F:] == 40)
+    _check_product(kept[:, :F], x, w_in[F:].t())
+    if M > 32:
+        return
+    w_in = _rand(2, 2 * F, C, std=C ** -0.5)
+    dy, ones, h = _rand(9, M, C), torch.ones(M, 2 * F, device=_dev()), torch.zeros(M, F, device=_dev())
+    hot = torch.eye(M, C, device=_dev())  # one-hot rows: dw_in's columns are the gradients of g and u
+    dx, dw_in = ops.gated_ffn_bwd(hot, w_in, w_out, h, ones, dy, needs=(True, True, False, False, False))[:2]
+    dgu = dw_in.t()[:M].contiguous()
+    assert torch.equal(dgu[:, :F], dgu[:, F:])
+    _check_product(dgu[:, :F], dy, w_out)
+    _check_product(dx, dgu, w_in)
