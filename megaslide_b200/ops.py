@@ -156,16 +156,20 @@ def status_word(device: torch.device) -> StatusWord:
 class HostFlag:
     """The status word of the operators around the attention (rotary positions, feed-forward): one pinned host
     word per device that their kernels write only when something went wrong, so a good call costs nothing.
-    The next call that finds a bit set raises MslError (the failed call's results are not valid)."""
+    The next call that finds a bit set waits for the device, so that no kernel sets another one while the word is
+    cleared, and raises MslError (the failed calls' results are not valid)."""
 
-    def __init__(self):
+    def __init__(self, index: Optional[int] = None):
+        self.index = index
         self.word = torch.zeros(1, dtype=torch.int32, device="cpu").pin_memory()
         self.ptr = self.word.data_ptr()
         self._view = self.word.numpy()
 
     def poll(self) -> None:
-        v = self._view[0]
-        if v:
+        if self._view[0]:
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.synchronize(self.index)
+            v = self._view[0]
             self._view[0] = 0
             what = []
             if v & _lib.MSL_STATUS_ROTARY_INDEX:
@@ -182,7 +186,7 @@ def host_flag(device: torch.device) -> HostFlag:
     """The process-wide HostFlag of a CUDA device."""
     f = _FLAGS.get(device.index)
     if f is None:
-        f = _FLAGS[device.index] = HostFlag()
+        f = _FLAGS[device.index] = HostFlag(device.index)
     return f
 
 

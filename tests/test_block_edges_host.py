@@ -161,3 +161,35 @@ def test_status_word_of_a_caller_is_checked():
     for bad in (torch.zeros(1), torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int32, device="meta")):
         with pytest.raises(ValueError, match="status"):
             ops._flag(dev, bad)
+
+
+def test_flag_loses_no_bit_that_is_set_while_it_is_read(monkeypatch):
+    """A kernel that is still running reports between the host's look at the word and its clearing it."""
+    flag = object.__new__(ops.HostFlag)
+    flag.index = None
+
+    class Word:
+        value, running = 0, False
+
+        def __getitem__(self, i):
+            v, self.value = self.value, self.value | (_lib.MSL_STATUS_TIMEOUT if self.running else 0)
+            self.running = False
+            return v
+
+        def __setitem__(self, i, v):
+            self.value = v
+
+    flag._view = word = Word()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: setattr(word, "running", False))
+    flag.poll()
+    word.value, word.running = _lib.MSL_STATUS_ROTARY_INDEX, True
+    texts = []
+    for _ in range(2):
+        try:
+            flag.poll()
+        except msl.MslError as e:
+            texts.append(str(e))
+    assert "outside its axis" in " ".join(texts) and "did not complete" in " ".join(texts)
+    assert word.value == 0
+    flag.poll()
