@@ -179,7 +179,8 @@ static int check(const msl_ffn_geometry* g, const msl_ffn_io* io) {
   if (g->rows < 0 || g->dim < 1 || g->hidden < 1) return failf(MSL_ERR_INVALID, "rows must be >= 0, dim and hidden >= 1");
   if (g->dtype != MSL_DTYPE_F32 && g->dtype != MSL_DTYPE_BF16) return failf(MSL_ERR_INVALID, "unknown dtype %d", g->dtype);
   if (g->activation != MSL_ACT_SILU && g->activation != MSL_ACT_GELU) return failf(MSL_ERR_INVALID, "unknown activation %d", g->activation);
-  if (g->dim > (1 << 21) || g->hidden > (1 << 20)) return failf(MSL_ERR_UNSUPPORTED, "dim or hidden is over 2^20");
+  if (g->dim > (1 << 21)) return failf(MSL_ERR_UNSUPPORTED, "dim is over 2^21");
+  if (g->hidden > (1 << 20)) return failf(MSL_ERR_UNSUPPORTED, "hidden is over 2^20");
   if (g->rows > (1LL << 31) - 256) return failf(MSL_ERR_UNSUPPORTED, "rows is over 2^31 - 256");
   if (!io) return failf(MSL_ERR_INVALID, "io is NULL");
   return MSL_OK;

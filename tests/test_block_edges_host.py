@@ -193,3 +193,12 @@ def test_flag_loses_no_bit_that_is_set_while_it_is_read(monkeypatch):
     assert "outside its axis" in " ".join(texts) and "did not complete" in " ".join(texts)
     assert word.value == 0
     flag.poll()
+
+
+@pytest.mark.parametrize("dim,hidden,text", [((1 << 21) + 1, 8, "dim is over 2^21"), (8, (1 << 20) + 1, "hidden is over 2^20")])
+def test_ffn_entry_names_the_limit_it_checks(dim, hidden, text):
+    lib = _lib.load()
+    g = _lib.FfnGeometry(4, dim, hidden, 0, 0)
+    io = _lib.FfnIO(x=16, x_ld=dim, w_in=16, w_out=16, h=16, y=16, y_ld=dim)
+    assert lib.msl_gated_ffn_fwd(ctypes.byref(g), ctypes.byref(io), None, 0, None) == _lib.MSL_ERR_UNSUPPORTED
+    assert lib.msl_last_error().decode().endswith(text)
