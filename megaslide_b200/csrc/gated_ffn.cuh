@@ -36,10 +36,6 @@ struct Product {
 };
 
 // act(g) and its derivative, in float32, for results in float32.
-__device__ __forceinline__ float act_value(float g, int act) {
-  if (act == MSL_ACT_SILU) return g / (1.f + expf(-g));
-  return 0.5f * g * (1.f + erff(g * 0.7071067811865476f));
-}
 __device__ __forceinline__ float act_value_grad(float g, int act, float& da) {
   if (act == MSL_ACT_SILU) {
     const float s = 1.f / (1.f + expf(-g));
