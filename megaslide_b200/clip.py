@@ -1,5 +1,6 @@
 """Global gradient norm over many tensors and clipping on the kernels of csrc/grad_norm.cu: two launches for the
-norm or for norm and scaling, whatever the number of tensors, and no wait for the GPU."""
+norm or for norm and scaling of up to 896 tensors with elements, one or two more for every further 896, and no wait for
+the GPU."""
 
 from __future__ import annotations
 

@@ -27,7 +27,7 @@ namespace clip {
 
 constexpr int kThreads = 256;
 constexpr int kLeastChunk = 2048, kMostChunk = 32768;  // elements
-constexpr int kMaxTensors = 896;   // of a launch: 30 KB of the 32 KB that parameters may take
+constexpr int kMaxTensors = 896;   // of a launch
 constexpr int kBlocksPerSm = 8;
 
 struct Table {
@@ -38,6 +38,7 @@ struct Table {
   unsigned char bf16[kMaxTensors];
   int count, chunk;
 };
+static_assert(sizeof(Table) + 64 <= 32764, "a kernel's parameters may take 32764 bytes, other ones than the table 40 of them");
 
 // last tensor whose first chunk is <= c (tensors without elements have no chunk and are never it)
 __device__ __forceinline__ int tensor_of(const Table& t, unsigned c) {
