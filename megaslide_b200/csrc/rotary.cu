@@ -629,8 +629,8 @@ int choose_v(const Params& P, bool inter, int dtype, bool bwd, int nops) {
   return 1;
 }
 
-// Blocks of a backward whose weights' gradients are wanted: resident ones only, each keeps its sums.  The
-// queries' share goes by the heads.
+// Blocks of a backward whose weights' gradients are wanted: each keeps its sums, so at most four a SM, in two rounds (two
+// or eight a SM take the same time).  The queries' share goes by the heads.
 int bwd_blocks(const msl_rotary_geometry* g, const msl_qk_norm_io* io, int* blocks0) {
   const long long most = static_cast<long long>(sm_count()) * kBwdBlocksPerSm;
   const long long need = (g->rows * io->heads + kWarps - 1) / kWarps, need1 = (g->rows * io->kv_heads + kWarps - 1) / kWarps;
@@ -684,8 +684,19 @@ template <typename T, bool INTER, int MODE>
 cudaError_t by_v(const Params& P, int v, cudaStream_t s, int blocks) {
   switch (v) {
     case 4:
-      if (MODE != kRotate && P.d == 64) return launch<T, 4, 1, INTER, MODE, 8>(P, s, blocks);
-      if (MODE != kRotate && P.d == 128) return launch<T, 4, 1, INTER, MODE, 16>(P, s, blocks);
+      // A head's sums: where its lanes are a power of two, shuffles of a number that the compiler knows, else a loop with
+      // a broadcast.  Norm and rotation of 131072 tokens of about 1536 channels in bf16, forward and backward: 4 lanes
+      // (head 32) 261 and 385 us, by the loop 268 and 429; 8 lanes 260 and 389, 277 and 459; 16 lanes 258 and 403, 290 and
+      // 495; 32 lanes 275 and 386, 302 and 527.  float32 within 6% either way.
+      if (MODE != kRotate) {
+        switch (P.d / 8) {
+          case 4: return launch<T, 4, 1, INTER, MODE, 4>(P, s, blocks);
+          case 8: return launch<T, 4, 1, INTER, MODE, 8>(P, s, blocks);
+          case 16: return launch<T, 4, 1, INTER, MODE, 16>(P, s, blocks);
+          case 32: return launch<T, 4, 1, INTER, MODE, 32>(P, s, blocks);
+          default: break;  // any other number; 1 and 2 lanes (heads of 8 and 16) are no or one step of the loop
+        }
+      }
       return launch<T, 4, 1, INTER, MODE, 0>(P, s, blocks);
     case 2: return launch<T, 2, 2, INTER, MODE, 0>(P, s, blocks);
     default: return launch<T, 1, 4, INTER, MODE, 0>(P, s, blocks);

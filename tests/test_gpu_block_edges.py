@@ -14,7 +14,8 @@ import megaslide_b200 as msl
 from megaslide_b200 import ops
 from megaslide_b200.dit import MegaSlideDiT, VideoDiTConfig
 from megaslide_b200.stream import CPUMasterVideoDiT, _HostAdamW
-from test_gpu_block_ops import DTYPES, EPS, HALF, IDS, RMS, _close, _dev, _ffn_case, _ffn_ref, _rand, _within
+from test_gpu_block_ops import (DTYPES, EPS, HALF, IDS, RMS, _angles, _close, _dev, _ffn_case, _ffn_ref, _positions, _rand,
+                                _ref_norm_rope, _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -342,3 +343,25 @@ def test_gated_ffn_float32_few_rows_of_wide_weights_keep_float32(M):
     assert torch.equal(dgu[:, :F], dgu[:, F:])
     _check_product(dgu[:, :F], dy, w_out)
     _check_product(dx, dgu, w_in)
+
+
+@pytest.mark.parametrize("interleaved", [True, False], ids=["interleaved", "split"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv,d", [(5, 5, 8), (7, 7, 16), (9, 3, 24), (11, 11, 32), (5, 5, 64), (4, 2, 96), (3, 3, 128), (2, 1, 256)])
+def test_qk_norm_rope_heads_of_every_number_of_lanes(heads, kv, d, dtype, interleaved):
+    """1 to 32 lanes of 8 channels, powers of two and others, heads that do not fill the last warp; bounds as in
+    test_gpu_block_ops.test_qk_norm_rope."""
+    vs, axes, B, N = (3, 4, 5), (d // 2, d // 4, d // 4), 2, 60
+    table = msl.rotary_table(vs, axes, theta=100.0, device=_dev())
+    cos, sin = _angles(table, vs, axes, _positions(vs, 0, N, None, B))
+    q, k = _rand(1, B, N, heads * d, dtype=dtype).requires_grad_(), _rand(2, B, N, kv * d, dtype=dtype).requires_grad_()
+    gq, gk = (1 + _rand(3, d, std=0.3)).to(dtype).requires_grad_(), (1 + _rand(4, d, std=0.3)).to(dtype).requires_grad_()
+    dq, dk = _rand(5, B, N, heads * d, dtype=dtype), _rand(6, B, N, kv * d, dtype=dtype)
+    q2, k2 = msl.qk_norm_rope(q, k, gq, gk, table, heads=heads, kv_heads=kv, video_shape=vs, axes=axes, interleaved=interleaved)
+    got = torch.autograd.grad([q2, k2], [q, k, gq, gk], [dq, dk])
+    half = HALF if dtype == torch.bfloat16 else 0.0
+    for y, x, g, dy, nh, dx, dg in ((q2, q, gq, dq, heads, got[0], got[2]), (k2, k, gk, dk, kv, got[1], got[3])):
+        w, wm, wdx, wdxm, wdg, wdgm = _ref_norm_rope(x, g, dy, nh, cos, sin, interleaved, 1e-6)
+        _within(y.detach(), w, wm, (d / 2 + 16) * EPS, half)
+        _within(dx, wdx, wdxm, (2 * d + 32) * EPS, half)
+        _within(dg, wdg, wdgm, (d / 2 + 16 + 6 * math.sqrt(B * N * nh)) * EPS, half)
