@@ -289,7 +289,8 @@ class DeformableSlideAttention3D(nn.Module):
 
     ``capture`` (not a parameter; None by default): a dict set here receives references to the
     intermediates of the next forward / backward (q/k/v, offsets, attention output, lse and their
-    gradients), which a checker compares with an independent implementation at sampled rows.
+    gradients), which a checker compares with an independent implementation at sampled rows.  Its q and k, and
+    their gradients, are the projections', before norm and rotation where those options are on.
     """
 
     def __init__(self, hidden_size: int, num_heads: int, kernel_size: Tuple[int, int, int] = (3, 7, 7),

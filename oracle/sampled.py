@@ -119,7 +119,10 @@ def check(module, cap: dict, video_shape, *, batch: int, dtype: torch.dtype, n_r
     """Compares one captured forward + backward (module.capture / TimeShardedDSA3D.capture) with the
     oracle at sampled rows.  Unsharded captures hold x2/qkv/dqkv; sharded ones xw/q/kv/dq/dkv plus the
     rank's frame windows (pass q_frame0/q_frames/kv_frame0/kv_frames).  Returns a dict of entries
-    {err, tol, ok} plus ``ok`` (all entries) and ``n_rows``."""
+    {err, tol, ok} plus ``ok`` (all entries) and ``n_rows``.  The oracle knows neither the norm of queries and keys nor
+    rotary positions, and a capture's q and k are those before them: modules with these options are refused."""
+    if getattr(module, "qk_norm", False) or getattr(module, "rotary_axes", None) is not None:
+        raise ValueError("the oracle does not restate qk_norm and rotary_axes")
     T, H, W = video_shape
     HW = H * W
     nh, d = module.num_heads, module.head_dim

@@ -9,6 +9,7 @@ import torch
 
 import megaslide_b200 as msl
 from megaslide_b200 import _lib, ops
+from oracle import sampled
 
 
 def _module(**kw):
@@ -202,3 +203,10 @@ def test_ffn_entry_names_the_limit_it_checks(dim, hidden, text):
     io = _lib.FfnIO(x=16, x_ld=dim, w_in=16, w_out=16, h=16, y=16, y_ld=dim)
     assert lib.msl_gated_ffn_fwd(ctypes.byref(g), ctypes.byref(io), None, 0, None) == _lib.MSL_ERR_UNSUPPORTED
     assert lib.msl_last_error().decode().endswith(text)
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_axes=None), dict(qk_norm=False)], ids=["norm", "rotary"])
+def test_sampled_check_refuses_options_that_the_oracle_does_not_restate(kw):
+    """It would compare the attention of normalised, turned q and k with that of the projections."""
+    with pytest.raises(ValueError, match="qk_norm and rotary_axes"):
+        sampled.check(_module(**kw), {}, (2, 3, 4), batch=1, dtype=torch.float32)
