@@ -57,7 +57,7 @@ class VideoDiTConfig:
     qk_norm: bool = False  # RMS norm of queries and keys for each head
     rotary_axes: Optional[Tuple[int, int, int]] = None  # channels of a head that turn with time, row and column
     rotary_theta: float = 10000.0
-    gated_mlp: bool = False  # act(gate) * up feed-forward block (GatedMLP) in place of fc1 - GELU - fc2
+    gated_mlp: bool = False  # act(gate) * up feed-forward block (GatedMLP; dropout on its result alone) for fc1 - GELU - fc2
     gated_activation: str = "silu"
     fused_clip: bool = False  # trainer: norm and clipping of the GPU-resident gradients by grad_norm and clip_grad_norm_
 

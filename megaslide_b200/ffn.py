@@ -66,7 +66,8 @@ def gated_ffn(x: Tensor, w_in: Tensor, w_out: Tensor, b_in: Optional[Tensor] = N
 
 class GatedMLP(nn.Module):
     """The gated block as a module: fc1 (2 * intermediate_size rows: gate, then the other) and fc2, as nn.Linear
-    parameters.  Under CUDA autocast to bfloat16 it computes in bfloat16, like nn.Linear."""
+    parameters.  Under CUDA autocast to bfloat16 it computes in bfloat16, like nn.Linear.  dropout acts on the result alone:
+    the hidden values stay inside the kernels (MLP in dit.py drops out both)."""
 
     def __init__(self, hidden_size: int, intermediate_size: int, dropout: float = 0.0, activation: str = "silu"):
         super().__init__()
