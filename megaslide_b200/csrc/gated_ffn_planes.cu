@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) planes_kernel(const __grid_consta
       const int sums = P.np == 3 ? w.k1 - w.k0 : 1;
       bool alive = true;
       for (int i = 0; i < sums; ++i) {
-        if (!wait(tfull + 8 * buf, tph, dead, P.status)) { alive = false; break; }
+        if (!wait_warp(tfull + 8 * buf, tph, dead, P.status)) { alive = false; break; }
         fence_after();
         const uint32_t from = tmem + buf * kAcc + lanes;
 #pragma unroll

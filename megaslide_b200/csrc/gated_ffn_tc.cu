@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         if (first + 1 < last) fetch(turn + 1, first + 1);
       }
       __syncwarp();
-      if (!wait(tfull + 8 * buf, tph, dead, P.status)) break;
+      if (!wait_warp(tfull + 8 * buf, tph, dead, P.status)) break;
       fence_after();
       bool alive = true;
       if (w.part >= 0) {
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         tmem_ld32(acc + c, v);
         if (EPI == kDgate) {
           const uint32_t g0 = mine + (turn & 1) * 2 * kTile, u0 = g0 + kTile;
-          if (!wait(mykept + 8 * (turn & 1), (turn >> 1) & 1, dead, P.status)) { alive = false; break; }
+          if (!wait_warp(mykept + 8 * (turn & 1), (turn >> 1) & 1, dead, P.status)) { alive = false; break; }
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const uint4 gv = lds(chunk32(g0, lane, q)), uv = lds(chunk32(u0, lane, q));

@@ -40,6 +40,11 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   }
   return true;
 }
+// The same for a whole warp: its lanes may see the end of a wait and the mark in any order, and must leave or go on together
+// (what follows is executed by all of them or none).
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* dead, uint32_t* status) {
+  return __all_sync(0xffffffffu, wait(bar, parity, dead, status));
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
