@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) planes_kernel(const __grid_consta
   const uint32_t tiles = base + kRing;
   const uint32_t bars = tiles + kEpiWarps * kTileBytes;
   const uint32_t full = bars, empty = bars + 8 * kMaxStages, peer = empty + 8 * kMaxStages, tfull = peer + 8 * kMaxStages, tempty = tfull + 16;
-  const uint32_t tmem_slot = tempty + 16;
+  const uint32_t tmem_slot = tempty + 16, last = tmem_slot + 8;
   volatile int* const dead = reinterpret_cast<volatile int*>(raw + (tmem_slot + 4 - smem_u32(raw)));
   volatile uint32_t* const slot = reinterpret_cast<volatile uint32_t*>(raw + (tmem_slot - smem_u32(raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) planes_kernel(const __grid_consta
       mbar_init(tfull + 8 * i, 1);
       mbar_init(tempty + 8 * i, 2 * kEpiWarps);
     }
+    mbar_init(last, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -305,6 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) planes_kernel(const __grid_consta
           }
         }
       }
+      if (!alive) mma_drain(last);
     } else if (lane == 0) {
       int st = 0;
       uint32_t ph = 0;

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   const uint32_t staging = base + kRing;
   const uint32_t bars = staging + kEpiWarps * kStaging;
   const uint32_t full = bars, empty = bars + 8 * kMaxStages, peer = empty + 8 * kMaxStages, tfull = peer + 8 * kMaxStages, tempty = tfull + 16;
-  const uint32_t kept = tempty + 16, tmem_slot = kept + 16 * kEpiWarps;
+  const uint32_t kept = tempty + 16, tmem_slot = kept + 16 * kEpiWarps, last = tmem_slot + 8;
   volatile int* const dead = reinterpret_cast<volatile int*>(raw + (tmem_slot + 4 - smem_u32(raw)));
   volatile uint32_t* const slot = reinterpret_cast<volatile uint32_t*>(raw + (tmem_slot - smem_u32(raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       mbar_init(tempty + 8 * i, 2 * kEpiWarps);
     }
     for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(kept + 8 * i, 1);
+    mbar_init(last, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       uint32_t ph = 0, tph = 0;
       bool alive = true;
       for (int t = t0; t < P.items && alive; t += tstep) {
-        if (!wait(tempty + 8 * buf, tph ^ 1, dead, P.status)) break;
+        if (!wait(tempty + 8 * buf, tph ^ 1, dead, P.status)) { alive = false; break; }
         fence_after();
         const Item w = item_at(P, t);
         for (int kb = w.k0; kb < w.k1; ++kb) {
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         buf ^= 1;
         if (buf == 0) tph ^= 1;
       }
+      if (!alive) mma_drain(last);
     } else if (lane == 0) {
       // the second CTA tells the first when its operands have landed
       int st = 0;

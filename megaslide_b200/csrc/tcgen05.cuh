@@ -92,6 +92,14 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
                "h"(static_cast<uint16_t>(3)) : "memory");
 }
+// A CTA that gives up: the multiplications issued so far end (within the limit) before their operands' CTAs leave and their
+// tensor memory is freed.
+__device__ __forceinline__ void mma_drain(uint32_t bar) {
+  mma_commit(bar);
+  const long long since = clock64();
+  while (!mbar_try(bar, 0) && clock64() - since < kWaitClocks) {
+  }
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // 32 columns of this warp's 32 lanes of tensor memory
