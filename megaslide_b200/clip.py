@@ -5,6 +5,7 @@ the GPU."""
 from __future__ import annotations
 
 import math
+from operator import attrgetter
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
@@ -13,15 +14,21 @@ from torch.autograd.graph import increment_version
 
 from . import ops
 
+_requires_grad = attrgetter("requires_grad")
 Tensors = Union[Tensor, Iterable[Optional[Tensor]]]
 
 
 def _list(tensors: Tensors) -> List[Tensor]:
-    """The tensors of a call; of parameters (which require gradients) their gradients, where they have one."""
+    """The tensors of a call; of parameters, and of other leaves that require gradients, their gradients, where they have
+    one."""
     ts = [tensors] if isinstance(tensors, Tensor) else tensors
     # plain tensors first: isinstance of Parameter runs a check in Python
     ts = [t if type(t) is Tensor else t.grad if isinstance(t, torch.nn.Parameter) else t for t in ts if t is not None]
-    return [t for t in ts if t is not None]
+    ts = [t for t in ts if t is not None]
+    if any(map(_requires_grad, ts)):
+        ts = [t.grad if t.requires_grad and t.is_leaf else t for t in ts]
+        ts = [t for t in ts if t is not None]
+    return ts
 
 
 def _check(extra_sumsq: float) -> float:
@@ -32,9 +39,9 @@ def _check(extra_sumsq: float) -> float:
 
 def grad_norm(tensors: Tensors, extra_sumsq: float = 0.0) -> Tensor:
     """2-norm of all elements of the tensors together (float32 or bfloat16, dense in any order of the axes, on one CUDA
-    device; parameters stand for their gradients), as a 0-dim float32 tensor on their device.  extra_sumsq: a sum of squares held
-    elsewhere (on the host, on other ranks) that belongs to the norm.  Without tensors the norm of extra_sumsq
-    alone, on the CPU.  Like torch's, it records no derivative."""
+    device; parameters and other leaves that require gradients stand for their gradients), as a 0-dim float32 tensor
+    on their device.  extra_sumsq: a sum of squares held elsewhere (on the host, on other ranks) that belongs to the
+    norm.  Without tensors the norm of extra_sumsq alone, on the CPU.  Like torch's, it records no derivative."""
     ts = _list(tensors)
     extra = _check(extra_sumsq)
     if not ts:
@@ -44,11 +51,11 @@ def grad_norm(tensors: Tensors, extra_sumsq: float = 0.0) -> Tensor:
 
 def clip_grad_norm_(tensors: Tensors, max_norm: float, *, out: Optional[Sequence[Tensor]] = None,
                     extra_sumsq: float = 0.0) -> Tensor:
-    """Scales the tensors (parameters: their gradients) by min(1, max_norm / (norm + 1e-6)) and returns the norm
-    before that, as grad_norm does; nothing waits for the GPU.  out: tensors of the same dtypes, sizes and
-    order that receive the result in place of the tensors themselves (slices of one flat buffer, say).  Results share memory with
-    nothing but their own tensor, in place: a tensor twice in the list is refused (MslError).  A norm that is not finite
-    reaches the results as the formula says (an infinite norm: zeros, and NaN for its infinite elements)."""
+    """Scales the tensors (as in grad_norm, gradients of parameters) by min(1, max_norm / (norm + 1e-6)) and returns the
+    norm before that; nothing waits for the GPU.  out: tensors of the same dtypes, sizes and order that receive the
+    result in place of the tensors themselves (slices of one flat buffer, say).  Results share memory with nothing but
+    their own tensor, in place: a tensor twice in the list is refused (MslError).  A norm that is not finite reaches the
+    results as the formula says (an infinite norm: zeros, and NaN for its infinite elements)."""
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     ts = _list(tensors)

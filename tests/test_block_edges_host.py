@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import megaslide_b200 as msl
-from megaslide_b200 import _lib, ops
+from megaslide_b200 import _lib, clip, ops
 from oracle import sampled
 
 
@@ -210,3 +210,16 @@ def test_sampled_check_refuses_options_that_the_oracle_does_not_restate(kw):
     """It would compare the attention of normalised, turned q and k with that of the projections."""
     with pytest.raises(ValueError, match="qk_norm and rotary_axes"):
         sampled.check(_module(**kw), {}, (2, 3, 4), batch=1, dtype=torch.float32)
+
+
+def test_leaves_that_require_gradients_stand_for_them():
+    """As torch's clip_grad_norm_ has it: a leaf is a parameter whether or not it is a Parameter, and it is not the weights
+    that are scaled."""
+    plain, leaf, bare = torch.ones(3), torch.ones(4, requires_grad=True), torch.ones(5, requires_grad=True)
+    param, frozen = torch.nn.Parameter(torch.ones(6)), torch.nn.Parameter(torch.ones(7), requires_grad=False)
+    leaf.grad, param.grad = torch.zeros(4), torch.zeros(6)
+    result = leaf * 2  # no leaf: itself
+    got = clip._list([plain, leaf, None, bare, param, frozen, result])
+    for a, b in zip(got, (plain, leaf.grad, param.grad, result), strict=True):
+        assert a is b
+    assert clip._list(leaf)[0] is leaf.grad and clip._list(bare) == []
