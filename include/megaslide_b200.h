@@ -332,7 +332,8 @@ typedef struct msl_ffn_geometry {
 
 /* Matrices are contiguous rows of their width except x, y, dy and dx (row strides given).  h [rows, hidden]
  * is the gated product that the second projection reads; kept [rows, 2*hidden] receives u act'(g), then act(g),
- * the factors the backward multiplies the gradient of h by (NULL = not kept).  Backward: dgu [rows, 2*hidden] is scratch (the gradients of g and u);
+ * the factors the backward multiplies the gradient of h by (NULL = not kept).  In bf16 they have 24 bits: kept holds the
+ * upper 16 of float32's 32, kept_low [rows, 2, hidden rounded up to 16] bytes, required beside kept, the next 8.  Backward: dgu [rows, 2*hidden] is scratch (the gradients of g and u);
  * dx, dw_in, dw_out, db_in, db_out are written where they are not NULL. */
 typedef struct msl_ffn_io {
   const void* x; int64_t x_ld;
@@ -345,6 +346,7 @@ typedef struct msl_ffn_io {
   void* dx; int64_t dx_ld;
   void* dw_in; void* dw_out; void* db_in; void* db_out;
   uint32_t* status; /* MSL_STATUS_TIMEOUT, as in the attention (may be NULL) */
+  void* kept_low;   /* bf16 */
 } msl_ffn_io;
 
 size_t msl_gated_ffn_workspace_bytes(const msl_ffn_geometry* geom, int32_t backward);

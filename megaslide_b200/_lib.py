@@ -124,7 +124,7 @@ class FfnIO(ctypes.Structure):
     _fields_ = [
         ("x", _vp), ("x_ld", _i64), ("w_in", _vp), ("b_in", _vp), ("w_out", _vp), ("b_out", _vp), ("h", _vp), ("kept", _vp),
         ("y", _vp), ("y_ld", _i64), ("dy", _vp), ("dy_ld", _i64), ("dgu", _vp), ("dx", _vp), ("dx_ld", _i64),
-        ("dw_in", _vp), ("dw_out", _vp), ("db_in", _vp), ("db_out", _vp), ("status", _vp),
+        ("dw_in", _vp), ("dw_out", _vp), ("db_in", _vp), ("db_out", _vp), ("status", _vp), ("kept_low", _vp),
     ]
 
 

@@ -304,6 +304,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   if (M == 0) return MSL_OK;
   if (!io->x || !io->h || !io->y) return failf(MSL_ERR_INVALID, "x, h and y are required");
   if (io->x_ld < C || io->y_ld < C) return failf(MSL_ERR_INVALID, "row strides must be >= dim = %lld", C);
+  if (io->kept && geom->dtype == MSL_DTYPE_BF16 && !io->kept_low) return failf(MSL_ERR_INVALID, "kept_low is required beside kept in bf16");
   const ffn::Workspace W = ffn::workspace_of(geom, false);
   rc = ffn::check_workspace(W, workspace, workspace_bytes);
   if (rc) return rc;
@@ -316,6 +317,7 @@ int msl_gated_ffn_fwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   p.out = io->h; p.ldo = F;
   p.bias = io->b_in;
   p.kept_out = io->kept;
+  p.low = static_cast<uint8_t*>(io->kept_low);
   p.M = M; p.N = F; p.K = C;
   ffn::Product q = ffn::product(geom, io, W, workspace);
   q.epilogue = ffn::kPlain;
@@ -349,6 +351,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
   const bool inner = io->dx || io->dw_in || io->db_in;  // wants the gradients of g and u
   if (!io->dy || io->dy_ld < C) return failf(MSL_ERR_INVALID, "dy (row stride >= dim) is required");
   if (inner && (!io->w_out || !io->kept || !io->dgu)) return failf(MSL_ERR_INVALID, "w_out, kept and dgu are required");
+  if (inner && geom->dtype == MSL_DTYPE_BF16 && !io->kept_low) return failf(MSL_ERR_INVALID, "kept_low is required beside kept in bf16");
   if (io->dx && (!io->w_in || io->dx_ld < C)) return failf(MSL_ERR_INVALID, "dx needs w_in and a row stride >= dim");
   if (io->dw_in && (!io->x || io->x_ld < C)) return failf(MSL_ERR_INVALID, "dw_in needs x");
   if (io->dw_out && !io->h) return failf(MSL_ERR_INVALID, "dw_out needs h");
@@ -364,6 +367,7 @@ int msl_gated_ffn_bwd(const msl_ffn_geometry* geom, const msl_ffn_io* io, void* 
     p.b = io->w_out; p.ldb = F; p.b_major = true;  // [K = dim, N = hidden]
     p.out = io->dgu; p.ldo = 2 * F;
     p.kept = io->kept;
+    p.low = static_cast<uint8_t*>(io->kept_low);
     p.M = M; p.N = F; p.K = C;
     rc = ffn::run(p, slots, 0, 2, s);
     if (rc) return rc;

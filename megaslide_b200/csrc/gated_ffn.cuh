@@ -27,6 +27,7 @@ struct Product {
   const void* bias;  // [N] (kGate: [2N]) or NULL
   const void* kept;  // kDgate: u act'(g), then act(g), [M, 2N]
   void* kept_out;    // kGate: [M, 2N] or NULL
+  uint8_t* low;      // bf16: the next 8 bits of the kept factors (read or written), [M, 2, low_width(N)]
   long long M, N, K;
   int dtype, act, epilogue;
   bool a_major, b_major;
@@ -34,6 +35,58 @@ struct Product {
   float* partial;  // workspace of tiles that are cut along k
   size_t partial_bytes;
 };
+
+// The factors that the forward keeps for the backward.  float32: as they are.  bf16: 24 bits of float32's 32, the upper 16
+// in `kept`, the next 8 in `low`, the rest cut off.  They are no operand of the tensor cores, and rounded to bf16 they put a
+// third rounding into the gradients, beside those of the gradients of g and u (an operand) and of the result: 0.0029
+// of the result in the 2-norm, where the two leave 0.0024.  All 32 bits would be another quarter of their bytes for nothing
+// that a bf16 result shows.  Reading puts the low byte into the last 8 bits as well: on average the middle of what was
+// cut off, and infinities, NaN and short numbers stay what they were.
+__host__ __device__ __forceinline__ long long low_width(long long N) { return (N + 15) / 16 * 16; }
+
+// one factor of one row, by the element; `which`: 0 u act'(g), 1 act(g)
+template <typename T>
+struct KeptRow {
+  T* at;
+  uint8_t* low;
+  long long N, W;
+
+  __device__ __forceinline__ KeptRow(const void* kept, const uint8_t* low_rows, long long row, long long n, long long N_)
+      : at(static_cast<T*>(const_cast<void*>(kept)) + row * 2 * N_ + n), low(nullptr), N(N_), W(0) {
+    if constexpr (sizeof(T) == 2) {
+      W = low_width(N_);
+      low = const_cast<uint8_t*>(low_rows) + row * 2 * W + n;
+    }
+  }
+  __device__ __forceinline__ void put(int which, float v) const {
+    if constexpr (sizeof(T) == 4) {
+      at[which * N] = v;
+    } else {
+      const uint32_t b = __float_as_uint(v);
+      reinterpret_cast<uint16_t*>(at)[which * N] = static_cast<uint16_t>(b >> 16);
+      low[which * W] = static_cast<uint8_t>(b >> 8);
+    }
+  }
+  __device__ __forceinline__ float get(int which) const {
+    if constexpr (sizeof(T) == 4) {
+      return at[which * N];
+    } else {
+      const uint32_t b = low[which * W];
+      return __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(at)[which * N]) << 16 | b << 8 | b);
+    }
+  }
+};
+
+// the same by words: the upper halves of two factors, the low bytes of four, and element j of both
+__device__ __forceinline__ uint32_t kept_high(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+__device__ __forceinline__ uint32_t kept_low(float a, float b, float c, float d) {
+  return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0051), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0051), 0x5410);
+}
+template <int J>
+__device__ __forceinline__ float kept_at(uint32_t high, uint32_t low) {  // J: place in the low word; its parity, that in the high word
+  constexpr unsigned h = J & 1 ? 0x3200 : 0x1000, l = (4 + J) * 0x11;
+  return __uint_as_float(__byte_perm(high, low, h | l));
+}
 
 // act(g) and its derivative, in float32, for results in float32.
 __device__ __forceinline__ float act_value_grad(float g, int act, float& da) {

@@ -43,6 +43,7 @@ struct Args {
   const void* bias;
   void* out;
   void* kept_out;
+  uint8_t* low;
   long long M, N, ldo;
   int np, act;
   int kblocks, mt, nt, gm;
@@ -176,16 +177,18 @@ __device__ __forceinline__ void gate_block(const Args& P, float* tile, int lane,
     if (!in || row0 >= P.M) continue;
     const int rows = static_cast<int>(min(16LL, P.M - row0));
     T* const h = static_cast<T*>(P.out) + row0 * P.ldo + x + lane;
-    T* const kept = P.kept_out ? static_cast<T*>(P.kept_out) + row0 * 2 * P.N + x + lane : nullptr;
+    KeptRow<T> kept(P.kept_out, P.low, row0, x + lane, P.N);
 #pragma unroll 2
     for (int r = 0; r < rows; ++r) {
       const float ur = tile[(16 + r) * kPitch + lane] + bu;
       float da;
       const float a = act_value_grad(tile[r * kPitch + lane] + bg, P.act, da);
       h[r * P.ldo] = from_f32<T>(a * ur);
-      if (kept) {
-        kept[r * 2 * P.N] = from_f32<T>(ur * da);
-        kept[r * 2 * P.N + P.N] = from_f32<T>(a);
+      if (P.kept_out) {
+        kept.put(0, ur * da);
+        kept.put(1, a);
+        kept.at += 2 * kept.N;
+        kept.low += 2 * kept.W;
       }
     }
   }
@@ -424,8 +427,9 @@ __global__ void __launch_bounds__(256) planes_join_kernel(const __grid_constant_
       float da;
       const float a = act_value_grad(v, P.act, da);
       if (P.kept_out) {
-        static_cast<T*>(P.kept_out)[row * 2 * P.N + x] = from_f32<T>(u * da);
-        static_cast<T*>(P.kept_out)[row * 2 * P.N + P.N + x] = from_f32<T>(a);
+        const KeptRow<T> kept(P.kept_out, P.low, row, x, P.N);
+        kept.put(0, u * da);
+        kept.put(1, a);
       }
       static_cast<T*>(P.out)[row * P.ldo + x] = from_f32<T>(a * u);
     }
@@ -437,16 +441,17 @@ __global__ void __launch_bounds__(256) planes_join_kernel(const __grid_constant_
 // of its own: in the product's epilogue it would hold up the sums that run through there (float32), and the factors' loads
 // would hold up the next tile (bf16, dx of 20001 x 1149 x 4605: 2410 us instead of 1180).
 template <typename T>
-__global__ void __launch_bounds__(256) dgate_kernel(const T* __restrict__ kept, const float* dh, long long ld, T* dgu, long long M, long long N) {
+__global__ void __launch_bounds__(256) dgate_kernel(const void* kept, const uint8_t* low, const float* dh, long long ld, T* dgu, long long M, long long N) {
   const long long row = blockIdx.x;
-  const T* const by = kept + row * 2 * N;
   const float* const from = dh + row * ld;
   T* const out = dgu + row * 2 * N;
 #pragma unroll 4
   for (long long c = blockIdx.y * 256LL + threadIdx.x; c < N; c += gridDim.y * 256LL) {
     const float v = from[c];
-    out[c] = from_f32<T>(v * to_f32<T>(by[c]));
-    out[N + c] = from_f32<T>(v * to_f32<T>(by[N + c]));
+    const KeptRow<T> by(kept, low, row, c, N);
+    const float g = by.get(0), u = by.get(1);
+    out[c] = from_f32<T>(v * g);
+    out[N + c] = from_f32<T>(v * u);
   }
 }
 
@@ -511,6 +516,7 @@ cudaError_t launch(const Product& p, const void* pa, const void* pb, cudaStream_
   a.bias = p.bias;
   a.out = p.out;
   a.kept_out = p.kept_out;
+  a.low = p.low;
   a.M = p.M;
   a.N = p.N;
   a.ldo = p.ldo;
@@ -633,9 +639,9 @@ cudaError_t launch_product_planes(const Product& p, const void* pa, const void* 
   const long long cols = (p.N + 1023) / 1024;
   const dim3 grid(static_cast<unsigned>(p.M), static_cast<unsigned>(cols < 64 ? cols : 64));
   if (f32)
-    planes::dgate_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(p.kept), dh, q.ldo, static_cast<float*>(p.out), p.M, p.N);
+    planes::dgate_kernel<float><<<grid, 256, 0, s>>>(p.kept, p.low, dh, q.ldo, static_cast<float*>(p.out), p.M, p.N);
   else
-    planes::dgate_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(p.kept), dh, q.ldo, static_cast<__nv_bfloat16*>(p.out), p.M, p.N);
+    planes::dgate_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p.kept, p.low, dh, q.ldo, static_cast<__nv_bfloat16*>(p.out), p.M, p.N);
   count_launches(1);
   return cudaGetLastError();
 }

@@ -27,6 +27,7 @@ struct Args {
   const void* bias;
   void* out;
   void* kept_out;
+  uint8_t* low;
   long long lda, ldb, ldo, N;
   int M, K, act, share;  // warps that share a pair of weight rows
 };
@@ -134,9 +135,9 @@ __global__ void __launch_bounds__(32 * kWarps) rows_kernel(const __grid_constant
     const float a = act_value_grad(s[0], P.act, da);
     out[n0] = from_f32<T>(a * s[1]);
     if (P.kept_out) {
-      T* const kept = static_cast<T*>(P.kept_out) + m * 2 * P.N;
-      kept[n0] = from_f32<T>(s[1] * da);
-      kept[P.N + n0] = from_f32<T>(a);
+      const KeptRow<T> kept(P.kept_out, P.low, m, n0, P.N);
+      kept.put(0, s[1] * da);
+      kept.put(1, a);
     }
   } else {
     out[n0] = from_f32<T>(s[0]);
@@ -262,9 +263,9 @@ __global__ void __launch_bounds__(32 * kMmaWarps) rows_mma_kernel(const __grid_c
         const float a = P.act == MSL_ACT_SILU ? act_grad_fast<MSL_ACT_SILU>(v0, da) : act_grad_fast<MSL_ACT_GELU>(v0, da);
         out[n0] = from_f32<T>(a * v1);
         if (P.kept_out) {
-          T* const kept = static_cast<T*>(P.kept_out) + m * 2LL * P.N;
-          kept[n0] = from_f32<T>(v1 * da);
-          kept[P.N + n0] = from_f32<T>(a);
+          const KeptRow<T> kept(P.kept_out, P.low, m, n0, P.N);
+          kept.put(0, v1 * da);
+          kept.put(1, a);
         }
       } else {
         if (in0) out[n0] = from_f32<T>(v0);
@@ -315,6 +316,7 @@ cudaError_t launch_product_rows(const Product& p, cudaStream_t s) {
   a.bias = p.bias;
   a.out = p.out; a.ldo = p.ldo;
   a.kept_out = p.kept_out;
+  a.low = p.low;
   a.N = p.N;
   a.M = static_cast<int>(p.M);
   a.K = static_cast<int>(p.K);

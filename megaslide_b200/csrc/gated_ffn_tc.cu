@@ -14,10 +14,11 @@
 // pairs walk over the tiles, one pair per two SMs.
 //   gate:  the tile's columns are BN/2 gate columns (the first CTA's half of B) and the same columns of the other
 //          projection, so g and u of an element meet in one epilogue thread: bias, activation and product; for
-//          the backward it also keeps u act'(g) and act(g), rounded to bf16 once each (g and u themselves would
-//          be rounded before the activation's derivative, and cost the backward the activation again)
-//   dgate: the sums are the gradient of h; the epilogue fetches the two kept factors by TMA, a step ahead, and
-//          writes the gradients of g and u over them in shared memory, from where they leave
+//          the backward it also keeps u act'(g) and act(g), 24 bits each (g and u themselves, in bf16, would
+//          be rounded before the activation's derivative, and cost the backward the activation again): the upper 16 by
+//          TMA, the lower 8 from the registers, 32 bytes a row
+//   dgate: the sums are the gradient of h; the epilogue fetches the two kept factors a step ahead, by TMA and into
+//          registers, and writes the gradients of g and u over the former in shared memory, from where they leave
 //
 // Tiles that do not fill a last round of all pairs are cut along k among the pairs left over: their parts' sums
 // go to the workspace in float32 and a small kernel joins them, in order, and does the epilogue.
@@ -59,6 +60,7 @@ struct Args {
   int bn, stages, stage_bytes, boxes;  // width of a tile, the ring, boxes of 64 that a CTA's half of B takes
   int full, items, parts, kper;        // tiles done whole; with the parts of the others; parts of a tile, their k-blocks
   float* partial;                      // [items - full][2 CTAs][4 x 32 rows][bn / 32][32 columns][32 rows]
+  uint8_t* low;                        // low bytes of the kept factors
   uint32_t* status;
 };
 
@@ -114,6 +116,23 @@ __device__ __forceinline__ void stage(uint32_t base, int row, const float (&v)[3
     const uint32_t w[4] = {pack(v[c * 8], v[c * 8 + 1]), pack(v[c * 8 + 2], v[c * 8 + 3]), pack(v[c * 8 + 4], v[c * 8 + 5]), pack(v[c * 8 + 6], v[c * 8 + 7])};
     sts(chunk32(base, row, c), w);
   }
+}
+
+// Kept factors: upper halves to a staging tile, low bytes to 32 bytes of a row of their own (columns from N to low_width(N)
+// are room for what is not read).
+__device__ __forceinline__ void stage_high(uint32_t base, int row, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t w[4] = {kept_high(v[c * 8], v[c * 8 + 1]), kept_high(v[c * 8 + 2], v[c * 8 + 3]), kept_high(v[c * 8 + 4], v[c * 8 + 5]), kept_high(v[c * 8 + 6], v[c * 8 + 7])};
+    sts(chunk32(base, row, c), w);
+  }
+}
+__device__ __forceinline__ void put_low(uint8_t* to, int cols, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (c * 16 < cols)
+      reinterpret_cast<uint4*>(to)[c] = make_uint4(kept_low(v[c * 16], v[c * 16 + 1], v[c * 16 + 2], v[c * 16 + 3]), kept_low(v[c * 16 + 4], v[c * 16 + 5], v[c * 16 + 6], v[c * 16 + 7]),
+                                                   kept_low(v[c * 16 + 8], v[c * 16 + 9], v[c * 16 + 10], v[c * 16 + 11]), kept_low(v[c * 16 + 12], v[c * 16 + 13], v[c * 16 + 14], v[c * 16 + 15]));
 }
 
 // adds bias[n .. n+32) to v (columns at or beyond N are clipped by the store)
@@ -278,6 +297,17 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         tma_load_3d(to, &maps.kept, bar, col0 + i * 32, 0, row0);
         tma_load_3d(to + kTile, &maps.kept, bar, col0 + i * 32, 1, row0);
       };
+      uint4 low[4];  // of the step to come: 32 low bytes of either factor
+      auto fetch_low = [&](int i) {
+        const long long W = low_width(P.N), x = col0 + i * 32;
+        const uint4* const from = reinterpret_cast<const uint4*>(P.low + (row0 + lane) * 2 * W + x);
+        const bool in = row0 + lane < P.M;
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) low[f * 2 + c] = in && x + c * 16 < P.N ? __ldg(from + f * (W / 16) + c) : make_uint4(0, 0, 0, 0);
+      };
+      if (EPI == kDgate && first < last && w.part < 0) fetch_low(first);
       if (EPI == kDgate && lane == 0 && first < last && w.part < 0) {  // on their way while the tile is still multiplied
         bulk_wait_read<0>();                             // the last tile's results have left
         fetch(turn, first);
@@ -306,18 +336,19 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         tmem_ld32(acc + c, v);
         if (EPI == kDgate) {
           const uint32_t g0 = mine + (turn & 1) * 2 * kTile, u0 = g0 + kTile;
+          const uint4 now[4] = {low[0], low[1], low[2], low[3]};
+          if (i + 1 < last) fetch_low(i + 1);
           if (!wait_warp(mykept + 8 * (turn & 1), (turn >> 1) & 1, dead, P.status)) { alive = false; break; }
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const uint4 gv = lds(chunk32(g0, lane, q)), uv = lds(chunk32(u0, lane, q));
-            const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
-            uint32_t dg[4], du[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float h0 = v[q * 8 + 2 * j], h1 = v[q * 8 + 2 * j + 1];
-              dg[j] = pack(h0 * bf16_lo(gw[j]), h1 * bf16_hi(gw[j]));
-              du[j] = pack(h0 * bf16_lo(uw[j]), h1 * bf16_hi(uw[j]));
-            }
+            const uint4 gl = now[q / 2], ul = now[2 + q / 2];
+            const uint32_t g01 = q & 1 ? gl.z : gl.x, g23 = q & 1 ? gl.w : gl.y, u01 = q & 1 ? ul.z : ul.x, u23 = q & 1 ? ul.w : ul.y;
+            const float* const h = v + q * 8;
+            const uint32_t dg[4] = {pack(h[0] * kept_at<0>(gv.x, g01), h[1] * kept_at<1>(gv.x, g01)), pack(h[2] * kept_at<2>(gv.y, g01), h[3] * kept_at<3>(gv.y, g01)),
+                                    pack(h[4] * kept_at<0>(gv.z, g23), h[5] * kept_at<1>(gv.z, g23)), pack(h[6] * kept_at<2>(gv.w, g23), h[7] * kept_at<3>(gv.w, g23))};
+            const uint32_t du[4] = {pack(h[0] * kept_at<0>(uv.x, u01), h[1] * kept_at<1>(uv.x, u01)), pack(h[2] * kept_at<2>(uv.y, u01), h[3] * kept_at<3>(uv.y, u01)),
+                                    pack(h[4] * kept_at<0>(uv.z, u23), h[5] * kept_at<1>(uv.z, u23)), pack(h[6] * kept_at<2>(uv.w, u23), h[7] * kept_at<3>(uv.w, u23))};
             sts(chunk32(g0, lane, q), dg);
             sts(chunk32(u0, lane, q), du);
           }
@@ -350,8 +381,15 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             }
             if (lane == 0) bulk_wait_read<0>();
             __syncwarp();
-            stage(mine, lane, d);
-            stage(mine + kTile, lane, v);
+            stage_high(mine, lane, d);
+            stage_high(mine + kTile, lane, v);
+            if (row0 + lane < P.M) {
+              const long long W = low_width(P.N);
+              uint8_t* const to = P.low + (row0 + lane) * 2 * W + x;
+              const int cols = static_cast<int>(min(32LL, P.N - x));  // under 1 where the tile's columns are none of the matrix'
+              put_low(to, cols, d);
+              put_low(to + W, cols, v);
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= u[j];
           } else {
@@ -453,6 +491,17 @@ __device__ __forceinline__ void put8(__nv_bfloat16* to, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(to) = make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
 }
 
+__device__ __forceinline__ void keep8(__nv_bfloat16* to, uint8_t* low, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(to) = make_uint4(kept_high(v[0], v[1]), kept_high(v[2], v[3]), kept_high(v[4], v[5]), kept_high(v[6], v[7]));
+  *reinterpret_cast<uint2*>(low) = make_uint2(kept_low(v[0], v[1], v[2], v[3]), kept_low(v[4], v[5], v[6], v[7]));
+}
+__device__ __forceinline__ void kept8(const __nv_bfloat16* from, const uint8_t* low, float (&v)[8]) {
+  const uint4 w = __ldg(reinterpret_cast<const uint4*>(from));
+  const uint2 l = __ldg(reinterpret_cast<const uint2*>(low));
+  v[0] = kept_at<0>(w.x, l.x); v[1] = kept_at<1>(w.x, l.x); v[2] = kept_at<2>(w.y, l.x); v[3] = kept_at<3>(w.y, l.x);
+  v[4] = kept_at<0>(w.z, l.y); v[5] = kept_at<1>(w.z, l.y); v[6] = kept_at<2>(w.w, l.y); v[7] = kept_at<3>(w.w, l.y);
+}
+
 template <int EPI, int ACT>
 __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ JoinArgs J) {
   const Args& P = J.tc;
@@ -478,22 +527,23 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ JoinA
       d[j] = u[j] * da;
     }
     if (J.kept_out) {
-      put8(J.kept_out + row * 2 * P.N + x, d);
-      put8(J.kept_out + row * 2 * P.N + P.N + x, v);
+      uint8_t* const low = P.low + row * 2 * low_width(P.N) + x;
+      keep8(J.kept_out + row * 2 * P.N + x, low, d);
+      keep8(J.kept_out + row * 2 * P.N + P.N + x, low + low_width(P.N), v);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= u[j];
   }
   if (EPI == kDgate) {
     const __nv_bfloat16* const kept = J.kept + row * 2 * P.N + x;
-    const uint4 gv = __ldg(reinterpret_cast<const uint4*>(kept)), uv = __ldg(reinterpret_cast<const uint4*>(kept + P.N));
-    const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+    const uint8_t* const low = P.low + row * 2 * low_width(P.N) + x;
+    float g[8], a[8];
+    kept8(kept, low, g);
+    kept8(kept + P.N, low + low_width(P.N), a);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u[2 * j] = v[2 * j] * bf16_lo(uw[j]);
-      u[2 * j + 1] = v[2 * j + 1] * bf16_hi(uw[j]);
-      v[2 * j] *= bf16_lo(gw[j]);
-      v[2 * j + 1] *= bf16_hi(gw[j]);
+    for (int j = 0; j < 8; ++j) {
+      u[j] = v[j] * a[j];
+      v[j] *= g[j];
     }
     put8(J.out + row * 2 * P.N + x, v);
     put8(J.out + row * 2 * P.N + P.N + x, u);
@@ -597,6 +647,7 @@ cudaError_t launch(const Product& p, cudaStream_t s) {
   a.nt = static_cast<int>(cut.nt);
   a.gm = a.mt <= 16 ? a.mt : 8;  // rows of tiles that go together: their operands stay in the L2 cache
   a.keep = p.kept_out != nullptr;
+  a.low = p.low;
   a.status = p.status;
   constexpr int smem = 1024 + kRing + kEpiWarps * kStaging + 24 * kMaxStages + 16 * kEpiWarps + 64;
   static_assert(smem <= 232448, "shared memory of a block");
@@ -631,7 +682,7 @@ bool tc_applies(const Product& p) {
   if (p.dtype != MSL_DTYPE_BF16 || !t5::encoder()) return false;
   if (!multiple_of(p.a, 16) || !multiple_of(p.b, 16) || !multiple_of(p.out, 16) || p.lda % 8 || p.ldb % 8 || p.ldo % 8 || p.N % 8) return false;
   if (p.bias && !multiple_of(p.bias, 16)) return false;
-  if ((p.kept && !multiple_of(p.kept, 16)) || (p.kept_out && !multiple_of(p.kept_out, 16))) return false;
+  if ((p.kept && !multiple_of(p.kept, 16)) || (p.kept_out && !multiple_of(p.kept_out, 16)) || ((p.kept || p.kept_out) && !multiple_of(p.low, 16))) return false;
   if (p.M > (1LL << 31) - 256 || p.N > (1LL << 30) || p.K > (1LL << 31) - 256) return false;
   if ((p.M + 127) / 128 * ((p.N + 63) / 64) > (1LL << 30)) return false;
   return true;

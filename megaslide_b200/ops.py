@@ -773,12 +773,18 @@ def _unaligned(*operands) -> int:
     return 1 if any(t is not None and t.data_ptr() & 15 for t in operands) else 0
 
 
+def _kept_bytes(M: int, F: int) -> Tuple[int, int]:
+    """Bytes of the kept factors of a bf16 block: the upper 16 bits [M, 2, F], and with the low 8 [M, 2, F rounded up to
+    16] after them."""
+    return 4 * M * F, 4 * M * F + 2 * M * ((F + 15) // 16 * 16)
+
+
 def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
                   b_out: Optional[torch.Tensor] = None, activation: str = "silu", keep: bool = False,
                   status: Optional[torch.Tensor] = None):
     """Gated feed-forward block on x [rows, >= dim] (row view).  Returns (y, h, kept): h [rows, hidden] the gated
-    product, kept [rows, 2 * hidden] what the backward needs (u act'(g), then act(g)) where ``keep``, else None.  status: a
-    device word for MSL_STATUS_TIMEOUT in place of the device's HostFlag."""
+    product, kept what the backward needs (u act'(g), then act(g)) where ``keep``, else None: [rows, 2 * hidden] in float32, in
+    bf16 bytes that hold 24 bits of each.  status: a device word for MSL_STATUS_TIMEOUT in place of the device's HostFlag."""
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
     dev, dt = x.device, x.dtype
     x_ld = _ld(x, "x")
@@ -786,10 +792,16 @@ def gated_ffn_fwd(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in
     off = (px | pi | po | (pbi or 0) | (pbo or 0)) & 15 or x_ld % 8
     g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation), 1 if off else 0)
     h = torch.empty(M, F, device=dev, dtype=dt)
-    kept = torch.empty(M, 2 * F, device=dev, dtype=dt) if keep else None
+    kept = low = None
+    if keep and dt == torch.float32:
+        kept = torch.empty(M, 2 * F, device=dev, dtype=dt)
+    elif keep:
+        high, both = _kept_bytes(M, F)
+        kept = torch.empty(both, device=dev, dtype=torch.uint8)
+        low = kept.data_ptr() + high
     y = torch.empty(x.shape, device=dev, dtype=dt)
     io = _lib.FfnIO(px, x_ld, pi, pbi, po, pbo, h.data_ptr(), _ptr(kept), y.data_ptr(), C)
-    io.status = _flag(dev, status)
+    io.status, io.kept_low = _flag(dev, status), low
     lib = _lib.load()
     with _on(dev):
         need = int(lib.msl_gated_ffn_workspace_bytes(ctypes.byref(g), 0))
@@ -807,8 +819,10 @@ def gated_ffn_bwd(x, w_in, w_out, h, kept, dy, b_in=None, b_out=None, activation
     M, C, F = _ffn_check(x, w_in, w_out, b_in, b_out)
     _need_cuda(h, kept, dy)
     dev, dt = x.device, x.dtype
-    for t, nm, width in ((h, "h", F), (kept, "kept", 2 * F), (dy, "dy", C)):
-        _operand(t, nm, M, width, dt, dev)
+    high, both = _kept_bytes(M, F)
+    rows = [(h, "h", M, F, dt), (dy, "dy", M, C, dt), (kept, "kept", M, 2 * F, dt) if dt == torch.float32 else (kept, "kept", 1, both, torch.uint8)]
+    for t, nm, n, width, kind in rows:
+        _operand(t, nm, n, width, kind, dev)
         if nm != "dy" and (t.shape[-1] != width or not t.is_contiguous()):
             raise ValueError(f"{nm} must be contiguous rows of {width} elements, got shape {tuple(t.shape)} strides {t.stride()}")
     if dy.shape[-1] != C:
@@ -824,7 +838,7 @@ def gated_ffn_bwd(x, w_in, w_out, h, kept, dy, b_in=None, b_out=None, activation
     g = _lib.FfnGeometry(M, C, F, dtype_code(dt), activation_code(activation), _unaligned(x, w_in, w_out, dy, h, kept) or int((x_ld | dy_ld) % 8 != 0))
     io = _lib.FfnIO(x.data_ptr(), x_ld, w_in.data_ptr(), None, w_out.data_ptr(), None, h.data_ptr(), kept.data_ptr(), None, 0,
                     dy.data_ptr(), dy_ld, _ptr(dgu), _ptr(dx), C, _ptr(dw_in), _ptr(dw_out), _ptr(db_in), _ptr(db_out),
-                    _flag(dev, status))
+                    _flag(dev, status), kept.data_ptr() + high if dt == torch.bfloat16 else None)
     lib = _lib.load()
     with _on(dev):
         need = int(lib.msl_gated_ffn_workspace_bytes(ctypes.byref(g), 1))

@@ -223,3 +223,15 @@ def test_leaves_that_require_gradients_stand_for_them():
     for a, b in zip(got, (plain, leaf.grad, param.grad, result), strict=True):
         assert a is b
     assert clip._list(leaf)[0] is leaf.grad and clip._list(bare) == []
+
+
+def test_ffn_entry_wants_the_low_bytes_beside_bf16_factors():
+    lib = _lib.load()
+    g = _lib.FfnGeometry(4, 8, 16, _lib.MSL_DTYPE_BF16, 0)
+    io = _lib.FfnIO(x=16, x_ld=8, w_in=16, w_out=16, h=16, y=16, y_ld=8, kept=16)
+    assert lib.msl_gated_ffn_fwd(ctypes.byref(g), ctypes.byref(io), None, 0, None) == _lib.MSL_ERR_INVALID
+    assert "kept_low" in lib.msl_last_error().decode()
+    io = _lib.FfnIO(x=16, x_ld=8, w_in=16, w_out=16, h=16, kept=16, dx=16, dx_ld=8, dy=16, dy_ld=8, dgu=16)
+    assert lib.msl_gated_ffn_bwd(ctypes.byref(g), ctypes.byref(io), None, 0, None) == _lib.MSL_ERR_INVALID
+    assert "kept_low" in lib.msl_last_error().decode()
+    assert ops._kept_bytes(3, 17) == (204, 204 + 2 * 3 * 32)

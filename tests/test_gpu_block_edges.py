@@ -291,6 +291,14 @@ def test_norm_weights_stay_float32_under_autocast(G, monkeypatch):
         assert not torch.equal(p.grad, p.grad.bfloat16().float())
 
 
+def _kept_factors(kept, M, F):
+    """The kept factors of a bf16 block as float32 [M, 2 F]: the upper 16 bits, then 8 more in rows of F rounded up to 16; the
+    last 8 are those 8 again."""
+    high = kept[:4 * M * F].view(torch.int16).view(M, 2, F).int() << 16
+    low = kept[4 * M * F:].view(M, 2, -1)[..., :F].int()
+    return (high | low << 8 | low).view(torch.float32).reshape(M, 2 * F)
+
+
 @pytest.mark.parametrize("M,C,F", [(1, 9, 30), (40, 77, 203), (130, 253, 635), (200, 1533, 2047)])
 def test_gated_ffn_widths_off_vectors_round_the_inner_gradients_once(M, C, F):
     """With one-hot rows of x, dw_in's columns are the gradients of g and u as the kernels hold them: the exact gradient
@@ -305,7 +313,7 @@ def test_gated_ffn_widths_off_vectors_round_the_inner_gradients_once(M, C, F):
     got = dw_in.t()[:rows].double()
     dh = dy.double() @ w_out.double()
     mag = dy.double().abs() @ w_out.double().abs()
-    kd = kept.double()
+    kd = _kept_factors(kept, M, F).double()
     want = torch.cat([dh * kd[:, :F], dh * kd[:, F:]], 1)[:rows]
     bound = torch.cat([mag * kd[:, :F].abs(), mag * kd[:, F:].abs()], 1)[:rows] * (C + 2) * EPS
     err = (got - want).abs()
@@ -365,3 +373,59 @@ def test_qk_norm_rope_heads_of_every_number_of_lanes(heads, kv, d, dtype, interl
         _within(y.detach(), w, wm, (d / 2 + 16) * EPS, half)
         _within(dx, wdx, wdxm, (2 * d + 32) * EPS, half)
         _within(dg, wdg, wdgm, (d / 2 + 16 + 6 * math.sqrt(B * N * nh)) * EPS, half)
+
+
+FACTORS = [(1, 64, 72), (5, 72, 200), (16, 256, 640), (17, 264, 328), (300, 256, 1024), (700, 1152, 1000), (1027, 256, 4040), (40, 77, 203), (700, 253, 635)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,C,F", FACTORS)
+def test_gated_ffn_keeps_its_factors_in_24_bits(M, C, F, act):
+    """u act'(g) and act(g) as the forward keeps them in bf16, by every form: off by the float32 sums (2 sqrt(C) + 16 EPS of
+    the absolute sums, through the activation's slope), the activation's own approximation (2^-15 of its value's scale) and
+    the 24th bit (2^-16)."""
+    x, w_in, w_out, b_in, b_out = (t.detach() for t in _ffn_case(M, C, F, torch.bfloat16, act, True))
+    kept = ops.gated_ffn_fwd(x, w_in, w_out, b_in, b_out, activation=act, keep=True)[2]
+    got = _kept_factors(kept, M, F).double()
+    gu = x.double() @ w_in.double().t() + b_in.double()
+    sums = (2 * math.sqrt(C) + 16) * EPS * (x.double().abs() @ w_in.double().abs().t() + b_in.double().abs())
+    g, u, eg, eu = gu[:, :F], gu[:, F:], sums[:, :F], sums[:, F:]
+    if act == "silu":
+        s = torch.sigmoid(g)
+        a, da = g * s, s * (1 + g * (1 - s))
+    else:
+        s = 0.5 * (1 + torch.erf(g / math.sqrt(2)))
+        a, da = g * s, s + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    # |act'| < 1.13 and |act''| < 1 for both
+    bound = torch.cat([2 * eg * u.abs() + 1.2 * eu, 1.2 * eg], 1) + 2.0 ** -15 * torch.cat([u.abs() * (da.abs() + 0.5), a.abs() + 0.5 * g.abs()], 1)
+    err = (got - torch.cat([u * da, a], 1)).abs()
+    assert torch.all(err <= bound + 2.0 ** -16 * got.abs() + 1e-37), float((err / bound).max())
+
+
+@pytest.mark.parametrize("M,C,F", FACTORS)
+def test_gated_ffn_bf16_gradients_have_two_roundings(M, C, F):
+    """The gradients of g and u are rounded as operands, then the result: RMS each, and no third one.  (RMS bounds a rounding's
+    root mean square at the foot of a binade; over all of it, it is 0.74 of that.  Two make 1.42, three 1.73.)"""
+    x, w_in, w_out, _, _ = _ffn_case(M, C, F, torch.bfloat16, "silu", False)
+    dy = _rand(9, M, C, dtype=torch.bfloat16)
+    y = msl.gated_ffn(x, w_in, w_out)
+    dx, dw_in = torch.autograd.grad(y, [x, w_in], dy)
+    _, wdx, wdw = _ffn_ref(x, w_in, w_out, None, None, "silu", dy)[:3]
+    for name, a, b in (("dx", dx, wdx), ("dw_in", dw_in, wdw)):
+        rel = float((a.double() - b).norm() / b.norm())
+        assert rel <= 1.5 * 0.74 * RMS, (name, rel)
+
+
+@pytest.mark.parametrize("C,F", [(64, 96), (61, 75)])
+@pytest.mark.parametrize("M", [1, 7, 200])
+def test_gated_ffn_kept_factors_that_are_not_finite(M, C, F):
+    """NaN and infinities keep what they are through the 24 bits: the row they are in, and no other."""
+    x, w_in, w_out, _, _ = (t.detach() if t is not None else None for t in _ffn_case(M, C, F, torch.bfloat16, "silu", False))
+    clean = _kept_factors(ops.gated_ffn_fwd(x, w_in, w_out, keep=True)[2], M, F)
+    for value in (float("nan"), float("inf")):
+        bad = x.clone()
+        bad[M - 1, 3] = value
+        got = _kept_factors(ops.gated_ffn_fwd(bad, w_in, w_out, keep=True)[2], M, F)
+        assert torch.equal(got[:M - 1], clean[:M - 1])
+        last = got[M - 1]
+        assert torch.isnan(last).all() if math.isnan(value) else not torch.isfinite(last[F:][clean[M - 1, F:].abs() < 1e30]).all()
