@@ -34,7 +34,13 @@ def dtype_code(dt: torch.dtype) -> int:
 def takes_derivatives(*ts) -> bool:
     """Whether a call goes through its autograd function: an operand requires a gradient, or a level of forward mode is
     open (a tangent asks for no gradient; the function refuses it, where the kernel alone would lose it)."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)) or forward_ad._current_level >= 0
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def once_only(backward):
@@ -557,16 +563,29 @@ def _ld(t: torch.Tensor, name: str) -> int:
     return _rows(t, name)
 
 
-def _operand(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype, dev: torch.device) -> None:
-    """Refuses an operand that is not `rows` rows of at least `width` elements of the call's type, on its device: the
-    kernels go by the call's geometry and would read or write beyond it."""
-    c = t.shape[-1] if t.dim() else 0
-    if c < width or t.numel() != rows * c:
-        raise ValueError(f"{name} must be {rows} rows of {width} elements, got {tuple(t.shape)}")
+def _extent(t: torch.Tensor, name: str, rows: int, width: int) -> int:
+    """Row stride of an operand; refuses one that is not `rows` rows of at least `width` elements: the kernels go by the
+    call's geometry and would read or write beyond it."""
+    shape = t.shape
+    if not shape or shape[-1] < width or t.numel() != rows * shape[-1]:
+        raise ValueError(f"{name} must be {rows} rows of {width} elements, got {tuple(shape)}")
+    return shape[-1] if t.is_contiguous() else _ld(t, name)
+
+
+def _operand(t: torch.Tensor, name: str, rows: int, width: int, dtype: torch.dtype, dev: torch.device) -> int:
+    """The same, and refuses one that is not of the call's type and on its device."""
     if t.dtype != dtype:
         raise TypeError(f"{name} must have the call's dtype {dtype}, got {t.dtype}")
     if t.device != dev:
         raise RuntimeError(f"{name} must be on the call's CUDA device {dev}, got {t.device}")
+    return _extent(t, name, rows, width)
+
+
+def _result(t: Optional[torch.Tensor], name: str, like: torch.Tensor, rows: int, width: int) -> Tuple[torch.Tensor, int]:
+    """A call's result and its row stride: the caller's tensor, checked, or a new one of like's rows."""
+    if t is None:
+        return torch.empty(*like.shape[:-1], width, device=like.device, dtype=like.dtype), width
+    return t, _operand(t, name, rows, width, like.dtype, like.device)
 
 
 class RotaryShape:
@@ -630,17 +649,15 @@ def rope3d(shape: RotaryShape, heads: int, x: torch.Tensor, table: torch.Tensor,
     _need_cuda(x, table, index)
     dev = x.device
     index_rows = _check_positions(shape, table, index, dev)
-    _operand(x, "x", shape.rows, heads * shape.head_dim, x.dtype, dev)
-    if out is None:
-        out = torch.empty(*x.shape[:-1], heads * shape.head_dim, device=dev, dtype=x.dtype)
-    else:
-        _operand(out, "out", shape.rows, heads * shape.head_dim, x.dtype, dev)
+    width = heads * shape.head_dim
+    x_ld = _extent(x, "x", shape.rows, width)
+    out, out_ld = _result(out, "out", x, shape.rows, width)
     g = shape.geometry(x.dtype)
     flag = _flag(dev, status) if index is not None else None
     with _on(dev):
         rc = _call("msl_rope3d", dev, lambda: _lib.load().msl_rope3d(
-            ctypes.byref(g), heads, x.data_ptr(), _ld(x, "x"), table.data_ptr(), _ptr(index), index_rows, 1 if inverse else 0,
-            out.data_ptr(), _ld(out, "out"), flag, _raw_stream(dev.index)))
+            ctypes.byref(g), heads, x.data_ptr(), x_ld, table.data_ptr(), _ptr(index), index_rows, 1 if inverse else 0,
+            out.data_ptr(), out_ld, flag, _raw_stream(dev.index)))
     _lib.check("msl_rope3d", rc)
     return out
 
@@ -648,11 +665,8 @@ def rope3d(shape: RotaryShape, heads: int, x: torch.Tensor, table: torch.Tensor,
 def _qk_io(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weight, k_weight, eps, table, index, status) -> "_lib.QkNormIO":
     _need_cuda(q, k, q_weight, k_weight, table, index)
     dev = q.device
-    if k is not None and k.dtype != q.dtype:
-        raise TypeError(f"q and k must have the same dtype, got {q.dtype} and {k.dtype}")
-    _operand(q, "q", shape.rows, heads * shape.head_dim, q.dtype, dev)
-    if kv_heads:
-        _operand(k, "k", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
+    q_ld = _extent(q, "q", shape.rows, heads * shape.head_dim)
+    k_ld = _operand(k, "k", shape.rows, kv_heads * shape.head_dim, q.dtype, dev) if kv_heads else 0
     wdt = torch.float32
     for w, nm in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if w is None:
@@ -665,7 +679,7 @@ def _qk_io(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weight, k_weig
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise TypeError("q_weight and k_weight must have the same dtype")
     return _lib.QkNormIO(
-        q.data_ptr(), _ld(q, "q"), _ptr(k) if kv_heads else None, _ld(k, "k") if kv_heads else 0, _ptr(q_weight), _ptr(k_weight),
+        q.data_ptr(), q_ld, _ptr(k) if kv_heads else None, k_ld, _ptr(q_weight), _ptr(k_weight),
         None, 0, None, 0, _ptr(table), _ptr(index), _check_positions(shape, table, index, dev),
         _flag(dev, status) if index is not None else None, heads, kv_heads, dtype_code(wdt), eps)
 
@@ -680,17 +694,11 @@ def qk_norm_rope_fwd(shape: RotaryShape, heads: int, kv_heads: int, q: torch.Ten
     takes q alone.  status as in rope3d."""
     io = _qk_io(shape, heads, kv_heads, q, k, q_weight, k_weight, eps, table, index, status)
     dev = q.device
-    if q_out is None:
-        q_out = torch.empty(*q.shape[:-1], heads * shape.head_dim, device=dev, dtype=q.dtype)
-    else:
-        _operand(q_out, "q_out", shape.rows, heads * shape.head_dim, q.dtype, dev)
-    io.q_out, io.q_out_ld = q_out.data_ptr(), _ld(q_out, "q_out")
+    q_out, io.q_out_ld = _result(q_out, "q_out", q, shape.rows, heads * shape.head_dim)
+    io.q_out = q_out.data_ptr()
     if kv_heads:
-        if k_out is None:
-            k_out = torch.empty(*k.shape[:-1], kv_heads * shape.head_dim, device=dev, dtype=k.dtype)
-        else:
-            _operand(k_out, "k_out", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
-        io.k_out, io.k_out_ld = k_out.data_ptr(), _ld(k_out, "k_out")
+        k_out, io.k_out_ld = _result(k_out, "k_out", k, shape.rows, kv_heads * shape.head_dim)
+        io.k_out = k_out.data_ptr()
     g = shape.geometry(q.dtype)
     with _on(dev):
         rc = _call("msl_qk_norm_rope_fwd", dev, lambda: _lib.load().msl_qk_norm_rope_fwd(
@@ -706,19 +714,15 @@ def qk_norm_rope_bwd(shape: RotaryShape, heads: int, kv_heads: int, q, k, q_weig
     io = _qk_io(shape, heads, kv_heads, q, k, q_weight, k_weight, eps, table, index, status)
     _need_cuda(dq_out, dk_out)
     dev = q.device
-    _operand(dq_out, "dq_out", shape.rows, heads * shape.head_dim, q.dtype, dev)
-    if dq is None:
-        dq = torch.empty(*q.shape[:-1], heads * shape.head_dim, device=dev, dtype=q.dtype)
-    else:
-        _operand(dq, "dq", shape.rows, heads * shape.head_dim, q.dtype, dev)
-    io.dq_out, io.dq_out_ld, io.dq, io.dq_ld = dq_out.data_ptr(), _ld(dq_out, "dq_out"), dq.data_ptr(), _ld(dq, "dq")
+    width = heads * shape.head_dim
+    io.dq_out, io.dq_out_ld = dq_out.data_ptr(), _operand(dq_out, "dq_out", shape.rows, width, q.dtype, dev)
+    dq, io.dq_ld = _result(dq, "dq", q, shape.rows, width)
+    io.dq = dq.data_ptr()
     if kv_heads:
-        _operand(dk_out, "dk_out", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
-        if dk is None:
-            dk = torch.empty(*k.shape[:-1], kv_heads * shape.head_dim, device=dev, dtype=k.dtype)
-        else:
-            _operand(dk, "dk", shape.rows, kv_heads * shape.head_dim, q.dtype, dev)
-        io.dk_out, io.dk_out_ld, io.dk, io.dk_ld = dk_out.data_ptr(), _ld(dk_out, "dk_out"), dk.data_ptr(), _ld(dk, "dk")
+        width = kv_heads * shape.head_dim
+        io.dk_out, io.dk_out_ld = dk_out.data_ptr(), _operand(dk_out, "dk_out", shape.rows, width, q.dtype, dev)
+        dk, io.dk_ld = _result(dk, "dk", k, shape.rows, width)
+        io.dk = dk.data_ptr()
     dgq = torch.empty_like(q_weight) if weight_grads and q_weight is not None else None
     dgk = torch.empty_like(k_weight) if weight_grads and k_weight is not None and kv_heads else None
     io.dq_weight, io.dk_weight = _ptr(dgq), _ptr(dgk)
