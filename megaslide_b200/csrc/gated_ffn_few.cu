@@ -1,5 +1,5 @@
-// The gated feed-forward block's float32 products for up to 64 rows (forward, and the gradients of h and x): the
-// weights are read once, split into bf16 planes in registers and multiplied on the tensor cores by mma.sync.
+// The gated feed-forward block's float32 products for up to 64 rows (forward, and from 9 rows on the gradients of h and
+// x): the weights are read once, split into bf16 planes in registers and multiplied on the tensor cores by mma.sync.
 //
 // An element is hi + mid + lo, eight bits each: hi its upper half, cut off (so no finite value becomes infinite), the
 // others rounded to nearest; the six products that reach 2^-24 of a product, the small ones of 32 k first.  Sums of 32 k
@@ -14,10 +14,9 @@
 // operand whatever order that has k and columns in, as long as x uses the same.  x goes through registers
 // into planes in shared memory, kChunk k at a time, once for the block.  Shares of k are joined by skinny_join_kernel.
 //
-// Measured, 7168 x 25088 (the four products that read weights, 1.08 GB each on average, joins included): 5, 13, 30 and 60
-// rows 338, 403, 470 and 683 us, where skinny_kernel took 309 (1 row), 430, 850 and about 1300.  What bounds it: up to 8
-// rows the splitting and the weights' bytes (3.2 TB/s), then the multiplications, 50 us for every 8 rows (2.4 clocks
-// an instruction).  12 or 16 warps a block are as fast; x by 64 k at a time and five stages 5% slower than by 128 and three.
+// Measured: at few_shape below.  What bounds it: up to 8 rows the splitting and the weights' bytes (7168 x 25088 forward, 2.16
+// GB: 620 us, 3.5 TB/s), then the multiplications, 50 us for every 8 rows of 1.08 GB (2.4 clocks an instruction).  12 or
+// 16 warps a block are as fast; x by 64 k at a time and five stages 5% slower than by 128 and three.
 
 #include "gated_ffn.cuh"
 
@@ -239,10 +238,13 @@ cudaError_t launch(const Args& a, int shares, cudaStream_t s) {
 
 }  // namespace few
 
-// Weights of 64 MB at least: 13, 30 and 60 rows of 2560 x 8960 a call 120, 142 and 205 us, by skinny_kernel 160, 266 and 288; of
-// 1152 x 4608 (21 and 42 MB) 53, 63 and 87 against 51, 60 and 89.
+// Weights of 64 MB at least, and more than 8 rows where the weights are stored [K, N] (the gradients of h and x).  Forward of 5,
+// 13, 30 and 60 rows of 2560 x 8960: 100, 113, 141 and 192 us, by skinny_kernel 170, 133, 242 and 282; 7168 x 25088: 628,
+// 751, 961 and 1325, 1193, 913, 1758 and 2136.  Gradients of h and x, 5, 13, 30 and 60 rows of 7168 x 25088: 728, 835, 902 and
+// 1389, 630, 823, 1658 and 2041; 2560 x 8960: 107, 120, 131 and 197, 105, 132, 253 and 292.  1152 x 4608 (21 and 42 MB),
+// 13, 30 and 60 rows forward 45, 57 and 76, 43, 72 and 78; gradients 47, 54 and 76, 37, 59 and 72.
 bool few_shape(long long M, long long cols, long long K, bool a_major, bool b_major) {
-  return !a_major && M <= kMostRowsFew && cols * K >= (1LL << 24) && (b_major ? cols % 4 == 0 : K % 4 == 0);
+  return !a_major && M <= kMostRowsFew && cols * K >= (1LL << 24) && (b_major ? M > 8 && cols % 4 == 0 : K % 4 == 0);
 }
 size_t few_bytes(long long M, long long N, long long K, int epilogue) {
   const long long cols = epilogue == kGate ? 2 * N : N;
@@ -268,7 +270,7 @@ cudaError_t launch_product_few(const Product& p, cudaStream_t s) {
   a.kper = cut.kper;
   a.M = static_cast<int>(p.M);
   cudaError_t e;
-  if (p.M <= 8) e = p.b_major ? few::launch<1, true>(a, cut.shares, s) : few::launch<1, false>(a, cut.shares, s);
+  if (p.M <= 8) e = few::launch<1, false>(a, cut.shares, s);
   else if (p.M <= 16) e = p.b_major ? few::launch<2, true>(a, cut.shares, s) : few::launch<2, false>(a, cut.shares, s);
   else if (p.M <= 32) e = p.b_major ? few::launch<4, true>(a, cut.shares, s) : few::launch<4, false>(a, cut.shares, s);
   else e = p.b_major ? few::launch<8, true>(a, cut.shares, s) : few::launch<8, false>(a, cut.shares, s);
