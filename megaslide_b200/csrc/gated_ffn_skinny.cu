@@ -237,8 +237,9 @@ __global__ void __launch_bounds__(256) skinny_join_kernel(const float* __restric
 
 // The weights' gradients of up to KM rows, out[m][n] = sum_k a[k][m] b[k][n]: bound by the bytes of the result.  A thread
 // has 4 columns, whose b stays in registers, and writes them for kOuterRows rows; a comes through shared memory.
-// 7168 x 25088, both gradients on average (0.72 GB): 1 row 159 us (4.5 TB/s of writes alone), 13 rows 215, 30 rows 528; by skinny_kernel
-// 421, 437, and by planes 586.
+// dw_out of 7168 x 25088 (0.72 GB), 1, 4 and 13 rows: 109, 111 and 159 us (6.6 TB/s of writes with one row), by
+// skinny_kernel 280, 283 and 293; 1152 x 4608 6.2, 6.2 and 8.2, 12.3, 12.3 and 12.4.  With 30 rows it was 326 and 16.4 against
+// 314 and 14.3, so beyond 16 skinny_kernel has them.
 constexpr int kOuterRows = 32;
 
 template <int KM>
@@ -358,12 +359,11 @@ cudaError_t launch_product_skinny(const Product& p, cudaStream_t s) {
   a.va = multiple_of(p.a, 16) && p.lda % 4 == 0;
   a.vb = multiple_of(p.b, 16) && p.ldb % 4 == 0;
   cudaError_t e;
-  if (direct && p.K <= 32 && p.N % 4 == 0 && a.vb && multiple_of(p.out, 16) && p.ldo % 4 == 0) {
+  if (direct && p.K <= 16 && p.N % 4 == 0 && a.vb && multiple_of(p.out, 16) && p.ldo % 4 == 0) {
     const dim3 grid(static_cast<unsigned>((p.M + skinny::kOuterRows - 1) / skinny::kOuterRows), static_cast<unsigned>((p.N + 1023) / 1024));
     if (p.K <= 4) skinny::outer_kernel<4><<<grid, 256, 0, s>>>(a);
     else if (p.K <= 8) skinny::outer_kernel<8><<<grid, 256, 0, s>>>(a);
-    else if (p.K <= 16) skinny::outer_kernel<16><<<grid, 256, 0, s>>>(a);
-    else skinny::outer_kernel<32><<<grid, 256, 0, s>>>(a);
+    else skinny::outer_kernel<16><<<grid, 256, 0, s>>>(a);
     return cudaGetLastError();
   }
   // rows on the grid's x, the axis that may be long (columns: at most 2^21 / 128)
