@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       uint4 low[4];  // of the step to come: 32 low bytes of either factor
       auto fetch_low = [&](int i) {
         const long long W = low_width(P.N), x = col0 + i * 32;
-        const uint4* const from = reinterpret_cast<const uint4*>(P.low + (row0 + lane) * 2 * W + x);
+        const uint4* const from = reinterpret_cast<const uint4*>(P.low + 2 * W * (row0 + lane) + x);
         const bool in = row0 + lane < P.M;
 #pragma unroll
         for (int f = 0; f < 2; ++f)
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             stage_high(mine + kTile, lane, v);
             if (row0 + lane < P.M) {
               const long long W = low_width(P.N);
-              uint8_t* const to = P.low + (row0 + lane) * 2 * W + x;
+              uint8_t* const to = P.low + 2 * W * (row0 + lane) + x;
               const int cols = static_cast<int>(min(32LL, P.N - x));  // under 1 where the tile's columns are none of the matrix'
               put_low(to, cols, d);
               put_low(to + W, cols, v);

@@ -429,3 +429,21 @@ def test_gated_ffn_kept_factors_that_are_not_finite(M, C, F):
         assert torch.equal(got[:M - 1], clean[:M - 1])
         last = got[M - 1]
         assert torch.isnan(last).all() if math.isnan(value) else not torch.isfinite(last[F:][clean[M - 1, F:].abs() < 1e30]).all()
+
+
+@pytest.mark.parametrize("dtype,C,F", [(torch.bfloat16, 8, 2056), (torch.bfloat16, 7, 2055), (torch.float32, 8, 2056)], ids=["bf16", "bf16-odd", "fp32"])
+def test_gated_ffn_beyond_2_31_elements(dtype, C, F):
+    """Hidden values, kept factors and inner gradients of over 2^31 elements: the last rows and, with a gradient in them
+    alone, the weights' gradients."""
+    M, n = 2 ** 19 + 37, 70
+    x = torch.empty(M, C, device=_dev(), dtype=dtype).normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    _, w_in, w_out, b_in, b_out = _ffn_case(1, C, F, dtype, "silu", True)
+    x.requires_grad_()
+    dy = torch.zeros_like(x)
+    dy[-n:] = _rand(9, n, C, dtype=dtype)
+    y = msl.gated_ffn(x, w_in, w_out, b_in, b_out)
+    got = torch.autograd.grad(y, [x, w_in, w_out, b_in, b_out], dy)
+    want = _ffn_ref(x[-n:], w_in, w_out, b_in, b_out, "silu", dy[-n:])
+    assert torch.count_nonzero(got[0][:-n]) == 0
+    for name, a, b in zip(("y", "dx", "dw_in", "dw_out", "db_in", "db_out"), (y.detach()[-n:], got[0][-n:], *got[1:]), want):
+        _close(a, b, (2 * math.sqrt(2 * F) + 16) * EPS if dtype == torch.float32 else (2 if name in ("y", "db_out") else 4) * RMS, name)
