@@ -12,8 +12,8 @@
 // (96 KB for three planes and 256 columns, two stages); results go through a transposing tile of shared memory, a
 // row of 32 at a time, whatever their alignment.
 //
-// What bounds it: six times the multiplications, so about 220 TFLOP/s of float32 products; the CUDA cores' limit
-// is 75.
+// What bounds it: six times the multiplications, so about 220 TFLOP/s of float32 products (4096 x 4096 x 4096 forward 214,
+// backward 219; 16384 x 2048 x 8192 219 and 214); the CUDA cores' limit is 75.
 
 #include <algorithm>
 

@@ -8,10 +8,13 @@
 // joined in a fixed order.  The second projection is launched so that it may start while the first still
 // runs: it loads weights first and waits for h only then.
 //
-// What bounds it: 1 x 1152 x 4608 in bf16 (32 MB of weights, which the L2 cache holds) 6.8 and 6.2 us, 8 rows 7.4 and
-// 8.0: the launches and one trip to the cache; 1 x 7168 x 28672 (1.23 GB) the memory, 131 us for the first
-// projection's 822 MB, 6.3 TB/s (by mma.sync 165 us, so one row does without; at the small size they are
-// even).  The tensor cores' own form takes 24 us and 260 us for 17 rows.
+// h is rounded to bf16 here too, though one row's second projection could read it unrounded: a token's result then is the
+// same whether it comes alone or among others, and what the backward reads is what the forward used.
+//
+// What bounds it: 1 x 1152 x 4608 in bf16 (32 MB of weights, which the L2 cache holds) 10.3 us, 8 rows 12.3, 16 rows 16.4,
+// both projections from a CUDA graph: the launches and one trip to the cache; 1 x 7168 x 28672 (1.23 GB) the memory, 249 us
+// (by mma.sync 260, so one row does without; at the small size they are even).  The tensor cores' own form takes 28.7
+// and 302 us for 17 rows.
 
 #include "gated_ffn.cuh"
 
@@ -294,9 +297,9 @@ cudaError_t launch_mma(Args a, cudaStream_t s) {
 
 }  // namespace rows
 
-// More rows only while the caches hold the weights: bf16, 7168 x 28672, 390 us for 16, against 260 on the tensor cores;
-// float32, 4 and 8 rows a call, 1152 x 4608: 27 and 40 us, against 48 by few_kernel, 7168 x 28672: 1064 and 1545
-// against 732 and 741.
+// More rows only while the caches hold the weights.  bf16, 7168 x 28672, 8, 9 and 16 rows: 281, 345 and 371 us, on the tensor
+// cores 337, 329 and 299; 1152 x 4608 12.3, 14.4 and 16.4 against 28.7.  float32, 2, 3, 4 and 8 rows of 7168 x 28672: 449,
+// 760, 1063 and 1556 us, by few_kernel 733, 737, 741 and 764; 1152 x 4608 16.5, 18.5, 22.5 and 36.8, by skinny_kernel 38.9.
 long long rows_most(int dtype, long long weights) {
   const bool cached = weights < (1LL << 25);
   return dtype == MSL_DTYPE_F32 ? (cached ? kMostRowsF32 : 2) : cached ? kMostRows : kMostRows / 2;

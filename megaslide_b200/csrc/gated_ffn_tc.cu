@@ -28,8 +28,9 @@
 // alone need 48 KB).  Where k is short the epilogue's bytes share that path: with 18 stages a tile (k = 1152) the gate's
 // results are 17% more and its stage takes 900 clocks, dgate's kept factors and results 44% more.  16 epilogue warps
 // instead of 8, or a second loading thread, change nothing.  In long runs the power limit holds the clock near
-// 1.4 to 1.6 GHz.  4096 x 7168 x 28672: 1.25 to 1.31 PFLOP/s a product; 32768 x 1152 x 4608: 1.13 (gate), 0.92
-// (dgate), 1.25 (the others).
+// 1.4 to 1.6 GHz.  16384 x 1152 x 4608: gate with kept factors 334 us (1.04 PFLOP/s), dgate 202 (0.86), the others 1.26 to
+// 1.32 PFLOP/s.  In a hot loop 4096 x 7168 x 28672 forward 1.23 (with kept factors 1.18) and backward 1.18, the same
+// products by cuBLAS 1.22 to 1.41 without the activations; 32768 x 1152 x 4608 1.20 (0.99) and 0.99, cuBLAS 1.20 to 1.30.
 
 #include "gated_ffn.cuh"
 #include "tcgen05.cuh"

@@ -18,11 +18,12 @@
 // two pairs at a time (fma.rn.f32x2), the weights are multiplied into the cosines and sines once per token, and
 // lanes without a head load a neighbour's instead of branching (they only never store).
 //
-// Measured in a steady loop, bf16 (of the measured copy bandwidth): rotation of 131072 x 16 x 72, 604 MB, 107 us, 5.6
-// TB/s (86%); norm and rotation of 262144 x 24 x 64 queries and keys, 3.2 GB, 593 us, 5.4 TB/s (83%); their backward,
-// 4.8 GB, 859 us, 5.6 TB/s (86%).  At these rates the GPU is at its 1000 W (a plain copy takes 770) and the clock falls
-// to 1.7 GHz, so instructions count beside bytes; a GPU that kept its clock took 518 and 807 us (95 and 91%).  With
-// loads straight to registers 145, 740 and 1035 us.
+// Measured, bf16 (of the measured copy bandwidth): rotation of 131072 x 16 x 72, 604 MB, 113 us, 5.4 TB/s (82%); norm and
+// rotation of 262144 x 24 x 64 queries and keys, 3.2 GB, 545 us, 5.9 TB/s (90%); their backward, 4.8 GB, 758 us, 6.4 TB/s
+// (97%); in a long loop 593 and 859.  At these rates the GPU comes to its 1000 W (a plain copy takes 770) and the clock
+// falls to 1.7 GHz, so instructions count beside bytes.  131072 x 16 x 72 queries and keys, whose 9 lanes a head sum by
+// the loop and leave 5 of 32 idle: 297 and 505 us, 4.1 and 3.6 TB/s.  With loads straight to registers 145, 740 and
+// 1035 us.
 
 #include "msl_abi.cuh"
 #include "msl_common.cuh"
