@@ -3,7 +3,6 @@ memory order or another default device, and where a trainer's gradients are not 
 test_gpu_block_ops.py: (2 sqrt(K) + 16) roundings of float32 for a product of K terms in the 2-norm, RMS for every rounding
 to bfloat16."""
 
-import copy
 import math
 
 import pytest
